@@ -1,0 +1,42 @@
+// kv_q8.cuh -- device helpers of the 8-bit cache's kernels: scale words and
+// code conversions.
+#pragma once
+
+#include "kv_q8.h"
+
+namespace kvb {
+namespace q8 {
+
+constexpr int kBad = -128;   // the code of a value that F16 does not hold as a finite number
+
+// A scale word is the float 2^e, or, for a block with a kBad code, a NaN that
+// keeps e + 127 in its low byte (so a rewound block can be stored again).
+__device__ __forceinline__ int scale_exp(uint32_t w)
+{
+    return (int)((w & 0x7f800000u) == 0x7f800000u ? (w & 0xffu) : w >> 23) - 127;
+}
+
+__device__ __forceinline__ uint32_t scale_word(int e, bool bad)
+{
+    return bad ? 0x7fc00000u | (uint32_t)(e + 127) : (uint32_t)(e + 127) << 23;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The smallest e in [kExpMin, kExpMax] at which amax (>= 0, finite) / 2^e
+// rounds to at most 127.  amax / 2^(floor(log2 amax) - 6) lies in [64, 128).
+__device__ __forceinline__ int block_exp(float amax)
+{
+    int e = (int)(__float_as_uint(amax) >> 23) - 127 - 6;
+    e = max(e, kExpMin);   // (also amax = 0)
+    if (__fmul_rn(amax, pow2(-e)) >= 127.5f) e++;
+    return min(e, kExpMax);
+}
+
+__device__ __forceinline__ int to_code(float y, float inv_scale)
+{
+    return max(-127, min(127, __float2int_rn(__fmul_rn(y, inv_scale))));
+}
+
+}  // namespace q8
+}  // namespace kvb

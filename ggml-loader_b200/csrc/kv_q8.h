@@ -1,0 +1,73 @@
+// kv_q8.h -- the 8-bit cache: what its kernels and the C entry points share.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace kvb {
+namespace q8 {
+
+constexpr int kBlock = 32;   // rows that share a scale (KV_Q8_BLOCK)
+constexpr int kExpMin = -24, kExpMax = 9;   // a scale is 2^e with e in this range
+
+struct Cache {
+    int8_t *k, *v;              // [H][rows][D]
+    float *k_scale, *v_scale;   // [H][rows / kBlock]
+    float *weight;              // [H][rows] or null
+    int64_t rows;
+    int32_t H, D;
+};
+
+struct StoreParams {
+    Cache c;
+    const void *k, *v;
+    int64_t k_stride, v_stride;   // elements a token
+    int64_t row0;
+    int32_t n_new;
+    int32_t f16;   // 1: __half rows, 0: float rows
+    int32_t vec;   // every row starts on a 16-byte boundary
+};
+cudaError_t launch_store(const StoreParams &p, cudaStream_t st);
+
+struct LoadParams {
+    Cache c;
+    void *k, *v;   // either may be null
+    int64_t stride;
+    int64_t row0, n;
+    int32_t f16, vec;
+};
+cudaError_t launch_load(const LoadParams &p, cudaStream_t st);
+
+struct EvictParams {
+    Cache src, dst;
+    int64_t n_rows, keep, recent;
+    int32_t *kept;   // [H][keep]
+};
+cudaError_t launch_evict(const EvictParams &p, cudaStream_t st);
+
+struct AttendParams {
+    Cache c;
+    int32_t Hq, r;          // query heads, query heads a KV head
+    int64_t n_past, n_kv;   // n_kv = n_past + n_new
+    int32_t n_new;
+    const void *q;
+    int64_t q_stride;
+    int32_t q_f16;
+    const void *mask;       // null: causal
+    int64_t mask_stride;
+    int32_t mask_f16;
+    int32_t flash;          // a row without a visible key gives 0 (else NaN)
+    void *out;
+    int64_t out_stride;
+    int32_t out_f16;
+    float scale;
+    char *ws;
+};
+// bytes of p.ws (a function of the sizes alone)
+uint64_t attend_workspace(const AttendParams &p);
+cudaError_t launch_attend(const AttendParams &p, cudaStream_t st);
+
+}  // namespace q8
+}  // namespace kvb

@@ -54,6 +54,11 @@ class KvConfig(ctypes.Structure):
     ]
 
 
+class KvQ8Cache(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("weight", _vp),
+                ("rows", _i64), ("n_head_kv", _i32), ("head_dim", _i32)]
+
+
 class KvError(RuntimeError):
     def __init__(self, code, what):
         self.code = code
@@ -102,6 +107,12 @@ def lib():
         "kv_launch_count": (_i64, [_vp]),
         "kv_debug_stamps": (_i64, [_vp, _vp, ctypes.POINTER(_i32), ctypes.POINTER(_i32)]),
         "kv_attend_decode_noalloc": (ctypes.c_int, [_vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp]),
+        "kv_q8_store": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _vp]),
+        "kv_q8_load": (ctypes.c_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp]),
+        "kv_q8_attend_workspace": (_u64, [_vp, _i32, _i64, _i32]),
+        "kv_q8_attend": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i64, ctypes.c_uint32,
+                                        _vp, _i64, _i32, _vp, _u64, _vp]),
+        "kv_q8_evict": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp]),
         "kv_status": (ctypes.c_int, [_vp, _vp]),
         "kv_debug_inject": (ctypes.c_int, [_vp, _i32, _u64]),
         "kv_rope_table_host": (ctypes.c_int, [cfgp, _i64, _i64, _vp]),
@@ -358,6 +369,114 @@ def attend_decode_noalloc(k_cache, v_cache, n_head, n_head_kv, head_dim, n_kv, q
     return _check(lib().kv_attend_decode_noalloc(_ptr(k_cache), _ptr(v_cache), n_head, n_head_kv, head_dim, n_kv,
                                                  _ptr(q), _ptr(out), _stream(stream)),
                   "kv_attend_decode_noalloc")
+
+
+Q8_BLOCK = 32
+
+
+class Q8Cache:
+    """One layer's 8-bit cache over the caller's CUDA tensors (kv_q8_cache): codes
+    k, v int8 [n_head_kv][rows][head_dim], scales float32 [n_head_kv][rows / 32]
+    and, where attention weights are kept, weight float32 [n_head_kv][rows], all
+    contiguous and on one device, which the calls run on.  Rows, queries, masks
+    and outputs are CUDA tensors whose last dimension is contiguous: a token's
+    heads are one row, its stride may be larger (a fused Q/K/V row)."""
+
+    def __init__(self, k, v, k_scale, v_scale, weight=None):
+        import torch
+        h, rows, d = k.shape
+        want = [("k", k, (h, rows, d), torch.int8), ("v", v, (h, rows, d), torch.int8),
+                ("k_scale", k_scale, (h, rows // Q8_BLOCK), torch.float32),
+                ("v_scale", v_scale, (h, rows // Q8_BLOCK), torch.float32)]
+        if weight is not None:
+            want.append(("weight", weight, (h, rows), torch.float32))
+        for name, t, shape, dtype in want:
+            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != k.device:
+                raise ValueError("%s must be a contiguous %s tensor %s on %s" % (name, dtype, shape, k.device))
+        self.tensors = k, v, k_scale, v_scale, weight   # kept alive
+        self.device = k.device
+        self.n_head_kv, self.rows, self.head_dim = h, rows, d
+        self._c = KvQ8Cache(*[_ptr(t) for t in self.tensors], rows, h, d)
+        self._ref = ctypes.addressof(self._c)
+
+    def _rows(self, name, t, n, width):
+        """(pointer, stride, type) of a tensor of n rows of `width` elements."""
+        import torch
+        if t.dtype not in (torch.float32, torch.float16):
+            raise ValueError("%s must be float32 or float16" % name)
+        shape, stride = t.shape, t.stride()
+        if shape[0] != n or t.numel() != n * width or t.device != self.device:
+            raise ValueError("%s must hold %d rows of %d elements on %s" % (name, n, width, self.device))
+        inner = 1
+        for i in range(len(shape) - 1, 0, -1):
+            if shape[i] != 1 and stride[i] != inner:
+                raise ValueError("the rows of %s must be contiguous" % name)
+            inner *= shape[i]
+        return t.data_ptr(), stride[0], int(t.dtype == torch.float16)
+
+    def _call(self, name, *args):
+        """The call on this cache's device."""
+        import torch
+        index = self.device.index
+        if index is not None and torch.cuda.is_available() and index != torch.cuda.current_device():
+            with torch.cuda.device(index):
+                return _check(getattr(lib(), name)(self._ref, *args), name)
+        return _check(getattr(lib(), name)(self._ref, *args), name)
+
+    def store(self, row0, n_new, k, v, stream=None):
+        """kv_q8_store: n_new rows of [n_head_kv][head_dim] at row0."""
+        width = self.n_head_kv * self.head_dim
+        kp, ks, kt = self._rows("k", k, n_new, width)
+        vp, vs, vt = self._rows("v", v, n_new, width)
+        if kt != vt:
+            raise ValueError("k and v must have one type")
+        return self._call("kv_q8_store", row0, n_new, kp, ks, vp, vs, kt, _stream(stream))
+
+    def load(self, row0, n, k_out, v_out, stream=None):
+        """kv_q8_load: the values of n rows from row0 into k_out and v_out (either may be None)."""
+        got = [None if t is None else self._rows(s, t, n, self.n_head_kv * self.head_dim)
+               for s, t in (("k_out", k_out), ("v_out", v_out))]
+        some = [g for g in got if g]
+        if some and any(g[1:] != some[0][1:] for g in some):
+            raise ValueError("k_out and v_out must have one type and row stride")
+        stride, kind = some[0][1:] if some else (0, 0)
+        return self._call("kv_q8_load", row0, n, got[0] and got[0][0], got[1] and got[1][0], stride, kind,
+                          _stream(stream))
+
+    def attend_workspace(self, n_head, n_past, n_new):
+        """Bytes of workspace attend needs for these sizes."""
+        n = int(lib().kv_q8_attend_workspace(self._ref, n_head, n_past, n_new))
+        if n == 0:
+            raise KvError(KV_E_ARG, "kv_q8_attend_workspace")
+        return n
+
+    def attend(self, n_head, n_past, n_new, q, out, mask=None, flash=False, workspace=None, stream=None):
+        """kv_q8_attend: n_new rows of [n_head][head_dim] queries over the rows
+        [0, n_past + n_new); workspace: a uint8 CUDA tensor of attend_workspace bytes."""
+        import torch
+        width = n_head * self.head_dim
+        qp, qs, qt = self._rows("q", q, n_new, width)
+        op, os_, ot = self._rows("out", out, n_new, width)
+        mp, mt, ms = None, 0, 0
+        if mask is not None:
+            if mask.dim() != 2 or mask.stride(1) != 1 or mask.shape[0] != n_new or mask.shape[1] < n_past + n_new or \
+                    mask.dtype not in (torch.float32, torch.float16) or mask.device != self.device:
+                raise ValueError("mask must be [n_new][>= n_past + n_new], float32 or float16, on %s" % self.device)
+            mp, mt, ms = mask.data_ptr(), int(mask.dtype == torch.float16), mask.stride(0)
+        if workspace is None or workspace.device != self.device or not workspace.is_contiguous():
+            raise ValueError("attend needs a contiguous workspace tensor on %s" % self.device)
+        return self._call("kv_q8_attend", n_head, n_past, n_new, qp, qs, qt, mp, mt, ms, 1 if flash else 0,
+                          op, os_, ot, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                          _stream(stream))
+
+    def evict(self, n_rows, keep, recent, dst, kept, stream=None):
+        """kv_q8_evict into the Q8Cache dst; kept: int32 [n_head_kv][keep]."""
+        import torch
+        if tuple(kept.shape) != (self.n_head_kv, keep) or kept.dtype != torch.int32 or not kept.is_contiguous() or \
+                kept.device != self.device or dst.device != self.device:
+            raise ValueError("kept must be a contiguous int32 [%d][%d] tensor on %s, with dst there too"
+                             % (self.n_head_kv, keep, self.device))
+        return self._call("kv_q8_evict", n_rows, keep, recent, dst._ref, kept.data_ptr(), _stream(stream))
 
 
 def gen_normal_device(dst, seed, stream_id, n, idx0=0, stream=None):

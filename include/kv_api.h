@@ -269,6 +269,104 @@ int kv_attend_decode_noalloc(const uint16_t *k_cache, const uint16_t *v_cache,
                              int32_t n_head, int32_t n_head_kv, int32_t head_dim, int64_t n_kv,
                              const float *q, float *out, void *stream);
 
+/* ---- the cache in 8 bits -------------------------------------------------- */
+/*
+ * One layer's K and V in 8-bit codes with one scale for each KV head and block
+ * of KV_Q8_BLOCK consecutive rows: half the bytes an attention call streams
+ * and half the memory of the F16 cache.  No counterpart in the reference,
+ * whose cache is F16.  The calls below work on the caller's buffers and
+ * allocate nothing, as kv_attend_decode_noalloc does.
+ *
+ *   code c of row i, block b = i / KV_Q8_BLOCK, stands for c * scale[h][b];
+ *   scale = 2^e with the smallest e in [-24, 9] at which the block's largest
+ *   magnitude rounds to a code <= 127 (e = 9 saturates there): a power of two,
+ *   so every value is an exact F16, and a row that moves to another block of
+ *   the same scale keeps its codes.  A value is first rounded to F16, as the
+ *   F16 cache would hold it.  What is not finite then (inf, NaN) has code -128,
+ *   which reads back as NaN, and its block's scale is NaN (the exponent kept in
+ *   the low byte): attention takes every row of such a block as NaN.
+ *
+ * All pointers are DEVICE pointers on the current device, k and v 16-byte
+ * aligned; rows is a multiple of KV_Q8_BLOCK, at most 2^31 - 32.  head_dim: 64,
+ * 96, 128 or 256.  n_head_kv: at most 1024.
+ */
+#define KV_Q8_BLOCK 32
+
+typedef struct kv_q8_cache {
+    int8_t *k, *v;              /* [n_head_kv][rows][head_dim] codes            */
+    float *k_scale, *v_scale;   /* [n_head_kv][rows / KV_Q8_BLOCK]              */
+    float *weight;              /* [n_head_kv][rows] accumulated attention weight,
+                                   or NULL: none is kept                        */
+    int64_t rows;
+    int32_t n_head_kv, head_dim;
+} kv_q8_cache;
+
+/* Element types of the calls below (those of the mask: KV_MASK_F32, KV_MASK_F16). */
+#define KV_F32 0
+#define KV_F16 1
+
+/*
+ * Store n_new rows (rotated and normed by the caller, as kv_append writes them)
+ * at cache rows [row0, row0+n_new): token t's K heads at k + t*k_stride
+ * elements, [n_head_kv][head_dim], V likewise.  Rows [0, row0) are kept; the
+ * first block's rows before row0 get the block's new scale where that changed
+ * (a growing scale rounds their codes once more).  Rows behind row0+n_new are
+ * not written, but a block's scale is that of its rows before row0+n_new: store
+ * them again before they are read.  The new rows' weights become 0.
+ * Returns KV_OK, KV_E_ARG, KV_E_RANGE (rows outside the cache) or KV_E_CUDA.
+ */
+int kv_q8_store(const kv_q8_cache *cache, int64_t row0, int32_t n_new, const void *k, int64_t k_stride,
+                const void *v, int64_t v_stride, int32_t type, void *stream);
+
+/*
+ * The values of rows [row0, row0+n) as F16 (exact) or F32: row i's heads at
+ * k_out + (i-row0)*stride elements, [n_head_kv][head_dim], V likewise; either
+ * may be NULL.
+ */
+int kv_q8_load(const kv_q8_cache *cache, int64_t row0, int64_t n, void *k_out, void *v_out, int64_t stride,
+               int32_t type, void *stream);
+
+/* Bytes of workspace kv_q8_attend needs for these sizes (0: bad arguments).  It
+ * grows with n_past and n_new: ask once for the largest of both.  The contents
+ * need no preparation; calls that overlap on the device need one each. */
+uint64_t kv_q8_attend_workspace(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32_t n_new);
+
+/*
+ * Attention of n_new tokens, whose rows [n_past, n_past+n_new) are stored, over
+ * rows [0, n_past+n_new) with scale 1/sqrt(head_dim): kv_attend's operator over
+ * the 8-bit cache.  q: token t's rotated query heads at q + t*q_stride elements,
+ * [n_head][head_dim], F32 (rounded to F16 as kv_attend does) or F16.  out: token
+ * t's heads at out + t*out_stride, F32 or F16 (q_type / out_type).
+ * mask, mask_type, mask_stride, flags: as kv_attend_mask (NULL: causal; the
+ * flags change only a row without a visible key: NaN, or 0 with KV_ATTN_FLASH).
+ * A key masked with -inf does not enter the row, whatever its block holds.
+ * With cache->weight, weight[h][i] of every attended row i grows by the softmax
+ * weights that the n_new tokens' query heads of KV head h gave it; a query row
+ * whose softmax is not finite (no visible key, NaN or inf scores) adds nothing.
+ * Results do not depend on timing (no atomics).
+ * workspace: 256-byte aligned device memory of at least kv_q8_attend_workspace
+ * bytes.  Returns KV_OK, KV_E_ARG, KV_E_RANGE (rows outside the cache, n_new or
+ * workspace too small or large) or KV_E_CUDA.  n_new: at most 65535.
+ */
+int kv_q8_attend(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32_t n_new,
+                 const void *q, int64_t q_stride, int32_t q_type,
+                 const void *mask, int32_t mask_type, int64_t mask_stride, uint32_t flags,
+                 void *out, int64_t out_stride, int32_t out_type,
+                 void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
+ * Evict rows by accumulated attention weight.  Of the first n_rows rows of
+ * `src`, each KV head keeps its last `recent` ones and, of those before, the
+ * keep-recent of largest weight (equal weights: the lower row; a NaN weight
+ * counts as the largest), in ascending order, at rows [0, keep) of `dst`: their
+ * values at the new blocks' scales, their weights (where dst has them), and
+ * their rows in src in kept, int32 [n_head_kv][keep].  dst is another cache of
+ * the same n_head_kv and head_dim; none of its buffers may overlap one of
+ * src's.  0 <= recent <= keep <= n_rows, keep >= 1.
+ */
+int kv_q8_evict(const kv_q8_cache *src, int64_t n_rows, int64_t keep, int64_t recent,
+                const kv_q8_cache *dst, int32_t *kept, void *stream);
+
 /* Copy cache rows [row0, row0+nrows) of K (which = 0) or V (which = 1) of
  * `layer` to / from host memory in the reference layout [row][head][dim] F16
  * (this context's heads only).  Synchronous.  Used for checking, for the

@@ -1,0 +1,147 @@
+"""CPU tests of the 8-bit cache's entry points: what they refuse (every check
+runs before any CUDA call), and the 64-bit restatement the GPU tests use
+against itself."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import kv_b200 as K
+import q8_reference as R
+
+P = 1 << 20   # a stand-in for a device pointer: refused calls never touch it
+
+
+def cache(**kw):
+    d = dict(k=P, v=2 * P, k_scale=3 * P, v_scale=4 * P, weight=5 * P, rows=1024, n_head_kv=2, head_dim=64)
+    d.update(kw)
+    return K.KvQ8Cache(*[d[n] for n, _ in K.KvQ8Cache._fields_])
+
+
+BAD_CACHES = [dict(k=0), dict(v=0), dict(k_scale=0), dict(v_scale=0), dict(k=P + 8), dict(v=P + 1), dict(k_scale=P + 2),
+              dict(weight=P + 1), dict(rows=0), dict(rows=-32), dict(rows=1000), dict(rows=1 << 31), dict(n_head_kv=0),
+              dict(n_head_kv=1025), dict(head_dim=80), dict(head_dim=0)]
+
+
+def store(c, row0=0, n=4, k=6 * P, ks=128, v=7 * P, vs=128, t=0):
+    return K.lib().kv_q8_store(ctypes.byref(c) if c else None, row0, n, k, ks, v, vs, t, None)
+
+
+def load(c, row0=0, n=4, k=6 * P, v=7 * P, s=128, t=0):
+    return K.lib().kv_q8_load(ctypes.byref(c) if c else None, row0, n, k, v, s, t, None)
+
+
+def attend(c, hq=4, past=10, n=2, q=6 * P, qs=256, qt=0, m=0, mt=0, ms=0, fl=0, o=7 * P, os=256, ot=0, w=8 * P,
+           wb=1 << 40):
+    return K.lib().kv_q8_attend(ctypes.byref(c) if c else None, hq, past, n, q, qs, qt, m, mt, ms, fl, o, os, ot, w, wb,
+                                None)
+
+
+def evict(src, dst, n=100, keep=50, recent=10, kept=100 * P):
+    return K.lib().kv_q8_evict(ctypes.byref(src) if src else None, n, keep, recent, ctypes.byref(dst) if dst else None,
+                               kept, None)
+
+
+def other(**kw):
+    return cache(**dict(dict(k=11 * P, v=12 * P, k_scale=13 * P, v_scale=14 * P, weight=15 * P), **kw))
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES, ids=lambda d: "%s=%s" % next(iter(d.items())))
+def test_every_call_refuses_a_bad_cache(bad):
+    c = cache(**bad)
+    assert store(c) == K.KV_E_ARG
+    assert load(c) == K.KV_E_ARG
+    assert attend(c) == K.KV_E_ARG
+    assert K.lib().kv_q8_attend_workspace(ctypes.byref(c), 4, 10, 2) == 0
+    assert evict(c, other()) == K.KV_E_ARG
+    assert evict(other(), c) == K.KV_E_ARG
+    assert K.last_error()
+
+
+def test_null_cache():
+    assert store(None) == load(None) == attend(None) == evict(None, other()) == evict(cache(), None) == K.KV_E_ARG
+
+
+@pytest.mark.parametrize("kw, rc", [
+    (dict(row0=-1), K.KV_E_RANGE), (dict(n=0), K.KV_E_RANGE), (dict(n=-5), K.KV_E_RANGE), (dict(row0=1021), K.KV_E_RANGE),
+    (dict(row0=1 << 62), K.KV_E_RANGE), (dict(n=1025), K.KV_E_RANGE), (dict(k=0), K.KV_E_ARG), (dict(v=0), K.KV_E_ARG),
+    (dict(k=6 * P + 2), K.KV_E_ARG), (dict(v=7 * P + 1, t=1), K.KV_E_ARG), (dict(ks=127), K.KV_E_ARG),
+    (dict(vs=-128), K.KV_E_ARG), (dict(t=2), K.KV_E_ARG)])
+def test_store_refusals(kw, rc):
+    assert store(cache(), **kw) == rc
+
+
+@pytest.mark.parametrize("kw, rc", [
+    (dict(row0=-1), K.KV_E_RANGE), (dict(n=0), K.KV_E_RANGE), (dict(row0=1000, n=25), K.KV_E_RANGE),
+    (dict(k=0, v=0), K.KV_E_ARG), (dict(s=127), K.KV_E_ARG), (dict(t=-1), K.KV_E_ARG), (dict(k=6 * P + 2), K.KV_E_ARG)])
+def test_load_refusals(kw, rc):
+    assert load(cache(), **kw) == rc
+
+
+@pytest.mark.parametrize("kw, rc", [
+    (dict(hq=3), K.KV_E_ARG), (dict(hq=0), K.KV_E_ARG), (dict(hq=2 * 129), K.KV_E_ARG), (dict(past=-1), K.KV_E_RANGE),
+    (dict(n=0), K.KV_E_RANGE), (dict(past=1023), K.KV_E_RANGE), (dict(n=65536), K.KV_E_RANGE), (dict(q=0), K.KV_E_ARG),
+    (dict(o=0), K.KV_E_ARG), (dict(w=0), K.KV_E_ARG), (dict(w=8 * P + 128), K.KV_E_ARG), (dict(q=6 * P + 2), K.KV_E_ARG),
+    (dict(o=7 * P + 1, ot=1), K.KV_E_ARG), (dict(qs=255), K.KV_E_ARG), (dict(os=0), K.KV_E_ARG), (dict(qt=2), K.KV_E_ARG),
+    (dict(ot=2), K.KV_E_ARG), (dict(m=9 * P, ms=11), K.KV_E_ARG), (dict(m=9 * P, ms=12, mt=2), K.KV_E_ARG),
+    (dict(m=9 * P + 2, ms=12), K.KV_E_ARG), (dict(fl=2), K.KV_E_ARG), (dict(wb=0), K.KV_E_RANGE)])
+def test_attend_refusals(kw, rc):
+    assert attend(cache(), **kw) == rc
+
+
+def test_attend_refuses_a_workspace_that_is_a_byte_short():
+    need = K.lib().kv_q8_attend_workspace(ctypes.byref(cache()), 4, 10, 2)
+    assert need > 0
+    assert attend(cache(), wb=need - 1) == K.KV_E_RANGE
+    assert "workspace" in K.last_error()
+
+
+def test_workspace_grows_with_the_sizes():
+    c = cache(rows=1 << 20, n_head_kv=8, head_dim=128)
+    ws = lambda past, n: K.lib().kv_q8_attend_workspace(ctypes.byref(c), 32, past, n)  # noqa: E731
+    last = 0
+    for past in (0, 1, 31, 500, 4096, 5000, 32768, 131072, 500000):
+        here = [ws(past, n) for n in (1, 2, 3, 4, 5, 8, 16, 17, 64, 512)]
+        assert here == sorted(here) and here[0] >= last, (past, here)
+        last = here[0]
+
+
+@pytest.mark.parametrize("kw, rc", [
+    (dict(keep=0), K.KV_E_ARG), (dict(recent=-1), K.KV_E_ARG), (dict(recent=51), K.KV_E_ARG), (dict(keep=101), K.KV_E_ARG),
+    (dict(n=1025), K.KV_E_RANGE), (dict(kept=0), K.KV_E_ARG), (dict(kept=100 * P + 2), K.KV_E_ARG),
+    (dict(n=0, keep=0, recent=0), K.KV_E_ARG)])
+def test_evict_refusals(kw, rc):
+    assert evict(cache(), other(), **kw) == rc
+
+
+def test_evict_refuses_mismatched_small_and_overlapping_caches():
+    assert evict(cache(), other(n_head_kv=1)) == K.KV_E_ARG
+    assert evict(cache(), other(head_dim=128)) == K.KV_E_ARG
+    assert evict(cache(weight=0), other()) == K.KV_E_ARG
+    assert evict(cache(), other(rows=32)) == K.KV_E_RANGE
+    assert evict(cache(), cache()) == K.KV_E_ARG
+    assert evict(cache(), other(k=2 * P + 16)) == K.KV_E_ARG
+    assert evict(cache(), other(v_scale=P + 1024)) == K.KV_E_ARG
+    assert evict(cache(), other(), kept=5 * P + 8) == K.KV_E_ARG
+
+
+def test_reference_block_round_trip():
+    rng = np.random.default_rng(1)
+    for top in (0.0, 2.0 ** -24, 1e-6, 0.3, 126.9, 127.4, 127.5, 128.0, 65504.0):
+        x = rng.uniform(-1, 1, (R.BLOCK, 8)) * top
+        x[3, 3] = top
+        x = x.astype(np.float16).astype(np.float64)
+        c, w = R.quantise_block(x)
+        y = R.row_values(c, np.array([w], np.uint32))
+        e = int(R.word_exp(w))
+        assert np.abs(y - x).max() <= 2.0 ** (e - 1) * (1 if e < 9 else 2)
+        c2, w2 = R.quantise_block(y)           # what is stored again keeps its codes and scale
+        assert (c2 == c).all() and w2 == w
+
+
+def test_reference_evict_order():
+    w = np.array([1.0, np.nan, 5.0, 5.0, 0.0, -0.0, 5.0, 2.0])
+    assert R.evict(w, 8, 4, 1) == [1, 2, 3, 7]
+    assert R.evict(w, 8, 8, 0) == list(range(8))
+    assert R.evict(w, 8, 3, 3) == [5, 6, 7]
+    assert R.evict(w, 7, 6, 0) == [0, 1, 2, 3, 4, 6]
