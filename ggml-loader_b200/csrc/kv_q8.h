@@ -63,11 +63,23 @@ struct AttendParams {
     int64_t out_stride;
     int32_t out_f16;
     float scale;
-    char *ws;
+    // scratch of the workspace, set by launch_attend
+    int32_t nb;             // blocks of kBlock keys: ceil(n_kv / kBlock)
+    int32_t n_tile;         // query-row tiles a KV head
+    int32_t n_vh;           // H * n_tile
+    int32_t n_cta;
+    float *part;            // [n_cta + n_vh][16][D] partial outputs of a (CTA, virtual head)
+    float2 *stat;           // [n_cta + n_vh][16] their (maximum, sum)
+    float *scores;          // [H][n_new * r][nb * kBlock] or null
+    float2 *row_stat;       // [H][n_new * r] (maximum, 1 / sum or 0) or null
 };
-// bytes of p.ws (a function of the sizes alone)
+// bytes of workspace (a function of the sizes alone)
 uint64_t attend_workspace(const AttendParams &p);
-cudaError_t launch_attend(const AttendParams &p, cudaStream_t st);
+cudaError_t launch_attend(AttendParams p, void *ws, cudaStream_t st);
+
+// kv_q8_rows.cu: the split of a call over CTAs, and its kernels
+void rows_split(AttendParams &p);
+cudaError_t launch_rows(const AttendParams &p, cudaStream_t st);
 
 }  // namespace q8
 }  // namespace kvb

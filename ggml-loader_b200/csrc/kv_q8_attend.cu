@@ -41,59 +41,6 @@ __device__ __forceinline__ float query(const AttendParams &p, int t, int hq, int
     return __half2float(__float2half_rn(static_cast<const float *>(p.q)[i]));
 }
 
-// One CTA a query row: scores of T keys, then their weighted values; the
-// running maximum and sum in float.  ws gets (max, 1 / sum), 0 for a row that adds no weight.
-template <int D>
-__global__ void __launch_bounds__(T) row_kernel(const AttendParams p)
-{
-    __shared__ float qs[D], ps[T], red[T / 32];
-    const int t = blockIdx.x / p.r, j = blockIdx.x % p.r, h = blockIdx.y, tid = threadIdx.x;
-    for (int d = tid; d < D; d += T) qs[d] = query(p, t, h * p.r + j, D, d);
-    float m = -CUDART_INF_F, l = 0.0f, o[(D + T - 1) / T] = {};
-    __syncthreads();
-    for (int64_t base = 0; base < p.n_kv; base += T) {
-        const float s = base + tid < p.n_kv ? score<D>(p, qs, h, t, base + tid) : -CUDART_INF_F;
-        float x = s;
-        for (int k = 16; k; k >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
-        if ((tid & 31) == 0) red[tid >> 5] = x;
-        __syncthreads();
-        float top = m;
-        for (int k = 0; k < T / 32; k++) top = fmaxf(top, red[k]);
-        const float ref = top == -CUDART_INF_F ? 0.0f : top, f = m == -CUDART_INF_F ? 0.0f : expf(m - ref);
-        ps[tid] = s == -CUDART_INF_F ? 0.0f : expf(s - ref);
-        __syncthreads();
-        l *= f;
-#pragma unroll
-        for (int k = 0; k < (D + T - 1) / T; k++) o[k] *= f;
-        for (int i = 0; i < T && base + i < p.n_kv; i++) {
-            const float w = ps[i];
-            if (w == 0.0f) continue;
-            l += w;
-            const int64_t key = base + i;
-            const float vs = p.c.v_scale[(int64_t)h * (p.c.rows / kBlock) + key / kBlock];
-#pragma unroll
-            for (int k = 0; k < (D + T - 1) / T; k++)
-                if (tid + k * T < D) o[k] += w * vs * (float)p.c.v[((int64_t)h * p.c.rows + key) * D + tid + k * T];
-        }
-        m = top;
-        __syncthreads();
-    }
-    const float z = l > 0.0f || l != l ? 1.0f / l : (p.flash ? 0.0f : CUDART_NAN_F);
-#pragma unroll
-    for (int k = 0; k < (D + T - 1) / T; k++) {
-        const int d = tid + k * T;
-        if (d >= D) continue;
-        const int64_t i = t * p.out_stride + (int64_t)(h * p.r + j) * D + d;
-        if (p.out_f16) static_cast<__half *>(p.out)[i] = __float2half_rn(o[k] * z);
-        else static_cast<float *>(p.out)[i] = o[k] * z;
-    }
-    if (tid == 0) {
-        const bool adds = l > 0.0f && l < CUDART_INF_F && m < CUDART_INF_F;
-        reinterpret_cast<float2 *>(p.ws)[(int64_t)h * p.n_new * p.r + blockIdx.x] =
-            adds ? make_float2(m, 1.0f / l) : make_float2(0.0f, 0.0f);
-    }
-}
-
 // A thread a (KV head, key): the weights of every query row.
 template <int D>
 __global__ void __launch_bounds__(T) weigh_kernel(const AttendParams p)
@@ -107,35 +54,57 @@ __global__ void __launch_bounds__(T) weigh_kernel(const AttendParams p)
         __syncthreads();
         for (int d = threadIdx.x; d < D; d += T) qs[d] = query(p, t, h * p.r + row % p.r, D, d);
         __syncthreads();
-        const float2 st = reinterpret_cast<const float2 *>(p.ws)[(int64_t)h * p.n_new * p.r + row];
+        const float2 st = p.row_stat[(int64_t)h * p.n_new * p.r + row];
         if (key < p.n_kv && st.y != 0.0f) sum += expf(score<D>(p, qs, h, t, key) - st.x) * st.y;
     }
     if (key < p.n_kv) p.c.weight[(int64_t)h * p.c.rows + key] += sum;
 }
 
 template <int D>
-cudaError_t run(const AttendParams &p, cudaStream_t st)
+cudaError_t weigh(const AttendParams &p, cudaStream_t st)
 {
-    row_kernel<D><<<dim3(p.n_new * p.r, p.c.H), T, 0, st>>>(p);
-    if (p.c.weight) weigh_kernel<D><<<dim3((unsigned)((p.n_kv + T - 1) / T), p.c.H), T, 0, st>>>(p);
+    weigh_kernel<D><<<dim3((unsigned)((p.n_kv + T - 1) / T), p.c.H), T, 0, st>>>(p);
     return cudaGetLastError();
+}
+
+// The workspace, laid out from `ws` on; returns its bytes.
+uint64_t lay_out(AttendParams &p, char *ws)
+{
+    rows_split(p);
+    uint64_t n = 0;
+    auto take = [&](uint64_t bytes) {
+        char *at = ws + n;
+        n += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    const uint64_t slots = (uint64_t)p.n_cta + p.n_vh, rows = (uint64_t)p.n_new * p.r;
+    p.part = reinterpret_cast<float *>(take(slots * 16 * p.c.D * sizeof(float)));
+    p.stat = reinterpret_cast<float2 *>(take(slots * 16 * sizeof(float2)));
+    p.scores = nullptr;
+    p.row_stat = nullptr;
+    if (p.c.weight && rows <= 16) p.scores = reinterpret_cast<float *>(take(p.c.H * rows * p.nb * kBlock * sizeof(float)));
+    if (p.c.weight && rows > 16) p.row_stat = reinterpret_cast<float2 *>(take(p.c.H * rows * sizeof(float2)));
+    return n;
 }
 
 }  // namespace
 
 uint64_t attend_workspace(const AttendParams &p)
 {
-    return (uint64_t)p.n_new * p.Hq * sizeof(float2);
+    AttendParams q = p;
+    return lay_out(q, nullptr);
 }
 
-cudaError_t launch_attend(const AttendParams &p, cudaStream_t st)
+cudaError_t launch_attend(AttendParams p, void *ws, cudaStream_t st)
 {
+    lay_out(p, static_cast<char *>(ws));
+    cudaError_t e = launch_rows(p, st);
+    if (e != cudaSuccess || !p.row_stat) return e;
     switch (p.c.D) {
-    case 64: return run<64>(p, st);
-    case 96: return run<96>(p, st);
-    case 128: return run<128>(p, st);
-    case 256: return run<256>(p, st);
-    default: return cudaErrorInvalidValue;
+    case 64: return weigh<64>(p, st);
+    case 96: return weigh<96>(p, st);
+    case 128: return weigh<128>(p, st);
+    default: return weigh<256>(p, st);
     }
 }
 

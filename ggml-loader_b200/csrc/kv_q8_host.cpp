@@ -184,8 +184,7 @@ int kv_q8_attend(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32
     p.out_stride = n_new > 1 ? out_stride : 0;
     p.out_f16 = out_type == KV_F16;
     p.scale = 1.0f / sqrtf((float)p.c.D);
-    p.ws = static_cast<char *>(workspace);
-    return cuda_rc(kvb::q8::launch_attend(p, static_cast<cudaStream_t>(stream)), what);
+    return cuda_rc(kvb::q8::launch_attend(p, workspace, static_cast<cudaStream_t>(stream)), what);
 }
 
 int kv_q8_evict(const kv_q8_cache *src, int64_t n_rows, int64_t keep, int64_t recent,

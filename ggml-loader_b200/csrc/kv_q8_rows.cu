@@ -1,0 +1,631 @@
+// kv_q8_rows.cu -- attention over the 8-bit cache for up to 16 query rows a KV
+// head (a token, a few draft tokens): one pass over the codes.
+//
+// For a query row, with t_k = (q . c_k) * ks * scale (c_k the codes of key k,
+// ks its block's scale, q rounded to F16) and v_k = c'_k * 2^ev:
+//   out = sum_k e^(t_k) 2^(ev) c'_k / sum_k e^(t_k).
+// Everything in sight of the tensor cores is an integer code or a weight
+// W = e^(t - m) 2^(ev - me), F16: a row's reference (m, me) is the score and
+// value exponent (less kBias) of the block in which t + ev ln 2 was largest, so
+// the largest W lies in [2^7, 2^15] whatever the scales are (a W in F16's
+// subnormals is below 2^-21 of it), and the output sums to O * 2^me.  The row's
+// sum of e^(t - m) adds W * 2^(me - ev) in float.  With a reference that only
+// moves when W would pass 2^15 the accumulators are seldom rescaled.
+//
+// A head's blocks are streamed once: warps take blocks of 32 keys in turn, each
+// with its own ring of shared memory (cp.async, nothing but warp barriers in
+// the loop), so HBM is the bound; partial (m, sum, out) rows of the CTAs of a
+// head are joined by a second kernel launched programmatically.
+#include <math_constants.h>
+
+#include "kv_internal.h"
+#include "kv_q8.cuh"
+#include "kv_sm100.cuh"
+
+namespace kvb {
+namespace q8 {
+namespace {
+
+using namespace sm100;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kBias = 7.0f;    // a new reference's weight is 2^kBias,
+constexpr float kTop = 15.0f;    // and it moves where a weight would pass 2^kTop
+
+template <int D>
+struct Rows {
+    static constexpr int W = D == 256 ? 4 : 8;                       // warps
+    static constexpr int stages = D == 64 ? 5 : 3;
+    static constexpr int pitch = D + 16;                             // bytes a row: 8 rows fall on different banks
+    static constexpr int tile = kBlock * pitch;                      // K or V of a block
+    static constexpr int ring = stages * 2 * tile;                   // a warp's
+    static constexpr int smem = W * ring;
+    static constexpr int nk = D / 16;                                // 16-wide steps over D
+};
+
+// two F16 pairs (codes 0, 1 | 2, 3 or 0, 2 | 1, 3) of four signed codes: 0x6400
+// | u is the half 1024 + u, u = code + 128
+template <bool BY_TWO>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &a, uint32_t &b)
+{
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));   // 1152
+    uint32_t x = __byte_perm(u, 0x64646464u, BY_TWO ? 0x4240 : 0x4140);
+    uint32_t y = __byte_perm(u, 0x64646464u, BY_TWO ? 0x4341 : 0x4342);
+    const __half2 hx = __hsub2(*reinterpret_cast<__half2 *>(&x), off), hy = __hsub2(*reinterpret_cast<__half2 *>(&y), off);
+    a = *reinterpret_cast<const uint32_t *>(&hx);
+    b = *reinterpret_cast<const uint32_t *>(&hy);
+}
+
+__device__ __forceinline__ uint32_t pack(float lo, float hi)
+{
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// 4 query elements as two F16 pairs
+__device__ __forceinline__ void load_q4(const AttendParams &p, int t, int hq, int D, int d, uint32_t &a, uint32_t &b)
+{
+    const int64_t i = t * p.q_stride + (int64_t)hq * D + d;
+    __half x[4];
+    if (p.q_f16) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = static_cast<const __half *>(p.q)[i + k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = __float2half_rn(static_cast<const float *>(p.q)[i + k]);
+    }
+    a = pack_half2(x[0], x[1]);
+    b = pack_half2(x[2], x[3]);
+}
+
+__device__ __forceinline__ float mask_value(const AttendParams &p, int t, int64_t key)
+{
+    const int64_t i = t * p.mask_stride + key;
+    return p.mask_f16 ? __half2float(static_cast<const __half *>(p.mask)[i]) : static_cast<const float *>(p.mask)[i];
+}
+
+__device__ __forceinline__ void store_out(const AttendParams &p, int64_t i, float x)
+{
+    if (p.out_f16) static_cast<__half *>(p.out)[i] = __float2half_rn(x);
+    else static_cast<float *>(p.out)[i] = x;
+}
+
+// sum -> 1 / sum, or what an empty row gives
+__device__ __forceinline__ float inverse_sum(float l, bool flash)
+{
+    return l == 0.0f ? (flash ? 0.0f : CUDART_NAN_F) : 1.0f / l;
+}
+
+// One query row of the warp's running softmax (a thread holds 8 of a block's
+// 32 keys of it; the 4 threads of a row agree on m, me and l's share is each one's own)
+struct RowState {
+    float m, me, l, bad;   // bad: 0, or NaN once a visible key's V block was not finite
+};
+
+// The block's 8 scores of this thread -> weights; rescale is the factor for
+// the sums so far (1 when the reference stays).
+template <bool MASKED>
+__device__ __forceinline__ void softmax_block(float (&s)[8], RowState &st, float ev, bool v_bad, float &rescale, float &orescale)
+{
+    // MASKED: natural units (a mask of the type's lowest value leaves no room for a factor); else log2
+    constexpr float unit = MASKED ? kLog2e : 1.0f;
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    rescale = orescale = 1.0f;
+    if (top > -CUDART_INF_F && (st.m == -CUDART_INF_F || __fmaf_rn(top - st.m, unit, ev - st.me) > kTop)) {
+        if (st.m > -CUDART_INF_F) {
+            rescale = ex2_approx((st.m - top) * unit);
+            orescale = ex2_approx(__fmaf_rn(st.m - top, unit, st.me - (ev - kBias)));
+        }
+        st.m = top;
+        st.me = ev - kBias;
+    }
+    if (v_bad && top > -CUDART_INF_F) st.bad = CUDART_NAN_F;
+    const float m = st.m == -CUDART_INF_F ? 0.0f : st.m, up = ev - st.me;
+    float sum = 0.0f;
+    if constexpr (MASKED) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) s[i] = ex2_approx(__fmaf_rn(s[i] - m, kLog2e, up));
+    } else {
+        const float ref = up - m;
+#pragma unroll
+        for (int i = 0; i < 8; i++) s[i] = ex2_approx(s[i] + ref);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum += s[i];
+    st.l = __fmaf_rn(sum, pow2((int)-up), st.l * rescale);
+}
+
+// HILO (up to 8 rows): the tensor cores' rows 8-15 carry the low half of rows
+// 0-7's weights, W - F16(W), so the weights enter with 22 bits at no cost.
+// Else rows 0-15, weights in F16 (11 bits, half a step 2^-12 of each: the
+// outputs' own F16 rounding is as large).
+template <int D, bool HILO, bool MASKED>
+__global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendParams p)
+{
+    using G = Rows<D>;
+    constexpr int RT = HILO ? 1 : 2;   // 8-row halves of softmax state
+    extern __shared__ __align__(128) char smem[];
+    __shared__ float2 s_stat[G::W][16];
+    __shared__ float s_bad[G::W][16];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    char *ring = smem + warp * G::ring;
+    const int64_t T = (int64_t)p.n_vh * p.nb, lo = blockIdx.x * T / p.n_cta, hi = (blockIdx.x + 1) * T / p.n_cta;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    for (int64_t pos = lo; pos < hi;) {
+        const int vh = (int)(pos / p.nb), b0 = (int)(pos - (int64_t)vh * p.nb);
+        const int b1 = (int)min((int64_t)p.nb, b0 + hi - pos);
+        pos += b1 - b0;
+        const int h = vh / p.n_tile, row0 = (vh - h * p.n_tile) * 16;   // (HILO: one tile)
+        const int nrows = min(HILO ? 8 : 16, p.n_new * p.r - row0);
+        const int8_t *kc = p.c.k + (int64_t)h * p.c.rows * D, *vc = p.c.v + (int64_t)h * p.c.rows * D;
+        const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)h * (p.c.rows / kBlock);
+        const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.c.v_scale) + (int64_t)h * (p.c.rows / kBlock);
+
+        auto fetch = [&](int b, int stage) {
+            if (b < b1) {
+                char *ks = ring + stage * 2 * G::tile, *vs = ks + G::tile;
+                const int8_t *ksrc = kc + (int64_t)b * kBlock * D, *vsrc = vc + (int64_t)b * kBlock * D;
+#pragma unroll
+                for (int j = 0; j < D / 16; j++) {
+                    const int i = lane + 32 * j, r = i / (D / 16), c = i % (D / 16);
+                    cp_async_16(ks + r * G::pitch + c * 16, ksrc + i * 16);
+                }
+#pragma unroll
+                for (int j = 0; j < D / 16; j++) {
+                    const int i = lane + 32 * j, r = i / (D / 16), c = i % (D / 16);
+                    cp_async_16(vs + r * G::pitch + c * 16, vsrc + i * 16);
+                }
+            }
+            cp_async_commit();
+        };
+        // this warp's blocks: b0 + warp, then every W-th
+        int fb = b0 + warp, fs = 0;
+#pragma unroll
+        for (int s = 0; s < G::stages - 1; s++) {
+            fetch(fb, fs);
+            fb += G::W;
+            fs++;
+        }
+
+        // Q as the A operand: rows g and g + 8, dims 4 t4 .. + 3 of each 16 (the
+        // order in which a thread holds a key's codes)
+        uint32_t qa[G::nk][HILO ? 2 : 4];
+        int tok[RT];
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            const int row = row0 + g + 8 * i;
+            const bool have = g + 8 * i < nrows;
+            tok[i] = have ? row / p.r : 0;
+            const int hq = h * p.r + (have ? row % p.r : 0);
+#pragma unroll
+            for (int k = 0; k < G::nk; k++) {
+                uint32_t a = 0, b = 0;
+                if (have) load_q4(p, tok[i], hq, D, k * 16 + t4 * 4, a, b);
+                qa[k][i] = a;
+                qa[k][RT + i] = b;
+            }
+        }
+
+        RowState st[RT];
+#pragma unroll
+        for (int i = 0; i < RT; i++) st[i] = RowState{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
+        float o[2 * G::nk][4];
+#pragma unroll
+        for (int i = 0; i < 2 * G::nk; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[i][j] = 0.0f;
+
+        int stage = 0;
+        uint32_t kw = 0, vw = 0;   // the scale words of this warp's next 32 blocks, one a lane
+        for (int b = b0 + warp, n = 0; b < b1; b += G::W, n++) {
+            if ((n & 31) == 0) {
+                const int mine = b + lane * G::W;
+                kw = mine < b1 ? ksc[mine] : 0;
+                vw = mine < b1 ? vsc[mine] : 0;
+            }
+            const uint32_t kword = __shfl_sync(0xffffffffu, kw, n & 31), vword = __shfl_sync(0xffffffffu, vw, n & 31);
+            const bool k_bad = (kword & 0x7f800000u) == 0x7f800000u, v_bad = (vword & 0x7f800000u) == 0x7f800000u;
+            const float ks = k_bad ? CUDART_NAN_F : pow2(scale_exp(kword)), ev = (float)scale_exp(vword);
+            const int64_t key0 = (int64_t)b * kBlock;
+            float mk[RT][8];
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int i = 0; i < RT; i++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int64_t key = key0 + (j >> 1) * 8 + 2 * t4 + (j & 1);
+                        mk[i][j] = key < p.n_kv ? mask_value(p, tok[i], key) : -CUDART_INF_F;
+                    }
+            }
+            cp_async_wait<G::stages - 2>();
+            __syncwarp();
+            fetch(fb, fs);   // into the stage the previous block left
+            fb += G::W;
+            if (++fs == G::stages) fs = 0;
+            const uint32_t kt = smem_addr(ring + stage * 2 * G::tile), vt = kt + G::tile;
+            if (++stage == G::stages) stage = 0;
+
+            // S = Q K^T: 4 groups of 8 keys
+            float acc[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
+                const uint32_t row = kt + (j * 8 + (lane & 7)) * G::pitch + (lane >> 3) * 16;
+#pragma unroll
+                for (int c = 0; c < D / 64; c++) {
+                    uint32_t w[4];
+                    ldsm_x4(row + c * 64, w[0], w[1], w[2], w[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t x, y;
+                        codes_to_half<false>(w[i], x, y);
+                        const int k = c * 4 + i;
+                        if constexpr (HILO) mma_16816(acc[j], qa[k][0], 0u, qa[k][1], 0u, x, y);
+                        else mma_16816(acc[j], qa[k][0], qa[k][1], qa[k][2], qa[k][3], x, y);
+                    }
+                }
+                if constexpr (D % 64 != 0) {   // 96: the last 32 dims
+                    uint32_t w0, w1;
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];"
+                                 : "=r"(w0), "=r"(w1)
+                                 : "r"(kt + (j * 8 + (lane & 7)) * G::pitch + (D / 64) * 64 + ((lane >> 3) & 1) * 16));
+                    uint32_t x, y;
+                    constexpr int k = D / 64 * 4;
+                    codes_to_half<false>(w0, x, y);
+                    if constexpr (HILO) mma_16816(acc[j], qa[k][0], 0u, qa[k][1], 0u, x, y);
+                    else mma_16816(acc[j], qa[k][0], qa[k][1], qa[k][2], qa[k][3], x, y);
+                    codes_to_half<false>(w1, x, y);
+                    if constexpr (HILO) mma_16816(acc[j], qa[k + 1][0], 0u, qa[k + 1][1], 0u, x, y);
+                    else mma_16816(acc[j], qa[k + 1][0], qa[k + 1][1], qa[k + 1][2], qa[k + 1][3], x, y);
+                }
+            }
+
+            // scores, then weights
+            const float cs = p.scale * ks * (MASKED ? 1.0f : kLog2e);
+            float w[RT][8];
+            float orescale[RT];
+            bool moved = false;
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float d = acc[j >> 1][2 * i + (j & 1)];
+                    if constexpr (MASKED) w[i][j] = mk[i][j] == -CUDART_INF_F ? mk[i][j] : __fmaf_rn(d, cs, mk[i][j]);
+                    else w[i][j] = d * cs;
+                }
+                if (!MASKED && key0 + kBlock > p.n_past) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (key0 + (j >> 1) * 8 + 2 * t4 + (j & 1) > p.n_past + tok[i]) w[i][j] = -CUDART_INF_F;
+                }
+                if (p.scores && g + 8 * i < nrows) {
+                    float *dst = p.scores + ((int64_t)h * p.n_new * p.r + g + 8 * i) * p.nb * kBlock + key0 + 2 * t4;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        *reinterpret_cast<float2 *>(dst + 8 * j) = make_float2(w[i][2 * j], w[i][2 * j + 1]);
+                }
+                float rescale;
+                softmax_block<MASKED>(w[i], st[i], ev, v_bad, rescale, orescale[i]);
+                moved |= orescale[i] != 1.0f;
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int i = 0; i < 2 * G::nk; i++) {
+                    o[i][0] *= orescale[0];
+                    o[i][1] *= orescale[0];
+                    o[i][2] *= orescale[RT - 1];
+                    o[i][3] *= orescale[RT - 1];
+                }
+            }
+
+            // O += W V: two steps of 16 keys
+            uint32_t pa[2][4];
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const float e0 = w[0][4 * s + 2 * x], e1 = w[0][4 * s + 2 * x + 1];
+                    pa[s][2 * x] = pack(e0, e1);
+                    if constexpr (HILO) {
+                        const __half2 hi2 = *reinterpret_cast<const __half2 *>(&pa[s][2 * x]);
+                        pa[s][2 * x + 1] = pack(e0 - __low2float(hi2), e1 - __high2float(hi2));
+                    } else {
+                        pa[s][2 * x + 1] = pack(w[RT - 1][4 * s + 2 * x], w[RT - 1][4 * s + 2 * x + 1]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < G::nk; c++) {
+                uint32_t v[4];
+                ldsm_x4_t(vt + lane * G::pitch + c * 16, v[0], v[1], v[2], v[3]);
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    uint32_t e0, d0, e1, d1;   // even and odd dims, keys 0-7 and 8-15 of the step
+                    codes_to_half<true>(v[2 * s], e0, d0);
+                    codes_to_half<true>(v[2 * s + 1], e1, d1);
+                    mma_16816(o[2 * c], pa[s][0], pa[s][1], pa[s][2], pa[s][3], e0, e1);
+                    mma_16816(o[2 * c + 1], pa[s][0], pa[s][1], pa[s][2], pa[s][3], d0, d1);
+                }
+            }
+        }
+
+        // the warps' rows: (m, l) and O 2^me to shared memory, summed there
+        constexpr int NR = 8 * RT;
+        float *os = reinterpret_cast<float *>(smem);
+        cp_async_wait<0>();
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RT; i++) {
+            float l = st[i].l;
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            const int row = g + 8 * i;
+            if (t4 == 0) {
+                s_stat[warp][row] = make_float2(st[i].m, l);
+                s_bad[warp][row] = st[i].bad;
+            }
+            const float f = pow2((int)st[i].me);
+            float *dst = os + ((int64_t)warp * NR + row) * D;
+#pragma unroll
+            for (int c = 0; c < G::nk; c++) {
+                // columns 2 t4, 2 t4 + 1 of the even and odd tile: dims 16 c + 4 t4 .. + 3
+                float4 x;
+                if constexpr (HILO)
+                    x = make_float4(o[2 * c][0] + o[2 * c][2], o[2 * c + 1][0] + o[2 * c + 1][2],
+                                    o[2 * c][1] + o[2 * c][3], o[2 * c + 1][1] + o[2 * c + 1][3]);
+                else
+                    x = make_float4(o[2 * c][2 * i], o[2 * c + 1][2 * i], o[2 * c][2 * i + 1], o[2 * c + 1][2 * i + 1]);
+                *reinterpret_cast<float4 *>(dst + c * 16 + t4 * 4) = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+            }
+        }
+        __syncthreads();
+        const bool whole = b0 == 0 && b1 == p.nb;
+        const int64_t slot = (int64_t)blockIdx.x + vh;   // (CTA, head) pairs in order: their sum counts them
+        constexpr float unit = MASKED ? kLog2e : 1.0f;
+        for (int i = threadIdx.x; i < nrows * (D / 4); i += G::W * 32) {
+            const int row = i / (D / 4), c = i % (D / 4) * 4;
+            float M = -CUDART_INF_F;
+#pragma unroll
+            for (int w = 0; w < G::W; w++) M = fmaxf(M, s_stat[w][row].x);
+            const float ref = M == -CUDART_INF_F ? 0.0f : M;
+            float l = 0.0f;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < G::W; w++) {
+                const float2 s = s_stat[w][row];
+                const float f = ex2_approx((s.x - ref) * unit), bad = s_bad[w][row];
+                const float4 y = *reinterpret_cast<const float4 *>(os + ((int64_t)w * NR + row) * D + c);
+                // (a warp without a visible key: m = -inf, f = 0, its sums 0 -- or NaN, which must stay)
+                l = __fmaf_rn(s.y, f, l);
+                x.x = __fmaf_rn(y.x, f, x.x + bad);
+                x.y = __fmaf_rn(y.y, f, x.y + bad);
+                x.z = __fmaf_rn(y.z, f, x.z + bad);
+                x.w = __fmaf_rn(y.w, f, x.w + bad);
+            }
+            if (whole) {
+                const float z = inverse_sum(l, p.flash != 0);
+                const int t = (row0 + row) / p.r, j = (row0 + row) % p.r;
+                const int64_t at = t * p.out_stride + (int64_t)(h * p.r + j) * D + c;
+                store_out(p, at, x.x * z);
+                store_out(p, at + 1, x.y * z);
+                store_out(p, at + 2, x.z * z);
+                store_out(p, at + 3, x.w * z);
+            } else {
+                *reinterpret_cast<float4 *>(p.part + (slot * 16 + row) * D + c) = x;
+            }
+            if (c == 0) p.stat[slot * 16 + row] = make_float2(M, l);
+        }
+        __syncthreads();   // the next head's ring takes the shared memory
+    }
+}
+
+// The CTAs of virtual head vh (the split of rows_kernel).
+__device__ __forceinline__ void span_of(const AttendParams &p, int vh, int &a, int &b)
+{
+    const int64_t T = (int64_t)p.n_vh * p.nb, x0 = (int64_t)vh * p.nb, x1 = x0 + p.nb - 1;
+    // CTA c holds [c T / C, (c + 1) T / C): position x is in floor(((x + 1) C - 1) / T)
+    a = (int)(((x0 + 1) * p.n_cta - 1) / T);
+    b = (int)(((x1 + 1) * p.n_cta - 1) / T);
+}
+
+// Joins the CTAs' partial rows: one CTA a (virtual head, row); with weights,
+// CTAs behind those add the softmax weights of 512 keys of a head.
+template <int D, bool MASKED>
+__global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
+{
+    constexpr float unit = MASKED ? kLog2e : 1.0f;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int n_join = p.n_vh * 16;
+    pdl_launch_dependents();
+    pdl_wait();
+    if ((int)blockIdx.x < n_join) {
+        __shared__ float4 s_o[4][D / 4];
+        __shared__ float2 s_ml[4];
+        const int vh = blockIdx.x >> 4, row = blockIdx.x & 15;
+        const int h = vh / p.n_tile, row0 = (vh - h * p.n_tile) * 16;
+        if (row0 + row >= p.n_new * p.r) return;
+        int a, b;
+        span_of(p, vh, a, b);
+        if (a == b && !p.row_stat) return;   // rows_kernel wrote the output
+        // each warp a quarter of the parts, then the four
+        float M = -CUDART_INF_F;
+        for (int c = a + lane; c <= b; c += 32) M = fmaxf(M, p.stat[((int64_t)c + vh) * 16 + row].x);
+#pragma unroll
+        for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
+        const float ref = M == -CUDART_INF_F ? 0.0f : M;
+        constexpr int V = (D / 4 + 31) / 32;
+        float4 x[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) x[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+#pragma unroll 4
+        for (int c = a + warp; c <= b; c += 4) {
+            const int64_t at = ((int64_t)c + vh) * 16 + row;
+            const float2 s = p.stat[at];
+            const float f = ex2_approx((s.x - ref) * unit);
+            l = __fmaf_rn(s.y, f, l);
+            if (a == b) continue;
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                if (lane + 32 * v >= D / 4) continue;
+                const float4 y = *reinterpret_cast<const float4 *>(p.part + at * D + (lane + 32 * v) * 4);
+                x[v].x = __fmaf_rn(y.x, f, x[v].x);
+                x[v].y = __fmaf_rn(y.y, f, x[v].y);
+                x[v].z = __fmaf_rn(y.z, f, x[v].z);
+                x[v].w = __fmaf_rn(y.w, f, x[v].w);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (lane + 32 * v < D / 4) s_o[warp][lane + 32 * v] = x[v];
+        if (lane == 0) s_ml[warp] = make_float2(M, l);
+        __syncthreads();
+        l = (s_ml[0].y + s_ml[1].y) + (s_ml[2].y + s_ml[3].y);
+        if (p.row_stat && tid == 0) {
+            const bool adds = l > 0.0f && l < CUDART_INF_F && M < CUDART_INF_F;
+            p.row_stat[(int64_t)h * p.n_new * p.r + row0 + row] =
+                adds ? make_float2(MASKED ? M : M / kLog2e, 1.0f / l) : make_float2(0.0f, 0.0f);
+        }
+        if (a == b) return;
+        const float z = inverse_sum(l, p.flash != 0);
+        const int t = (row0 + row) / p.r, j = (row0 + row) % p.r;
+        const int64_t at = t * p.out_stride + (int64_t)(h * p.r + j) * D;
+        for (int d = tid; d < D; d += 128) {
+            const float *o0 = reinterpret_cast<const float *>(s_o);
+            store_out(p, at + d, ((o0[d] + o0[D + d]) + (o0[2 * D + d] + o0[3 * D + d])) * z);
+        }
+        return;
+    }
+    // weight[h][key] += sum over rows of e^(score - M) / Z
+    __shared__ float2 s_row[16];
+    const int chunks = (int)(((int64_t)p.nb * kBlock + 511) / 512);
+    const int w = blockIdx.x - n_join, h = w / chunks;
+    const int64_t key = (int64_t)(w - h * chunks) * 512 + tid * 4;
+    const int R = p.n_new * p.r;
+    int a, b;
+    span_of(p, h, a, b);
+    {
+        const int row = tid >> 3, sub = tid & 7;
+        float M = -CUDART_INF_F, l = 0.0f;
+        if (row < R) {
+            for (int c = a + sub; c <= b; c += 8) {
+                const float2 s = p.stat[((int64_t)c + h) * 16 + row];
+                const float top = fmaxf(M, s.x);
+                if (top > -CUDART_INF_F) l = __fmaf_rn(l, ex2_approx((M - top) * unit), s.y * ex2_approx((s.x - top) * unit));
+                else l += s.y;   // (0, or NaN)
+                M = top;
+            }
+        }
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) {
+            const float M2 = __shfl_xor_sync(0xffffffffu, M, k), l2 = __shfl_xor_sync(0xffffffffu, l, k);
+            const float top = fmaxf(M, M2);
+            if (top > -CUDART_INF_F) l = __fmaf_rn(l, ex2_approx((M - top) * unit), l2 * ex2_approx((M2 - top) * unit));
+            else l += l2;
+            M = top;
+        }
+        if (sub == 0) {
+            const bool adds = row < R && l > 0.0f && l < CUDART_INF_F && M < CUDART_INF_F;
+            s_row[row] = adds ? make_float2(M, 1.0f / l) : make_float2(0.0f, 0.0f);
+        }
+    }
+    __syncthreads();
+    if (key >= p.n_kv) return;
+    const float *src = p.scores + (int64_t)h * R * p.nb * kBlock + key;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int row = 0; row < R; row++) {
+        const float2 s = s_row[row];
+        const float4 x = *reinterpret_cast<const float4 *>(src + (int64_t)row * p.nb * kBlock);
+        if (s.y == 0.0f) continue;   // (adds nothing, whatever its scores are)
+        sum[0] = __fmaf_rn(ex2_approx((x.x - s.x) * unit), s.y, sum[0]);
+        sum[1] = __fmaf_rn(ex2_approx((x.y - s.x) * unit), s.y, sum[1]);
+        sum[2] = __fmaf_rn(ex2_approx((x.z - s.x) * unit), s.y, sum[2]);
+        sum[3] = __fmaf_rn(ex2_approx((x.w - s.x) * unit), s.y, sum[3]);
+    }
+    float *dst = p.c.weight + (int64_t)h * p.c.rows + key;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (key + i < p.n_kv) dst[i] += sum[i];
+}
+
+template <class K>
+cudaError_t launch_pdl(K kernel, unsigned grid, unsigned block, size_t smem, const AttendParams &p, cudaStream_t st)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int D, bool HILO, bool MASKED>
+cudaError_t run(const AttendParams &p, cudaStream_t st)
+{
+    using G = Rows<D>;
+    cudaError_t e = cudaFuncSetAttribute(rows_kernel<D, HILO, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
+    if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, HILO, MASKED>, p.n_cta, G::W * 32, G::smem, p, st);
+    if (e != cudaSuccess) return e;
+    const bool split = p.n_cta > p.n_vh || p.n_vh % p.n_cta != 0;   // else every head lies in one CTA
+    if (!split && !p.scores && !p.row_stat) return cudaSuccess;
+    unsigned grid = (unsigned)p.n_vh * 16;
+    if (p.scores) grid += (unsigned)(p.c.H * (((int64_t)p.nb * kBlock + 511) / 512));
+    return launch_pdl(join_kernel<D, MASKED>, grid, 128, 0, p, st);
+}
+
+template <int D>
+cudaError_t run_d(const AttendParams &p, cudaStream_t st)
+{
+    const bool hilo = (int64_t)p.n_new * p.r <= 8;
+    if (p.mask) return hilo ? run<D, true, true>(p, st) : run<D, false, true>(p, st);
+    return hilo ? run<D, true, false>(p, st) : run<D, false, false>(p, st);
+}
+
+}  // namespace
+
+// CTAs: one an SM, at least a block a warp each, and a multiple of the heads
+// when that idles at most 5 % of them (a CTA then works on one head).
+void rows_split(AttendParams &p)
+{
+    constexpr int kSMs = 148;
+    p.n_tile = (int)(((int64_t)p.n_new * p.r + 15) / 16);
+    p.n_vh = p.c.H * p.n_tile;
+    p.nb = (int)((p.n_kv + kBlock - 1) / kBlock);
+    const int W = p.c.D == 256 ? 4 : 8;
+    const int64_t T = (int64_t)p.n_vh * p.nb;
+    int64_t C = (T + W - 1) / W;
+    if (C > kSMs) C = kSMs;
+    if (C >= p.n_vh) {
+        const int64_t even = C / p.n_vh * p.n_vh;
+        if (even * 20 >= C * 19) C = even;
+    }
+    p.n_cta = (int)C;
+}
+
+cudaError_t launch_rows(const AttendParams &p, cudaStream_t st)
+{
+    switch (p.c.D) {
+    case 64: return run_d<64>(p, st);
+    case 96: return run_d<96>(p, st);
+    case 128: return run_d<128>(p, st);
+    case 256: return run_d<256>(p, st);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace q8
+}  // namespace kvb

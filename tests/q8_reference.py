@@ -54,10 +54,10 @@ def evict(w, n, keep, recent):
     return sorted(heavy) + list(range(n - recent, n))
 
 
-def attend(k, v, q, n_past, mask=None, flash=False):
-    """One head group in 64 bits.  k, v float64 [n_kv][D] (NaN rows allowed), q float64 [T][r][D], mask float32
+def attend(k, v, vs, q, n_past, mask=None, flash=False):
+    """One head group in 64 bits.  k, v float64 [n_kv][D] (NaN rows allowed), vs [n_kv] V's scales, q float64 [T][r][D], mask float32
     [T][>= n_kv] or None.  Returns out [T][r][D], the rows' weights summed over tokens and heads [n_kv], and what the
-    tolerances go by: sum p |v| [T][r][D] and the error of a score [T][r]."""
+    tolerances go by: sum p |v| [T][r][D], the error of a score [T][r] and max p vs [T][r]."""
     T, r, D = q.shape
     n_kv = k.shape[0]
     scale = float(np.float32(1.0) / np.sqrt(np.float32(D)))
@@ -90,4 +90,4 @@ def attend(k, v, q, n_past, mask=None, flash=False):
     dot = torch.nan_to_num(torch.einsum("trd,nd->trn", q.abs(), torch.nan_to_num(k).abs()) * scale)
     big = torch.where(hidden | ~torch.isfinite(t), torch.zeros_like(t), t.abs()).clamp(max=1e6).amax(-1)
     err = (D + 4) * 2.0 ** -24 * torch.where(hidden, torch.zeros_like(dot), dot).amax(-1) + 2.0 ** -22 * big
-    return out, weight, mag, err
+    return out, weight, mag, err, (torch.nan_to_num(p) * vs).amax(-1)

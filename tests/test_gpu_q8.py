@@ -159,7 +159,8 @@ def test_store_clears_the_new_rows_weights_only():
 def check(c, hq, n_past, n_new, q, mask=None, flash=False, out_f16=False, w0=None, out=None, workspace=None):
     """Runs attend and compares.  Tolerance of an output: a weight's relative error is at most twice the error of a
     score (its own and the sum's), 2^-21 for the exponential, n 2^-24 for the sum of n weights, and half a step of F16
-    (2^-11) where the weights are rounded to it; an F16 output adds half a step of itself."""
+    (2^-11) where the weights are rounded to it: of itself, or 2^-25 below F16's normal numbers, where the largest weight
+    times scale is held at 2^7 or more, so 2^-32 of that a key of at most 127; an F16 output adds half a step of itself."""
     n_kv, r, d = n_past + n_new, hq // c.h, c.d
     if out is None:
         out = torch.full((n_new, hq * d), 7.0, device="cuda", dtype=torch.float16 if out_f16 else torch.float32)
@@ -171,9 +172,10 @@ def check(c, hq, n_past, n_new, q, mask=None, flash=False, out_f16=False, w0=Non
     m = None if mask is None else mask.float().cpu()
     for h in range(c.h):
         k, v = c.values(n_kv, h, True)
-        want, weight, mag, err = R.attend(k, v, qq[:, h], n_past, m, flash)
+        vs = torch.from_numpy(2.0 ** R.word_exp(np.repeat(c.words[1][h], B)[:n_kv]))
+        want, weight, mag, err, top = R.attend(k, v, vs, qq[:, h], n_past, m, flash)
         rel = (2 * err + 2.0 ** -21 + n_kv * 2.0 ** -24)[..., None]
-        tol = mag * (rel + 2.0 ** -11) + 2.0 ** -24
+        tol = mag * (rel + 2.0 ** -11) + (n_kv * 127 * 2.0 ** -32 * top)[..., None] + 2.0 ** -24
         if out_f16:
             tol = tol + want.abs().nan_to_num() * 2.0 ** -11 + 2.0 ** -25
         assert torch.equal(torch.isnan(got[:, h]), torch.isnan(want)), "NaN rows of head %d" % h
