@@ -54,7 +54,7 @@ struct AttendParams {
     int32_t n_new;
     const void *q;
     int64_t q_stride;
-    int32_t q_f16;
+    int32_t q_f16, q_vec;   // q_vec: every head starts on a 16-byte boundary
     const void *mask;       // null: causal
     int64_t mask_stride;
     int32_t mask_f16;

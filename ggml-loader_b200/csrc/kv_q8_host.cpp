@@ -176,6 +176,7 @@ int kv_q8_attend(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32
     p.q = q;
     p.q_stride = n_new > 1 ? q_stride : 0;
     p.q_f16 = q_type == KV_F16;
+    p.q_vec = vec_ok(q, p.q_stride, q_type);
     p.mask = mask;
     p.mask_stride = n_new > 1 ? mask_stride : 0;
     p.mask_f16 = mask_type == KV_MASK_F16;

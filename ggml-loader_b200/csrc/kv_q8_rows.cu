@@ -18,6 +18,9 @@
 // head are joined by a second kernel launched programmatically.
 #include <math_constants.h>
 
+#include <algorithm>
+#include <atomic>
+
 #include "kv_internal.h"
 #include "kv_q8.cuh"
 #include "kv_sm100.cuh"
@@ -34,13 +37,15 @@ constexpr float kTop = 15.0f;    // and it moves where a weight would pass 2^kTo
 
 template <int D>
 struct Rows {
-    static constexpr int W = D == 256 ? 4 : 8;                       // warps
-    static constexpr int stages = D == 64 ? 5 : 3;
+    static constexpr int W = 8;                                      // warps
+    static constexpr int E = D == 64 ? 10 : D == 96 ? 7 : D == 128 ? 6 : 3;   // tiles in a warp's ring
     static constexpr int pitch = D + 16;                             // bytes a row: 8 rows fall on different banks
     static constexpr int tile = kBlock * pitch;                      // K or V of a block
-    static constexpr int ring = stages * 2 * tile;                   // a warp's
-    static constexpr int smem = W * ring;
+    static constexpr int ring = E * tile;                            // a warp's
+    static constexpr int smem = W * ring;                            // (also holds the W warps' 16 output rows at the end)
     static constexpr int nk = D / 16;                                // 16-wide steps over D
+    static constexpr bool q_regs = D <= 128;                         // the queries stay in registers, else in shared memory
+    static_assert(smem >= W * 16 * D * 4 && smem <= 225 * 1024, "shared memory");
 };
 
 // two F16 pairs (codes 0, 1 | 2, 3 or 0, 2 | 1, 3) of four signed codes: 0x6400
@@ -64,19 +69,25 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi)
 }
 
 // 4 query elements as two F16 pairs
-__device__ __forceinline__ void load_q4(const AttendParams &p, int t, int hq, int D, int d, uint32_t &a, uint32_t &b)
+__device__ __forceinline__ uint2 load_q4(const AttendParams &p, int t, int hq, int D, int d)
 {
     const int64_t i = t * p.q_stride + (int64_t)hq * D + d;
     __half x[4];
     if (p.q_f16) {
+        if (p.q_vec) return *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + i);
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = static_cast<const __half *>(p.q)[i + k];
+    } else if (p.q_vec) {
+        const float4 v = *reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + i);
+        x[0] = __float2half_rn(v.x);
+        x[1] = __float2half_rn(v.y);
+        x[2] = __float2half_rn(v.z);
+        x[3] = __float2half_rn(v.w);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = __float2half_rn(static_cast<const float *>(p.q)[i + k]);
     }
-    a = pack_half2(x[0], x[1]);
-    b = pack_half2(x[2], x[3]);
+    return make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
 }
 
 __device__ __forceinline__ float mask_value(const AttendParams &p, int t, int64_t key)
@@ -152,6 +163,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
     extern __shared__ __align__(128) char smem[];
     __shared__ float2 s_stat[G::W][16];
     __shared__ float s_bad[G::W][16];
+    __shared__ uint2 s_q[G::q_regs ? 1 : 16][G::q_regs ? 1 : D / 4 + 4];   // (the pad: 8 rows fall on different banks)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     char *ring = smem + warp * G::ring;
     const int64_t T = (int64_t)p.n_vh * p.nb, lo = blockIdx.x * T / p.n_cta, hi = (blockIdx.x + 1) * T / p.n_cta;
@@ -168,50 +180,70 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
         const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)h * (p.c.rows / kBlock);
         const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.c.v_scale) + (int64_t)h * (p.c.rows / kBlock);
 
-        auto fetch = [&](int b, int stage) {
-            if (b < b1) {
-                char *ks = ring + stage * 2 * G::tile, *vs = ks + G::tile;
-                const int8_t *ksrc = kc + (int64_t)b * kBlock * D, *vsrc = vc + (int64_t)b * kBlock * D;
-#pragma unroll
-                for (int j = 0; j < D / 16; j++) {
-                    const int i = lane + 32 * j, r = i / (D / 16), c = i % (D / 16);
-                    cp_async_16(ks + r * G::pitch + c * 16, ksrc + i * 16);
-                }
-#pragma unroll
-                for (int j = 0; j < D / 16; j++) {
-                    const int i = lane + 32 * j, r = i / (D / 16), c = i % (D / 16);
-                    cp_async_16(vs + r * G::pitch + c * 16, vsrc + i * 16);
-                }
-            }
-            cp_async_commit();
-        };
-        // this warp's blocks: b0 + warp, then every W-th
-        int fb = b0 + warp, fs = 0;
-#pragma unroll
-        for (int s = 0; s < G::stages - 1; s++) {
-            fetch(fb, fs);
-            fb += G::W;
-            fs++;
-        }
-
+        // The small loads first: behind the ring's they would wait for all of them.
         // Q as the A operand: rows g and g + 8, dims 4 t4 .. + 3 of each 16 (the
         // order in which a thread holds a key's codes)
-        uint32_t qa[G::nk][HILO ? 2 : 4];
+        uint2 q[G::q_regs ? G::nk : 1][RT];
         int tok[RT];
 #pragma unroll
         for (int i = 0; i < RT; i++) {
             const int row = row0 + g + 8 * i;
             const bool have = g + 8 * i < nrows;
             tok[i] = have ? row / p.r : 0;
-            const int hq = h * p.r + (have ? row % p.r : 0);
+            if constexpr (G::q_regs) {
+                const int hq = h * p.r + (have ? row % p.r : 0);
 #pragma unroll
-            for (int k = 0; k < G::nk; k++) {
-                uint32_t a = 0, b = 0;
-                if (have) load_q4(p, tok[i], hq, D, k * 16 + t4 * 4, a, b);
-                qa[k][i] = a;
-                qa[k][RT + i] = b;
+                for (int k = 0; k < G::nk; k++)
+                    q[k][i] = have ? load_q4(p, tok[i], hq, D, k * 16 + t4 * 4) : make_uint2(0, 0);
             }
         }
+        if constexpr (!G::q_regs) {
+            for (int i = threadIdx.x; i < 8 * RT * (D / 4); i += G::W * 32) {
+                const int row = i / (D / 4), c = i % (D / 4);
+                s_q[row][c] = row < nrows ? load_q4(p, (row0 + row) / p.r, h * p.r + (row0 + row) % p.r, D, c * 4)
+                                          : make_uint2(0, 0);
+            }
+        }
+        // the scale words of this warp's next 32 blocks, one a lane
+        uint32_t kw = 0, vw = 0;
+        auto scales = [&](int b) {
+            const int mine = b + lane * G::W;
+            kw = mine < b1 ? ksc[mine] : 0;
+            vw = mine < b1 ? vsc[mine] : 0;
+        };
+        scales(b0 + warp);
+
+        // this warp's blocks: b0 + warp, then every W-th; their tiles K, V, K, V ... through the ring
+        int fb = b0 + warp, fs = 0;
+        bool fv = false;
+        auto fetch = [&] {
+            if (fb < b1) {
+                char *dst = ring + fs * G::tile;
+                const int8_t *src = (fv ? vc : kc) + (int64_t)fb * kBlock * D;
+#pragma unroll
+                for (int j = 0; j < D / 16; j++) {
+                    const int i = lane + 32 * j, r = i / (D / 16), c = i % (D / 16);
+                    cp_async_16(dst + r * G::pitch + c * 16, src + i * 16);
+                }
+            }
+            cp_async_commit();
+            if (fv) fb += G::W;
+            fv = !fv;
+            if (++fs == G::E) fs = 0;
+        };
+        int slot = 0;
+        // the next tile's address, once it has arrived; the one before it is read again by nobody
+        auto next_tile = [&] {
+            cp_async_wait<G::E - 2>();
+            __syncwarp();
+            fetch();
+            const uint32_t at = smem_addr(ring + slot * G::tile);
+            if (++slot == G::E) slot = 0;
+            return at;
+        };
+#pragma unroll 1
+        for (int i = 0; i < G::E - 1; i++) fetch();
+        if constexpr (!G::q_regs) __syncthreads();
 
         RowState st[RT];
 #pragma unroll
@@ -222,14 +254,8 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
 #pragma unroll
             for (int j = 0; j < 4; j++) o[i][j] = 0.0f;
 
-        int stage = 0;
-        uint32_t kw = 0, vw = 0;   // the scale words of this warp's next 32 blocks, one a lane
         for (int b = b0 + warp, n = 0; b < b1; b += G::W, n++) {
-            if ((n & 31) == 0) {
-                const int mine = b + lane * G::W;
-                kw = mine < b1 ? ksc[mine] : 0;
-                vw = mine < b1 ? vsc[mine] : 0;
-            }
+            if (n && (n & 31) == 0) scales(b);
             const uint32_t kword = __shfl_sync(0xffffffffu, kw, n & 31), vword = __shfl_sync(0xffffffffu, vw, n & 31);
             const bool k_bad = (kword & 0x7f800000u) == 0x7f800000u, v_bad = (vword & 0x7f800000u) == 0x7f800000u;
             const float ks = k_bad ? CUDART_NAN_F : pow2(scale_exp(kword)), ev = (float)scale_exp(vword);
@@ -244,47 +270,37 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
                         mk[i][j] = key < p.n_kv ? mask_value(p, tok[i], key) : -CUDART_INF_F;
                     }
             }
-            cp_async_wait<G::stages - 2>();
-            __syncwarp();
-            fetch(fb, fs);   // into the stage the previous block left
-            fb += G::W;
-            if (++fs == G::stages) fs = 0;
-            const uint32_t kt = smem_addr(ring + stage * 2 * G::tile), vt = kt + G::tile;
-            if (++stage == G::stages) stage = 0;
-
-            // S = Q K^T: 4 groups of 8 keys
+            // S = Q K^T: 4 groups of 8 keys, 32 dims at a time
+            const uint32_t kt = next_tile() + (lane & 7) * G::pitch + (lane >> 3) * 16;
             float acc[4][4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
-                const uint32_t row = kt + (j * 8 + (lane & 7)) * G::pitch + (lane >> 3) * 16;
 #pragma unroll
-                for (int c = 0; c < D / 64; c++) {
+            for (int c = 0; c < D / 32; c++) {
+                uint2 qa[2][RT];
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int i = 0; i < RT; i++) {
+                        if constexpr (G::q_regs) qa[k][i] = q[2 * c + k][i];
+                        else qa[k][i] = s_q[g + 8 * i][(2 * c + k) * 4 + t4];
+                    }
+#pragma unroll
+                for (int jj = 0; jj < 2; jj++) {
+                    // lanes 0-15: keys of group 2 jj (two 16-dim chunks), 16-31: of group 2 jj + 1
                     uint32_t w[4];
-                    ldsm_x4(row + c * 64, w[0], w[1], w[2], w[3]);
+                    ldsm_x4(kt + (jj * 16 + (lane >> 4) * 8) * G::pitch + c * 32 - (lane >> 4) * 32, w[0], w[1], w[2], w[3]);
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         uint32_t x, y;
                         codes_to_half<false>(w[i], x, y);
-                        const int k = c * 4 + i;
-                        if constexpr (HILO) mma_16816(acc[j], qa[k][0], 0u, qa[k][1], 0u, x, y);
-                        else mma_16816(acc[j], qa[k][0], qa[k][1], qa[k][2], qa[k][3], x, y);
+                        float(&d)[4] = acc[2 * jj + (i >> 1)];
+                        const uint2 *a = qa[i & 1];
+                        if constexpr (HILO) mma_16816(d, a[0].x, 0u, a[0].y, 0u, x, y);
+                        else mma_16816(d, a[0].x, a[RT - 1].x, a[0].y, a[RT - 1].y, x, y);
                     }
-                }
-                if constexpr (D % 64 != 0) {   // 96: the last 32 dims
-                    uint32_t w0, w1;
-                    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];"
-                                 : "=r"(w0), "=r"(w1)
-                                 : "r"(kt + (j * 8 + (lane & 7)) * G::pitch + (D / 64) * 64 + ((lane >> 3) & 1) * 16));
-                    uint32_t x, y;
-                    constexpr int k = D / 64 * 4;
-                    codes_to_half<false>(w0, x, y);
-                    if constexpr (HILO) mma_16816(acc[j], qa[k][0], 0u, qa[k][1], 0u, x, y);
-                    else mma_16816(acc[j], qa[k][0], qa[k][1], qa[k][2], qa[k][3], x, y);
-                    codes_to_half<false>(w1, x, y);
-                    if constexpr (HILO) mma_16816(acc[j], qa[k + 1][0], 0u, qa[k + 1][1], 0u, x, y);
-                    else mma_16816(acc[j], qa[k + 1][0], qa[k + 1][1], qa[k + 1][2], qa[k + 1][3], x, y);
                 }
             }
 
@@ -342,6 +358,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
                     }
                 }
             }
+            const uint32_t vt = next_tile();
 #pragma unroll
             for (int c = 0; c < G::nk; c++) {
                 uint32_t v[4];
@@ -388,7 +405,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
         }
         __syncthreads();
         const bool whole = b0 == 0 && b1 == p.nb;
-        const int64_t slot = (int64_t)blockIdx.x + vh;   // (CTA, head) pairs in order: their sum counts them
+        const int64_t part = (int64_t)blockIdx.x + vh;   // (CTA, head) pairs in order: their sum counts them
         constexpr float unit = MASKED ? kLog2e : 1.0f;
         for (int i = threadIdx.x; i < nrows * (D / 4); i += G::W * 32) {
             const int row = i / (D / 4), c = i % (D / 4) * 4;
@@ -419,9 +436,9 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
                 store_out(p, at + 2, x.z * z);
                 store_out(p, at + 3, x.w * z);
             } else {
-                *reinterpret_cast<float4 *>(p.part + (slot * 16 + row) * D + c) = x;
+                *reinterpret_cast<float4 *>(p.part + (part * 16 + row) * D + c) = x;
             }
-            if (c == 0) p.stat[slot * 16 + row] = make_float2(M, l);
+            if (c == 0) p.stat[part * 16 + row] = make_float2(M, l);
         }
         __syncthreads();   // the next head's ring takes the shared memory
     }
@@ -557,6 +574,23 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
         if (key + i < p.n_kv) dst[i] += sum[i];
 }
 
+// Runs a function once a device (a kernel's attributes last); devices past 63 run it every time.
+struct Once {
+    std::atomic<uint64_t> done{0};
+    template <class F>
+    cudaError_t on_device(F &&f)
+    {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        e = f();
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+};
+
 template <class K>
 cudaError_t launch_pdl(K kernel, unsigned grid, unsigned block, size_t smem, const AttendParams &p, cudaStream_t st)
 {
@@ -577,7 +611,10 @@ template <int D, bool HILO, bool MASKED>
 cudaError_t run(const AttendParams &p, cudaStream_t st)
 {
     using G = Rows<D>;
-    cudaError_t e = cudaFuncSetAttribute(rows_kernel<D, HILO, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
+    static Once once;
+    cudaError_t e = once.on_device([] {
+        return cudaFuncSetAttribute(rows_kernel<D, HILO, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
+    });
     if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, HILO, MASKED>, p.n_cta, G::W * 32, G::smem, p, st);
     if (e != cudaSuccess) return e;
     const bool split = p.n_cta > p.n_vh || p.n_vh % p.n_cta != 0;   // else every head lies in one CTA
@@ -597,21 +634,26 @@ cudaError_t run_d(const AttendParams &p, cudaStream_t st)
 
 }  // namespace
 
-// CTAs: one an SM, at least a block a warp each, and a multiple of the heads
-// when that idles at most 5 % of them (a CTA then works on one head).
+// CTAs: one an SM, about a block a warp each at least, and a multiple of the
+// heads where there are SMs for it or it idles at most 5 % of them (a CTA then
+// works on one head; 8 heads of 2000 keys: 63 CTAs 11.0 us, 64 CTAs 8.0 us).
 void rows_split(AttendParams &p)
 {
     constexpr int kSMs = 148;
     p.n_tile = (int)(((int64_t)p.n_new * p.r + 15) / 16);
     p.n_vh = p.c.H * p.n_tile;
     p.nb = (int)((p.n_kv + kBlock - 1) / kBlock);
-    const int W = p.c.D == 256 ? 4 : 8;
+    constexpr int W = 8;
     const int64_t T = (int64_t)p.n_vh * p.nb;
     int64_t C = (T + W - 1) / W;
     if (C > kSMs) C = kSMs;
+    // a head costs a CTA about 4 us besides its blocks (2.3 us a block of each
+    // warp at most): short heads go to CTAs of their own, in waves if need be
+    if (C < p.n_vh && (C < kSMs || p.nb <= 4 * W)) C = p.n_vh;
     if (C >= p.n_vh) {
-        const int64_t even = C / p.n_vh * p.n_vh;
-        if (even * 20 >= C * 19) C = even;
+        const int64_t up = (C + p.n_vh - 1) / p.n_vh * p.n_vh, down = C / p.n_vh * p.n_vh;
+        if (up <= kSMs) C = std::min(up, T);
+        else if (down * 20 >= C * 19) C = down;
     }
     p.n_cta = (int)C;
 }

@@ -394,34 +394,37 @@ class Q8Cache:
             if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != k.device:
                 raise ValueError("%s must be a contiguous %s tensor %s on %s" % (name, dtype, shape, k.device))
         self.tensors = k, v, k_scale, v_scale, weight   # kept alive
-        self.device = k.device
         self.n_head_kv, self.rows, self.head_dim = h, rows, d
         self._c = KvQ8Cache(*[_ptr(t) for t in self.tensors], rows, h, d)
         self._ref = ctypes.addressof(self._c)
+        # what each call looks up, once: a decoded token's call is a few microseconds
+        self._torch, self._lib, self._index = torch, lib(), k.get_device()
+        self._types = {torch.float32: 0, torch.float16: 1}
+        self._current = torch._C._cuda_getDevice if self._index >= 0 else None
 
     def _rows(self, name, t, n, width):
         """(pointer, stride, type) of a tensor of n rows of `width` elements."""
-        import torch
-        if t.dtype not in (torch.float32, torch.float16):
+        kind = self._types.get(t.dtype)
+        if kind is None:
             raise ValueError("%s must be float32 or float16" % name)
         shape, stride = t.shape, t.stride()
-        if shape[0] != n or t.numel() != n * width or t.device != self.device:
-            raise ValueError("%s must hold %d rows of %d elements on %s" % (name, n, width, self.device))
+        if t.get_device() != self._index or not shape or shape[0] != n or t.numel() != n * width:
+            raise ValueError("%s must hold %d rows of %d elements on the cache's device" % (name, n, width))
         inner = 1
         for i in range(len(shape) - 1, 0, -1):
             if shape[i] != 1 and stride[i] != inner:
                 raise ValueError("the rows of %s must be contiguous" % name)
             inner *= shape[i]
-        return t.data_ptr(), stride[0], int(t.dtype == torch.float16)
+        return t.data_ptr(), stride[0], kind
 
-    def _call(self, name, *args):
-        """The call on this cache's device."""
-        import torch
-        index = self.device.index
-        if index is not None and torch.cuda.is_available() and index != torch.cuda.current_device():
-            with torch.cuda.device(index):
-                return _check(getattr(lib(), name)(self._ref, *args), name)
-        return _check(getattr(lib(), name)(self._ref, *args), name)
+    def _call(self, fn, *args):
+        """fn on this cache, on its device."""
+        if self._current is not None and self._current() != self._index:
+            with self._torch.cuda.device(self._index):
+                rc = fn(self._ref, *args)
+        else:
+            rc = fn(self._ref, *args)
+        return rc if rc == KV_OK else _check(rc, fn.__name__)
 
     def store(self, row0, n_new, k, v, stream=None):
         """kv_q8_store: n_new rows of [n_head_kv][head_dim] at row0."""
@@ -430,53 +433,50 @@ class Q8Cache:
         vp, vs, vt = self._rows("v", v, n_new, width)
         if kt != vt:
             raise ValueError("k and v must have one type")
-        return self._call("kv_q8_store", row0, n_new, kp, ks, vp, vs, kt, _stream(stream))
+        return self._call(self._lib.kv_q8_store, row0, n_new, kp, ks, vp, vs, kt, _stream(stream))
 
     def load(self, row0, n, k_out, v_out, stream=None):
         """kv_q8_load: the values of n rows from row0 into k_out and v_out (either may be None)."""
-        got = [None if t is None else self._rows(s, t, n, self.n_head_kv * self.head_dim)
-               for s, t in (("k_out", k_out), ("v_out", v_out))]
-        some = [g for g in got if g]
-        if some and any(g[1:] != some[0][1:] for g in some):
+        width = self.n_head_kv * self.head_dim
+        k = (None,) if k_out is None else self._rows("k_out", k_out, n, width)
+        v = (None,) if v_out is None else self._rows("v_out", v_out, n, width)
+        if k[1:] != v[1:] and k[0] and v[0]:
             raise ValueError("k_out and v_out must have one type and row stride")
-        stride, kind = some[0][1:] if some else (0, 0)
-        return self._call("kv_q8_load", row0, n, got[0] and got[0][0], got[1] and got[1][0], stride, kind,
-                          _stream(stream))
+        stride, kind = k[1:] or v[1:] or (0, 0)
+        return self._call(self._lib.kv_q8_load, row0, n, k[0], v[0], stride, kind, _stream(stream))
 
     def attend_workspace(self, n_head, n_past, n_new):
         """Bytes of workspace attend needs for these sizes."""
-        n = int(lib().kv_q8_attend_workspace(self._ref, n_head, n_past, n_new))
+        n = int(self._lib.kv_q8_attend_workspace(self._ref, n_head, n_past, n_new))
         if n == 0:
             raise KvError(KV_E_ARG, "kv_q8_attend_workspace")
         return n
 
     def attend(self, n_head, n_past, n_new, q, out, mask=None, flash=False, workspace=None, stream=None):
         """kv_q8_attend: n_new rows of [n_head][head_dim] queries over the rows
-        [0, n_past + n_new); workspace: a uint8 CUDA tensor of attend_workspace bytes."""
-        import torch
+        [0, n_past + n_new); workspace: a contiguous CUDA tensor of attend_workspace bytes."""
         width = n_head * self.head_dim
         qp, qs, qt = self._rows("q", q, n_new, width)
         op, os_, ot = self._rows("out", out, n_new, width)
         mp, mt, ms = None, 0, 0
         if mask is not None:
-            if mask.dim() != 2 or mask.stride(1) != 1 or mask.shape[0] != n_new or mask.shape[1] < n_past + n_new or \
-                    mask.dtype not in (torch.float32, torch.float16) or mask.device != self.device:
-                raise ValueError("mask must be [n_new][>= n_past + n_new], float32 or float16, on %s" % self.device)
-            mp, mt, ms = mask.data_ptr(), int(mask.dtype == torch.float16), mask.stride(0)
-        if workspace is None or workspace.device != self.device or not workspace.is_contiguous():
-            raise ValueError("attend needs a contiguous workspace tensor on %s" % self.device)
-        return self._call("kv_q8_attend", n_head, n_past, n_new, qp, qs, qt, mp, mt, ms, 1 if flash else 0,
-                          op, os_, ot, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                          _stream(stream))
+            mt = self._types.get(mask.dtype)
+            if mt is None or mask.dim() != 2 or mask.stride(1) != 1 or mask.shape[0] != n_new or \
+                    mask.shape[1] < n_past + n_new or mask.get_device() != self._index:
+                raise ValueError("mask must be [n_new][>= n_past + n_new], float32 or float16, on the cache's device")
+            mp, ms = mask.data_ptr(), mask.stride(0)
+        if workspace is None or workspace.get_device() != self._index or not workspace.is_contiguous():
+            raise ValueError("attend needs a contiguous workspace tensor on the cache's device")
+        return self._call(self._lib.kv_q8_attend, n_head, n_past, n_new, qp, qs, qt, mp, mt, ms, 1 if flash else 0,
+                          op, os_, ot, workspace.data_ptr(), workspace.nbytes, _stream(stream))
 
     def evict(self, n_rows, keep, recent, dst, kept, stream=None):
         """kv_q8_evict into the Q8Cache dst; kept: int32 [n_head_kv][keep]."""
-        import torch
-        if tuple(kept.shape) != (self.n_head_kv, keep) or kept.dtype != torch.int32 or not kept.is_contiguous() or \
-                kept.device != self.device or dst.device != self.device:
-            raise ValueError("kept must be a contiguous int32 [%d][%d] tensor on %s, with dst there too"
-                             % (self.n_head_kv, keep, self.device))
-        return self._call("kv_q8_evict", n_rows, keep, recent, dst._ref, kept.data_ptr(), _stream(stream))
+        if kept.shape != (self.n_head_kv, keep) or kept.dtype != self._torch.int32 or not kept.is_contiguous() or \
+                kept.get_device() != self._index or dst._index != self._index:
+            raise ValueError("kept must be a contiguous int32 [%d][%d] tensor on the cache's device, dst there too"
+                             % (self.n_head_kv, keep))
+        return self._call(self._lib.kv_q8_evict, n_rows, keep, recent, dst._ref, kept.data_ptr(), _stream(stream))
 
 
 def gen_normal_device(dst, seed, stream_id, n, idx0=0, stream=None):
