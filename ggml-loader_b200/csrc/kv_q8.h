@@ -4,12 +4,14 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace kvb {
 namespace q8 {
 
 constexpr int kBlock = 32;   // rows that share a scale (KV_Q8_BLOCK)
+constexpr int kSMs = 148;    // the most CTAs a split uses
 constexpr int kExpMin = -24, kExpMax = 9;   // a scale is 2^e with e in this range
 
 struct Cache {
@@ -61,15 +63,18 @@ struct AttendParams {
     int32_t flash;          // a row without a visible key gives 0 (else NaN)
     void *out;
     int64_t out_stride;
-    int32_t out_f16;
+    int32_t out_f16, out_vec;
     float scale;
     // scratch of the workspace, set by launch_attend
     int32_t nb;             // blocks of kBlock keys: ceil(n_kv / kBlock)
-    int32_t n_tile;         // query-row tiles a KV head
-    int32_t n_vh;           // H * n_tile
+    int32_t n_tile;         // query-row tiles a CTA holds
+    int32_t n_vh;           // what CTAs work on at a time: KV heads, or (chunk) pairs of one and a block, H * n_blk
     int32_t n_cta;
-    float *part;            // [n_cta + n_vh][16][D] partial outputs of a (CTA, virtual head)
-    float2 *stat;           // [n_cta + n_vh][16] their (maximum, sum)
+    int32_t tok_tile, tok_blk, n_blk;   // chunk: tokens of a query tile and of a CTA's tiles, such blocks
+    int64_t subs;           // chunk: sub-tiles of 64 keys of one KV head, over its blocks
+    float *part;            // [n_cta + n_vh][rows][D] partial outputs of a (CTA, head or pair); rows: 16,
+                            // or a chunk block's 128 * n_tile
+    float2 *stat;           // [n_cta + n_vh][rows] their (maximum, sum)
     float *scores;          // [H][n_new * r][nb * kBlock] or null
     float2 *row_stat;       // [H][n_new * r] (maximum, 1 / sum or 0) or null
 };
@@ -80,6 +85,28 @@ cudaError_t launch_attend(AttendParams p, void *ws, cudaStream_t st);
 // kv_q8_rows.cu: the split of a call over CTAs, and its kernels
 void rows_split(AttendParams &p);
 cudaError_t launch_rows(const AttendParams &p, cudaStream_t st);
+// kv_q8_chunk.cu: the same for more than 16 query rows a KV head
+void chunk_split(AttendParams &p);
+cudaError_t launch_chunk(const AttendParams &p, cudaStream_t st);
+// the bits of device waits that expired since the last call (0: none)
+cudaError_t take_error(unsigned *word);
+
+// Runs a function once a device (a kernel's attributes last); devices past 63 run it every time.
+struct Once {
+    std::atomic<uint64_t> done{0};
+    template <class F>
+    cudaError_t on_device(F &&f)
+    {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+        e = f();
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+};
 
 }  // namespace q8
 }  // namespace kvb

@@ -1,6 +1,8 @@
 // kv_q8_attend.cu -- attention over the 8-bit cache.
 #include <math_constants.h>
 
+#include <algorithm>
+
 #include "kv_internal.h"
 #include "kv_q8.cuh"
 
@@ -55,7 +57,8 @@ __global__ void __launch_bounds__(T) weigh_kernel(const AttendParams p)
         for (int d = threadIdx.x; d < D; d += T) qs[d] = query(p, t, h * p.r + row % p.r, D, d);
         __syncthreads();
         const float2 st = p.row_stat[(int64_t)h * p.n_new * p.r + row];
-        if (key < p.n_kv && st.y != 0.0f) sum += expf(score<D>(p, qs, h, t, key) - st.x) * st.y;
+        if (key < p.n_kv && st.y != 0.0f)
+            sum += (p.mask ? expf(score<D>(p, qs, h, t, key) - st.x) : exp2f(score<D>(p, qs, h, t, key) * 1.4426950408889634f - st.x)) * st.y;
     }
     if (key < p.n_kv) p.c.weight[(int64_t)h * p.c.rows + key] += sum;
 }
@@ -70,20 +73,24 @@ cudaError_t weigh(const AttendParams &p, cudaStream_t st)
 // The workspace, laid out from `ws` on; returns its bytes.
 uint64_t lay_out(AttendParams &p, char *ws)
 {
-    rows_split(p);
+    const uint64_t rows = (uint64_t)p.n_new * p.r;
+    const bool chunk = rows > 16;
+    if (chunk) chunk_split(p);
+    else rows_split(p);
     uint64_t n = 0;
     auto take = [&](uint64_t bytes) {
         char *at = ws + n;
         n += (bytes + 255) / 256 * 256;
         return at;
     };
-    const uint64_t slots = (uint64_t)p.n_cta + p.n_vh, rows = (uint64_t)p.n_new * p.r;
-    p.part = reinterpret_cast<float *>(take(slots * 16 * p.c.D * sizeof(float)));
-    p.stat = reinterpret_cast<float2 *>(take(slots * 16 * sizeof(float2)));
+    // (the most CTAs any call of these heads has, so that larger sizes never need less)
+    const uint64_t slots = ((uint64_t)std::max(p.n_vh, kSMs) + p.n_vh) * (chunk ? 128 * p.n_tile : 16);
+    p.part = reinterpret_cast<float *>(take(slots * p.c.D * sizeof(float)));
+    p.stat = reinterpret_cast<float2 *>(take(slots * sizeof(float2)));
     p.scores = nullptr;
     p.row_stat = nullptr;
-    if (p.c.weight && rows <= 16) p.scores = reinterpret_cast<float *>(take(p.c.H * rows * p.nb * kBlock * sizeof(float)));
-    if (p.c.weight && rows > 16) p.row_stat = reinterpret_cast<float2 *>(take(p.c.H * rows * sizeof(float2)));
+    if (p.c.weight && !chunk) p.scores = reinterpret_cast<float *>(take(p.c.H * rows * p.nb * kBlock * sizeof(float)));
+    if (p.c.weight && chunk) p.row_stat = reinterpret_cast<float2 *>(take(p.c.H * rows * sizeof(float2)));
     return n;
 }
 
@@ -92,13 +99,20 @@ uint64_t lay_out(AttendParams &p, char *ws)
 uint64_t attend_workspace(const AttendParams &p)
 {
     AttendParams q = p;
-    return lay_out(q, nullptr);
+    uint64_t n = lay_out(q, nullptr);
+    if ((int64_t)p.n_new * p.r > 16 && p.r <= 16) {   // what the most rows of the other kernel need, so that it suffices for fewer tokens
+        q = p;
+        q.n_new = 16 / p.r;
+        n = std::max(n, lay_out(q, nullptr));
+    }
+    return n;
 }
 
 cudaError_t launch_attend(AttendParams p, void *ws, cudaStream_t st)
 {
     lay_out(p, static_cast<char *>(ws));
-    cudaError_t e = launch_rows(p, st);
+    const bool chunk = (int64_t)p.n_new * p.r > 16;
+    cudaError_t e = chunk ? launch_chunk(p, st) : launch_rows(p, st);
     if (e != cudaSuccess || !p.row_stat) return e;
     switch (p.c.D) {
     case 64: return weigh<64>(p, st);

@@ -1,0 +1,853 @@
+// kv_q8_chunk.cu -- attention over the 8-bit cache for more than 16 query rows
+// a KV head (a prompt's chunk), on the 5th-generation tensor cores: tcgen05.mma
+// with F32 accumulators in TMEM, operands in shared memory.
+//
+// The mathematics is kv_q8_rows.cu's: scores t = (q . codes) * ks * scale,
+// weights W = e^t 2^ev relative to a running reference of the row, F16, and
+//   out = sum W codes_v / sum W 2^-ev,
+// so both operands from the cache are its integer codes, exact in F16.
+// Reference: unmasked rows keep one number M (log2 units of e^t 2^ev); with a
+// mask it is a pair (m, me), since a mask of the type's lowest value leaves no
+// room next to it for an exponent.
+//
+// Work: a tile is 128 query rows of one KV head (row = token * r + head of the
+// group); a CTA holds two of them (one at head_dim 256), so a sub-tile of 64
+// keys staged once feeds both.  A pair is (KV head, block of two tiles), its
+// keys the sub-tiles up to the block's last visible key; the pairs' sub-tiles,
+// laid end to end, are cut into equal ranges, one CTA each; pairs cut between
+// CTAs are joined by fold_kernel.
+//
+// chunk_kernel (512 threads, registers moved to where they are needed):
+//   warps 0-2   issue the MMAs: S_A, S_B (64 columns each, double buffered) and
+//               the products P.V; three threads because one thread's issue rate
+//               bounds MMAs this narrow.  Warp 3 owns TMEM.
+//   warps 4-7   stage: codes from global memory into registers some units ahead
+//               (32 KB in flight an SM), converted to F16 and stored in the
+//               128-byte-swizzled layout the tensor cores read; also the queries
+//   warps 8-15  softmax of tile A and tile B, a query row a thread: S from TMEM,
+//               weights back as F16 pairs; rescales O when the reference moves;
+//               writes a segment's O
+// Every wait is inside the CTA and bounded; an expired one sets the error word.
+#include <math_constants.h>
+
+#include <algorithm>
+
+#include "kv_internal.h"
+#include "kv_q8.cuh"
+#include "kv_sm100.cuh"
+
+namespace kvb {
+namespace q8 {
+
+__device__ unsigned g_error;   // bits of waits that expired (kv_q8_status)
+
+namespace {
+
+using namespace sm100;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kBias = 7.0f, kTop = 15.0f;   // as kv_q8_rows.cu: a new reference's weight is 2^7, it moves past 2^15
+constexpr uint64_t kLimitNs = 1000000000ull;
+constexpr int kThreads = 512;
+constexpr int kSub = 64;   // keys of a sub-tile
+
+template <int D>
+struct CL {
+    static constexpr int NT = D == 256 ? 1 : 2;              // query tiles a CTA holds
+    static constexpr int NB = (D + 63) / 64;                 // 64-wide swizzled boxes a row
+    static constexpr uint32_t q_tile = NB * 128 * 128;       // bytes
+    static constexpr uint32_t box = kSub * 128;              // [64 keys][64 halves]
+    static constexpr uint32_t tile = NB * box;               // a K or V sub-tile
+    static constexpr int KS = D == 256 ? 3 : D >= 96 ? 5 : 8;
+    static constexpr int VS = D == 256 ? 2 : D >= 96 ? 5 : 8;
+    static constexpr int n_ld = kSub * D / 16 / 128;         // 16-byte loads a staging thread makes a unit
+    static constexpr int PF = D == 64 ? 8 : D == 256 ? 2 : 4;   // units in flight: 32 KB an SM (64 registers a thread; 24 KB at 96)
+    static constexpr size_t o_q = 0;
+    static constexpr size_t o_k = o_q + NT * (size_t)q_tile;
+    static constexpr size_t o_v = o_k + KS * (size_t)tile;
+    static constexpr size_t o_bar = o_v + VS * (size_t)tile;
+    static constexpr int n_bar = 2 + 2 * KS + 2 * VS + 12 + 2 + 3;
+    static constexpr size_t o_tm = o_bar + n_bar * 8;
+    static constexpr size_t bytes = o_tm + 16;
+    static_assert(bytes <= 227 * 1024, "shared memory");
+};
+
+// ---- the work split --------------------------------------------------------------
+__device__ __forceinline__ int subs_of(const AttendParams &p, int b)
+{
+    const int64_t last = p.mask ? p.n_kv : p.n_past + min((int64_t)p.n_new, (int64_t)(b + 1) * p.tok_blk);
+    return (int)((last + kSub - 1) / kSub);
+}
+
+__device__ __forceinline__ int64_t pair_start(const AttendParams &p, int pair)
+{
+    const int b = pair % p.n_blk;
+    int64_t x = (int64_t)(pair / p.n_blk) * p.subs;
+    for (int i = 0; i < b; i++) x += subs_of(p, i);
+    return x;
+}
+
+__device__ __forceinline__ int64_t cta_begin(const AttendParams &p, int c)
+{
+    return (int64_t)c * (p.c.H * p.subs) / p.n_cta;
+}
+
+// A walk over a CTA's sub-tiles: pair, sub-tile t of [t0, t1) of it (whole: all of the pair's).
+struct Walk {
+    int pair, t0, t, t1, n;
+    int64_t left;   // sub-tiles from t0 of this pair on
+    __device__ __forceinline__ void begin(const AttendParams &p, int c)
+    {
+        const int64_t x = cta_begin(p, c);
+        left = cta_begin(p, c + 1) - x;
+        const int h = (int)(x / p.subs);
+        int64_t rem = x - (int64_t)h * p.subs;
+        int b = 0;
+        for (; b < p.n_blk - 1; b++) {
+            const int k = subs_of(p, b);
+            if (rem < k) break;
+            rem -= k;
+        }
+        pair = h * p.n_blk + b;
+        t0 = t = (int)rem;
+        span(p);
+    }
+    __device__ __forceinline__ void span(const AttendParams &p)
+    {
+        n = subs_of(p, pair % p.n_blk);
+        t1 = (int)min((int64_t)n, t0 + left);
+    }
+    __device__ __forceinline__ bool more() const { return left > 0; }
+    __device__ __forceinline__ void next_pair(const AttendParams &p)
+    {
+        left -= t1 - t0;
+        pair++;
+        t0 = t = 0;
+        if (left > 0) span(p);
+    }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == n; }
+};
+
+// query tiles of block b that hold rows
+__device__ __forceinline__ int tiles_of(const AttendParams &p, int b)
+{
+    return p.n_tile == 2 && b * p.tok_blk + p.tok_tile < p.n_new ? 2 : 1;
+}
+
+__device__ __forceinline__ void give_up(volatile int *flag, unsigned bit)
+{
+    if (!*flag) {
+        atomicOr(&g_error, bit);
+        *flag = 1;
+    }
+}
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <int N>
+__device__ __forceinline__ void regs_inc()
+{
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_dec()
+{
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// four signed codes -> four halves in order (0x6400 | u is the half 1024 + u)
+__device__ __forceinline__ uint2 codes_to_half4(uint32_t w)
+{
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 hx = __hsub2(*reinterpret_cast<__half2 *>(&x), off), hy = __hsub2(*reinterpret_cast<__half2 *>(&y), off);
+    return make_uint2(*reinterpret_cast<const uint32_t *>(&hx), *reinterpret_cast<const uint32_t *>(&hy));
+}
+
+// 8 query elements at d as F16
+__device__ __forceinline__ uint4 load_q8(const AttendParams &p, int t, int hq, int D, int d)
+{
+    const int64_t i = t * p.q_stride + (int64_t)hq * D + d;
+    uint4 w;
+    __half2 *h = reinterpret_cast<__half2 *>(&w);
+    if (p.q_f16) {
+        const __half *src = static_cast<const __half *>(p.q) + i;
+        if (p.q_vec) return *reinterpret_cast<const uint4 *>(src);
+#pragma unroll
+        for (int k = 0; k < 4; k++) h[k] = __halves2half2(src[2 * k], src[2 * k + 1]);
+    } else {
+        const float *src = static_cast<const float *>(p.q) + i;
+        if (p.q_vec) {
+            const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
+            h[0] = __floats2half2_rn(a.x, a.y);
+            h[1] = __floats2half2_rn(a.z, a.w);
+            h[2] = __floats2half2_rn(b.x, b.y);
+            h[3] = __floats2half2_rn(b.z, b.w);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) h[k] = __floats2half2_rn(src[2 * k], src[2 * k + 1]);
+        }
+    }
+    return w;
+}
+
+__device__ __forceinline__ void sts128(uint32_t at, uint4 v)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// A unit's codes (64 keys from key0) into registers; keys past the cache are zeros.
+template <int D>
+__device__ __forceinline__ void load_unit(const AttendParams &p, const int8_t *head, int64_t key0, int tid,
+                                          uint4 (&buf)[CL<D>::n_ld])
+{
+    const uint4 *src = reinterpret_cast<const uint4 *>(head + key0 * D);
+#pragma unroll
+    for (int j = 0; j < CL<D>::n_ld; j++) {
+        const int i = tid + 128 * j;
+        buf[j] = key0 + i / (D / 16) < p.c.rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+    }
+}
+
+// The same codes as F16 in the swizzled layout: row r of box b at r * 128, its
+// 16-byte chunk j at (j ^ (r & 7)) * 16.  16 codes are two chunks; half of the
+// lanes store their second one first, so 8 lanes fall on different banks.
+template <int D>
+__device__ __forceinline__ void store_unit(uint32_t tile, int tid, const uint4 (&buf)[CL<D>::n_ld])
+{
+#pragma unroll
+    for (int j = 0; j < CL<D>::n_ld; j++) {
+        const int i = tid + 128 * j, r = i / (D / 16), c = i % (D / 16);
+        const uint2 a = codes_to_half4(buf[j].x), b = codes_to_half4(buf[j].y), e = codes_to_half4(buf[j].z),
+                    f = codes_to_half4(buf[j].w);
+        const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(e.x, e.y, f.x, f.y);
+        const uint32_t row = tile + (c >> 2) * CL<D>::box + r * 128;
+        const int ch = 2 * (c & 3), flip = (c >> 2) & 1;
+        sts128(row + (((ch + flip) ^ (r & 7)) << 4), flip ? hi : lo);
+        sts128(row + (((ch + 1 - flip) ^ (r & 7)) << 4), flip ? lo : hi);
+    }
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+__device__ __forceinline__ uint64_t pk2(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ float2 up2(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ float max32(const uint32_t *v)
+{
+    float m[4];
+#pragma unroll
+    for (int a = 0; a < 4; a++) m[a] = fmaxf(__uint_as_float(v[a]), __uint_as_float(v[4 + a]));
+#pragma unroll
+    for (int e = 8; e < 32; e += 8)
+#pragma unroll
+        for (int a = 0; a < 4; a++) m[a] = max3(m[a], __uint_as_float(v[e + a]), __uint_as_float(v[e + 4 + a]));
+    return max3(m[0], m[1], fmaxf(m[2], m[3]));
+}
+
+__device__ __forceinline__ bool bad_scale(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+
+// v[e] = v[e] * scale of its block + mask (natural units); a key masked with -inf stays out whatever v holds
+__device__ __forceinline__ void add_mask(const AttendParams &p, int tok, int64_t kb, int nvis, float sc0, float sc1,
+                                         uint32_t (&v)[64])
+{
+    const int64_t base = (int64_t)tok * p.mask_stride + kb;
+#pragma unroll 1
+    for (int q = 0; q < 4; q++) {
+        float m[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            m[e] = -CUDART_INF_F;
+            if (16 * q + e < nvis)
+                m[e] = p.mask_f16 ? __half2float(static_cast<const __half *>(p.mask)[base + 16 * q + e])
+                                  : static_cast<const float *>(p.mask)[base + 16 * q + e];
+        }
+        const float sc = q < 2 ? sc0 : sc1;
+#pragma unroll
+        for (int qq = 0; qq < 4; qq++) {
+            if (qq != q) continue;
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                v[16 * qq + e] = __float_as_uint(m[e] == -CUDART_INF_F ? m[e] : __fmaf_rn(__uint_as_float(v[16 * qq + e]), sc, m[e]));
+        }
+    }
+}
+
+__device__ __forceinline__ void store_out4(const AttendParams &p, int64_t i, float4 x)
+{
+    if (p.out_f16) {
+        __half *dst = static_cast<__half *>(p.out) + i;
+        const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+        if (p.out_vec) {
+            *reinterpret_cast<uint2 *>(dst) =
+                make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+        } else {
+            dst[0] = __low2half(a);
+            dst[1] = __high2half(a);
+            dst[2] = __low2half(b);
+            dst[3] = __high2half(b);
+        }
+    } else {
+        float *dst = static_cast<float *>(p.out) + i;
+        if (p.out_vec) {
+            *reinterpret_cast<float4 *>(dst) = x;
+        } else {
+            dst[0] = x.x;
+            dst[1] = x.y;
+            dst[2] = x.z;
+            dst[3] = x.w;
+        }
+    }
+}
+
+__device__ __forceinline__ float inverse_sum(float l, bool flash)
+{
+    return l == 0.0f ? (flash ? 0.0f : CUDART_NAN_F) : 1.0f / l;
+}
+
+// what the weights' pass reads of a row: weight = 2^((t - m) * unit) * y
+__device__ __forceinline__ float2 row_stat_of(float m, float l)
+{
+    return l > 0.0f && l < CUDART_INF_F && m < CUDART_INF_F ? make_float2(m, 1.0f / l) : make_float2(0.0f, 0.0f);
+}
+
+template <int D, bool MASKED>
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p)
+{
+    using L = CL<D>;
+    constexpr int KS = L::KS, VS = L::VS;
+    constexpr uint32_t kTmO = 256;   // TMEM column of O_A (O_B at + D); S buffers: g * 128 + {0, 64}
+    extern __shared__ __align__(1024) unsigned char smem[];
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::o_bar);
+    uint64_t *q_full = bar, *q_empty = bar + 1;
+    uint64_t *k_full = bar + 2, *k_empty = k_full + KS;
+    uint64_t *v_full = k_empty + KS, *v_empty = v_full + VS;
+    uint64_t *s_full = v_empty + VS, *p_full = s_full + 4, *o_ready = p_full + 4;   // [tile][buffer]
+    uint64_t *o_full = o_ready + 4, *o_empty = o_full + 1, *drain = o_empty + 1;
+    uint32_t *tm_slot = reinterpret_cast<uint32_t *>(smem + L::o_tm);
+    volatile int *flag = reinterpret_cast<volatile int *>(smem + L::o_tm + 8);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
+
+    if (tid == 0) {
+        for (int i = 0; i < L::n_bar; i++) {
+            const uint64_t *b = &bar[i];
+            const bool staged = b == q_full || (b >= k_full && b < k_full + KS) || (b >= v_full && b < v_full + VS);
+            const bool both = b == q_empty || (b >= k_empty && b < k_empty + KS);   // both S issuers
+            mbar_init(&bar[i], staged || (b >= p_full && b < p_full + 4) ? 4 : b == o_empty ? 8 : both ? 2 : 1);
+        }
+        *flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 3) {
+        tmem_alloc(tm_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tm_slot;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    Walk w;
+    if (warp < 4) {
+        regs_dec<56>();
+        if (lane == 0 && warp < 3) {
+            constexpr uint32_t idS = idesc_f16_f32(128, kSub, false), idO = idesc_f16_f32(128, D, true);
+            const uint32_t sq = smem_addr(smem + L::o_q), sk = smem_addr(smem + L::o_k), sv = smem_addr(smem + L::o_v);
+            auto wait = [&](uint64_t *b, uint32_t par) {
+                if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
+                give_up(flag, 1u);
+                return false;
+            };
+            int i = 0;   // sub-tiles of the CTA so far
+            bool ok = true;
+            w.begin(p, cta);
+            if (warp < 2) {
+                const int g = warp;
+                int n = 0;   // sub-tiles of tile g so far
+                for (int seg = 0; ok && w.more(); seg++, w.next_pair(p)) {
+                    const bool active = g < tiles_of(p, w.pair % p.n_blk);
+                    if (active && !(ok = wait(q_full, seg & 1))) break;
+                    for (int t = w.t0; t < w.t1; t++, i++) {
+                        const int s = i % KS;
+                        if (!(ok = wait(&k_full[s], (i / KS) & 1))) break;
+                        if (!active) {   // (in step with the other tile's issuer)
+                            mbar_arrive(&k_empty[s]);
+                            if (t == w.t1 - 1) mbar_arrive(q_empty);
+                            continue;
+                        }
+                        // the buffer is free once the product that read its weights is done
+                        if (n >= 2 && !(ok = wait(&o_ready[g * 2 + (n & 1)], ((n - 2) >> 1) & 1))) break;
+                        tc_fence_after();
+                        const uint32_t kt = sk + s * L::tile;
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; kk++)
+                            umma_ss(tmem + g * 128 + (n & 1) * 64,
+                                    sdesc_k_sw128(sq + g * L::q_tile + (kk >> 2) * 16384 + (kk & 3) * 32),
+                                    sdesc_k_sw128(kt + (kk >> 2) * L::box + (kk & 3) * 32), idS, kk > 0);
+                        umma_commit(&s_full[g * 2 + (n & 1)]);
+                        umma_commit(&k_empty[s]);
+                        if (t == w.t1 - 1) umma_commit(q_empty);
+                        n++;
+                    }
+                }
+            } else {
+                int n[2] = {0, 0};
+                for (int seg = 0; ok && w.more(); seg++, w.next_pair(p)) {
+                    const int nt = tiles_of(p, w.pair % p.n_blk);
+                    for (int t = w.t0; ok && t < w.t1; t++, i++) {
+                        const int s = i % VS;
+                        if (!(ok = wait(&v_full[s], (i / VS) & 1))) break;
+                        if (t == w.t0 && seg > 0 && !(ok = wait(o_empty, (seg - 1) & 1))) break;
+#pragma unroll
+                        for (int g = 0; g < L::NT; g++) {
+                            if (g >= nt) continue;
+                            if (!(ok = wait(&p_full[g * 2 + (n[g] & 1)], (n[g] >> 1) & 1))) break;
+                            tc_fence_after();
+                            const uint32_t vt = sv + s * L::tile;
+#pragma unroll
+                            for (int kk = 0; kk < kSub / 16; kk++)   // 16 keys a step: 8 columns of F16 pairs
+                                umma_ts(tmem + kTmO + g * D, tmem + g * 128 + (n[g] & 1) * 64 + kk * 8,
+                                        sdesc_mn_sw128(vt + kk * 2048, L::box), idO, !(t == w.t0 && kk == 0));
+                            umma_commit(&o_ready[g * 2 + (n[g] & 1)]);
+                            n[g]++;
+                        }
+                        if (!ok) break;
+                        umma_commit(&v_empty[s]);
+                        if (t == w.t1 - 1) umma_commit(o_full);
+                    }
+                }
+            }
+            // every MMA of this thread has completed before TMEM is freed
+            umma_commit(&drain[warp]);
+            mbar_wait(&drain[warp], 0, kLimitNs);
+        }
+    } else if (warp < 8) {
+        regs_dec<120>();
+        const int st = tid - 128;
+        auto wait = [&](uint64_t *b, uint32_t par) {
+            // (one answer for the warp: its lanes arrive together)
+            const bool got = mbar_wait_ab(b, par, kLimitNs, flag);
+            if (!__all_sync(0xffffffffu, got)) {
+                give_up(flag, 2u);
+                return false;
+            }
+            return true;
+        };
+        const uint32_t sk = smem_addr(smem + L::o_k), sv = smem_addr(smem + L::o_v);
+        uint4 buf[L::PF][L::n_ld];
+        Walk f;   // the units being fetched: K then V of each sub-tile
+        f.begin(p, cta);
+        bool fv = false;
+        auto fetch = [&](uint4 (&b)[L::n_ld]) {
+            if (!f.more()) return;
+            const int8_t *head = (fv ? p.c.v : p.c.k) + (int64_t)(f.pair / p.n_blk) * p.c.rows * D;
+            load_unit<D>(p, head, (int64_t)f.t * kSub, st, b);
+            if (fv && ++f.t == f.t1) f.next_pair(p);
+            fv = !fv;
+        };
+#pragma unroll
+        for (int u = 0; u < L::PF; u++) fetch(buf[u]);
+        w.begin(p, cta);
+        int i = 0, seg = 0;
+        bool ok = true, first = true;
+        while (ok && w.more()) {
+#pragma unroll
+            for (int u = 0; u < L::PF; u += 2) {
+                if (!ok || !w.more()) break;
+                if (first) {   // a segment's queries
+                    const int h = w.pair / p.n_blk, b = w.pair % p.n_blk;
+                    if (seg > 0 && !(ok = wait(q_empty, (seg - 1) & 1))) break;
+                    const int nt = tiles_of(p, b);
+                    for (int g = 0; g < nt; g++) {
+                        const int tok0 = b * p.tok_blk + g * p.tok_tile;
+                        const uint32_t dst = smem_addr(smem + L::o_q) + g * L::q_tile;
+#pragma unroll 8
+                        for (int x = st; x < 128 * (D / 8); x += 128) {
+                            const int row = x / (D / 8), c = x % (D / 8);
+                            const int tk = row / p.r, t = tok0 + tk;
+                            uint4 v = make_uint4(0, 0, 0, 0);
+                            if (tk < p.tok_tile && t < p.n_new) v = load_q8(p, t, h * p.r + row - tk * p.r, D, c * 8);
+                            sts128(dst + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), v);
+                        }
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(q_full);
+                    first = false;
+                }
+                {
+                    const int s = i % KS;
+                    if (i >= KS && !(ok = wait(&k_empty[s], (i / KS - 1) & 1))) break;
+                    store_unit<D>(sk + s * L::tile, st, buf[u]);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&k_full[s]);
+                    fetch(buf[u]);
+                }
+                {
+                    const int s = i % VS;
+                    if (i >= VS && !(ok = wait(&v_empty[s], (i / VS - 1) & 1))) break;
+                    store_unit<D>(sv + s * L::tile, st, buf[u + 1]);
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_full[s]);
+                    fetch(buf[u + 1]);
+                }
+                i++;
+                if (++w.t == w.t1) {
+                    w.next_pair(p);
+                    seg++;
+                    first = true;
+                }
+            }
+        }
+    } else {
+        regs_inc<168>();
+        const int g = (warp - 8) >> 2, q4 = warp & 3;
+        const int row = q4 * 32 + lane;   // of the tile
+        const uint32_t lanes = (uint32_t)(q4 * 32) << 16;
+        const uint32_t tS = tmem + lanes + g * 128, tO = tmem + lanes + kTmO + g * D;
+        const int tok_in = row / p.r, hd = row - tok_in * p.r;
+        auto wait = [&](uint64_t *b, uint32_t par) {
+            if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
+            give_up(flag, 4u);
+            return false;
+        };
+        const int64_t n_sc = p.c.rows / kBlock;
+        int n = 0;
+        bool ok = true;
+        w.begin(p, cta);
+        for (int seg = 0; ok && w.more(); seg++, w.next_pair(p)) {
+            const int h = w.pair / p.n_blk, b = w.pair % p.n_blk;
+            if (g >= tiles_of(p, b)) {   // no rows in this tile: keep step with the other one
+                ok = __all_sync(0xffffffffu, wait(o_full, seg & 1));
+                if (ok && lane == 0) mbar_arrive(o_empty);
+                continue;
+            }
+            const int tok = b * p.tok_blk + g * p.tok_tile + tok_in;
+            const bool valid = tok_in < p.tok_tile && tok < p.n_new;
+            const int64_t lim = !valid ? -1 : MASKED ? p.n_kv - 1 : p.n_past + tok;   // the last key it may see
+            const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.c.k_scale) + h * n_sc;
+            const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.c.v_scale) + h * n_sc;
+            float m = -CUDART_INF_F, me = 0.0f, l = 0.0f, bad = 0.0f;
+            // a sub-tile's scale words, one sub-tile ahead (the last block of a cache may be the first of the two)
+            uint32_t kw[2], vw[2];
+            auto scales = [&](int t) {
+                const int64_t i0 = min(2 * (int64_t)t, n_sc - 1), i1 = min(2 * (int64_t)t + 1, n_sc - 1);
+                kw[0] = __ldg(ksc + i0);
+                kw[1] = __ldg(ksc + i1);
+                vw[0] = __ldg(vsc + i0);
+                vw[1] = __ldg(vsc + i1);
+            };
+            scales(w.t0);
+            const int n0 = n;
+            for (int t = w.t0; t < w.t1; t++, n++) {
+                const int bf = n & 1;
+                const uint32_t k0 = kw[0], k1 = kw[1], v0 = vw[0], v1 = vw[1];
+                if (t + 1 < w.t1) scales(t + 1);
+                if (!(ok = __all_sync(0xffffffffu, wait(&s_full[g * 2 + bf], (n >> 1) & 1)))) break;
+                tc_fence_after();
+                uint32_t v[64];
+                tmem_ld32(tS + bf * 64, *reinterpret_cast<uint32_t(*)[32]>(v));
+                tmem_ld32(tS + bf * 64 + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+                tmem_wait_ld();
+                const int64_t kb = (int64_t)t * kSub;
+                const int nvis = (int)max((int64_t)0, min((int64_t)kSub, lim - kb + 1));
+                const bool k_bad = bad_scale(k0) || bad_scale(k1);
+                if (k_bad) {   // visible keys of such a block are NaN
+#pragma unroll
+                    for (int e = 0; e < 64; e++)
+                        if (bad_scale(e < 32 ? k0 : k1)) v[e] = 0x7fc00000u;
+                }
+                if (!MASKED && !__all_sync(0xffffffffu, nvis == 64)) {
+#pragma unroll
+                    for (int e = 0; e < 64; e++)
+                        if (e >= nvis) v[e] = __float_as_uint(-CUDART_INF_F);
+                }
+                const float ev0 = (float)scale_exp(v0), ev1 = (float)scale_exp(v1);
+                float c0 = p.scale * pow2(scale_exp(k0)), c1 = p.scale * pow2(scale_exp(k1));
+                float f = 1.0f;
+                bool moved = false;
+                uint64_t s0 = 0ull, s1 = 0ull;
+                if constexpr (MASKED) {
+                    add_mask(p, valid ? tok : 0, kb, nvis, c0, c1, v);
+                    const float x0 = max32(v), x1 = max32(v + 32);
+                    // the block whose top counts for more
+                    const bool second = x0 == -CUDART_INF_F || (x1 - x0) * kLog2e + (ev1 - ev0) > 0.0f;
+                    const float top = second ? x1 : x0, tev = second ? ev1 : ev0;
+                    if (top > -CUDART_INF_F && (m == -CUDART_INF_F || __fmaf_rn(top - m, kLog2e, tev - me) > kTop)) {
+                        if (m > -CUDART_INF_F) {
+                            f = ex2_approx(__fmaf_rn(m - top, kLog2e, me - (tev - kBias)));
+                            moved = true;
+                        }
+                        m = top;
+                        me = tev - kBias;
+                    }
+                    if ((bad_scale(v0) && x0 > -CUDART_INF_F) || (bad_scale(v1) && x1 > -CUDART_INF_F)) bad = CUDART_NAN_F;
+                    const float mm = m == -CUDART_INF_F ? 0.0f : m;
+                    // (its own loop: the difference is taken before the exponent is added)
+                    float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        uint32_t pkd[16];
+                        const float up = (u ? ev1 : ev0) - me;
+                        float a = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const float y0 = ex2_approx(__fmaf_rn(__uint_as_float(v[u * 32 + 2 * e]) - mm, kLog2e, up));
+                            const float y1 = ex2_approx(__fmaf_rn(__uint_as_float(v[u * 32 + 2 * e + 1]) - mm, kLog2e, up));
+                            a += y0 + y1;
+                            const __half2 h2 = __floats2half2_rn(y0, y1);
+                            pkd[e] = *reinterpret_cast<const uint32_t *>(&h2);
+                        }
+                        if (u) a1 = a;
+                        else a0 = a;
+                        tmem_st16(tS + bf * 64 + u * 16, pkd);
+                    }
+                    l = __fmaf_rn(a1, pow2(-(int)ev1), __fmaf_rn(a0, pow2(-(int)ev0), l * f));
+                } else {
+                    c0 *= kLog2e;
+                    c1 *= kLog2e;
+                    const float x0 = max32(v), x1 = max32(v + 32);
+                    const float z = fmaxf(__fmaf_rn(x0, c0, ev0), __fmaf_rn(x1, c1, ev1));
+                    if (z > m + kTop) {   // (never without a visible key: z = -inf)
+                        f = ex2_approx(m - (z - kBias));   // 0 while m = -inf
+                        moved = m != -CUDART_INF_F;
+                        m = z - kBias;
+                    }
+                    if ((bad_scale(v0) && x0 > -CUDART_INF_F) || (bad_scale(v1) && x1 > -CUDART_INF_F)) bad = CUDART_NAN_F;
+                    const float ref = m == -CUDART_INF_F ? 0.0f : m;
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        uint32_t pkd[16];
+                        const uint64_t c2 = u ? pk2(c1, c1) : pk2(c0, c0), a2 = u ? pk2(ev1 - ref, ev1 - ref) : pk2(ev0 - ref, ev0 - ref);
+                        uint64_t sum = 0ull;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const float2 xy = up2(fma2(pk2(__uint_as_float(v[u * 32 + 2 * e]), __uint_as_float(v[u * 32 + 2 * e + 1])), c2, a2));
+                            const float y0 = ex2_approx(xy.x), y1 = ex2_approx(xy.y);
+                            sum = add2(sum, pk2(y0, y1));
+                            const __half2 h2 = __floats2half2_rn(y0, y1);
+                            pkd[e] = *reinterpret_cast<const uint32_t *>(&h2);
+                        }
+                        if (u) s1 = sum;
+                        else s0 = sum;
+                        tmem_st16(tS + bf * 64 + u * 16, pkd);
+                    }
+                    const float2 a0 = up2(s0), a1 = up2(s1);
+                    l = __fmaf_rn(a1.x + a1.y, pow2(-(int)ev1), __fmaf_rn(a0.x + a0.y, pow2(-(int)ev0), l * f));
+                }
+                // O holds the segment's earlier sub-tiles: scaled once the last product into it is done
+                if (n > n0 && __any_sync(0xffffffffu, moved)) {
+                    if (!(ok = __all_sync(0xffffffffu, wait(&o_ready[g * 2 + ((n - 1) & 1)], ((n - 1) >> 1) & 1)))) break;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int ch = 0; ch < D / 16; ch++) {
+                        uint32_t o[16];
+                        tmem_ld16(tO + ch * 16, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        tmem_st16(tO + ch * 16, o);
+                    }
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[g * 2 + bf]);
+            }
+            if (!ok || !(ok = __all_sync(0xffffffffu, wait(o_full, seg & 1)))) break;
+            tc_fence_after();
+            const bool whole = w.whole();
+            const int64_t at = ((int64_t)cta + w.pair) * (128 * L::NT) + g * 128 + row;   // (CTA, pair) in order: their sum counts them
+            float scl = 1.0f;
+            if constexpr (MASKED) {   // both sums relative to e^m alone
+                scl = pow2((int)me);
+                l *= scl;
+            }
+            if (whole) scl *= inverse_sum(l, p.flash != 0);
+            if (valid) {
+                if (!whole) p.stat[at] = make_float2(m, l);
+                else if (p.row_stat) p.row_stat[(int64_t)h * p.n_new * p.r + (int64_t)tok * p.r + hd] = row_stat_of(m, l);
+            }
+            const int64_t dst = (int64_t)tok * p.out_stride + (int64_t)(h * p.r + hd) * D;
+            const uint64_t pol = policy_evict_last();   // a cut pair's rows stay in L2 for the fold
+#pragma unroll 1
+            for (int ch = 0; ch < D / 32; ch++) {
+                uint32_t o[32];
+                tmem_ld32(tO + ch * 32, o);
+                tmem_wait_ld();
+                if (!valid) continue;
+#pragma unroll
+                for (int q = 0; q < 8; q++) {
+                    const float4 x = make_float4(__fmaf_rn(__uint_as_float(o[4 * q]), scl, bad), __fmaf_rn(__uint_as_float(o[4 * q + 1]), scl, bad),
+                                                 __fmaf_rn(__uint_as_float(o[4 * q + 2]), scl, bad), __fmaf_rn(__uint_as_float(o[4 * q + 3]), scl, bad));
+                    if (whole) store_out4(p, dst + ch * 32 + 4 * q, x);
+                    else st_v4_hint(p.part + at * D + ch * 32 + 4 * q, x, pol);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(o_empty);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 3) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the pairs cut between CTAs, a warp a query row; row_stat of their rows.
+template <int D, bool MASKED>
+__global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
+{
+    constexpr int rows_blk = 128 * CL<D>::NT;
+    constexpr float unit = MASKED ? kLog2e : 1.0f;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch_dependents();
+    const int pair = blockIdx.x / (rows_blk / 8), in = blockIdx.x % (rows_blk / 8) * 8 + warp;
+    const int h = pair / p.n_blk, b = pair % p.n_blk, tk = (in & 127) / p.r, hd = (in & 127) - tk * p.r;
+    const int tok = b * p.tok_blk + (in >> 7) * p.tok_tile + tk;
+    const int64_t W = p.c.H * p.subs, x0 = pair_start(p, pair), x1 = x0 + subs_of(p, b) - 1;
+    const int c0 = (int)(((x0 + 1) * p.n_cta - 1) / W), c1 = (int)(((x1 + 1) * p.n_cta - 1) / W);
+    pdl_wait();
+    if (c0 == c1 || tk >= p.tok_tile || tok >= p.n_new) return;
+    float M = -CUDART_INF_F;
+    for (int c = c0; c <= c1; c++) M = fmaxf(M, p.stat[((int64_t)c + pair) * rows_blk + in].x);
+    const float ref = M == -CUDART_INF_F ? 0.0f : M;
+    constexpr int V = (D / 4 + 31) / 32;
+    float4 x[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) x[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float l = 0.0f;
+#pragma unroll 4
+    for (int c = c0; c <= c1; c++) {
+        const int64_t at = ((int64_t)c + pair) * rows_blk + in;
+        const float2 s = p.stat[at];
+        const float f = ex2_approx((s.x - ref) * unit);
+        l = __fmaf_rn(s.y, f, l);
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            if (lane + 32 * v >= D / 4) continue;
+            const float4 y = __ldcg(reinterpret_cast<const float4 *>(p.part + at * D) + lane + 32 * v);
+            x[v].x = __fmaf_rn(y.x, f, x[v].x);
+            x[v].y = __fmaf_rn(y.y, f, x[v].y);
+            x[v].z = __fmaf_rn(y.z, f, x[v].z);
+            x[v].w = __fmaf_rn(y.w, f, x[v].w);
+        }
+    }
+    const float z = inverse_sum(l, p.flash != 0);
+    const int64_t dst = (int64_t)tok * p.out_stride + (int64_t)(h * p.r + hd) * D;
+#pragma unroll
+    for (int v = 0; v < V; v++)
+        if (lane + 32 * v < D / 4)
+            store_out4(p, dst + (lane + 32 * v) * 4, make_float4(x[v].x * z, x[v].y * z, x[v].z * z, x[v].w * z));
+    if (lane == 0 && p.row_stat) p.row_stat[(int64_t)h * p.n_new * p.r + (int64_t)tok * p.r + hd] = row_stat_of(M, l);
+}
+
+template <class K>
+cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, const AttendParams &p, cudaStream_t st)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int D, bool MASKED>
+cudaError_t run(const AttendParams &p, cudaStream_t st)
+{
+    using L = CL<D>;
+    static Once once;
+    cudaError_t e = once.on_device([] {
+        return cudaFuncSetAttribute(chunk_kernel<D, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::bytes);
+    });
+    if (e == cudaSuccess) e = launch_pdl(chunk_kernel<D, MASKED>, p.n_cta, kThreads, L::bytes, p, st);
+    if (e != cudaSuccess) return e;
+    // every pair in one CTA: as many CTAs as pairs of equal length, or one CTA
+    if (p.n_cta == 1 || (p.n_blk == 1 && p.c.H % p.n_cta == 0)) return cudaSuccess;
+    return launch_pdl(fold_kernel<D, MASKED>, (unsigned)p.n_vh * (128 * L::NT / 8), 256, 0, p, st);
+}
+
+}  // namespace
+
+void chunk_split(AttendParams &p)
+{
+    p.n_tile = p.c.D == 256 ? 1 : 2;
+    p.tok_tile = 128 / p.r;
+    p.tok_blk = p.n_tile * p.tok_tile;
+    p.n_blk = (p.n_new + p.tok_blk - 1) / p.tok_blk;
+    p.n_vh = p.c.H * p.n_blk;
+    p.subs = 0;
+    for (int b = 0; b < p.n_blk; b++) {
+        const int64_t last = p.mask ? p.n_kv : p.n_past + std::min<int64_t>(p.n_new, (int64_t)(b + 1) * p.tok_blk);
+        p.subs += (last + kSub - 1) / kSub;
+    }
+    p.n_cta = (int)std::min<int64_t>(kSMs, p.c.H * p.subs);
+}
+
+cudaError_t launch_chunk(const AttendParams &p, cudaStream_t st)
+{
+    switch (p.c.D) {
+    case 64: return p.mask ? run<64, true>(p, st) : run<64, false>(p, st);
+    case 96: return p.mask ? run<96, true>(p, st) : run<96, false>(p, st);
+    case 128: return p.mask ? run<128, true>(p, st) : run<128, false>(p, st);
+    case 256: return p.mask ? run<256, true>(p, st) : run<256, false>(p, st);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+cudaError_t take_error(unsigned *word)
+{
+    cudaError_t e = cudaMemcpyFromSymbol(word, g_error, sizeof(unsigned));
+    if (e == cudaSuccess && *word) {
+        const unsigned zero = 0;
+        e = cudaMemcpyToSymbol(g_error, &zero, sizeof(unsigned));
+    }
+    return e;
+}
+
+}  // namespace q8
+}  // namespace kvb

@@ -184,8 +184,21 @@ int kv_q8_attend(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32
     p.out = out;
     p.out_stride = n_new > 1 ? out_stride : 0;
     p.out_f16 = out_type == KV_F16;
+    p.out_vec = vec_ok(out, p.out_stride, out_type);
     p.scale = 1.0f / sqrtf((float)p.c.D);
     return cuda_rc(kvb::q8::launch_attend(p, workspace, static_cast<cudaStream_t>(stream)), what);
+}
+
+int kv_q8_status(void *stream)
+{
+    const char *what = "kv_q8_status";
+    int rc = cuda_rc(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)), what);
+    unsigned word = 0;
+    if (rc == KV_OK) rc = cuda_rc(kvb::q8::take_error(&word), what);
+    if (rc == KV_OK && word)
+        return fail(KV_E_TIMEOUT, "%s: a wait in an attention kernel expired (bits 0x%x); its outputs are not valid", what,
+                    word);
+    return rc;
 }
 
 int kv_q8_evict(const kv_q8_cache *src, int64_t n_rows, int64_t keep, int64_t recent,

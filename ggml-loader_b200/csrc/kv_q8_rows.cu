@@ -19,7 +19,6 @@
 #include <math_constants.h>
 
 #include <algorithm>
-#include <atomic>
 
 #include "kv_internal.h"
 #include "kv_q8.cuh"
@@ -174,8 +173,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
         const int vh = (int)(pos / p.nb), b0 = (int)(pos - (int64_t)vh * p.nb);
         const int b1 = (int)min((int64_t)p.nb, b0 + hi - pos);
         pos += b1 - b0;
-        const int h = vh / p.n_tile, row0 = (vh - h * p.n_tile) * 16;   // (HILO: one tile)
-        const int nrows = min(HILO ? 8 : 16, p.n_new * p.r - row0);
+        const int h = vh, nrows = p.n_new * p.r;   // (at most 8 with HILO, else 16)
         const int8_t *kc = p.c.k + (int64_t)h * p.c.rows * D, *vc = p.c.v + (int64_t)h * p.c.rows * D;
         const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)h * (p.c.rows / kBlock);
         const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.c.v_scale) + (int64_t)h * (p.c.rows / kBlock);
@@ -187,8 +185,8 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
         int tok[RT];
 #pragma unroll
         for (int i = 0; i < RT; i++) {
-            const int row = row0 + g + 8 * i;
-            const bool have = g + 8 * i < nrows;
+            const int row = g + 8 * i;
+            const bool have = row < nrows;
             tok[i] = have ? row / p.r : 0;
             if constexpr (G::q_regs) {
                 const int hq = h * p.r + (have ? row % p.r : 0);
@@ -200,7 +198,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
         if constexpr (!G::q_regs) {
             for (int i = threadIdx.x; i < 8 * RT * (D / 4); i += G::W * 32) {
                 const int row = i / (D / 4), c = i % (D / 4);
-                s_q[row][c] = row < nrows ? load_q4(p, (row0 + row) / p.r, h * p.r + (row0 + row) % p.r, D, c * 4)
+                s_q[row][c] = row < nrows ? load_q4(p, row / p.r, h * p.r + row % p.r, D, c * 4)
                                           : make_uint2(0, 0);
             }
         }
@@ -429,7 +427,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
             }
             if (whole) {
                 const float z = inverse_sum(l, p.flash != 0);
-                const int t = (row0 + row) / p.r, j = (row0 + row) % p.r;
+                const int t = row / p.r, j = row % p.r;
                 const int64_t at = t * p.out_stride + (int64_t)(h * p.r + j) * D + c;
                 store_out(p, at, x.x * z);
                 store_out(p, at + 1, x.y * z);
@@ -444,7 +442,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
     }
 }
 
-// The CTAs of virtual head vh (the split of rows_kernel).
+// The CTAs of head vh (the split of rows_kernel).
 __device__ __forceinline__ void span_of(const AttendParams &p, int vh, int &a, int &b)
 {
     const int64_t T = (int64_t)p.n_vh * p.nb, x0 = (int64_t)vh * p.nb, x1 = x0 + p.nb - 1;
@@ -453,7 +451,7 @@ __device__ __forceinline__ void span_of(const AttendParams &p, int vh, int &a, i
     b = (int)(((x1 + 1) * p.n_cta - 1) / T);
 }
 
-// Joins the CTAs' partial rows: one CTA a (virtual head, row); with weights,
+// Joins the CTAs' partial rows: one CTA a (head, row); with weights,
 // CTAs behind those add the softmax weights of 512 keys of a head.
 template <int D, bool MASKED>
 __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
@@ -466,12 +464,11 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
     if ((int)blockIdx.x < n_join) {
         __shared__ float4 s_o[4][D / 4];
         __shared__ float2 s_ml[4];
-        const int vh = blockIdx.x >> 4, row = blockIdx.x & 15;
-        const int h = vh / p.n_tile, row0 = (vh - h * p.n_tile) * 16;
-        if (row0 + row >= p.n_new * p.r) return;
+        const int vh = blockIdx.x >> 4, h = vh, row = blockIdx.x & 15;
+        if (row >= p.n_new * p.r) return;
         int a, b;
         span_of(p, vh, a, b);
-        if (a == b && !p.row_stat) return;   // rows_kernel wrote the output
+        if (a == b) return;   // rows_kernel wrote the output
         // each warp a quarter of the parts, then the four
         float M = -CUDART_INF_F;
         for (int c = a + lane; c <= b; c += 32) M = fmaxf(M, p.stat[((int64_t)c + vh) * 16 + row].x);
@@ -489,7 +486,6 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
             const float2 s = p.stat[at];
             const float f = ex2_approx((s.x - ref) * unit);
             l = __fmaf_rn(s.y, f, l);
-            if (a == b) continue;
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 if (lane + 32 * v >= D / 4) continue;
@@ -506,14 +502,8 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
         if (lane == 0) s_ml[warp] = make_float2(M, l);
         __syncthreads();
         l = (s_ml[0].y + s_ml[1].y) + (s_ml[2].y + s_ml[3].y);
-        if (p.row_stat && tid == 0) {
-            const bool adds = l > 0.0f && l < CUDART_INF_F && M < CUDART_INF_F;
-            p.row_stat[(int64_t)h * p.n_new * p.r + row0 + row] =
-                adds ? make_float2(MASKED ? M : M / kLog2e, 1.0f / l) : make_float2(0.0f, 0.0f);
-        }
-        if (a == b) return;
         const float z = inverse_sum(l, p.flash != 0);
-        const int t = (row0 + row) / p.r, j = (row0 + row) % p.r;
+        const int t = row / p.r, j = row % p.r;
         const int64_t at = t * p.out_stride + (int64_t)(h * p.r + j) * D;
         for (int d = tid; d < D; d += 128) {
             const float *o0 = reinterpret_cast<const float *>(s_o);
@@ -574,23 +564,6 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
         if (key + i < p.n_kv) dst[i] += sum[i];
 }
 
-// Runs a function once a device (a kernel's attributes last); devices past 63 run it every time.
-struct Once {
-    std::atomic<uint64_t> done{0};
-    template <class F>
-    cudaError_t on_device(F &&f)
-    {
-        int dev = 0;
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) return e;
-        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-        if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
-        e = f();
-        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
-        return e;
-    }
-};
-
 template <class K>
 cudaError_t launch_pdl(K kernel, unsigned grid, unsigned block, size_t smem, const AttendParams &p, cudaStream_t st)
 {
@@ -618,7 +591,7 @@ cudaError_t run(const AttendParams &p, cudaStream_t st)
     if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, HILO, MASKED>, p.n_cta, G::W * 32, G::smem, p, st);
     if (e != cudaSuccess) return e;
     const bool split = p.n_cta > p.n_vh || p.n_vh % p.n_cta != 0;   // else every head lies in one CTA
-    if (!split && !p.scores && !p.row_stat) return cudaSuccess;
+    if (!split && !p.scores) return cudaSuccess;
     unsigned grid = (unsigned)p.n_vh * 16;
     if (p.scores) grid += (unsigned)(p.c.H * (((int64_t)p.nb * kBlock + 511) / 512));
     return launch_pdl(join_kernel<D, MASKED>, grid, 128, 0, p, st);
@@ -639,9 +612,8 @@ cudaError_t run_d(const AttendParams &p, cudaStream_t st)
 // works on one head; 8 heads of 2000 keys: 63 CTAs 11.0 us, 64 CTAs 8.0 us).
 void rows_split(AttendParams &p)
 {
-    constexpr int kSMs = 148;
-    p.n_tile = (int)(((int64_t)p.n_new * p.r + 15) / 16);
-    p.n_vh = p.c.H * p.n_tile;
+    p.n_tile = 1;
+    p.n_vh = p.c.H;
     p.nb = (int)((p.n_kv + kBlock - 1) / kBlock);
     constexpr int W = 8;
     const int64_t T = (int64_t)p.n_vh * p.nb;

@@ -113,6 +113,7 @@ def lib():
         "kv_q8_attend": (ctypes.c_int, [_vp, _i32, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i64, ctypes.c_uint32,
                                         _vp, _i64, _i32, _vp, _u64, _vp]),
         "kv_q8_evict": (ctypes.c_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp]),
+        "kv_q8_status": (ctypes.c_int, [_vp]),
         "kv_status": (ctypes.c_int, [_vp, _vp]),
         "kv_debug_inject": (ctypes.c_int, [_vp, _i32, _u64]),
         "kv_rope_table_host": (ctypes.c_int, [cfgp, _i64, _i64, _vp]),
@@ -469,6 +470,11 @@ class Q8Cache:
             raise ValueError("attend needs a contiguous workspace tensor on the cache's device")
         return self._call(self._lib.kv_q8_attend, n_head, n_past, n_new, qp, qs, qt, mp, mt, ms, 1 if flash else 0,
                           op, os_, ot, workspace.data_ptr(), workspace.nbytes, _stream(stream))
+
+    def status(self, stream=None):
+        """KV_OK, or KV_E_TIMEOUT if a bounded device-side wait of an attend expired (raises)."""
+        with self._torch.cuda.device(self._index):
+            return _check(self._lib.kv_q8_status(_stream(stream)), "kv_q8_status")
 
     def evict(self, n_rows, keep, recent, dst, kept, stream=None):
         """kv_q8_evict into the Q8Cache dst; kept: int32 [n_head_kv][keep]."""

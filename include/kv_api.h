@@ -354,6 +354,12 @@ int kv_q8_attend(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32
                  void *out, int64_t out_stride, int32_t out_type,
                  void *workspace, uint64_t workspace_bytes, void *stream);
 
+/* Deferred device-side errors of kv_q8_attend on the current device, as
+ * kv_status: waits for `stream`, then returns KV_E_TIMEOUT (and clears the
+ * record) if a bounded wait inside one of its kernels expired since the last
+ * check (the outputs of that call are not valid), else KV_OK. */
+int kv_q8_status(void *stream);
+
 /*
  * Evict rows by accumulated attention weight.  Of the first n_rows rows of
  * `src`, each KV head keeps its last `recent` ones and, of those before, the
