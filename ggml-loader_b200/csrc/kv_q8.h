@@ -77,6 +77,8 @@ struct AttendParams {
     float2 *stat;           // [n_cta + n_vh][rows] their (maximum, sum)
     float *scores;          // [H][n_new * r][nb * kBlock] or null
     float2 *row_stat;       // [H][n_new * r] (maximum, 1 / sum or 0) or null
+    int32_t n_kt;           // weigh: tiles of 128 keys, ceil(n_kv / 128)
+    unsigned *error;        // the device's record of waits that expired
 };
 // bytes of workspace (a function of the sizes alone)
 uint64_t attend_workspace(const AttendParams &p);
@@ -88,7 +90,10 @@ cudaError_t launch_rows(const AttendParams &p, cudaStream_t st);
 // kv_q8_chunk.cu: the same for more than 16 query rows a KV head
 void chunk_split(AttendParams &p);
 cudaError_t launch_chunk(const AttendParams &p, cudaStream_t st);
-// the bits of device waits that expired since the last call (0: none)
+// kv_q8_weigh.cu: a chunk's softmax weights into the cache's accumulator
+cudaError_t launch_weigh(const AttendParams &p, cudaStream_t st);
+// the current device's record of waits that expired: its address, and its bits since the last call
+cudaError_t error_word(unsigned **dev);
 cudaError_t take_error(unsigned *word);
 
 // Runs a function once a device (a kernel's attributes last); devices past 63 run it every time.

@@ -33,13 +33,12 @@
 #include <algorithm>
 
 #include "kv_internal.h"
-#include "kv_q8.cuh"
-#include "kv_sm100.cuh"
+#include "kv_q8_stage.cuh"
 
 namespace kvb {
 namespace q8 {
 
-__device__ unsigned g_error;   // bits of waits that expired (kv_q8_status)
+__device__ unsigned g_error;
 
 namespace {
 
@@ -47,7 +46,6 @@ using namespace sm100;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kBias = 7.0f, kTop = 15.0f;   // as kv_q8_rows.cu: a new reference's weight is 2^7, it moves past 2^15
-constexpr uint64_t kLimitNs = 1000000000ull;
 constexpr int kThreads = 512;
 constexpr int kSub = 64;   // keys of a sub-tile
 
@@ -134,16 +132,6 @@ __device__ __forceinline__ int tiles_of(const AttendParams &p, int b)
     return p.n_tile == 2 && b * p.tok_blk + p.tok_tile < p.n_new ? 2 : 1;
 }
 
-__device__ __forceinline__ void give_up(volatile int *flag, unsigned bit)
-{
-    if (!*flag) {
-        atomicOr(&g_error, bit);
-        *flag = 1;
-    }
-}
-
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
 template <int N>
 __device__ __forceinline__ void regs_inc()
 {
@@ -153,48 +141,6 @@ template <int N>
 __device__ __forceinline__ void regs_dec()
 {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// four signed codes -> four halves in order (0x6400 | u is the half 1024 + u)
-__device__ __forceinline__ uint2 codes_to_half4(uint32_t w)
-{
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));
-    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 hx = __hsub2(*reinterpret_cast<__half2 *>(&x), off), hy = __hsub2(*reinterpret_cast<__half2 *>(&y), off);
-    return make_uint2(*reinterpret_cast<const uint32_t *>(&hx), *reinterpret_cast<const uint32_t *>(&hy));
-}
-
-// 8 query elements at d as F16
-__device__ __forceinline__ uint4 load_q8(const AttendParams &p, int t, int hq, int D, int d)
-{
-    const int64_t i = t * p.q_stride + (int64_t)hq * D + d;
-    uint4 w;
-    __half2 *h = reinterpret_cast<__half2 *>(&w);
-    if (p.q_f16) {
-        const __half *src = static_cast<const __half *>(p.q) + i;
-        if (p.q_vec) return *reinterpret_cast<const uint4 *>(src);
-#pragma unroll
-        for (int k = 0; k < 4; k++) h[k] = __halves2half2(src[2 * k], src[2 * k + 1]);
-    } else {
-        const float *src = static_cast<const float *>(p.q) + i;
-        if (p.q_vec) {
-            const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
-            h[0] = __floats2half2_rn(a.x, a.y);
-            h[1] = __floats2half2_rn(a.z, a.w);
-            h[2] = __floats2half2_rn(b.x, b.y);
-            h[3] = __floats2half2_rn(b.z, b.w);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++) h[k] = __floats2half2_rn(src[2 * k], src[2 * k + 1]);
-        }
-    }
-    return w;
-}
-
-__device__ __forceinline__ void sts128(uint32_t at, uint4 v)
-{
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
 // A unit's codes (64 keys from key0) into registers; keys past the cache are zeros.
@@ -210,22 +156,13 @@ __device__ __forceinline__ void load_unit(const AttendParams &p, const int8_t *h
     }
 }
 
-// The same codes as F16 in the swizzled layout: row r of box b at r * 128, its
-// 16-byte chunk j at (j ^ (r & 7)) * 16.  16 codes are two chunks; half of the
-// lanes store their second one first, so 8 lanes fall on different banks.
 template <int D>
 __device__ __forceinline__ void store_unit(uint32_t tile, int tid, const uint4 (&buf)[CL<D>::n_ld])
 {
 #pragma unroll
     for (int j = 0; j < CL<D>::n_ld; j++) {
-        const int i = tid + 128 * j, r = i / (D / 16), c = i % (D / 16);
-        const uint2 a = codes_to_half4(buf[j].x), b = codes_to_half4(buf[j].y), e = codes_to_half4(buf[j].z),
-                    f = codes_to_half4(buf[j].w);
-        const uint4 lo = make_uint4(a.x, a.y, b.x, b.y), hi = make_uint4(e.x, e.y, f.x, f.y);
-        const uint32_t row = tile + (c >> 2) * CL<D>::box + r * 128;
-        const int ch = 2 * (c & 3), flip = (c >> 2) & 1;
-        sts128(row + (((ch + flip) ^ (r & 7)) << 4), flip ? hi : lo);
-        sts128(row + (((ch + 1 - flip) ^ (r & 7)) << 4), flip ? lo : hi);
+        const int i = tid + 128 * j;
+        store_codes(tile, CL<D>::box, i / (D / 16), i % (D / 16), buf[j]);
     }
 }
 
@@ -388,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const uint32_t sq = smem_addr(smem + L::o_q), sk = smem_addr(smem + L::o_k), sv = smem_addr(smem + L::o_v);
             auto wait = [&](uint64_t *b, uint32_t par) {
                 if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
-                give_up(flag, 1u);
+                give_up(p.error, flag, 1u);
                 return false;
             };
             int i = 0;   // sub-tiles of the CTA so far
@@ -461,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             // (one answer for the warp: its lanes arrive together)
             const bool got = mbar_wait_ab(b, par, kLimitNs, flag);
             if (!__all_sync(0xffffffffu, got)) {
-                give_up(flag, 2u);
+                give_up(p.error, flag, 2u);
                 return false;
             }
             return true;
@@ -543,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         const int tok_in = row / p.r, hd = row - tok_in * p.r;
         auto wait = [&](uint64_t *b, uint32_t par) {
             if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
-            give_up(flag, 4u);
+            give_up(p.error, flag, 4u);
             return false;
         };
         const int64_t n_sc = p.c.rows / kBlock;
@@ -837,6 +774,19 @@ cudaError_t launch_chunk(const AttendParams &p, cudaStream_t st)
     case 256: return p.mask ? run<256, true>(p, st) : run<256, false>(p, st);
     default: return cudaErrorInvalidValue;
     }
+}
+
+cudaError_t error_word(unsigned **dev)
+{
+    // (looked up once a device: its address does not change)
+    static std::atomic<unsigned *> known[64];
+    int id = 0;
+    cudaError_t e = cudaGetDevice(&id);
+    if (e != cudaSuccess) return e;
+    if (id < 64 && (*dev = known[id].load(std::memory_order_relaxed))) return cudaSuccess;
+    e = cudaGetSymbolAddress(reinterpret_cast<void **>(dev), g_error);
+    if (e == cudaSuccess && id < 64) known[id].store(*dev, std::memory_order_relaxed);
+    return e;
 }
 
 cudaError_t take_error(unsigned *word)

@@ -1,0 +1,341 @@
+// kv_q8_weigh.cu -- the softmax weights of a chunk's query rows, summed for each
+// cached row: weight[h][k] += sum over rows of e^(t - m) / Z, with every row's
+// (m, 1 / Z) known from the attention kernels.
+//
+// The scores are formed again as S^T = K Q^T on the tensor cores (keys on the
+// 128 TMEM lanes, 128 query rows in the columns), so a thread holds one key and
+// its sum never leaves its registers: no atomics, one order.  Half the products
+// of the attention itself; the exponentials are the bound (16 a clock and SM).
+//
+// An item is (KV head, 128 keys); a CTA takes a range of items and for each
+// walks the query tiles that see them.  288 threads, two CTAs an SM up to
+// head_dim 128:
+//   warps 0-3  a key a thread: S^T from TMEM, exponentials, the sum
+//   warps 4-7  stage: the item's codes as F16, query tiles and their rows' (m, 1 / Z)
+//   warp 8     issues the MMAs, owns TMEM
+#include <math_constants.h>
+
+#include <algorithm>
+
+#include "kv_internal.h"
+#include "kv_q8_stage.cuh"
+
+namespace kvb {
+namespace q8 {
+namespace {
+
+using namespace sm100;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kThreads = 288;
+
+template <int D>
+struct WL {
+    static constexpr int NB = (D + 63) / 64;
+    static constexpr uint32_t box = 128 * 128;         // [128 rows][64 halves]
+    static constexpr uint32_t tile = NB * box;         // K or Q tile
+    static constexpr int n_ld = 128 * D / 16 / 128;    // 16-byte loads a staging thread makes for an item's codes
+    static constexpr int ctas = D == 256 ? 1 : 2;      // an SM
+    static constexpr size_t o_k = 0, o_q = tile;
+    static constexpr size_t o_st = o_q + 2 * (size_t)tile;   // [2][128] (m, 1 / Z)
+    static constexpr size_t o_lim = o_st + 2 * 128 * 8;      // [2][128] the last key a row may see
+    static constexpr size_t o_bar = o_lim + 2 * 128 * 4;
+    static constexpr int n_bar = 2 + 4 + 4 + 1;
+    static constexpr size_t o_tm = o_bar + n_bar * 8;
+    static constexpr size_t bytes = o_tm + 16;
+    static_assert(bytes * ctas <= 226 * 1024, "shared memory");
+};
+
+// A walk over a CTA's (item, query tile) steps, the same in every warp.
+struct Steps {
+    int64_t item, end;
+    int h, qt, n_qt;
+    int64_t key0;
+    int staged_h;      // the head whose only query tile is staged (-1: none)
+    bool fresh;        // this step's query tile is staged anew
+    __device__ __forceinline__ void begin(const AttendParams &p, int cta, int ctas)
+    {
+        const int64_t n = (int64_t)p.c.H * p.n_kt;
+        item = cta * n / ctas;
+        end = (cta + 1) * n / ctas;
+        n_qt = (int)(((int64_t)p.n_new * p.r + 127) / 128);
+        staged_h = -1;
+        if (more()) enter(p);
+    }
+    __device__ __forceinline__ bool more() const { return item < end; }
+    __device__ __forceinline__ void enter(const AttendParams &p)
+    {
+        h = (int)(item / p.n_kt);
+        key0 = (item - (int64_t)h * p.n_kt) * 128;
+        // tiles whose last token comes before the keys do not see them
+        const int64_t tok0 = p.mask ? 0 : max((int64_t)0, key0 - p.n_past);
+        qt = (int)(tok0 * p.r / 128);
+        step();
+    }
+    __device__ __forceinline__ void step()
+    {
+        fresh = n_qt > 1 || staged_h != h;
+        staged_h = h;
+    }
+    __device__ __forceinline__ bool last() const { return qt == n_qt - 1; }
+    // whether the staged tile is not used after this step
+    __device__ __forceinline__ bool done_with_q(const AttendParams &p) const
+    {
+        return n_qt > 1 || item + 1 >= end || (item + 1) / p.n_kt != h;
+    }
+    __device__ __forceinline__ void next(const AttendParams &p)
+    {
+        if (!last()) {
+            qt++;
+            step();
+        } else {
+            item++;
+            if (more()) enter(p);
+        }
+    }
+};
+
+template <int D, bool MASKED>
+__global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const AttendParams p)
+{
+    using L = WL<D>;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::o_bar);
+    uint64_t *k_full = bar, *k_empty = bar + 1, *q_full = bar + 2, *q_empty = bar + 4, *s_full = bar + 6, *s_empty = bar + 8;
+    uint64_t *drain = bar + 10;
+    uint32_t *tm_slot = reinterpret_cast<uint32_t *>(smem + L::o_tm);
+    volatile int *flag = reinterpret_cast<volatile int *>(smem + L::o_tm + 8);
+    float2 *row_st = reinterpret_cast<float2 *>(smem + L::o_st);
+    int *row_lim = reinterpret_cast<int *>(smem + L::o_lim);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        mbar_init(k_full, 4);
+        mbar_init(k_empty, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&q_full[i], 4);
+            mbar_init(&q_empty[i], 5);   // the MMAs that read it, and the 4 warps that read its rows' numbers
+            mbar_init(&s_full[i], 1);
+            mbar_init(&s_empty[i], 4);
+        }
+        mbar_init(drain, 1);
+        *flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        tmem_alloc(tm_slot, 256);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tm_slot;
+    pdl_launch_dependents();
+    pdl_wait();
+    auto wait = [&](uint64_t *b, uint32_t par) {
+        if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
+        give_up(p.error, flag, 8u);
+        return false;
+    };
+
+    Steps w;
+    w.begin(p, blockIdx.x, gridDim.x);
+    bool ok = true;
+    int q = -1, s = 0, items = 0;   // query tiles staged (the present one's number), steps, items begun
+    if (warp < 4) {
+        const uint32_t tS = tmem + ((uint32_t)(warp * 32) << 16);
+        float sum = 0.0f;
+        for (; ok && w.more(); s++) {
+            if (w.fresh) q++;
+            const int64_t key = w.key0 + tid;
+            // (key 0 of the tile is a row of the cache: the block of a lane past the cache is the last one)
+            const int64_t blk = min(key / kBlock, p.c.rows / kBlock - 1);
+            const uint32_t kw = __ldg(reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)w.h * (p.c.rows / kBlock) + blk);
+            const float c = p.scale * pow2(scale_exp(kw)) * (MASKED ? 1.0f : kLog2e);
+            ok = __all_sync(0xffffffffu, wait(&q_full[q & 1], (q >> 1) & 1) && wait(&s_full[s & 1], (s >> 1) & 1));
+            if (!ok) break;
+            tc_fence_after();
+            const float4 *st = reinterpret_cast<const float4 *>(row_st + (q & 1) * 128);
+            const int *lim = row_lim + (q & 1) * 128;
+            const int row0 = w.qt * 128, n_rows = min(128, p.n_new * p.r - row0);
+            const bool all = MASKED || w.key0 + 127 <= p.n_past + row0 / p.r;   // every row sees every key
+            const bool in = key < p.n_kv;
+            float part = 0.0f;
+#pragma unroll 1
+            for (int ch = 0; ch < 4; ch++) {
+                if (ch * 32 >= n_rows) break;
+                uint32_t v[32];
+                tmem_ld32(tS + (s & 1) * 128 + ch * 32, v);
+                tmem_wait_ld();
+                if constexpr (MASKED) {
+                    int tok = -1;
+                    float mk = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        const int row = row0 + ch * 32 + e;
+                        if (row - row0 >= n_rows) break;
+                        const float2 y = row_st[(q & 1) * 128 + ch * 32 + e];
+                        if (row / p.r != tok) {   // (the same for all lanes)
+                            tok = row / p.r;
+                            const int64_t i = tok * p.mask_stride + key;
+                            mk = -CUDART_INF_F;
+                            if (in) mk = p.mask_f16 ? __half2float(static_cast<const __half *>(p.mask)[i]) : static_cast<const float *>(p.mask)[i];
+                        }
+                        if (y.y == 0.0f) continue;   // (its mask may be infinite)
+                        part = __fmaf_rn(ex2_approx((__fmaf_rn(__uint_as_float(v[e]), c, mk) - y.x) * kLog2e), y.y, part);
+                    }
+                } else {
+                    if (!all) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++)
+                            if (key > lim[ch * 32 + e]) v[e] = __float_as_uint(-CUDART_INF_F);
+                    }
+                    float a = 0.0f, b = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float4 y = st[ch * 16 + e];   // two rows' (m, 1 / Z)
+                        a = __fmaf_rn(ex2_approx(__fmaf_rn(__uint_as_float(v[2 * e]), c, -y.x)), y.y, a);
+                        b = __fmaf_rn(ex2_approx(__fmaf_rn(__uint_as_float(v[2 * e + 1]), c, -y.z)), y.w, b);
+                    }
+                    part += a + b;
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&s_empty[s & 1]);
+                if (w.done_with_q(p)) mbar_arrive(&q_empty[q & 1]);
+            }
+            sum += part;
+            if (w.last()) {
+                if (in) p.c.weight[(int64_t)w.h * p.c.rows + key] += sum;
+                sum = 0.0f;
+            }
+            w.next(p);
+        }
+    } else if (warp < 8) {
+        const int t = tid - 128;
+        uint4 buf[L::n_ld];
+        auto load = [&](int64_t item) {
+            const int h = (int)(item / p.n_kt);
+            const int64_t key0 = (item - (int64_t)h * p.n_kt) * 128;
+            const uint4 *src = reinterpret_cast<const uint4 *>(p.c.k + ((int64_t)h * p.c.rows + key0) * D);
+#pragma unroll
+            for (int j = 0; j < L::n_ld; j++) {
+                const int i = t + 128 * j;
+                buf[j] = key0 + i / (D / 16) < p.c.rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        if (w.more()) load(w.item);
+        auto all_wait = [&](uint64_t *b, uint32_t par) { return __all_sync(0xffffffffu, wait(b, par)); };
+        const uint32_t sk = smem_addr(smem + L::o_k), sq = smem_addr(smem + L::o_q);
+        for (int64_t now = -1; ok && w.more(); w.next(p)) {
+            if (w.item != now) {
+                if (items > 0 && !(ok = all_wait(k_empty, (items - 1) & 1))) break;
+#pragma unroll
+                for (int j = 0; j < L::n_ld; j++) {
+                    const int i = t + 128 * j;
+                    store_codes(sk, L::box, i / (D / 16), i % (D / 16), buf[j]);
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(k_full);
+                now = w.item;
+                items++;
+                if (w.item + 1 < w.end) load(w.item + 1);
+            }
+            if (!w.fresh) continue;
+            q++;
+            if (q >= 2 && !(ok = all_wait(&q_empty[q & 1], ((q >> 1) - 1) & 1))) break;
+            const int row0 = w.qt * 128, R = p.n_new * p.r;
+            const float2 *stat = p.row_stat + (int64_t)w.h * R + row0;
+            {
+                // a row that adds nothing has 1 / Z = 0: its queries are zeros, so that its products are finite
+                const float2 y = row0 + t < R ? stat[t] : make_float2(0.0f, 0.0f);
+                row_st[(q & 1) * 128 + t] = y;
+                row_lim[(q & 1) * 128 + t] = (int)(p.n_past + (row0 + t) / p.r);
+            }
+            const uint32_t dst = sq + (q & 1) * L::tile;
+#pragma unroll 8
+            for (int x = t; x < 128 * (D / 8); x += 128) {
+                const int row = x / (D / 8), c = x % (D / 8);
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row0 + row < R && stat[row].y != 0.0f)
+                    v = load_q8(p, (row0 + row) / p.r, w.h * p.r + (row0 + row) % p.r, D, c * 8);
+                sts128(dst + (c >> 3) * L::box + row * 128 + (((c & 7) ^ (row & 7)) << 4), v);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[q & 1]);
+        }
+    } else if (lane == 0) {
+        constexpr uint32_t id = idesc_f16_f32(128, 128, false);
+        const uint32_t sk = smem_addr(smem + L::o_k), sq = smem_addr(smem + L::o_q);
+        for (int64_t now = -1; ok && w.more(); s++, w.next(p)) {
+            if (w.item != now) {
+                if (!(ok = wait(k_full, items & 1))) break;
+                now = w.item;
+                items++;
+            }
+            if (w.fresh) {
+                q++;
+                if (!(ok = wait(&q_full[q & 1], (q >> 1) & 1))) break;
+            }
+            if (s >= 2 && !(ok = wait(&s_empty[s & 1], ((s >> 1) - 1) & 1))) break;
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++) {
+                const uint32_t off = (kk >> 2) * L::box + (kk & 3) * 32;
+                umma_ss(tmem + (s & 1) * 128, sdesc_k_sw128(sk + off), sdesc_k_sw128(sq + (q & 1) * L::tile + off), id, kk > 0);
+            }
+            umma_commit(&s_full[s & 1]);
+            if (w.done_with_q(p)) umma_commit(&q_empty[q & 1]);
+            if (w.last()) umma_commit(k_empty);
+        }
+        umma_commit(drain);
+        mbar_wait(drain, 0, kLimitNs);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 256);
+    }
+}
+
+template <int D, bool MASKED>
+cudaError_t run(const AttendParams &p, cudaStream_t st)
+{
+    using L = WL<D>;
+    static Once once;
+    cudaError_t e = once.on_device([] {
+        return cudaFuncSetAttribute(weigh_kernel<D, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::bytes);
+    });
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)p.c.H * p.n_kt, kSMs * L::ctas));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = L::bytes;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, weigh_kernel<D, MASKED>, p);
+}
+
+}  // namespace
+
+cudaError_t launch_weigh(const AttendParams &p, cudaStream_t st)
+{
+    switch (p.c.D) {
+    case 64: return p.mask ? run<64, true>(p, st) : run<64, false>(p, st);
+    case 96: return p.mask ? run<96, true>(p, st) : run<96, false>(p, st);
+    case 128: return p.mask ? run<128, true>(p, st) : run<128, false>(p, st);
+    case 256: return p.mask ? run<256, true>(p, st) : run<256, false>(p, st);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace q8
+}  // namespace kvb
