@@ -20,10 +20,12 @@
 // chunk_kernel (512 threads, registers moved to where they are needed):
 //   warps 0-2   issue the MMAs: S_A, S_B (64 columns each, double buffered) and
 //               the products P.V; three threads because one thread's issue rate
-//               bounds MMAs this narrow.  Warp 3 owns TMEM.
-//   warps 4-7   stage: codes from global memory into registers some units ahead
-//               (32 KB in flight an SM), converted to F16 and stored in the
-//               128-byte-swizzled layout the tensor cores read; also the queries
+//               bounds MMAs this narrow
+//   warp 3      brings the codes in (bulk copies, 32 KB in flight); owns TMEM
+//   warps 4-7   convert them to F16 in the 128-byte-swizzled layout the tensor
+//               cores read; also the queries.  (Codes loaded into registers some
+//               units ahead measured 262 us against 160: the fence before a
+//               tile is handed over waits for every load in flight)
 //   warps 8-15  softmax of tile A and tile B, a query row a thread: S from TMEM,
 //               weights back as F16 pairs; rescales O when the reference moves;
 //               writes a segment's O
@@ -56,15 +58,18 @@ struct CL {
     static constexpr uint32_t q_tile = NB * 128 * 128;       // bytes
     static constexpr uint32_t box = kSub * 128;              // [64 keys][64 halves]
     static constexpr uint32_t tile = NB * box;               // a K or V sub-tile
-    static constexpr int KS = D == 256 ? 3 : D >= 96 ? 5 : 8;
-    static constexpr int VS = D == 256 ? 2 : D >= 96 ? 5 : 8;
-    static constexpr int n_ld = kSub * D / 16 / 128;         // 16-byte loads a staging thread makes a unit
-    static constexpr int PF = D == 64 ? 8 : D == 256 ? 2 : 4;   // units in flight: 32 KB an SM (64 registers a thread; 24 KB at 96)
+    static constexpr int KS = D == 256 ? 2 : D >= 96 ? 4 : 8;
+    static constexpr int VS = KS;
+    static constexpr uint32_t unit = kSub * D;               // bytes of codes of a sub-tile
+    static constexpr int RS = D == 96 ? 5 : 32768 / (int)unit;   // units of codes in flight or waiting: 32 KB
+    static constexpr int n_ld = unit / 16 / 128;             // 16-byte pieces a staging thread converts a unit
     static constexpr size_t o_q = 0;
     static constexpr size_t o_k = o_q + NT * (size_t)q_tile;
     static constexpr size_t o_v = o_k + KS * (size_t)tile;
-    static constexpr size_t o_bar = o_v + VS * (size_t)tile;
-    static constexpr int n_bar = 2 + 2 * KS + 2 * VS + 12 + 2 + 3;
+    static constexpr size_t o_raw = o_v + VS * (size_t)tile;
+    static constexpr size_t o_off = o_raw + RS * (size_t)unit;   // [128] where a tile's query rows are
+    static constexpr size_t o_bar = o_off + 128 * 8;
+    static constexpr int n_bar = 2 + 2 * KS + 2 * VS + 12 + 2 + 3 + 2 * RS;
     static constexpr size_t o_tm = o_bar + n_bar * 8;
     static constexpr size_t bytes = o_tm + 16;
     static_assert(bytes <= 227 * 1024, "shared memory");
@@ -141,29 +146,6 @@ template <int N>
 __device__ __forceinline__ void regs_dec()
 {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
-// A unit's codes (64 keys from key0) into registers; keys past the cache are zeros.
-template <int D>
-__device__ __forceinline__ void load_unit(const AttendParams &p, const int8_t *head, int64_t key0, int tid,
-                                          uint4 (&buf)[CL<D>::n_ld])
-{
-    const uint4 *src = reinterpret_cast<const uint4 *>(head + key0 * D);
-#pragma unroll
-    for (int j = 0; j < CL<D>::n_ld; j++) {
-        const int i = tid + 128 * j;
-        buf[j] = key0 + i / (D / 16) < p.c.rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-    }
-}
-
-template <int D>
-__device__ __forceinline__ void store_unit(uint32_t tile, int tid, const uint4 (&buf)[CL<D>::n_ld])
-{
-#pragma unroll
-    for (int j = 0; j < CL<D>::n_ld; j++) {
-        const int i = tid + 128 * j;
-        store_codes(tile, CL<D>::box, i / (D / 16), i % (D / 16), buf[j]);
-    }
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c)
@@ -292,6 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     uint64_t *v_full = k_empty + KS, *v_empty = v_full + VS;
     uint64_t *s_full = v_empty + VS, *p_full = s_full + 4, *o_ready = p_full + 4;   // [tile][buffer]
     uint64_t *o_full = o_ready + 4, *o_empty = o_full + 1, *drain = o_empty + 1;
+    uint64_t *raw_full = drain + 3, *raw_empty = raw_full + L::RS;
     uint32_t *tm_slot = reinterpret_cast<uint32_t *>(smem + L::o_tm);
     volatile int *flag = reinterpret_cast<volatile int *>(smem + L::o_tm + 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cta = blockIdx.x;
@@ -299,7 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     if (tid == 0) {
         for (int i = 0; i < L::n_bar; i++) {
             const uint64_t *b = &bar[i];
-            const bool staged = b == q_full || (b >= k_full && b < k_full + KS) || (b >= v_full && b < v_full + VS);
+            const bool staged = b == q_full || (b >= k_full && b < k_full + KS) || (b >= v_full && b < v_full + VS) ||
+                                b >= raw_empty;   // the four staging warps
             const bool both = b == q_empty || (b >= k_empty && b < k_empty + KS);   // both S issuers
             mbar_init(&bar[i], staged || (b >= p_full && b < p_full + 4) ? 4 : b == o_empty ? 8 : both ? 2 : 1);
         }
@@ -319,8 +303,33 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
 
     Walk w;
     if (warp < 4) {
-        regs_dec<56>();
-        if (lane == 0 && warp < 3) {
+        regs_dec<96>();
+        if (lane == 0 && warp == 3) {
+            // a unit's codes lie in one piece: one bulk copy; rows past the cache are left out (their weights are 0)
+            const uint32_t raw = smem_addr(smem + L::o_raw);
+            int u = 0;
+            bool ok = true;
+            for (w.begin(p, cta); ok && w.more(); w.next_pair(p)) {
+                const int64_t head = (int64_t)(w.pair / p.n_blk) * p.c.rows;
+                for (int t = w.t0; ok && t < w.t1; t++) {
+                    const int64_t key0 = (int64_t)t * kSub;
+                    const uint32_t n = (uint32_t)min((int64_t)kSub, p.c.rows - key0) * D;
+#pragma unroll
+                    for (int v = 0; v < 2; v++, u++) {
+                        const int s = u % L::RS;
+                        if (u >= L::RS && !mbar_wait_ab(&raw_empty[s], (u / L::RS - 1) & 1, kLimitNs, flag)) {
+                            give_up(p.error, flag, 2u);
+                            ok = false;
+                            break;
+                        }
+                        mbar_arrive_expect_tx(&raw_full[s], n);
+                        bulk_load(raw + s * L::unit, (v ? p.c.v : p.c.k) + (head + key0) * D, n, &raw_full[s]);
+                    }
+                }
+            }
+            // none may land after the CTA has gone
+            for (int x = u > L::RS ? u - L::RS : 0; x < u; x++) mbar_wait(&raw_full[x % L::RS], (x / L::RS) & 1, kLimitNs);
+        } else if (lane == 0) {
             constexpr uint32_t idS = idesc_f16_f32(128, kSub, false), idO = idesc_f16_f32(128, D, true);
             const uint32_t sq = smem_addr(smem + L::o_q), sk = smem_addr(smem + L::o_k), sv = smem_addr(smem + L::o_v);
             auto wait = [&](uint64_t *b, uint32_t par) {
@@ -392,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             mbar_wait(&drain[warp], 0, kLimitNs);
         }
     } else if (warp < 8) {
-        regs_dec<120>();
+        regs_dec<80>();
         const int st = tid - 128;
         auto wait = [&](uint64_t *b, uint32_t par) {
             // (one answer for the warp: its lanes arrive together)
@@ -403,72 +412,51 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             }
             return true;
         };
-        const uint32_t sk = smem_addr(smem + L::o_k), sv = smem_addr(smem + L::o_v);
-        uint4 buf[L::PF][L::n_ld];
-        Walk f;   // the units being fetched: K then V of each sub-tile
-        f.begin(p, cta);
-        bool fv = false;
-        auto fetch = [&](uint4 (&b)[L::n_ld]) {
-            if (!f.more()) return;
-            const int8_t *head = (fv ? p.c.v : p.c.k) + (int64_t)(f.pair / p.n_blk) * p.c.rows * D;
-            load_unit<D>(p, head, (int64_t)f.t * kSub, st, b);
-            if (fv && ++f.t == f.t1) f.next_pair(p);
-            fv = !fv;
+        int64_t *off = reinterpret_cast<int64_t *>(smem + L::o_off);
+        int i = 0, u = 0;   // sub-tiles and units so far
+        bool ok = true;
+        // the next unit, as F16 into `tile` once `empty` (phase par) says it is free
+        auto convert = [&](unsigned char *tile, uint64_t *full, uint64_t *empty, bool used, uint32_t par) {
+            const int s = u % L::RS;
+            if (!wait(&raw_full[s], (u / L::RS) & 1)) return false;
+            u++;
+            uint4 c[L::n_ld];
+            const uint4 *src = reinterpret_cast<const uint4 *>(smem + L::o_raw + s * L::unit);
+#pragma unroll
+            for (int j = 0; j < L::n_ld; j++) c[j] = src[st + 128 * j];
+            if (used && !wait(empty, par)) return false;
+#pragma unroll
+            for (int j = 0; j < L::n_ld; j++) {
+                const int x = st + 128 * j;
+                store_codes(smem_addr(tile), L::box, x / (D / 16), x % (D / 16), c[j]);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(full);
+                mbar_arrive(&raw_empty[s]);
+            }
+            return true;
         };
-#pragma unroll
-        for (int u = 0; u < L::PF; u++) fetch(buf[u]);
         w.begin(p, cta);
-        int i = 0, seg = 0;
-        bool ok = true, first = true;
-        while (ok && w.more()) {
-#pragma unroll
-            for (int u = 0; u < L::PF; u += 2) {
-                if (!ok || !w.more()) break;
-                if (first) {   // a segment's queries
-                    const int h = w.pair / p.n_blk, b = w.pair % p.n_blk;
-                    if (seg > 0 && !(ok = wait(q_empty, (seg - 1) & 1))) break;
-                    const int nt = tiles_of(p, b);
-                    for (int g = 0; g < nt; g++) {
-                        const int tok0 = b * p.tok_blk + g * p.tok_tile;
-                        const uint32_t dst = smem_addr(smem + L::o_q) + g * L::q_tile;
-#pragma unroll 8
-                        for (int x = st; x < 128 * (D / 8); x += 128) {
-                            const int row = x / (D / 8), c = x % (D / 8);
-                            const int tk = row / p.r, t = tok0 + tk;
-                            uint4 v = make_uint4(0, 0, 0, 0);
-                            if (tk < p.tok_tile && t < p.n_new) v = load_q8(p, t, h * p.r + row - tk * p.r, D, c * 8);
-                            sts128(dst + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), v);
-                        }
-                    }
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(q_full);
-                    first = false;
-                }
-                {
-                    const int s = i % KS;
-                    if (i >= KS && !(ok = wait(&k_empty[s], (i / KS - 1) & 1))) break;
-                    store_unit<D>(sk + s * L::tile, st, buf[u]);
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&k_full[s]);
-                    fetch(buf[u]);
-                }
-                {
-                    const int s = i % VS;
-                    if (i >= VS && !(ok = wait(&v_empty[s], (i / VS - 1) & 1))) break;
-                    store_unit<D>(sv + s * L::tile, st, buf[u + 1]);
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&v_full[s]);
-                    fetch(buf[u + 1]);
-                }
-                i++;
-                if (++w.t == w.t1) {
-                    w.next_pair(p);
-                    seg++;
-                    first = true;
-                }
+        for (int seg = 0; ok && w.more(); seg++, w.next_pair(p)) {
+            const int h = w.pair / p.n_blk, b = w.pair % p.n_blk, nt = tiles_of(p, b);
+            if (seg > 0 && !(ok = wait(q_empty, (seg - 1) & 1))) break;
+            for (int g = 0; g < nt; g++) {
+                const int tk = st / p.r, tok = b * p.tok_blk + g * p.tok_tile + tk;
+                named_sync(1, 128);   // (the tile before has been staged)
+                off[st] = tk < p.tok_tile && tok < p.n_new
+                              ? tok * p.q_stride + (int64_t)(h * p.r + st - tk * p.r) * D : -1;
+                named_sync(1, 128);
+                stage_queries<D>(p, smem_addr(smem + L::o_q) + g * L::q_tile, 16384, off, st);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+            for (int t = w.t0; t < w.t1; t++, i++) {
+                const int ks = i % KS, vs = i % VS;
+                if (!(ok = convert(smem + L::o_k + ks * L::tile, &k_full[ks], &k_empty[ks], i >= KS, (i / KS - 1) & 1))) break;
+                if (!(ok = convert(smem + L::o_v + vs * L::tile, &v_full[vs], &v_empty[vs], i >= VS, (i / VS - 1) & 1))) break;
             }
         }
     } else {

@@ -30,36 +30,78 @@ __device__ __forceinline__ uint2 codes_to_half4(uint32_t w)
     return make_uint2(*reinterpret_cast<const uint32_t *>(&hx), *reinterpret_cast<const uint32_t *>(&hy));
 }
 
-// 8 query elements at d as F16
-__device__ __forceinline__ uint4 load_q8(const AttendParams &p, int t, int hq, int D, int d)
-{
-    const int64_t i = t * p.q_stride + (int64_t)hq * D + d;
-    uint4 w;
-    __half2 *h = reinterpret_cast<__half2 *>(&w);
-    if (p.q_f16) {
-        const __half *src = static_cast<const __half *>(p.q) + i;
-        if (p.q_vec) return *reinterpret_cast<const uint4 *>(src);
-#pragma unroll
-        for (int k = 0; k < 4; k++) h[k] = __halves2half2(src[2 * k], src[2 * k + 1]);
-    } else {
-        const float *src = static_cast<const float *>(p.q) + i;
-        if (p.q_vec) {
-            const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
-            h[0] = __floats2half2_rn(a.x, a.y);
-            h[1] = __floats2half2_rn(a.z, a.w);
-            h[2] = __floats2half2_rn(b.x, b.y);
-            h[3] = __floats2half2_rn(b.z, b.w);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; k++) h[k] = __floats2half2_rn(src[2 * k], src[2 * k + 1]);
-        }
-    }
-    return w;
-}
-
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// n bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory, completed on `bar`
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t n, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(n), "r"(sm100::smem_addr(bar))
+                 : "memory");
+}
+
+// 16 bytes into shared memory, or 16 zeros
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void *src, bool have)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(have ? 16 : 0) : "memory");
+}
+
+// 128 query rows as F16 in the swizzled layout, by 128 threads (t); off[row] is
+// where a row's elements start, -1 for a row of zeros (shared memory, complete).
+// Aligned F16 rows go straight to shared memory; others through registers, four
+// loads in flight.
+template <int D>
+__device__ __forceinline__ void stage_queries(const AttendParams &p, uint32_t dst, uint32_t box, const int64_t *off, int t)
+{
+    constexpr int C = D / 8;
+    if (p.q_f16 && p.q_vec) {
+        const __half *q = static_cast<const __half *>(p.q);
+#pragma unroll 4
+        for (int x = t; x < 128 * C; x += 128) {
+            const int row = x / C, c = x % C;
+            const int64_t at = off[row];
+            cp_async_16_or_zero(dst + (c >> 3) * box + row * 128 + (((c & 7) ^ (row & 7)) << 4),
+                                q + (at < 0 ? 0 : at + c * 8), at >= 0);
+        }
+        sm100::cp_async_commit();
+        sm100::cp_async_wait<0>();
+    } else {
+#pragma unroll 1
+        for (int x0 = t; x0 < 128 * C; x0 += 4 * 128) {
+            float v[4][8];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int x = x0 + 128 * k;
+                const int64_t at = off[x / C], i = at < 0 ? 0 : at + x % C * 8;   // (element 0 exists)
+                if (p.q_f16) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[k][e] = __half2float(static_cast<const __half *>(p.q)[at < 0 ? 0 : i + e]);
+                } else if (p.q_vec) {
+                    const float4 *src = reinterpret_cast<const float4 *>(static_cast<const float *>(p.q) + i);
+                    const float4 a = src[0], b = src[1];
+                    v[k][0] = a.x; v[k][1] = a.y; v[k][2] = a.z; v[k][3] = a.w;
+                    v[k][4] = b.x; v[k][5] = b.y; v[k][6] = b.z; v[k][7] = b.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[k][e] = static_cast<const float *>(p.q)[at < 0 ? 0 : i + e];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int x = x0 + 128 * k, row = x / C, c = x % C;
+                const bool have = off[row] >= 0;
+                uint4 w;
+                __half2 *h = reinterpret_cast<__half2 *>(&w);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    h[e] = have ? __floats2half2_rn(v[k][2 * e], v[k][2 * e + 1]) : __half2half2(__ushort_as_half(0));
+                sts128(dst + (c >> 3) * box + row * 128 + (((c & 7) ^ (row & 7)) << 4), w);
+            }
+        }
+    }
 }
 
 // 16 codes (chunk c of row r) as F16 in the swizzled layout: box c / 4 (64

@@ -39,7 +39,8 @@ struct WL {
     static constexpr size_t o_k = 0, o_q = tile;
     static constexpr size_t o_st = o_q + 2 * (size_t)tile;   // [2][128] (m, 1 / Z)
     static constexpr size_t o_lim = o_st + 2 * 128 * 8;      // [2][128] the last key a row may see
-    static constexpr size_t o_bar = o_lim + 2 * 128 * 4;
+    static constexpr size_t o_off = o_lim + 2 * 128 * 4;     // [2][128] where a row's queries are, -1: nowhere
+    static constexpr size_t o_bar = o_off + 2 * 128 * 8;
     static constexpr int n_bar = 2 + 4 + 4 + 1;
     static constexpr size_t o_tm = o_bar + n_bar * 8;
     static constexpr size_t bytes = o_tm + 16;
@@ -107,6 +108,7 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
     volatile int *flag = reinterpret_cast<volatile int *>(smem + L::o_tm + 8);
     float2 *row_st = reinterpret_cast<float2 *>(smem + L::o_st);
     int *row_lim = reinterpret_cast<int *>(smem + L::o_lim);
+    int64_t *row_off = reinterpret_cast<int64_t *>(smem + L::o_off);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         mbar_init(k_full, 4);
@@ -248,21 +250,17 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
             if (q >= 2 && !(ok = all_wait(&q_empty[q & 1], ((q >> 1) - 1) & 1))) break;
             const int row0 = w.qt * 128, R = p.n_new * p.r;
             const float2 *stat = p.row_stat + (int64_t)w.h * R + row0;
+            int64_t *off = row_off + (q & 1) * 128;
             {
                 // a row that adds nothing has 1 / Z = 0: its queries are zeros, so that its products are finite
                 const float2 y = row0 + t < R ? stat[t] : make_float2(0.0f, 0.0f);
+                const int tok = (row0 + t) / p.r, j = row0 + t - tok * p.r;
                 row_st[(q & 1) * 128 + t] = y;
-                row_lim[(q & 1) * 128 + t] = (int)(p.n_past + (row0 + t) / p.r);
+                row_lim[(q & 1) * 128 + t] = (int)(p.n_past + tok);
+                off[t] = y.y != 0.0f ? tok * p.q_stride + (int64_t)(w.h * p.r + j) * D : -1;
             }
-            const uint32_t dst = sq + (q & 1) * L::tile;
-#pragma unroll 8
-            for (int x = t; x < 128 * (D / 8); x += 128) {
-                const int row = x / (D / 8), c = x % (D / 8);
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row0 + row < R && stat[row].y != 0.0f)
-                    v = load_q8(p, (row0 + row) / p.r, w.h * p.r + (row0 + row) % p.r, D, c * 8);
-                sts128(dst + (c >> 3) * L::box + row * 128 + (((c & 7) ^ (row & 7)) << 4), v);
-            }
+            named_sync(1, 128);
+            stage_queries<D>(p, sq + (q & 1) * L::tile, L::box, off, t);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[q & 1]);
