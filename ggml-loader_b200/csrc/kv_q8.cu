@@ -6,10 +6,24 @@
 // are exact but for the one rounding to the integer.
 #include "kv_internal.h"
 #include "kv_q8.cuh"
+#include "kv_sm100.cuh"
 
 namespace kvb {
 namespace q8 {
 namespace {
+
+using sm100::cluster_rank;
+using sm100::cluster_sync_all;
+using sm100::mapa;
+using sm100::pdl_launch_dependents;
+using sm100::pdl_wait;
+
+__device__ __forceinline__ int ld_cluster_s32(uint32_t addr)
+{
+    int v;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 
 __device__ __forceinline__ bool finite(float x)
 {
@@ -113,6 +127,8 @@ __global__ void __launch_bounds__(kBlock *D / 8) store_kernel(const StoreParams 
     float *scale = (is_v ? p.c.v_scale : p.c.k_scale) + (int64_t)h * (p.c.rows / kBlock) + blk;
     float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     int e0 = 0;
+    pdl_launch_dependents();
+    pdl_wait();
     if (fresh) {
         const int64_t at = (row - p.row0) * (is_v ? p.v_stride : p.k_stride) + h * D + c;
         load8<F16>(is_v ? p.v : p.k, at, p.vec, x);
@@ -127,46 +143,61 @@ __global__ void __launch_bounds__(kBlock *D / 8) store_kernel(const StoreParams 
     if (fresh && !is_v && c == 0 && p.c.weight) p.c.weight[(int64_t)h * p.c.rows + row] = 0.0f;
 }
 
+// kLoadU pieces of 8 codes a thread, their loads in flight together; a token's
+// heads are neighbours in the output.  Bound by the output's bytes.
+constexpr int kLoadU = 4;
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(256) load_kernel(const LoadParams p)
 {
-    const int64_t n = p.n * p.c.H * (D / 8), step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += step) {
-        const bool is_v = i >= n;
-        void *out = is_v ? p.v : p.k;
-        if (!out) continue;
-        // a token's heads are neighbours in the output
-        const int64_t j = is_v ? i - n : i;
-        const int c = (int)(j % (D / 8)) * 8;
-        const int64_t th = j / (D / 8);
-        const int h = (int)(th % p.c.H);
-        const int64_t t = th / p.c.H, row = p.row0 + t;
-        const int8_t *codes = is_v ? p.c.v : p.c.k;
-        const float *scale = is_v ? p.c.v_scale : p.c.k_scale;
-        const uint32_t s = __float_as_uint(scale[(int64_t)h * (p.c.rows / kBlock) + row / kBlock]);
-        const uint2 w = *reinterpret_cast<const uint2 *>(codes + ((int64_t)h * p.c.rows + row) * D + c);
+    pdl_launch_dependents();
+    pdl_wait();
+    const bool is_v = p.k ? blockIdx.y != 0 : true;
+    void *out = is_v ? p.v : p.k;
+    const int8_t *codes = is_v ? p.c.v : p.c.k;
+    const uint32_t *scale = reinterpret_cast<const uint32_t *>(is_v ? p.c.v_scale : p.c.k_scale);
+    // (a row has at most 1024 * 32 pieces, a CTA's rows are few: 32 bits from its first row on)
+    const uint32_t pieces = p.c.H * (D / 8);
+    const int64_t first = (int64_t)blockIdx.x * (256 * kLoadU), t0 = first / pieces;
+    const uint32_t base = (uint32_t)(first - t0 * pieces);
+    uint2 w[kLoadU];
+    uint32_t s[kLoadU];
+    int64_t at[kLoadU];
+#pragma unroll
+    for (int k = 0; k < kLoadU; k++) {
+        const uint32_t j = base + threadIdx.x + 256 * k, dt = j / pieces, c = j - dt * pieces;
+        const int64_t t = t0 + dt, row = p.row0 + t;
+        const uint32_t h = c / (D / 8), d = c % (D / 8) * 8;
+        at[k] = t < p.n ? t * p.stride + c * 8 : -1;
+        if (at[k] >= 0) {
+            w[k] = *reinterpret_cast<const uint2 *>(codes + ((int64_t)h * p.c.rows + row) * D + d);
+            s[k] = scale[(int64_t)h * (p.c.rows / kBlock) + row / kBlock];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kLoadU; k++) {
+        if (at[k] < 0) continue;
         float x[8];
-        decode8(w, scale_exp(s), x);
-        const int64_t at = t * p.stride + h * D + c;
+        decode8(w[k], scale_exp(s[k]), x);
         if constexpr (F16) {
-            __half *dst = static_cast<__half *>(out) + at;
+            __half *dst = static_cast<__half *>(out) + at[k];
             __half y[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) y[k] = __float2half_rn(x[k]);
+            for (int e = 0; e < 8; e++) y[e] = __float2half_rn(x[e]);
             if (p.vec) {
                 *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++) dst[k] = y[k];
+                for (int e = 0; e < 8; e++) dst[e] = y[e];
             }
         } else {
-            float *dst = static_cast<float *>(out) + at;
+            float *dst = static_cast<float *>(out) + at[k];
             if (p.vec) {
                 reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
                 reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++) dst[k] = x[k];
+                for (int e = 0; e < 8; e++) dst[e] = x[e];
             }
         }
     }
@@ -183,115 +214,225 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
+constexpr int kSelCtas = 8;                      // a KV head's cluster
+constexpr int kSelSlice = 48 * 1024;             // keys a CTA holds in shared memory; with more it reads them each time
 
-// One CTA a KV head: the (keep - recent)-th largest key among the candidates by
-// four 8-bit digits, then one ordered pass that writes the kept rows.
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const EvictParams p)
+// A cluster a KV head, each CTA a contiguous slice of its candidates: the
+// (keep - recent)-th largest key by four 8-bit digits (histograms in shared
+// memory, added up over the cluster), then the kept rows in order from each
+// CTA's place on.  The weights are read once; what is left are the cluster's
+// barriers, two a digit (32k candidates, 8 heads: 191 us with one CTA a head).
+__global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) select_kernel(const EvictParams p)
 {
-    __shared__ int hist[256];
-    __shared__ uint32_t s_prefix;
-    __shared__ int64_t s_want;
-    __shared__ int warp_n[kSelThreads / 32], warp_t[kSelThreads / 32];
-    const int h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    extern __shared__ uint32_t s_key[];
+    __shared__ int s_hist[8][256];     // (copies: fewer warps on one counter)
+    __shared__ int s_sum[256];         // this CTA's, read by the others
+    __shared__ int s_all[256];
+    __shared__ int s_scan[kSelWarps];
+    __shared__ int s_count[2];         // this CTA's keys above the edge, and on it
+    __shared__ uint32_t s_digit;
+    __shared__ int s_want;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = (int)cluster_rank(), h = blockIdx.x / kSelCtas;
+    const int cand = (int)(p.n_rows - p.recent), take = (int)(p.keep - p.recent);
     const float *w = p.src.weight + (int64_t)h * p.src.rows;
     int32_t *kept = p.kept + (int64_t)h * p.keep;
-    const int64_t cand = p.n_rows - p.recent, take = p.keep - p.recent;
+    // slices of a multiple of 4 keys
+    const int per = (int)(((int64_t)cand + kSelCtas * 4 - 1) / (kSelCtas * 4) * 4);
+    const int lo = (int)min((int64_t)cand, (int64_t)rank * per), n = min(per, cand - lo);
+    const bool held = per <= kSelSlice;
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int64_t j = (int64_t)rank * kSelThreads + tid; j < p.recent; j += kSelCtas * kSelThreads)
+        kept[take + j] = cand + (int32_t)j;
+    if (take == 0) return;   // (the whole cluster)
+    if (held)
+        for (int i = tid; i < n; i += kSelThreads) s_key[i] = weight_key(w[lo + i]);
+    auto key = [&](int i) { return held ? s_key[i] : weight_key(w[lo + i]); };
+
+    uint32_t prefix = 0;
+    int want = take;   // still to be taken among the keys with the prefix
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 8 * 256; i += kSelThreads) (&s_hist[0][0])[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kSelThreads) {
+            const uint32_t k = key(i);
+            if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&s_hist[warp & 7][(k >> shift) & 255u], 1);
+        }
+        __syncthreads();
+        if (tid < 256) {
+            int x = 0;
+#pragma unroll
+            for (int c = 0; c < 8; c++) x += s_hist[c][tid];
+            s_sum[tid] = x;
+        }
+        cluster_sync_all();
+        if (tid < 256) {
+            int x = 0;
+#pragma unroll
+            for (int c = 0; c < kSelCtas; c++) x += ld_cluster_s32(mapa(sm100::smem_addr(&s_sum[tid]), c));
+            s_all[tid] = x;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            // lane l: digits 255 - 8 l down; the digit in which the want-th largest lies
+            int x[8], total = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) total += x[j] = s_all[255 - 8 * lane - j];
+            int before = total;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += y;
+            }
+            before -= total;
+            if (before < want && want <= before + total) {
+                int d = 0;
+                while (before + x[0] < want) {
+                    before += x[0];
+                    d++;
+#pragma unroll
+                    for (int j = 0; j < 7; j++) x[j] = x[j + 1];
+                }
+                s_digit = 255 - 8 * lane - d;
+                s_want = want - before;
+            }
+        }
+        __syncthreads();
+        prefix = prefix << 8 | s_digit;
+        want = s_want;
+        cluster_sync_all();   // (s_sum is written again)
+    }
+
+    // a thread's keys are neighbours: 4 m of them from 4 m tid on
+    const int m = (n + kSelThreads * 4 - 1) / (kSelThreads * 4) * 4, i0 = min(n, m * tid), i1 = min(n, i0 + m);
+    int above = 0, on = 0;
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = key(i);
+        above += k > prefix;
+        on += k == prefix;
+    }
+    // exclusive sums over the CTA
+    auto scan = [&](int x, int &total) {
+        int y = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) y += z;
+        }
+        __syncthreads();
+        if (lane == 31) s_scan[warp] = y;
+        __syncthreads();
+        int b = 0;
+        total = 0;
+#pragma unroll
+        for (int k = 0; k < kSelWarps; k++) {
+            if (k < warp) b += s_scan[k];
+            total += s_scan[k];
+        }
+        return b + y - x;
+    };
+    int n_above, n_on;
+    int a = scan(above, n_above), e = scan(on, n_on);
     if (tid == 0) {
-        s_prefix = 0;
-        s_want = take;   // still to be taken among the keys with the prefix
+        s_count[0] = n_above;
+        s_count[1] = n_on;
     }
-    __syncthreads();
-    for (int shift = 24; shift >= 0 && take > 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        const uint32_t prefix = s_prefix;
-        for (int64_t i = tid; i < cand; i += kSelThreads) {
-            const uint32_t key = weight_key(w[i]);
-            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            int64_t want = s_want;
-            int d = 255;
-            while (d > 0 && hist[d] < want) want -= hist[d--];
-            s_want = want;
-            s_prefix = prefix << 8 | (uint32_t)d;
-        }
-        __syncthreads();
+    cluster_sync_all();
+    for (int c = 0; c < rank; c++) {
+        const uint32_t at = mapa(sm100::smem_addr(s_count), c);
+        a += ld_cluster_s32(at);
+        e += ld_cluster_s32(at + 4);
     }
-    const uint32_t edge = s_prefix;
-    int64_t ties = take > 0 ? s_want : 0, at = 0;   // rows of key == edge still to take, rows written
-    for (int64_t base = 0; base < cand && take > 0; base += kSelThreads) {
-        const int64_t i = base + tid;
-        const uint32_t key = i < cand ? weight_key(w[i]) : 0;
-        const bool tie = i < cand && key == edge;
-        const uint32_t tb = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) warp_t[warp] = __popc(tb);
-        __syncthreads();
-        int before = __popc(tb & ((1u << lane) - 1u)), all = 0;
-        for (int k = 0; k < kSelThreads / 32; k++) {
-            if (k < warp) before += warp_t[k];
-            all += warp_t[k];
-        }
-        const bool in = i < cand && (key > edge || (tie && before < ties));
-        const uint32_t nb = __ballot_sync(0xffffffffu, in);
-        if (lane == 0) warp_n[warp] = __popc(nb);
-        __syncthreads();
-        int pos = __popc(nb & ((1u << lane) - 1u)), n = 0;
-        for (int k = 0; k < kSelThreads / 32; k++) {
-            if (k < warp) pos += warp_n[k];
-            n += warp_n[k];
-        }
-        if (in) kept[at + pos] = (int32_t)i;
-        at += n;
-        ties -= min((int64_t)all, ties);
-        __syncthreads();
+    cluster_sync_all();   // (no CTA leaves while its counts are read)
+    // rows before this thread's first: a above the edge and min(e, want) on it
+    for (int i = i0; i < i1; i++) {
+        const uint32_t k = key(i);
+        const bool tie = k == prefix;
+        if (k > prefix || (tie && e < want)) kept[a + min(e, want)] = lo + i;
+        a += k > prefix;
+        e += tie;
     }
-    for (int64_t j = tid; j < p.recent; j += kSelThreads) kept[take + j] = (int32_t)(cand + j);
 }
 
-// One CTA a block of dst, KV head and K/V: gathers its rows and stores them.
+// One CTA a block of dst and KV head, K and V: a row is D/16 threads, 16 codes
+// each of K and of V, so both gathers are in flight together.
 template <int D>
-__global__ void __launch_bounds__(kBlock *D / 8) gather_kernel(const EvictParams p)
+__global__ void __launch_bounds__(kBlock *D / 16) gather_kernel(const EvictParams p)
 {
-    constexpr int T = kBlock * D / 8;
-    const int r = threadIdx.x / (D / 8), c = threadIdx.x % (D / 8) * 8;
+    constexpr int T = kBlock * D / 16;
+    __shared__ uint32_t part[2][T / 32];
+    const int r = threadIdx.x / (D / 16), c = threadIdx.x % (D / 16) * 16;
     const int h = blockIdx.y;
-    const bool is_v = blockIdx.z != 0;
     const int64_t blk = blockIdx.x, row = blk * kBlock + r;
     const bool used = row < p.keep;
-    float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    int e0[2] = {kExpMin, kExpMin};
+    pdl_launch_dependents();
+    pdl_wait();
     if (used) {
-        const int64_t from = p.kept[(int64_t)h * p.keep + row];
-        const int8_t *codes = is_v ? p.src.v : p.src.k;
-        const float *scale = is_v ? p.src.v_scale : p.src.k_scale;
-        const uint32_t s = __float_as_uint(scale[(int64_t)h * (p.src.rows / kBlock) + from / kBlock]);
-        decode8(*reinterpret_cast<const uint2 *>(codes + ((int64_t)h * p.src.rows + from) * D + c), scale_exp(s), x);
-        if (!is_v && c == 0 && p.dst.weight)
-            p.dst.weight[(int64_t)h * p.dst.rows + row] = p.src.weight[(int64_t)h * p.src.rows + from];
+        const int64_t from = p.kept[(int64_t)h * p.keep + row], at = ((int64_t)h * p.src.rows + from) * D + c;
+        const int64_t sc = (int64_t)h * (p.src.rows / kBlock) + from / kBlock;
+        w[0] = *reinterpret_cast<const uint4 *>(p.src.k + at);
+        w[1] = *reinterpret_cast<const uint4 *>(p.src.v + at);
+        e0[0] = scale_exp(reinterpret_cast<const uint32_t *>(p.src.k_scale)[sc]);
+        e0[1] = scale_exp(reinterpret_cast<const uint32_t *>(p.src.v_scale)[sc]);
+        if (c == 0 && p.dst.weight) p.dst.weight[(int64_t)h * p.dst.rows + row] = p.src.weight[(int64_t)h * p.src.rows + from];
     }
-    bool bad;
-    const int e = block_scale<T>(x, bad);
-    if (used)
-        *reinterpret_cast<uint2 *>((is_v ? p.dst.v : p.dst.k) + ((int64_t)h * p.dst.rows + row) * D + c) = encode8(x, e);
-    if (threadIdx.x == 0)
-        (is_v ? p.dst.v_scale : p.dst.k_scale)[(int64_t)h * (p.dst.rows / kBlock) + blk] =
-            __uint_as_float(scale_word(e, bad));
+    // the largest magnitude, code * 2^e: exact in float, whose bits order as it does
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+        const int8_t *x = reinterpret_cast<const int8_t *>(&w[v]);
+        int top = 0;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            bad |= x[i] == kBad;
+            top = max(top, x[i] == kBad ? 0 : abs((int)x[i]));
+        }
+        const uint32_t best = __reduce_max_sync(0xffffffffu, __float_as_uint(__fmul_rn((float)top, pow2(e0[v]))));
+        const bool any = __any_sync(0xffffffffu, bad);
+        if ((threadIdx.x & 31) == 0) part[v][threadIdx.x >> 5] = best | (any ? 0x80000000u : 0u);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+        uint32_t best = 0, flag = 0;
+#pragma unroll
+        for (int i = 0; i < T / 32; i++) {
+            best = max(best, part[v][i] & 0x7fffffffu);
+            flag |= part[v][i];
+        }
+        const int e = block_exp(__uint_as_float(best));
+        if (used) {
+            int8_t *x = reinterpret_cast<int8_t *>(&w[v]);
+            if (e != e0[v]) {   // (exact in float: |code| < 128, the factor a power of two)
+                const float f = pow2(e0[v] - e);
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (x[i] != kBad) x[i] = (int8_t)to_code((float)x[i], f);
+            }
+            *reinterpret_cast<uint4 *>((v ? p.dst.v : p.dst.k) + ((int64_t)h * p.dst.rows + row) * D + c) = w[v];
+        }
+        if (threadIdx.x == 0)
+            (v ? p.dst.v_scale : p.dst.k_scale)[(int64_t)h * (p.dst.rows / kBlock) + blk] =
+                __uint_as_float(scale_word(e, (flag & 0x80000000u) != 0));
+    }
 }
 
 template <int D>
-void store_d(const StoreParams &p, dim3 grid, cudaStream_t st)
+cudaError_t store_d(const StoreParams &p, dim3 grid, cudaStream_t st)
 {
-    if (p.f16) store_kernel<D, true><<<grid, kBlock * D / 8, 0, st>>>(p);
-    else store_kernel<D, false><<<grid, kBlock * D / 8, 0, st>>>(p);
+    return p.f16 ? launch_pdl(store_kernel<D, true>, grid, kBlock * D / 8, 0, p, st)
+                 : launch_pdl(store_kernel<D, false>, grid, kBlock * D / 8, 0, p, st);
 }
 
 template <int D>
-void load_d(const LoadParams &p, unsigned grid, cudaStream_t st)
+cudaError_t load_d(const LoadParams &p, dim3 grid, cudaStream_t st)
 {
-    if (p.f16) load_kernel<D, true><<<grid, 256, 0, st>>>(p);
-    else load_kernel<D, false><<<grid, 256, 0, st>>>(p);
+    return p.f16 ? launch_pdl(load_kernel<D, true>, grid, 256, 0, p, st)
+                 : launch_pdl(load_kernel<D, false>, grid, 256, 0, p, st);
 }
 
 }  // namespace
@@ -301,43 +442,45 @@ cudaError_t launch_store(const StoreParams &p, cudaStream_t st)
     const int64_t b0 = p.row0 / kBlock, b1 = (p.row0 + p.n_new + kBlock - 1) / kBlock;
     const dim3 grid((unsigned)(b1 - b0), p.c.H, 2);
     switch (p.c.D) {
-    case 64: store_d<64>(p, grid, st); break;
-    case 96: store_d<96>(p, grid, st); break;
-    case 128: store_d<128>(p, grid, st); break;
-    case 256: store_d<256>(p, grid, st); break;
+    case 64: return store_d<64>(p, grid, st);
+    case 96: return store_d<96>(p, grid, st);
+    case 128: return store_d<128>(p, grid, st);
+    case 256: return store_d<256>(p, grid, st);
     default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 cudaError_t launch_load(const LoadParams &p, cudaStream_t st)
 {
-    const int64_t n = 2 * p.n * p.c.H * (p.c.D / 8);
-    const unsigned grid = (unsigned)((n + 255) / 256 < 148 * 64 ? (n + 255) / 256 : 148 * 64);
+    const int64_t pieces = p.n * p.c.H * (p.c.D / 8);   // (at most 2^31 * 2^15 / 2^10 CTAs: checked by the entry point)
+    const dim3 grid((unsigned)((pieces + 256 * kLoadU - 1) / (256 * kLoadU)), p.k && p.v ? 2 : 1);
     switch (p.c.D) {
-    case 64: load_d<64>(p, grid, st); break;
-    case 96: load_d<96>(p, grid, st); break;
-    case 128: load_d<128>(p, grid, st); break;
-    case 256: load_d<256>(p, grid, st); break;
+    case 64: return load_d<64>(p, grid, st);
+    case 96: return load_d<96>(p, grid, st);
+    case 128: return load_d<128>(p, grid, st);
+    case 256: return load_d<256>(p, grid, st);
     default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 cudaError_t launch_evict(const EvictParams &p, cudaStream_t st)
 {
-    select_kernel<<<p.src.H, kSelThreads, 0, st>>>(p);
-    cudaError_t e = cudaGetLastError();
+    static Once once;
+    cudaError_t e = once.on_device([] {
+        return cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSlice * 4);
+    });
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)((p.keep + kBlock - 1) / kBlock), p.src.H, 2);
+    const int64_t cand = p.n_rows - p.recent, per = (cand + kSelCtas * 4 - 1) / (kSelCtas * 4) * 4;
+    e = launch_pdl(select_kernel, dim3(p.src.H * kSelCtas), kSelThreads, per <= kSelSlice ? (size_t)per * 4 : 0, p, st);
+    if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)((p.keep + kBlock - 1) / kBlock), p.src.H);
     switch (p.src.D) {
-    case 64: gather_kernel<64><<<grid, kBlock * 8, 0, st>>>(p); break;
-    case 96: gather_kernel<96><<<grid, kBlock * 12, 0, st>>>(p); break;
-    case 128: gather_kernel<128><<<grid, kBlock * 16, 0, st>>>(p); break;
-    case 256: gather_kernel<256><<<grid, kBlock * 32, 0, st>>>(p); break;
+    case 64: return launch_pdl(gather_kernel<64>, grid, kBlock * 4, 0, p, st);
+    case 96: return launch_pdl(gather_kernel<96>, grid, kBlock * 6, 0, p, st);
+    case 128: return launch_pdl(gather_kernel<128>, grid, kBlock * 8, 0, p, st);
+    case 256: return launch_pdl(gather_kernel<256>, grid, kBlock * 16, 0, p, st);
     default: return cudaErrorInvalidValue;
     }
-    return cudaGetLastError();
 }
 
 }  // namespace q8

@@ -38,5 +38,23 @@ __device__ __forceinline__ int to_code(float y, float inv_scale)
     return max(-127, min(127, __float2int_rn(__fmul_rn(y, inv_scale))));
 }
 
+// A launch that may begin its set-up while the kernel before it in the stream
+// ends; every kernel launched so waits (pdl_wait) before it touches memory.
+template <class K, class P>
+cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, const P &p, cudaStream_t st)
+{
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 }  // namespace q8
 }  // namespace kvb

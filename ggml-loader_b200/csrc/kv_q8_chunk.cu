@@ -705,22 +705,6 @@ __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
     if (lane == 0 && p.row_stat) p.row_stat[(int64_t)h * p.n_new * p.r + (int64_t)tok * p.r + hd] = row_stat_of(M, l);
 }
 
-template <class K>
-cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, const AttendParams &p, cudaStream_t st)
-{
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 template <int D, bool MASKED>
 cudaError_t run(const AttendParams &p, cudaStream_t st)
 {

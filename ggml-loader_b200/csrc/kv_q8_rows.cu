@@ -564,22 +564,6 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
         if (key + i < p.n_kv) dst[i] += sum[i];
 }
 
-template <class K>
-cudaError_t launch_pdl(K kernel, unsigned grid, unsigned block, size_t smem, const AttendParams &p, cudaStream_t st)
-{
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(block);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 template <int D, bool HILO, bool MASKED>
 cudaError_t run(const AttendParams &p, cudaStream_t st)
 {

@@ -309,17 +309,8 @@ cudaError_t run(const AttendParams &p, cudaStream_t st)
         return cudaFuncSetAttribute(weigh_kernel<D, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::bytes);
     });
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)p.c.H * p.n_kt, kSMs * L::ctas));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = L::bytes;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, weigh_kernel<D, MASKED>, p);
+    const unsigned grid = (unsigned)std::min<int64_t>((int64_t)p.c.H * p.n_kt, kSMs * L::ctas);
+    return launch_pdl(weigh_kernel<D, MASKED>, grid, kThreads, L::bytes, p, st);
 }
 
 }  // namespace
