@@ -177,13 +177,25 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadParams p)
 #pragma unroll
     for (int k = 0; k < kLoadU; k++) {
         if (at[k] < 0) continue;
-        float x[8];
-        decode8(w[k], scale_exp(s[k]), x);
+        const int e0 = scale_exp(s[k]);
         if constexpr (F16) {
             __half *dst = static_cast<__half *>(out) + at[k];
             __half y[8];
+            if ((s[k] & 0x7f800000u) == 0x7f800000u) {   // a block with values that are not finite
+                float x[8];
+                decode8(w[k], e0, x);
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = __float2half_rn(x[e]);
+                for (int e = 0; e < 8; e++) y[e] = __float2half_rn(x[e]);
+            } else {
+                // the codes as halves times 2^e0, both exact (2^-24 is the smallest half)
+                const __half2 f = __half2half2(__float2half_rn(pow2(e0)));
+                const uint2 a = codes_to_half4(w[k].x), b = codes_to_half4(w[k].y);
+                __half2 *y2 = reinterpret_cast<__half2 *>(y);
+                y2[0] = __hmul2(*reinterpret_cast<const __half2 *>(&a.x), f);
+                y2[1] = __hmul2(*reinterpret_cast<const __half2 *>(&a.y), f);
+                y2[2] = __hmul2(*reinterpret_cast<const __half2 *>(&b.x), f);
+                y2[3] = __hmul2(*reinterpret_cast<const __half2 *>(&b.y), f);
+            }
             if (p.vec) {
                 *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);
             } else {
@@ -192,6 +204,8 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadParams p)
             }
         } else {
             float *dst = static_cast<float *>(out) + at[k];
+            float x[8];
+            decode8(w[k], e0, x);
             if (p.vec) {
                 reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
                 reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -356,69 +370,102 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
     }
 }
 
-// One CTA a block of dst and KV head, K and V: a row is D/16 threads, 16 codes
-// each of K and of V, so both gathers are in flight together.
-template <int D>
+// U blocks of dst of a KV head a CTA, K and V: a row is D/16 threads, 16 codes
+// each of K and of V of every block, so 2 U gathers a thread are in flight
+// together (32k rows to 16k: 38 us with one block a CTA).
+template <int D, int U>
 __global__ void __launch_bounds__(kBlock *D / 16) gather_kernel(const EvictParams p)
 {
     constexpr int T = kBlock * D / 16;
-    __shared__ uint32_t part[2][T / 32];
+    __shared__ uint32_t part[2 * U][T / 32];
     const int r = threadIdx.x / (D / 16), c = threadIdx.x % (D / 16) * 16;
     const int h = blockIdx.y;
-    const int64_t blk = blockIdx.x, row = blk * kBlock + r;
-    const bool used = row < p.keep;
-    uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-    int e0[2] = {kExpMin, kExpMin};
+    const int64_t row0 = (int64_t)blockIdx.x * (U * kBlock) + r;
+    const int32_t *kept = p.kept + (int64_t)h * p.keep;
+    const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.src.k_scale) + (int64_t)h * (p.src.rows / kBlock);
+    const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.src.v_scale) + (int64_t)h * (p.src.rows / kBlock);
+    uint4 w[U][2];
+    uint32_t sc[U][2];
+    int32_t from[U];
     pdl_launch_dependents();
     pdl_wait();
-    if (used) {
-        const int64_t from = p.kept[(int64_t)h * p.keep + row], at = ((int64_t)h * p.src.rows + from) * D + c;
-        const int64_t sc = (int64_t)h * (p.src.rows / kBlock) + from / kBlock;
-        w[0] = *reinterpret_cast<const uint4 *>(p.src.k + at);
-        w[1] = *reinterpret_cast<const uint4 *>(p.src.v + at);
-        e0[0] = scale_exp(reinterpret_cast<const uint32_t *>(p.src.k_scale)[sc]);
-        e0[1] = scale_exp(reinterpret_cast<const uint32_t *>(p.src.v_scale)[sc]);
-        if (c == 0 && p.dst.weight) p.dst.weight[(int64_t)h * p.dst.rows + row] = p.src.weight[(int64_t)h * p.src.rows + from];
+#pragma unroll
+    for (int u = 0; u < U; u++) from[u] = row0 + u * kBlock < p.keep ? kept[row0 + u * kBlock] : -1;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+        sc[u][0] = sc[u][1] = scale_word(kExpMin, false);
+        if (from[u] < 0) continue;
+        const int64_t at = ((int64_t)h * p.src.rows + from[u]) * D + c;
+        w[u][0] = *reinterpret_cast<const uint4 *>(p.src.k + at);
+        w[u][1] = *reinterpret_cast<const uint4 *>(p.src.v + at);
+        sc[u][0] = ksc[from[u] / kBlock];
+        sc[u][1] = vsc[from[u] / kBlock];
+    }
+    if (c == 0 && p.dst.weight) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (from[u] >= 0)
+                p.dst.weight[(int64_t)h * p.dst.rows + row0 + u * kBlock] = p.src.weight[(int64_t)h * p.src.rows + from[u]];
     }
     // the largest magnitude, code * 2^e: exact in float, whose bits order as it does
 #pragma unroll
-    for (int v = 0; v < 2; v++) {
-        const int8_t *x = reinterpret_cast<const int8_t *>(&w[v]);
-        int top = 0;
-        bool bad = false;
+    for (int v = 0; v < 2 * U; v++) {
+        const uint4 &x = w[v >> 1][v & 1];
+        // magnitudes of four codes at once (-128 gives 128, which marks a value that is not finite)
+        uint32_t m = __vmaxu4(__vmaxu4(__vabs4(x.x), __vabs4(x.y)), __vmaxu4(__vabs4(x.z), __vabs4(x.w)));
+        bool bad = (m & 0x80808080u) != 0;
+        if (bad) {
+            const int8_t *q = reinterpret_cast<const int8_t *>(&x);
+            int top = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            bad |= x[i] == kBad;
-            top = max(top, x[i] == kBad ? 0 : abs((int)x[i]));
+            for (int i = 0; i < 16; i++) top = max(top, q[i] == kBad ? 0 : abs((int)q[i]));
+            m = top;
         }
-        const uint32_t best = __reduce_max_sync(0xffffffffu, __float_as_uint(__fmul_rn((float)top, pow2(e0[v]))));
+        m = max(max(m & 255u, (m >> 8) & 255u), max((m >> 16) & 255u, m >> 24));
+        const float f = __fmul_rn((float)m, pow2(scale_exp(sc[v >> 1][v & 1])));
+        const uint32_t best = __reduce_max_sync(0xffffffffu, __float_as_uint(f));
         const bool any = __any_sync(0xffffffffu, bad);
         if ((threadIdx.x & 31) == 0) part[v][threadIdx.x >> 5] = best | (any ? 0x80000000u : 0u);
     }
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < 2; v++) {
+    for (int v = 0; v < 2 * U; v++) {
+        const int u = v >> 1;
+        const bool is_v = (v & 1) != 0;
+        if ((int64_t)blockIdx.x * (U * kBlock) + u * kBlock >= p.keep) break;   // (a block without rows)
         uint32_t best = 0, flag = 0;
 #pragma unroll
         for (int i = 0; i < T / 32; i++) {
             best = max(best, part[v][i] & 0x7fffffffu);
             flag |= part[v][i];
         }
-        const int e = block_exp(__uint_as_float(best));
-        if (used) {
-            int8_t *x = reinterpret_cast<int8_t *>(&w[v]);
-            if (e != e0[v]) {   // (exact in float: |code| < 128, the factor a power of two)
-                const float f = pow2(e0[v] - e);
+        const int e = block_exp(__uint_as_float(best)), e0 = scale_exp(sc[u][v & 1]);
+        if (from[u] >= 0) {
+            uint4 &x4 = w[u][v & 1];
+            if (e != e0) {   // (exact in float: |code| < 128, the factor a power of two)
+                int8_t *x = reinterpret_cast<int8_t *>(&x4);
+                const float f = pow2(e0 - e);
 #pragma unroll
                 for (int i = 0; i < 16; i++)
                     if (x[i] != kBad) x[i] = (int8_t)to_code((float)x[i], f);
             }
-            *reinterpret_cast<uint4 *>((v ? p.dst.v : p.dst.k) + ((int64_t)h * p.dst.rows + row) * D + c) = w[v];
+            *reinterpret_cast<uint4 *>((is_v ? p.dst.v : p.dst.k) + ((int64_t)h * p.dst.rows + row0 + u * kBlock) * D + c) = x4;
         }
         if (threadIdx.x == 0)
-            (v ? p.dst.v_scale : p.dst.k_scale)[(int64_t)h * (p.dst.rows / kBlock) + blk] =
+            (is_v ? p.dst.v_scale : p.dst.k_scale)[(int64_t)h * (p.dst.rows / kBlock) + (int64_t)blockIdx.x * U + u] =
                 __uint_as_float(scale_word(e, (flag & 0x80000000u) != 0));
     }
+}
+
+template <int D>
+cudaError_t gather_d(const EvictParams &p, cudaStream_t st)
+{
+    const int64_t blocks = (p.keep + kBlock - 1) / kBlock;
+    // four blocks a CTA once that leaves two CTAs an SM
+    if (blocks * p.src.H >= 4 * 2 * kSMs)
+        return launch_pdl(gather_kernel<D, 4>, dim3((unsigned)((blocks + 3) / 4), p.src.H), kBlock * D / 16, 0, p, st);
+    return launch_pdl(gather_kernel<D, 1>, dim3((unsigned)blocks, p.src.H), kBlock * D / 16, 0, p, st);
 }
 
 template <int D>
@@ -473,12 +520,11 @@ cudaError_t launch_evict(const EvictParams &p, cudaStream_t st)
     const int64_t cand = p.n_rows - p.recent, per = (cand + kSelCtas * 4 - 1) / (kSelCtas * 4) * 4;
     e = launch_pdl(select_kernel, dim3(p.src.H * kSelCtas), kSelThreads, per <= kSelSlice ? (size_t)per * 4 : 0, p, st);
     if (e != cudaSuccess) return e;
-    const dim3 grid((unsigned)((p.keep + kBlock - 1) / kBlock), p.src.H);
     switch (p.src.D) {
-    case 64: return launch_pdl(gather_kernel<64>, grid, kBlock * 4, 0, p, st);
-    case 96: return launch_pdl(gather_kernel<96>, grid, kBlock * 6, 0, p, st);
-    case 128: return launch_pdl(gather_kernel<128>, grid, kBlock * 8, 0, p, st);
-    case 256: return launch_pdl(gather_kernel<256>, grid, kBlock * 16, 0, p, st);
+    case 64: return gather_d<64>(p, st);
+    case 96: return gather_d<96>(p, st);
+    case 128: return gather_d<128>(p, st);
+    case 256: return gather_d<256>(p, st);
     default: return cudaErrorInvalidValue;
     }
 }

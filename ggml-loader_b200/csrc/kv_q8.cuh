@@ -38,6 +38,16 @@ __device__ __forceinline__ int to_code(float y, float inv_scale)
     return max(-127, min(127, __float2int_rn(__fmul_rn(y, inv_scale))));
 }
 
+// four signed codes -> four halves in order (0x6400 | u is the half 1024 + u)
+__device__ __forceinline__ uint2 codes_to_half4(uint32_t w)
+{
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 hx = __hsub2(*reinterpret_cast<__half2 *>(&x), off), hy = __hsub2(*reinterpret_cast<__half2 *>(&y), off);
+    return make_uint2(*reinterpret_cast<const uint32_t *>(&hx), *reinterpret_cast<const uint32_t *>(&hy));
+}
+
 // A launch that may begin its set-up while the kernel before it in the stream
 // ends; every kernel launched so waits (pdl_wait) before it touches memory.
 template <class K, class P>

@@ -20,16 +20,6 @@ __device__ __forceinline__ void give_up(unsigned *error, volatile int *flag, uns
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// four signed codes -> four halves in order (0x6400 | u is the half 1024 + u)
-__device__ __forceinline__ uint2 codes_to_half4(uint32_t w)
-{
-    const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));
-    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 hx = __hsub2(*reinterpret_cast<__half2 *>(&x), off), hy = __hsub2(*reinterpret_cast<__half2 *>(&y), off);
-    return make_uint2(*reinterpret_cast<const uint32_t *>(&hx), *reinterpret_cast<const uint32_t *>(&hy));
-}
-
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v)
 {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
