@@ -1,4 +1,5 @@
-"""Build the KV path library in-tree: ggml-loader_b200/lib/libkv_b200.so.
+"""Build the KV path library in-tree: ggml-loader_b200/lib/libkv_b200.so (and
+the Python binding's C module, ggml-loader_b200/kv_b200/_q8call.so).
 
 Every CUDA source is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a); host sources go through nvcc to
@@ -11,6 +12,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -18,6 +20,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "lib", "libkv_b200.so")
 INCLUDE = os.path.join(ROOT, "include")
+CALLS = os.path.join(HERE, "kv_b200", "_q8call.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -68,7 +71,19 @@ def build(verbose=False, lib=LIB, obj_dir=OBJ, defines=()):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (" ".join(cmd), r.stderr))
+    build_calls()
     return lib
+
+
+def build_calls():
+    """The Python binding's C module (kv_b200/q8call.c)."""
+    src = os.path.join(HERE, "kv_b200", "q8call.c")
+    if _stale(CALLS, [src] + _headers()):
+        cmd = ["gcc", "-O2", "-shared", "-fPIC", "-Wall", "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], src, "-o", CALLS]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("gcc failed for %s:\n%s\n%s" % (src, " ".join(cmd), r.stderr))
+    return CALLS
 
 
 # the phase-stamp measurement build (kv_debug_stamps; python -m kv_b200.stamps)

@@ -373,6 +373,22 @@ def attend_decode_noalloc(k_cache, v_cache, n_head, n_head_kv, head_dim, n_kv, q
 
 
 Q8_BLOCK = 32
+_q8calls = None
+
+
+def _calls():
+    """The binding's C module with the loaded library's entry points (raises if it is not built)."""
+    global _q8calls
+    if _q8calls is None:
+        import torch
+        try:
+            from . import _q8call
+        except ImportError as e:
+            raise ImportError("kv_b200/_q8call.so is not built (%s); run ggml-loader_b200/build.py" % e)
+        address = [ctypes.cast(getattr(lib(), n), _vp).value for n in ("kv_q8_store", "kv_q8_load", "kv_q8_attend")]
+        _q8call.init(torch.float32, torch.float16, *address)
+        _q8calls = _q8call
+    return _q8calls
 
 
 class Q8Cache:
@@ -398,53 +414,27 @@ class Q8Cache:
         self.n_head_kv, self.rows, self.head_dim = h, rows, d
         self._c = KvQ8Cache(*[_ptr(t) for t in self.tensors], rows, h, d)
         self._ref = ctypes.addressof(self._c)
-        # what each call looks up, once: a decoded token's call is a few microseconds
-        self._torch, self._lib, self._index = torch, lib(), k.get_device()
-        self._types = {torch.float32: 0, torch.float16: 1}
+        self._lib, self._calls, self._index = lib(), _calls(), k.get_device()
+        self._width = h * d
+        self._torch = torch
         self._current = torch._C._cuda_getDevice if self._index >= 0 else None
 
-    def _rows(self, name, t, n, width):
-        """(pointer, stride, type) of a tensor of n rows of `width` elements."""
-        kind = self._types.get(t.dtype)
-        if kind is None:
-            raise ValueError("%s must be float32 or float16" % name)
-        shape, stride = t.shape, t.stride()
-        if t.get_device() != self._index or not shape or shape[0] != n or t.numel() != n * width:
-            raise ValueError("%s must hold %d rows of %d elements on the cache's device" % (name, n, width))
-        inner = 1
-        for i in range(len(shape) - 1, 0, -1):
-            if shape[i] != 1 and stride[i] != inner:
-                raise ValueError("the rows of %s must be contiguous" % name)
-            inner *= shape[i]
-        return t.data_ptr(), stride[0], kind
-
-    def _call(self, fn, *args):
-        """fn on this cache, on its device."""
-        if self._current is not None and self._current() != self._index:
-            with self._torch.cuda.device(self._index):
-                rc = fn(self._ref, *args)
+    def _on_device(self, fn, *args):
+        """fn(*args), which returns a KV_* code, on the cache's device."""
+        if self._current is None or self._current() == self._index:
+            rc = fn(*args)
         else:
-            rc = fn(self._ref, *args)
-        return rc if rc == KV_OK else _check(rc, fn.__name__)
+            with self._torch.cuda.device(self._index):
+                rc = fn(*args)
+        return rc if rc == KV_OK else _check(rc, "kv_q8_" + fn.__name__.replace("kv_q8_", ""))
 
     def store(self, row0, n_new, k, v, stream=None):
         """kv_q8_store: n_new rows of [n_head_kv][head_dim] at row0."""
-        width = self.n_head_kv * self.head_dim
-        kp, ks, kt = self._rows("k", k, n_new, width)
-        vp, vs, vt = self._rows("v", v, n_new, width)
-        if kt != vt:
-            raise ValueError("k and v must have one type")
-        return self._call(self._lib.kv_q8_store, row0, n_new, kp, ks, vp, vs, kt, _stream(stream))
+        return self._on_device(self._calls.store, self._ref, self._index, self._width, row0, n_new, k, v, stream)
 
     def load(self, row0, n, k_out, v_out, stream=None):
         """kv_q8_load: the values of n rows from row0 into k_out and v_out (either may be None)."""
-        width = self.n_head_kv * self.head_dim
-        k = (None,) if k_out is None else self._rows("k_out", k_out, n, width)
-        v = (None,) if v_out is None else self._rows("v_out", v_out, n, width)
-        if k[1:] != v[1:] and k[0] and v[0]:
-            raise ValueError("k_out and v_out must have one type and row stride")
-        stride, kind = k[1:] or v[1:] or (0, 0)
-        return self._call(self._lib.kv_q8_load, row0, n, k[0], v[0], stride, kind, _stream(stream))
+        return self._on_device(self._calls.load, self._ref, self._index, self._width, row0, n, k_out, v_out, stream)
 
     def attend_workspace(self, n_head, n_past, n_new):
         """Bytes of workspace attend needs for these sizes."""
@@ -456,20 +446,8 @@ class Q8Cache:
     def attend(self, n_head, n_past, n_new, q, out, mask=None, flash=False, workspace=None, stream=None):
         """kv_q8_attend: n_new rows of [n_head][head_dim] queries over the rows
         [0, n_past + n_new); workspace: a contiguous CUDA tensor of attend_workspace bytes."""
-        width = n_head * self.head_dim
-        qp, qs, qt = self._rows("q", q, n_new, width)
-        op, os_, ot = self._rows("out", out, n_new, width)
-        mp, mt, ms = None, 0, 0
-        if mask is not None:
-            mt = self._types.get(mask.dtype)
-            if mt is None or mask.dim() != 2 or mask.stride(1) != 1 or mask.shape[0] != n_new or \
-                    mask.shape[1] < n_past + n_new or mask.get_device() != self._index:
-                raise ValueError("mask must be [n_new][>= n_past + n_new], float32 or float16, on the cache's device")
-            mp, ms = mask.data_ptr(), mask.stride(0)
-        if workspace is None or workspace.get_device() != self._index or not workspace.is_contiguous():
-            raise ValueError("attend needs a contiguous workspace tensor on the cache's device")
-        return self._call(self._lib.kv_q8_attend, n_head, n_past, n_new, qp, qs, qt, mp, mt, ms, 1 if flash else 0,
-                          op, os_, ot, workspace.data_ptr(), workspace.nbytes, _stream(stream))
+        return self._on_device(self._calls.attend, self._ref, self._index, self.head_dim, n_head, n_past, n_new, q, out,
+                               mask, flash, workspace, stream)
 
     def status(self, stream=None):
         """KV_OK, or KV_E_TIMEOUT if a bounded device-side wait of an attend expired (raises)."""
@@ -482,7 +460,8 @@ class Q8Cache:
                 kept.get_device() != self._index or dst._index != self._index:
             raise ValueError("kept must be a contiguous int32 [%d][%d] tensor on the cache's device, dst there too"
                              % (self.n_head_kv, keep))
-        return self._call(self._lib.kv_q8_evict, n_rows, keep, recent, dst._ref, kept.data_ptr(), _stream(stream))
+        return self._on_device(self._lib.kv_q8_evict, self._ref, n_rows, keep, recent, dst._ref, kept.data_ptr(),
+                               _stream(stream))
 
 
 def gen_normal_device(dst, seed, stream_id, n, idx0=0, stream=None):
