@@ -67,10 +67,9 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi)
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// 4 query elements as two F16 pairs
-__device__ __forceinline__ uint2 load_q4(const AttendParams &p, int t, int hq, int D, int d)
+// 4 query elements from element i on, as two F16 pairs
+__device__ __forceinline__ uint2 load_q4(const AttendParams &p, int64_t i)
 {
-    const int64_t i = t * p.q_stride + (int64_t)hq * D + d;
     __half x[4];
     if (p.q_f16) {
         if (p.q_vec) return *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + i);
@@ -87,6 +86,11 @@ __device__ __forceinline__ uint2 load_q4(const AttendParams &p, int t, int hq, i
         for (int k = 0; k < 4; k++) x[k] = __float2half_rn(static_cast<const float *>(p.q)[i + k]);
     }
     return make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+}
+
+__device__ __forceinline__ void l2_prefetch_bulk(const void *p, uint32_t bytes)
+{
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ float mask_value(const AttendParams &p, int t, int64_t key)
@@ -167,41 +171,38 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
     char *ring = smem + warp * G::ring;
     const int64_t T = (int64_t)p.n_vh * p.nb, lo = blockIdx.x * T / p.n_cta, hi = (blockIdx.x + 1) * T / p.n_cta;
     pdl_launch_dependents();
-    pdl_wait();
-
+    if (threadIdx.x < 2 && lo < hi) {
+        // While the kernel before this one ends, HBM brings the CTA's first codes
+        // to L2 (a hint: what that kernel still writes is read anew below).
+        const int h = (int)(lo / p.nb), b0 = (int)(lo - (int64_t)h * p.nb);
+        const int n = min(min(p.nb - b0, (int)(hi - lo)), p.l2_ahead);
+        if (n > 0)
+            l2_prefetch_bulk((threadIdx.x ? p.c.v : p.c.k) + ((int64_t)h * p.c.rows + (int64_t)b0 * kBlock) * D, n * kBlock * D);
+    }
+    bool waited = false;
     for (int64_t pos = lo; pos < hi;) {
-        const int vh = (int)(pos / p.nb), b0 = (int)(pos - (int64_t)vh * p.nb);
+        const int h = (int)(pos / p.nb), b0 = (int)(pos - (int64_t)h * p.nb);
         const int b1 = (int)min((int64_t)p.nb, b0 + hi - pos);
         pos += b1 - b0;
-        const int h = vh, nrows = p.n_new * p.r;   // (at most 8 with HILO, else 16)
+        const int nrows = p.n_new * p.r;   // (at most 8 with HILO, else 16)
         const int8_t *kc = p.c.k + (int64_t)h * p.c.rows * D, *vc = p.c.v + (int64_t)h * p.c.rows * D;
         const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)h * (p.c.rows / kBlock);
         const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.c.v_scale) + (int64_t)h * (p.c.rows / kBlock);
-
-        // The small loads first: behind the ring's they would wait for all of them.
-        // Q as the A operand: rows g and g + 8, dims 4 t4 .. + 3 of each 16 (the
-        // order in which a thread holds a key's codes)
-        uint2 q[G::q_regs ? G::nk : 1][RT];
+        // rows g and g + 8: token and where their queries start
         int tok[RT];
+        int64_t qat[RT];
+        bool have[RT];
 #pragma unroll
         for (int i = 0; i < RT; i++) {
             const int row = g + 8 * i;
-            const bool have = row < nrows;
-            tok[i] = have ? row / p.r : 0;
-            if constexpr (G::q_regs) {
-                const int hq = h * p.r + (have ? row % p.r : 0);
-#pragma unroll
-                for (int k = 0; k < G::nk; k++)
-                    q[k][i] = have ? load_q4(p, tok[i], hq, D, k * 16 + t4 * 4) : make_uint2(0, 0);
-            }
+            have[i] = row < nrows;
+            tok[i] = have[i] ? row / p.r : 0;
+            qat[i] = tok[i] * p.q_stride + (int64_t)(h * p.r + (have[i] ? row - tok[i] * p.r : 0)) * D + t4 * 4;
         }
-        if constexpr (!G::q_regs) {
-            for (int i = threadIdx.x; i < 8 * RT * (D / 4); i += G::W * 32) {
-                const int row = i / (D / 4), c = i % (D / 4);
-                s_q[row][c] = row < nrows ? load_q4(p, row / p.r, h * p.r + row % p.r, D, c * 4)
-                                          : make_uint2(0, 0);
-            }
-        }
+        if (!waited) pdl_wait();   // (nothing before it reads memory)
+        waited = true;
+
+        // The small loads first: behind the ring's they would wait for all of them.
         // the scale words of this warp's next 32 blocks, one a lane
         uint32_t kw = 0, vw = 0;
         auto scales = [&](int b) {
@@ -210,6 +211,30 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
             vw = mine < b1 ? vsc[mine] : 0;
         };
         scales(b0 + warp);
+        // Q as the A operand: dims 4 t4 .. + 3 of each 16 (the order in which a
+        // thread holds a key's codes)
+        uint2 q[G::q_regs ? G::nk : 1][RT];
+        if constexpr (G::q_regs) {
+            if (p.q_f16 && p.q_vec) {
+#pragma unroll
+                for (int i = 0; i < RT; i++)
+#pragma unroll
+                    for (int k = 0; k < G::nk; k++)
+                        q[k][i] = have[i] ? *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + qat[i] + k * 16)
+                                          : make_uint2(0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < RT; i++)
+#pragma unroll
+                    for (int k = 0; k < G::nk; k++) q[k][i] = have[i] ? load_q4(p, qat[i] + k * 16) : make_uint2(0, 0);
+            }
+        } else {
+            for (int i = threadIdx.x; i < 8 * RT * (D / 4); i += G::W * 32) {
+                const int row = i / (D / 4), c = i % (D / 4), t = row / p.r;
+                s_q[row][c] = row < nrows ? load_q4(p, t * p.q_stride + (int64_t)(h * p.r + row - t * p.r) * D + c * 4)
+                                          : make_uint2(0, 0);
+            }
+        }
 
         // this warp's blocks: b0 + warp, then every W-th; their tiles K, V, K, V ... through the ring
         int fb = b0 + warp, fs = 0;
@@ -252,22 +277,24 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
 #pragma unroll
             for (int j = 0; j < 4; j++) o[i][j] = 0.0f;
 
+        // a block's mask values, one block ahead
+        float mk[MASKED ? RT : 1][8];
+        auto masks = [&](int b) {
+#pragma unroll
+            for (int i = 0; i < RT; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int64_t key = (int64_t)b * kBlock + (j >> 1) * 8 + 2 * t4 + (j & 1);
+                    mk[MASKED ? i : 0][j] = key < p.n_kv ? mask_value(p, tok[i], key) : -CUDART_INF_F;
+                }
+        };
+        if (MASKED && b0 + warp < b1) masks(b0 + warp);
         for (int b = b0 + warp, n = 0; b < b1; b += G::W, n++) {
             if (n && (n & 31) == 0) scales(b);
             const uint32_t kword = __shfl_sync(0xffffffffu, kw, n & 31), vword = __shfl_sync(0xffffffffu, vw, n & 31);
             const bool k_bad = (kword & 0x7f800000u) == 0x7f800000u, v_bad = (vword & 0x7f800000u) == 0x7f800000u;
             const float ks = k_bad ? CUDART_NAN_F : pow2(scale_exp(kword)), ev = (float)scale_exp(vword);
             const int64_t key0 = (int64_t)b * kBlock;
-            float mk[RT][8];
-            if constexpr (MASKED) {
-#pragma unroll
-                for (int i = 0; i < RT; i++)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int64_t key = key0 + (j >> 1) * 8 + 2 * t4 + (j & 1);
-                        mk[i][j] = key < p.n_kv ? mask_value(p, tok[i], key) : -CUDART_INF_F;
-                    }
-            }
             // S = Q K^T: 4 groups of 8 keys, 32 dims at a time
             const uint32_t kt = next_tile() + (lane & 7) * G::pitch + (lane >> 3) * 16;
             float acc[4][4];
@@ -315,6 +342,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
                     if constexpr (MASKED) w[i][j] = mk[i][j] == -CUDART_INF_F ? mk[i][j] : __fmaf_rn(d, cs, mk[i][j]);
                     else w[i][j] = d * cs;
                 }
+                if (MASKED && i == RT - 1 && b + G::W < b1) masks(b + G::W);
                 if (!MASKED && key0 + kBlock > p.n_past) {
 #pragma unroll
                     for (int j = 0; j < 8; j++)
@@ -403,7 +431,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
         }
         __syncthreads();
         const bool whole = b0 == 0 && b1 == p.nb;
-        const int64_t part = (int64_t)blockIdx.x + vh;   // (CTA, head) pairs in order: their sum counts them
+        const int64_t part = (int64_t)blockIdx.x + h;   // (CTA, head) pairs in order: their sum counts them
         constexpr float unit = MASKED ? kLog2e : 1.0f;
         for (int i = threadIdx.x; i < nrows * (D / 4); i += G::W * 32) {
             const int row = i / (D / 4), c = i % (D / 4) * 4;
@@ -442,58 +470,76 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
     }
 }
 
-// The CTAs of head vh (the split of rows_kernel).
-__device__ __forceinline__ void span_of(const AttendParams &p, int vh, int &a, int &b)
+// The CTAs of head h (the split of rows_kernel).
+__device__ __forceinline__ void span_of(const AttendParams &p, int h, int &a, int &b)
 {
-    const int64_t T = (int64_t)p.n_vh * p.nb, x0 = (int64_t)vh * p.nb, x1 = x0 + p.nb - 1;
+    const int64_t T = (int64_t)p.n_vh * p.nb, x0 = (int64_t)h * p.nb, x1 = x0 + p.nb - 1;
     // CTA c holds [c T / C, (c + 1) T / C): position x is in floor(((x + 1) C - 1) / T)
     a = (int)(((x0 + 1) * p.n_cta - 1) / T);
     b = (int)(((x1 + 1) * p.n_cta - 1) / T);
 }
 
-// Joins the CTAs' partial rows: one CTA a (head, row); with weights,
-// CTAs behind those add the softmax weights of 512 keys of a head.
+// Joins the CTAs' partial rows: one CTA a (head, row), each of its four warps a
+// quarter of the parts, kJoinU of them and their (m, l) in flight together.
+// With weights, CTAs behind those add the softmax weights of 512 keys of a head.
+constexpr int kJoinU = 5;
+
 template <int D, bool MASKED>
 __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
 {
     constexpr float unit = MASKED ? kLog2e : 1.0f;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int n_join = p.n_vh * 16;
+    const int R = p.n_new * p.r, n_join = p.n_vh * R;
     pdl_launch_dependents();
-    pdl_wait();
     if ((int)blockIdx.x < n_join) {
         __shared__ float4 s_o[4][D / 4];
         __shared__ float2 s_ml[4];
-        const int vh = blockIdx.x >> 4, h = vh, row = blockIdx.x & 15;
-        if (row >= p.n_new * p.r) return;
+        const int h = blockIdx.x / R, row = blockIdx.x - h * R;
         int a, b;
-        span_of(p, vh, a, b);
+        span_of(p, h, a, b);
+        const int t = row / p.r;
+        const int64_t out = t * p.out_stride + (int64_t)(h * p.r + row - t * p.r) * D;
+        pdl_wait();
         if (a == b) return;   // rows_kernel wrote the output
-        // each warp a quarter of the parts, then the four
-        float M = -CUDART_INF_F;
-        for (int c = a + lane; c <= b; c += 32) M = fmaxf(M, p.stat[((int64_t)c + vh) * 16 + row].x);
-#pragma unroll
-        for (int k = 16; k; k >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, k));
-        const float ref = M == -CUDART_INF_F ? 0.0f : M;
         constexpr int V = (D / 4 + 31) / 32;
         float4 x[V];
 #pragma unroll
         for (int v = 0; v < V; v++) x[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float l = 0.0f;
-#pragma unroll 4
-        for (int c = a + warp; c <= b; c += 4) {
-            const int64_t at = ((int64_t)c + vh) * 16 + row;
-            const float2 s = p.stat[at];
-            const float f = ex2_approx((s.x - ref) * unit);
-            l = __fmaf_rn(s.y, f, l);
+        float M = -CUDART_INF_F, l = 0.0f;
+        for (int c0 = a + warp; c0 <= b; c0 += 4 * kJoinU) {
+            float2 s[kJoinU];
+            float4 y[kJoinU][V];
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                if (lane + 32 * v >= D / 4) continue;
-                const float4 y = *reinterpret_cast<const float4 *>(p.part + at * D + (lane + 32 * v) * 4);
-                x[v].x = __fmaf_rn(y.x, f, x[v].x);
-                x[v].y = __fmaf_rn(y.y, f, x[v].y);
-                x[v].z = __fmaf_rn(y.z, f, x[v].z);
-                x[v].w = __fmaf_rn(y.w, f, x[v].w);
+            for (int u = 0; u < kJoinU; u++) {
+                const int c = c0 + 4 * u;
+                const int64_t at = ((int64_t)c + h) * 16 + row;
+                s[u] = c <= b ? p.stat[at] : make_float2(-CUDART_INF_F, 0.0f);
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    y[u][v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (c <= b && lane + 32 * v < D / 4)
+                        y[u][v] = *reinterpret_cast<const float4 *>(p.part + at * D + (lane + 32 * v) * 4);
+                }
+            }
+            float top = M;
+#pragma unroll
+            for (int u = 0; u < kJoinU; u++) top = fmaxf(top, s[u].x);
+            const float ref = top == -CUDART_INF_F ? 0.0f : top, f0 = ex2_approx((M - ref) * unit);
+            M = top;
+            l *= f0;
+#pragma unroll
+            for (int v = 0; v < V; v++) x[v] = make_float4(x[v].x * f0, x[v].y * f0, x[v].z * f0, x[v].w * f0);
+#pragma unroll
+            for (int u = 0; u < kJoinU; u++) {
+                const float f = ex2_approx((s[u].x - ref) * unit);
+                l = __fmaf_rn(s[u].y, f, l);
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    x[v].x = __fmaf_rn(y[u][v].x, f, x[v].x);
+                    x[v].y = __fmaf_rn(y[u][v].y, f, x[v].y);
+                    x[v].z = __fmaf_rn(y[u][v].z, f, x[v].z);
+                    x[v].w = __fmaf_rn(y[u][v].w, f, x[v].w);
+                }
             }
         }
 #pragma unroll
@@ -501,13 +547,23 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
             if (lane + 32 * v < D / 4) s_o[warp][lane + 32 * v] = x[v];
         if (lane == 0) s_ml[warp] = make_float2(M, l);
         __syncthreads();
-        l = (s_ml[0].y + s_ml[1].y) + (s_ml[2].y + s_ml[3].y);
+        // the four warps' sums, each relative to its own maximum
+        M = fmaxf(fmaxf(s_ml[0].x, s_ml[1].x), fmaxf(s_ml[2].x, s_ml[3].x));
+        const float ref = M == -CUDART_INF_F ? 0.0f : M;
+        float f[4];
+        l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            f[k] = ex2_approx((s_ml[k].x - ref) * unit);
+            l = __fmaf_rn(s_ml[k].y, f[k], l);
+        }
         const float z = inverse_sum(l, p.flash != 0);
-        const int t = row / p.r, j = row % p.r;
-        const int64_t at = t * p.out_stride + (int64_t)(h * p.r + j) * D;
+        const float *o0 = reinterpret_cast<const float *>(s_o);
         for (int d = tid; d < D; d += 128) {
-            const float *o0 = reinterpret_cast<const float *>(s_o);
-            store_out(p, at + d, ((o0[d] + o0[D + d]) + (o0[2 * D + d] + o0[3 * D + d])) * z);
+            float y = o0[d] * f[0];
+#pragma unroll
+            for (int k = 1; k < 4; k++) y = __fmaf_rn(o0[k * D + d], f[k], y);
+            store_out(p, out + d, y * z);
         }
         return;
     }
@@ -516,9 +572,9 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
     const int chunks = (int)(((int64_t)p.nb * kBlock + 511) / 512);
     const int w = blockIdx.x - n_join, h = w / chunks;
     const int64_t key = (int64_t)(w - h * chunks) * 512 + tid * 4;
-    const int R = p.n_new * p.r;
     int a, b;
     span_of(p, h, a, b);
+    pdl_wait();
     {
         const int row = tid >> 3, sub = tid & 7;
         float M = -CUDART_INF_F, l = 0.0f;
@@ -576,7 +632,7 @@ cudaError_t run(const AttendParams &p, cudaStream_t st)
     if (e != cudaSuccess) return e;
     const bool split = p.n_cta > p.n_vh || p.n_vh % p.n_cta != 0;   // else every head lies in one CTA
     if (!split && !p.scores) return cudaSuccess;
-    unsigned grid = (unsigned)p.n_vh * 16;
+    unsigned grid = (unsigned)(p.n_vh * p.n_new * p.r);
     if (p.scores) grid += (unsigned)(p.c.H * (((int64_t)p.nb * kBlock + 511) / 512));
     return launch_pdl(join_kernel<D, MASKED>, grid, 128, 0, p, st);
 }
@@ -591,9 +647,11 @@ cudaError_t run_d(const AttendParams &p, cudaStream_t st)
 
 }  // namespace
 
-// CTAs: one an SM, about a block a warp each at least, and a multiple of the
-// heads where there are SMs for it or it idles at most 5 % of them (a CTA then
-// works on one head; 8 heads of 2000 keys: 63 CTAs 11.0 us, 64 CTAs 8.0 us).
+// CTAs: one an SM, about a block a warp each at least.  A CTA that crosses from
+// one head to the next ends and begins a head once more, about 4 us, the time
+// of 21 blocks of its 8 warps: a multiple of the heads (no CTA crosses) where
+// there are SMs for it, or where idling the rest costs less than that (8 heads
+// of 2000 keys: 63 CTAs 11.0 us, 64 CTAs 8.0 us).
 void rows_split(AttendParams &p)
 {
     p.n_tile = 1;
@@ -609,9 +667,10 @@ void rows_split(AttendParams &p)
     if (C >= p.n_vh) {
         const int64_t up = (C + p.n_vh - 1) / p.n_vh * p.n_vh, down = C / p.n_vh * p.n_vh;
         if (up <= kSMs) C = std::min(up, T);
-        else if (down * 20 >= C * 19) C = down;
+        else if (T / down - T / C <= 21) C = down;
     }
     p.n_cta = (int)C;
+    p.l2_ahead = W;   // a block of each warp: 20.5 -> 19.5 us at 32k keys of 8 heads; 16 gain the same, 32 nothing
 }
 
 cudaError_t launch_rows(const AttendParams &p, cudaStream_t st)
