@@ -51,18 +51,21 @@ __device__ __forceinline__ uint2 codes_to_half4(uint32_t w)
 // A launch that may begin its set-up while the kernel before it in the stream
 // ends; every kernel launched so waits (pdl_wait) before it touches memory.
 template <class K, class P>
-cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, const P &p, cudaStream_t st)
+cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, const P &p, cudaStream_t st, unsigned cluster = 0)
 {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 

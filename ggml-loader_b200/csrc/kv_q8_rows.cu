@@ -31,6 +31,7 @@ namespace {
 using namespace sm100;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMaxCluster = 8;
 constexpr float kBias = 7.0f;    // a new reference's weight is 2^kBias,
 constexpr float kTop = 15.0f;    // and it moves where a weight would pass 2^kTop
 
@@ -41,10 +42,10 @@ struct Rows {
     static constexpr int pitch = D + 16;                             // bytes a row: 8 rows fall on different banks
     static constexpr int tile = kBlock * pitch;                      // K or V of a block
     static constexpr int ring = E * tile;                            // a warp's
-    static constexpr int smem = W * ring;                            // (also holds the W warps' 16 output rows at the end)
+    static constexpr int smem = W * ring;                            // (at the end also the W warps' 16 output rows, and their sum)
     static constexpr int nk = D / 16;                                // 16-wide steps over D
     static constexpr bool q_regs = D <= 128;                         // the queries stay in registers, else in shared memory
-    static_assert(smem >= W * 16 * D * 4 && smem <= 225 * 1024, "shared memory");
+    static_assert(smem >= (W + 1) * 16 * D * 4 && smem <= 225 * 1024, "shared memory");
 };
 
 // two F16 pairs (codes 0, 1 | 2, 3 or 0, 2 | 1, 3) of four signed codes: 0x6400
@@ -103,6 +104,44 @@ __device__ __forceinline__ void store_out(const AttendParams &p, int64_t i, floa
 {
     if (p.out_f16) static_cast<__half *>(p.out)[i] = __float2half_rn(x);
     else static_cast<float *>(p.out)[i] = x;
+}
+
+__device__ __forceinline__ int64_t out_at(const AttendParams &p, int h, int row, int D)
+{
+    const int t = row / p.r;
+    return t * p.out_stride + (int64_t)(h * p.r + row - t * p.r) * D;
+}
+
+// x * z at four elements from i on
+__device__ __forceinline__ void store_out4(const AttendParams &p, int64_t i, float4 x, float z)
+{
+    if (p.out_f16 && p.out_vec) {
+        *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + i) = make_uint2(pack(x.x * z, x.y * z), pack(x.z * z, x.w * z));
+    } else if (p.out_vec) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + i) = make_float4(x.x * z, x.y * z, x.z * z, x.w * z);
+    } else {
+        store_out(p, i, x.x * z);
+        store_out(p, i + 1, x.y * z);
+        store_out(p, i + 2, x.z * z);
+        store_out(p, i + 3, x.w * z);
+    }
+}
+
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr)
+{
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
 }
 
 // sum -> 1 / sum, or what an empty row gives
@@ -166,6 +205,7 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
     extern __shared__ __align__(128) char smem[];
     __shared__ float2 s_stat[G::W][16];
     __shared__ float s_bad[G::W][16];
+    __shared__ float2 s_row[16];
     __shared__ uint2 s_q[G::q_regs ? 1 : 16][G::q_regs ? 1 : D / 4 + 4];   // (the pad: 8 rows fall on different banks)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     char *ring = smem + warp * G::ring;
@@ -453,18 +493,52 @@ __global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendPa
                 x.z = __fmaf_rn(y.z, f, x.z + bad);
                 x.w = __fmaf_rn(y.w, f, x.w + bad);
             }
-            if (whole) {
-                const float z = inverse_sum(l, p.flash != 0);
-                const int t = row / p.r, j = row % p.r;
-                const int64_t at = t * p.out_stride + (int64_t)(h * p.r + j) * D + c;
-                store_out(p, at, x.x * z);
-                store_out(p, at + 1, x.y * z);
-                store_out(p, at + 2, x.z * z);
-                store_out(p, at + 3, x.w * z);
-            } else {
-                *reinterpret_cast<float4 *>(p.part + (part * 16 + row) * D + c) = x;
+            if (p.cq) {
+                *reinterpret_cast<float4 *>(os + G::W * NR * D + row * D + c) = x;
+                if (c == 0) s_row[row] = make_float2(M, l);
+                continue;
             }
+            if (whole) store_out4(p, out_at(p, h, row, D) + c, x, inverse_sum(l, p.flash != 0));
+            else *reinterpret_cast<float4 *>(p.part + (part * 16 + row) * D + c) = x;
             if (c == 0) p.stat[part * 16 + row] = make_float2(M, l);
+        }
+        if (p.cq) {
+            // The head's CTAs are one cluster: each takes a share of the output
+            // and reads the others' sums through distributed shared memory (no
+            // second kernel).
+            cluster_sync_all();
+            for (int i = cluster_rank() * (G::W * 32) + threadIdx.x; i < nrows * (D / 4); i += p.cq * G::W * 32) {
+                const int row = i / (D / 4), c = i % (D / 4) * 4;
+                const uint32_t at = smem_addr(&s_row[row]), xat = smem_addr(os + G::W * NR * D + row * D + c);
+                float2 s[kMaxCluster];
+                float4 y[kMaxCluster];
+                float M = -CUDART_INF_F;
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; k++) {
+                    s[k] = make_float2(-CUDART_INF_F, 0.0f);
+                    y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (k >= p.cq) continue;
+                    s[k] = ld_cluster_f2(mapa(at, k));
+                    y[k] = ld_cluster_f4(mapa(xat, k));
+                }
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; k++) M = fmaxf(M, s[k].x);
+                const float ref = M == -CUDART_INF_F ? 0.0f : M;
+                float l = 0.0f;
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int k = 0; k < kMaxCluster; k++) {
+                    const float f = ex2_approx((s[k].x - ref) * unit);
+                    l = __fmaf_rn(s[k].y, f, l);
+                    x.x = __fmaf_rn(y[k].x, f, x.x);
+                    x.y = __fmaf_rn(y[k].y, f, x.y);
+                    x.z = __fmaf_rn(y[k].z, f, x.z);
+                    x.w = __fmaf_rn(y[k].w, f, x.w);
+                }
+                store_out4(p, out_at(p, h, row, D) + c, x, inverse_sum(l, p.flash != 0));
+            }
+            cluster_sync_all();   // (no CTA leaves while its sums are read)
+            return;
         }
         __syncthreads();   // the next head's ring takes the shared memory
     }
@@ -628,8 +702,8 @@ cudaError_t run(const AttendParams &p, cudaStream_t st)
     cudaError_t e = once.on_device([] {
         return cudaFuncSetAttribute(rows_kernel<D, HILO, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
     });
-    if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, HILO, MASKED>, p.n_cta, G::W * 32, G::smem, p, st);
-    if (e != cudaSuccess) return e;
+    if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, HILO, MASKED>, p.n_cta, G::W * 32, G::smem, p, st, p.cq);
+    if (e != cudaSuccess || p.cq) return e;
     const bool split = p.n_cta > p.n_vh || p.n_vh % p.n_cta != 0;   // else every head lies in one CTA
     if (!split && !p.scores) return cudaSuccess;
     unsigned grid = (unsigned)(p.n_vh * p.n_new * p.r);
@@ -668,6 +742,19 @@ void rows_split(AttendParams &p)
         const int64_t up = (C + p.n_vh - 1) / p.n_vh * p.n_vh, down = C / p.n_vh * p.n_vh;
         if (up <= kSMs) C = std::min(up, T);
         else if (T / down - T / C <= 21) C = down;
+    }
+    // Up to 8 CTAs a head join in their cluster instead of by a second kernel,
+    // where the device holds all clusters at once (these numbers of them, by
+    // the occupancy query at this shared memory).  Heads of up to 128 blocks of
+    // 128-wide rows are cut in 8 for it, two blocks a warp.  2000 keys, device
+    // time with the join and without: 2 heads of 64 4.9 and 4.1 us, 8 of 128
+    // 8.0 and 5.2 us.
+    constexpr int most[kMaxCluster + 1] = {0, 0, 74, 45, 33, 22, 22, 15, 15};
+    p.cq = 0;
+    if (!p.c.weight) {
+        if (C > kMaxCluster * p.n_vh && (int64_t)p.nb * p.c.D <= 2 * W * kMaxCluster * 128 && p.n_vh <= most[kMaxCluster]) C = kMaxCluster * p.n_vh;
+        const int64_t q = C / p.n_vh;
+        if (C % p.n_vh == 0 && q >= 2 && q <= kMaxCluster && p.n_vh <= most[q]) p.cq = (int)q;
     }
     p.n_cta = (int)C;
     p.l2_ahead = W;   // a block of each warp: 20.5 -> 19.5 us at 32k keys of 8 heads; 16 gain the same, 32 nothing
