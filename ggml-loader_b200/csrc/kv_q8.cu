@@ -229,24 +229,85 @@ __device__ __forceinline__ uint32_t weight_key(float w)
 }
 
 constexpr int kSelThreads = 1024, kSelWarps = kSelThreads / 32;
-constexpr int kSelCtas = 8;                      // a KV head's cluster
-constexpr int kSelSlice = 48 * 1024;             // keys a CTA holds in shared memory; with more it reads them each time
+constexpr int kSelCtas = 8;               // a KV head's cluster
+constexpr int kSelSlice = 32 * 1024;      // keys a CTA holds in shared memory; with more it reads them each time
+constexpr int kSelBins = 4096;
+
+__device__ __forceinline__ void red_cluster_add(uint32_t addr, int v)
+{
+    asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// This CTA's counts added to the cluster's in every CTA; few of the counters
+// are not zero, so they are sent one by one (all 4096 read from each CTA
+// instead: 44 us against 13).  Leaves zeros behind.
+template <int BINS>
+__device__ __forceinline__ void send_counts(int *s_mine, int *s_all)
+{
+    for (int i = threadIdx.x; i < BINS; i += kSelThreads) {
+        const int x = s_mine[i];
+        if (!x) continue;
+        s_mine[i] = 0;
+        const uint32_t at = sm100::smem_addr(&s_all[i]);
+#pragma unroll
+        for (int c = 0; c < kSelCtas; c++) red_cluster_add(mapa(at, c), x);
+    }
+}
+
+// The digit (from the top) in which the want-th largest key lies, by the
+// cluster's counts: thread t takes BINS / 1024 digits from the top down.
+// `want` becomes what is to be taken within it.
+template <int BINS>
+__device__ __forceinline__ uint32_t find_digit(const int *s_all, int *s_scan, int *s_found, int &want)
+{
+    constexpr int M = BINS / kSelThreads;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int x[M], total = 0;
+#pragma unroll
+    for (int j = 0; j < M; j++) total += x[j] = s_all[BINS - 1 - M * tid - j];
+    int y = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) y += z;
+    }
+    if (lane == 31) s_scan[warp] = y;
+    __syncthreads();
+    int before = y - total;
+#pragma unroll
+    for (int k = 0; k < kSelWarps; k++) before += k < warp ? s_scan[k] : 0;
+    if (before < want && want <= before + total) {   // one thread
+        int digit = BINS - 1 - M * tid;
+#pragma unroll
+        for (int j = 0; j < M - 1; j++)
+            if (before + x[j] < want && digit == BINS - 1 - M * tid - j) {
+                before += x[j];
+                digit--;
+            }
+        s_found[0] = digit;
+        s_found[1] = want - before;
+    }
+    __syncthreads();
+    want = s_found[1];
+    return s_found[0];
+}
 
 // A cluster a KV head, each CTA a contiguous slice of its candidates: the
-// (keep - recent)-th largest key by four 8-bit digits (histograms in shared
-// memory, added up over the cluster), then the kept rows in order from each
-// CTA's place on.  The weights are read once; what is left are the cluster's
-// barriers, two a digit (32k candidates, 8 heads: 191 us with one CTA a head).
+// (keep - recent)-th largest key by digits of 12, 10 and 10 bits (histograms in
+// shared memory, added up over the cluster; the first digit takes the sign, the
+// exponent and 3 bits of the fraction, so that like weights do not meet in one
+// counter), then the kept rows in order from each CTA's place on.  The weights
+// are read once; what is left are the cluster's barriers, one a digit (32k
+// candidates, 8 heads: one CTA a head 140 us, four 8-bit digits 17 us).
 __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) select_kernel(const EvictParams p)
 {
-    extern __shared__ uint32_t s_key[];
-    __shared__ int s_hist[8][256];     // (copies: fewer warps on one counter)
-    __shared__ int s_sum[256];         // this CTA's, read by the others
-    __shared__ int s_all[256];
+    extern __shared__ uint32_t s_dyn[];
+    int *s_mine = reinterpret_cast<int *>(s_dyn);        // this CTA's counts
+    int *s_all = s_mine + kSelBins;                      // [2][kSelBins] the cluster's, by digit in turn
+    uint32_t *s_key = s_dyn + 3 * kSelBins;
     __shared__ int s_scan[kSelWarps];
+    __shared__ int s_found[2];
     __shared__ int s_count[2];         // this CTA's keys above the edge, and on it
-    __shared__ uint32_t s_digit;
-    __shared__ int s_want;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = (int)cluster_rank(), h = blockIdx.x / kSelCtas;
     const int cand = (int)(p.n_rows - p.recent), take = (int)(p.keep - p.recent);
@@ -256,70 +317,43 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
     const int per = (int)(((int64_t)cand + kSelCtas * 4 - 1) / (kSelCtas * 4) * 4);
     const int lo = (int)min((int64_t)cand, (int64_t)rank * per), n = min(per, cand - lo);
     const bool held = per <= kSelSlice;
+    for (int i = tid; i < 3 * kSelBins; i += kSelThreads) s_mine[i] = 0;
     pdl_launch_dependents();
+    cluster_sync_all();   // (counts may come in)
     pdl_wait();
     for (int64_t j = (int64_t)rank * kSelThreads + tid; j < p.recent; j += kSelCtas * kSelThreads)
         kept[take + j] = cand + (int32_t)j;
     if (take == 0) return;   // (the whole cluster)
-    if (held)
-        for (int i = tid; i < n; i += kSelThreads) s_key[i] = weight_key(w[lo + i]);
+    // the first digit with the reading of the weights
+#pragma unroll 4
+    for (int i = tid; i < n; i += kSelThreads) {
+        const uint32_t k = weight_key(w[lo + i]);
+        if (held) s_key[i] = k;
+        atomicAdd(&s_mine[k >> 20], 1);
+    }
     auto key = [&](int i) { return held ? s_key[i] : weight_key(w[lo + i]); };
-
-    uint32_t prefix = 0;
     int want = take;   // still to be taken among the keys with the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 8 * 256; i += kSelThreads) (&s_hist[0][0])[i] = 0;
-        __syncthreads();
+    __syncthreads();
+    send_counts<4096>(s_mine, s_all);
+    cluster_sync_all();
+    uint32_t prefix = find_digit<4096>(s_all, s_scan, s_found, want);
+    // (find_digit's barrier: the first counts are read; they are zeros again before the last digit's come in)
+    s_all[tid] = 0;
+#pragma unroll 1
+    for (int d = 0; d < 2; d++) {
+        const int shift = 10 - 10 * d;
+        int *all = s_all + (d ? 0 : kSelBins);
         for (int i = tid; i < n; i += kSelThreads) {
             const uint32_t k = key(i);
-            if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&s_hist[warp & 7][(k >> shift) & 255u], 1);
+            if (k >> (shift + 10) == prefix) atomicAdd(&s_mine[(k >> shift) & 1023u], 1);
         }
         __syncthreads();
-        if (tid < 256) {
-            int x = 0;
-#pragma unroll
-            for (int c = 0; c < 8; c++) x += s_hist[c][tid];
-            s_sum[tid] = x;
-        }
+        send_counts<1024>(s_mine, all);
         cluster_sync_all();
-        if (tid < 256) {
-            int x = 0;
-#pragma unroll
-            for (int c = 0; c < kSelCtas; c++) x += ld_cluster_s32(mapa(sm100::smem_addr(&s_sum[tid]), c));
-            s_all[tid] = x;
-        }
-        __syncthreads();
-        if (warp == 0) {
-            // lane l: digits 255 - 8 l down; the digit in which the want-th largest lies
-            int x[8], total = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) total += x[j] = s_all[255 - 8 * lane - j];
-            int before = total;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, before, o);
-                if (lane >= o) before += y;
-            }
-            before -= total;
-            if (before < want && want <= before + total) {
-                int d = 0;
-                while (before + x[0] < want) {
-                    before += x[0];
-                    d++;
-#pragma unroll
-                    for (int j = 0; j < 7; j++) x[j] = x[j + 1];
-                }
-                s_digit = 255 - 8 * lane - d;
-                s_want = want - before;
-            }
-        }
-        __syncthreads();
-        prefix = prefix << 8 | s_digit;
-        want = s_want;
-        cluster_sync_all();   // (s_sum is written again)
+        prefix = prefix << 10 | find_digit<1024>(all, s_scan, s_found, want);
     }
 
-    // a thread's keys are neighbours: 4 m of them from 4 m tid on
+    // a thread's keys are neighbours: m of them from m tid on
     const int m = (n + kSelThreads * 4 - 1) / (kSelThreads * 4) * 4, i0 = min(n, m * tid), i1 = min(n, i0 + m);
     int above = 0, on = 0;
     for (int i = i0; i < i1; i++) {
@@ -359,7 +393,7 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
         a += ld_cluster_s32(at);
         e += ld_cluster_s32(at + 4);
     }
-    cluster_sync_all();   // (no CTA leaves while its counts are read)
+    sm100::cluster_arrive();
     // rows before this thread's first: a above the edge and min(e, want) on it
     for (int i = i0; i < i1; i++) {
         const uint32_t k = key(i);
@@ -368,11 +402,12 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
         a += k > prefix;
         e += tie;
     }
+    sm100::cluster_wait();   // (no CTA leaves while its counts are read)
 }
 
 // U blocks of dst of a KV head a CTA, K and V: a row is D/16 threads, 16 codes
 // each of K and of V of every block, so 2 U gathers a thread are in flight
-// together (32k rows to 16k: 38 us with one block a CTA).
+// together.
 template <int D, int U>
 __global__ void __launch_bounds__(kBlock *D / 16) gather_kernel(const EvictParams p)
 {
@@ -462,9 +497,10 @@ template <int D>
 cudaError_t gather_d(const EvictParams &p, cudaStream_t st)
 {
     const int64_t blocks = (p.keep + kBlock - 1) / kBlock;
-    // four blocks a CTA once that leaves two CTAs an SM
-    if (blocks * p.src.H >= 4 * 2 * kSMs)
-        return launch_pdl(gather_kernel<D, 4>, dim3((unsigned)((blocks + 3) / 4), p.src.H), kBlock * D / 16, 0, p, st);
+    // two blocks a CTA once that leaves four CTAs an SM (32k rows to 16k, 4096 blocks of 128-wide rows, device
+    // time with the selection and the read-back: 1 a CTA 68 us, 2 54 us, 4 58 us, 8 68 us)
+    if (blocks * p.src.H >= 2 * 4 * kSMs)
+        return launch_pdl(gather_kernel<D, 2>, dim3((unsigned)((blocks + 1) / 2), p.src.H), kBlock * D / 16, 0, p, st);
     return launch_pdl(gather_kernel<D, 1>, dim3((unsigned)blocks, p.src.H), kBlock * D / 16, 0, p, st);
 }
 
@@ -514,11 +550,12 @@ cudaError_t launch_evict(const EvictParams &p, cudaStream_t st)
 {
     static Once once;
     cudaError_t e = once.on_device([] {
-        return cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelSlice * 4);
+        return cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (3 * kSelBins + kSelSlice) * 4);
     });
     if (e != cudaSuccess) return e;
     const int64_t cand = p.n_rows - p.recent, per = (cand + kSelCtas * 4 - 1) / (kSelCtas * 4) * 4;
-    e = launch_pdl(select_kernel, dim3(p.src.H * kSelCtas), kSelThreads, per <= kSelSlice ? (size_t)per * 4 : 0, p, st);
+    e = launch_pdl(select_kernel, dim3(p.src.H * kSelCtas), kSelThreads,
+                   (size_t)(3 * kSelBins + (per <= kSelSlice ? per : 0)) * 4, p, st);
     if (e != cudaSuccess) return e;
     switch (p.src.D) {
     case 64: return gather_d<64>(p, st);

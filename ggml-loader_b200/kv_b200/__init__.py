@@ -385,8 +385,9 @@ def _calls():
             from . import _q8call
         except ImportError as e:
             raise ImportError("kv_b200/_q8call.so is not built (%s); run ggml-loader_b200/build.py" % e)
-        address = [ctypes.cast(getattr(lib(), n), _vp).value for n in ("kv_q8_store", "kv_q8_load", "kv_q8_attend")]
-        _q8call.init(torch.float32, torch.float16, *address)
+        address = [ctypes.cast(getattr(lib(), n), _vp).value
+                   for n in ("kv_q8_store", "kv_q8_load", "kv_q8_attend", "kv_q8_evict")]
+        _q8call.init(torch.float32, torch.float16, torch.int32, *address)
         _q8calls = _q8call
     return _q8calls
 
@@ -426,7 +427,7 @@ class Q8Cache:
         else:
             with self._torch.cuda.device(self._index):
                 rc = fn(*args)
-        return rc if rc == KV_OK else _check(rc, "kv_q8_" + fn.__name__.replace("kv_q8_", ""))
+        return rc if rc == KV_OK else _check(rc, "kv_q8_" + fn.__name__)
 
     def store(self, row0, n_new, k, v, stream=None):
         """kv_q8_store: n_new rows of [n_head_kv][head_dim] at row0."""
@@ -456,12 +457,8 @@ class Q8Cache:
 
     def evict(self, n_rows, keep, recent, dst, kept, stream=None):
         """kv_q8_evict into the Q8Cache dst; kept: int32 [n_head_kv][keep]."""
-        if kept.shape != (self.n_head_kv, keep) or kept.dtype != self._torch.int32 or not kept.is_contiguous() or \
-                kept.get_device() != self._index or dst._index != self._index:
-            raise ValueError("kept must be a contiguous int32 [%d][%d] tensor on the cache's device, dst there too"
-                             % (self.n_head_kv, keep))
-        return self._on_device(self._lib.kv_q8_evict, self._ref, n_rows, keep, recent, dst._ref, kept.data_ptr(),
-                               _stream(stream))
+        return self._on_device(self._calls.evict, self._ref, self._index, self.n_head_kv, n_rows, keep, recent, dst._ref,
+                               dst._index, kept, stream)
 
 
 def gen_normal_device(dst, seed, stream_id, n, idx0=0, stream=None):

@@ -13,12 +13,13 @@
 
 #include "kv_api.h"
 
-static PyObject *g_f32, *g_f16;   /* torch.float32, torch.float16 */
+static PyObject *g_f32, *g_f16, *g_i32;   /* torch.float32, torch.float16, torch.int32 */
 static PyObject *s_dtype, *s_shape, *s_stride, *s_get_device, *s_data_ptr, *s_cuda_stream, *s_is_contiguous, *s_nbytes;
 static int (*p_store)(const kv_q8_cache *, int64_t, int32_t, const void *, int64_t, const void *, int64_t, int32_t, void *);
 static int (*p_load)(const kv_q8_cache *, int64_t, int64_t, void *, void *, int64_t, int32_t, void *);
 static int (*p_attend)(const kv_q8_cache *, int32_t, int64_t, int32_t, const void *, int64_t, int32_t, const void *, int32_t,
                        int64_t, uint32_t, void *, int64_t, int32_t, void *, uint64_t, void *);
+static int (*p_evict)(const kv_q8_cache *, int64_t, int64_t, int64_t, const kv_q8_cache *, int32_t *, void *);
 
 /* an integer attribute, or the integer a method without arguments returns; -1 with an error set */
 static int64_t int_of(PyObject *o, PyObject *name, int call)
@@ -188,19 +189,49 @@ static PyObject *q8_attend(PyObject *self, PyObject *const *a, Py_ssize_t n)
                                     flash ? KV_ATTN_FLASH : 0u, out.ptr, out.stride, out.type, ws, (uint64_t)bytes, st));
 }
 
-/* init(torch.float32, torch.float16, address of kv_q8_store, _load, _attend) */
+/* evict(cache, device, n_head_kv, n_rows, keep, recent, dst, dst's device, kept, stream) */
+static PyObject *q8_evict(PyObject *self, PyObject *const *a, Py_ssize_t n)
+{
+    if (!arity("evict", n, 10)) return NULL;
+    const kv_q8_cache *c = PyLong_AsVoidPtr(a[0]), *dst = PyLong_AsVoidPtr(a[6]);
+    const int64_t dev = as_i64(a[1]), heads = as_i64(a[2]), keep = as_i64(a[4]), ddev = as_i64(a[7]);
+    void *st = stream_of(a[9]);
+    PyObject *type = PyErr_Occurred() ? NULL : PyObject_GetAttr(a[8], s_dtype);
+    PyObject *shape = type ? PyObject_GetAttr(a[8], s_shape) : NULL, *whole = shape ? PyObject_CallMethodNoArgs(a[8], s_is_contiguous) : NULL;
+    const int ok = whole == Py_True && type == g_i32 && PyTuple_Check(shape) && PyTuple_GET_SIZE(shape) == 2 &&
+                   PyLong_AsLongLong(PyTuple_GET_ITEM(shape, 0)) == heads && PyLong_AsLongLong(PyTuple_GET_ITEM(shape, 1)) == keep &&
+                   ddev == dev && int_of(a[8], s_get_device, 1) == dev;
+    Py_XDECREF(type);
+    Py_XDECREF(shape);
+    Py_XDECREF(whole);
+    if (!ok) {
+        if (!PyErr_Occurred())
+            PyErr_Format(PyExc_ValueError, "kept must be a contiguous int32 [%lld][%lld] tensor on the cache's device, dst there too",
+                         (long long)heads, (long long)keep);
+        return NULL;
+    }
+    int32_t *kept = (int32_t *)(intptr_t)int_of(a[8], s_data_ptr, 1);
+    const int64_t rows = as_i64(a[3]), recent = as_i64(a[5]);
+    if (PyErr_Occurred()) return NULL;
+    return PyLong_FromLong(p_evict(c, rows, keep, recent, dst, kept, st));
+}
+
+/* init(torch.float32, torch.float16, torch.int32, address of kv_q8_store, _load, _attend, _evict) */
 static PyObject *q8_init(PyObject *self, PyObject *args)
 {
-    PyObject *f32, *f16;
-    unsigned long long s, l, a;
-    if (!PyArg_ParseTuple(args, "OOKKK", &f32, &f16, &s, &l, &a)) return NULL;
+    PyObject *f32, *f16, *i32;
+    unsigned long long s, l, a, e;
+    if (!PyArg_ParseTuple(args, "OOOKKKK", &f32, &f16, &i32, &s, &l, &a, &e)) return NULL;
     Py_INCREF(f32);
     Py_INCREF(f16);
+    Py_INCREF(i32);
     Py_XSETREF(g_f32, f32);
     Py_XSETREF(g_f16, f16);
+    Py_XSETREF(g_i32, i32);
     *(void **)&p_store = (void *)(uintptr_t)s;
     *(void **)&p_load = (void *)(uintptr_t)l;
     *(void **)&p_attend = (void *)(uintptr_t)a;
+    *(void **)&p_evict = (void *)(uintptr_t)e;
     Py_RETURN_NONE;
 }
 
@@ -208,6 +239,7 @@ static PyMethodDef methods[] = {{"init", q8_init, METH_VARARGS, NULL},
                                 {"store", (PyCFunction)(void (*)(void))q8_store, METH_FASTCALL, NULL},
                                 {"load", (PyCFunction)(void (*)(void))q8_load, METH_FASTCALL, NULL},
                                 {"attend", (PyCFunction)(void (*)(void))q8_attend, METH_FASTCALL, NULL},
+                                {"evict", (PyCFunction)(void (*)(void))q8_evict, METH_FASTCALL, NULL},
                                 {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_q8call", NULL, -1, methods};
 
