@@ -254,6 +254,20 @@ __device__ __forceinline__ void send_counts(int *s_mine, int *s_all)
     }
 }
 
+// Sum of the warps' totals before `warp` (s_scan: one a warp), and of all.
+__device__ __forceinline__ int before_warp(const int *s_scan, int warp, int lane, int &total)
+{
+    int y = s_scan[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int z = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) y += z;
+    }
+    total = __shfl_sync(0xffffffffu, y, 31);
+    const int b = __shfl_sync(0xffffffffu, y, warp ? warp - 1 : 0);
+    return warp ? b : 0;
+}
+
 // The digit (from the top) in which the want-th largest key lies, by the
 // cluster's counts: thread t takes BINS / 1024 digits from the top down.
 // `want` becomes what is to be taken within it.
@@ -273,9 +287,8 @@ __device__ __forceinline__ uint32_t find_digit(const int *s_all, int *s_scan, in
     }
     if (lane == 31) s_scan[warp] = y;
     __syncthreads();
-    int before = y - total;
-#pragma unroll
-    for (int k = 0; k < kSelWarps; k++) before += k < warp ? s_scan[k] : 0;
+    int all;
+    int before = y - total + before_warp(s_scan, warp, lane, all);
     if (before < want && want <= before + total) {   // one thread
         int digit = BINS - 1 - M * tid;
 #pragma unroll
@@ -305,7 +318,7 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
     int *s_mine = reinterpret_cast<int *>(s_dyn);        // this CTA's counts
     int *s_all = s_mine + kSelBins;                      // [2][kSelBins] the cluster's, by digit in turn
     uint32_t *s_key = s_dyn + 3 * kSelBins;
-    __shared__ int s_scan[kSelWarps];
+    __shared__ int s_scan[2 * kSelWarps];
     __shared__ int s_found[2];
     __shared__ int s_count[2];         // this CTA's keys above the edge, and on it
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -361,37 +374,35 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
         above += k > prefix;
         on += k == prefix;
     }
-    // exclusive sums over the CTA
-    auto scan = [&](int x, int &total) {
-        int y = x;
+    // exclusive sums over the CTA of both
+    int a = above, e = on;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int z = __shfl_up_sync(0xffffffffu, y, o);
-            if (lane >= o) y += z;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, a, o), z = __shfl_up_sync(0xffffffffu, e, o);
+        if (lane >= o) {
+            a += y;
+            e += z;
         }
-        __syncthreads();
-        if (lane == 31) s_scan[warp] = y;
-        __syncthreads();
-        int b = 0;
-        total = 0;
-#pragma unroll
-        for (int k = 0; k < kSelWarps; k++) {
-            if (k < warp) b += s_scan[k];
-            total += s_scan[k];
-        }
-        return b + y - x;
-    };
+    }
+    if (lane == 31) {
+        s_scan[warp] = a;
+        s_scan[kSelWarps + warp] = e;
+    }
+    __syncthreads();
     int n_above, n_on;
-    int a = scan(above, n_above), e = scan(on, n_on);
+    a += before_warp(s_scan, warp, lane, n_above) - above;
+    e += before_warp(s_scan + kSelWarps, warp, lane, n_on) - on;
     if (tid == 0) {
         s_count[0] = n_above;
         s_count[1] = n_on;
     }
     cluster_sync_all();
-    for (int c = 0; c < rank; c++) {
-        const uint32_t at = mapa(sm100::smem_addr(s_count), c);
-        a += ld_cluster_s32(at);
-        e += ld_cluster_s32(at + 4);
+    {
+        // lane c: the counts of CTA c, where it comes before this one
+        const uint32_t at = mapa(sm100::smem_addr(s_count), lane & (kSelCtas - 1));
+        const bool take_it = lane < rank;
+        a += __reduce_add_sync(0xffffffffu, take_it ? ld_cluster_s32(at) : 0);
+        e += __reduce_add_sync(0xffffffffu, take_it ? ld_cluster_s32(at + 4) : 0);
     }
     sm100::cluster_arrive();
     // rows before this thread's first: a above the edge and min(e, want) on it
