@@ -416,103 +416,97 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
     sm100::cluster_wait();   // (no CTA leaves while its counts are read)
 }
 
-// U blocks of dst of a KV head a CTA, K and V: a row is D/16 threads, 16 codes
-// each of K and of V of every block, so 2 U gathers a thread are in flight
-// together.
-template <int D, int U>
+// 16 codes times 2^k, rounded: as halves, whose numbers from 1024 to 2048 are
+// the integers, so 1536 + code * 2^k is the rounded code in the low byte (one
+// rounding, to even; the factor is exact from 2^-24 on, and 0 below, where every
+// code rounds to 0; a code that is not 0 stays below 128, so k < 7 for it).
+// bad: kBad codes may be among them.
+__device__ __forceinline__ void move_codes(uint4 &x, int k, bool bad)
+{
+    const __half2 f = __half2half2(__float2half_rn(pow2(min(k, 15)))), one = __half2half2(__ushort_as_half(0x6600));
+    uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint2 y = codes_to_half4(w[i]);
+        const __half2 a = __hfma2(*reinterpret_cast<const __half2 *>(&y.x), f, one);
+        const __half2 b = __hfma2(*reinterpret_cast<const __half2 *>(&y.y), f, one);
+        uint32_t z = __byte_perm(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b), 0x6420);
+        if (bad) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+                if (((w[i] >> j) & 255u) == 0x80u) z = (z & ~(255u << j)) | (0x80u << j);
+        }
+        w[i] = z;
+    }
+}
+
+// One block of dst of a KV head a CTA, K and V: a row is D/16 threads, 16 codes
+// each of K and of V.  Many small CTAs keep the gathers in flight (32k rows to
+// 16k with the selection and the read-back: 46 us, two blocks a CTA 47 us, four
+// 51 us); the codes' arithmetic is in halves, two at a time (with conversions
+// to float and back the conversions were the bound, 50 us).
+template <int D>
 __global__ void __launch_bounds__(kBlock *D / 16) gather_kernel(const EvictParams p)
 {
     constexpr int T = kBlock * D / 16;
-    __shared__ uint32_t part[2 * U][T / 32];
+    __shared__ uint32_t part[2][T / 32];
     const int r = threadIdx.x / (D / 16), c = threadIdx.x % (D / 16) * 16;
     const int h = blockIdx.y;
-    const int64_t row0 = (int64_t)blockIdx.x * (U * kBlock) + r;
-    const int32_t *kept = p.kept + (int64_t)h * p.keep;
-    const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.src.k_scale) + (int64_t)h * (p.src.rows / kBlock);
-    const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.src.v_scale) + (int64_t)h * (p.src.rows / kBlock);
-    uint4 w[U][2];
-    uint32_t sc[U][2];
-    int32_t from[U];
+    const int64_t row = (int64_t)blockIdx.x * kBlock + r;
+    uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+    int e0[2] = {kExpMin, kExpMin};
     pdl_launch_dependents();
     pdl_wait();
-#pragma unroll
-    for (int u = 0; u < U; u++) from[u] = row0 + u * kBlock < p.keep ? kept[row0 + u * kBlock] : -1;
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
-        sc[u][0] = sc[u][1] = scale_word(kExpMin, false);
-        if (from[u] < 0) continue;
-        const int64_t at = ((int64_t)h * p.src.rows + from[u]) * D + c;
-        w[u][0] = *reinterpret_cast<const uint4 *>(p.src.k + at);
-        w[u][1] = *reinterpret_cast<const uint4 *>(p.src.v + at);
-        sc[u][0] = ksc[from[u] / kBlock];
-        sc[u][1] = vsc[from[u] / kBlock];
-    }
-    if (c == 0 && p.dst.weight) {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (from[u] >= 0)
-                p.dst.weight[(int64_t)h * p.dst.rows + row0 + u * kBlock] = p.src.weight[(int64_t)h * p.src.rows + from[u]];
+    const bool used = row < p.keep;
+    if (used) {
+        const int64_t from = p.kept[(int64_t)h * p.keep + row], at = ((int64_t)h * p.src.rows + from) * D + c;
+        const int64_t sc = (int64_t)h * (p.src.rows / kBlock) + from / kBlock;
+        w[0] = *reinterpret_cast<const uint4 *>(p.src.k + at);
+        w[1] = *reinterpret_cast<const uint4 *>(p.src.v + at);
+        e0[0] = scale_exp(reinterpret_cast<const uint32_t *>(p.src.k_scale)[sc]);
+        e0[1] = scale_exp(reinterpret_cast<const uint32_t *>(p.src.v_scale)[sc]);
+        if (c == 0 && p.dst.weight) p.dst.weight[(int64_t)h * p.dst.rows + row] = p.src.weight[(int64_t)h * p.src.rows + from];
     }
     // the largest magnitude, code * 2^e: exact in float, whose bits order as it does
 #pragma unroll
-    for (int v = 0; v < 2 * U; v++) {
-        const uint4 &x = w[v >> 1][v & 1];
-        // magnitudes of four codes at once (-128 gives 128, which marks a value that is not finite)
-        uint32_t m = __vmaxu4(__vmaxu4(__vabs4(x.x), __vabs4(x.y)), __vmaxu4(__vabs4(x.z), __vabs4(x.w)));
-        bool bad = (m & 0x80808080u) != 0;
+    for (int v = 0; v < 2; v++) {
+        __half2 m2 = __half2half2(__ushort_as_half(0));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint2 y = codes_to_half4(reinterpret_cast<const uint32_t *>(&w[v])[i]);
+            m2 = __hmax2(m2, __hmax2(__habs2(*reinterpret_cast<const __half2 *>(&y.x)), __habs2(*reinterpret_cast<const __half2 *>(&y.y))));
+        }
+        float m = __half2float(__hmax(__low2half(m2), __high2half(m2)));
+        const bool bad = m == 128.0f;
         if (bad) {
-            const int8_t *q = reinterpret_cast<const int8_t *>(&x);
+            const int8_t *q = reinterpret_cast<const int8_t *>(&w[v]);
             int top = 0;
 #pragma unroll
             for (int i = 0; i < 16; i++) top = max(top, q[i] == kBad ? 0 : abs((int)q[i]));
-            m = top;
+            m = (float)top;
         }
-        m = max(max(m & 255u, (m >> 8) & 255u), max((m >> 16) & 255u, m >> 24));
-        const float f = __fmul_rn((float)m, pow2(scale_exp(sc[v >> 1][v & 1])));
-        const uint32_t best = __reduce_max_sync(0xffffffffu, __float_as_uint(f));
+        const uint32_t best = __reduce_max_sync(0xffffffffu, __float_as_uint(__fmul_rn(m, pow2(e0[v]))));
         const bool any = __any_sync(0xffffffffu, bad);
         if ((threadIdx.x & 31) == 0) part[v][threadIdx.x >> 5] = best | (any ? 0x80000000u : 0u);
     }
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < 2 * U; v++) {
-        const int u = v >> 1;
-        const bool is_v = (v & 1) != 0;
-        if ((int64_t)blockIdx.x * (U * kBlock) + u * kBlock >= p.keep) break;   // (a block without rows)
+    for (int v = 0; v < 2; v++) {
         uint32_t best = 0, flag = 0;
 #pragma unroll
         for (int i = 0; i < T / 32; i++) {
             best = max(best, part[v][i] & 0x7fffffffu);
             flag |= part[v][i];
         }
-        const int e = block_exp(__uint_as_float(best)), e0 = scale_exp(sc[u][v & 1]);
-        if (from[u] >= 0) {
-            uint4 &x4 = w[u][v & 1];
-            if (e != e0) {   // (exact in float: |code| < 128, the factor a power of two)
-                int8_t *x = reinterpret_cast<int8_t *>(&x4);
-                const float f = pow2(e0 - e);
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (x[i] != kBad) x[i] = (int8_t)to_code((float)x[i], f);
-            }
-            *reinterpret_cast<uint4 *>((is_v ? p.dst.v : p.dst.k) + ((int64_t)h * p.dst.rows + row0 + u * kBlock) * D + c) = x4;
+        const bool bad = (flag & 0x80000000u) != 0;
+        const int e = block_exp(__uint_as_float(best));
+        if (used) {
+            if (e != e0[v]) move_codes(w[v], e0[v] - e, bad);
+            *reinterpret_cast<uint4 *>((v ? p.dst.v : p.dst.k) + ((int64_t)h * p.dst.rows + row) * D + c) = w[v];
         }
         if (threadIdx.x == 0)
-            (is_v ? p.dst.v_scale : p.dst.k_scale)[(int64_t)h * (p.dst.rows / kBlock) + (int64_t)blockIdx.x * U + u] =
-                __uint_as_float(scale_word(e, (flag & 0x80000000u) != 0));
+            (v ? p.dst.v_scale : p.dst.k_scale)[(int64_t)h * (p.dst.rows / kBlock) + blockIdx.x] = __uint_as_float(scale_word(e, bad));
     }
-}
-
-template <int D>
-cudaError_t gather_d(const EvictParams &p, cudaStream_t st)
-{
-    const int64_t blocks = (p.keep + kBlock - 1) / kBlock;
-    // two blocks a CTA once that leaves four CTAs an SM (32k rows to 16k, 4096 blocks of 128-wide rows, device
-    // time with the selection and the read-back: 1 a CTA 68 us, 2 54 us, 4 58 us, 8 68 us)
-    if (blocks * p.src.H >= 2 * 4 * kSMs)
-        return launch_pdl(gather_kernel<D, 2>, dim3((unsigned)((blocks + 1) / 2), p.src.H), kBlock * D / 16, 0, p, st);
-    return launch_pdl(gather_kernel<D, 1>, dim3((unsigned)blocks, p.src.H), kBlock * D / 16, 0, p, st);
 }
 
 template <int D>
@@ -568,11 +562,12 @@ cudaError_t launch_evict(const EvictParams &p, cudaStream_t st)
     e = launch_pdl(select_kernel, dim3(p.src.H * kSelCtas), kSelThreads,
                    (size_t)(3 * kSelBins + (per <= kSelSlice ? per : 0)) * 4, p, st);
     if (e != cudaSuccess) return e;
+    const dim3 grid((unsigned)((p.keep + kBlock - 1) / kBlock), p.src.H);
     switch (p.src.D) {
-    case 64: return gather_d<64>(p, st);
-    case 96: return gather_d<96>(p, st);
-    case 128: return gather_d<128>(p, st);
-    case 256: return gather_d<256>(p, st);
+    case 64: return launch_pdl(gather_kernel<64>, grid, kBlock * 4, 0, p, st);
+    case 96: return launch_pdl(gather_kernel<96>, grid, kBlock * 6, 0, p, st);
+    case 128: return launch_pdl(gather_kernel<128>, grid, kBlock * 8, 0, p, st);
+    case 256: return launch_pdl(gather_kernel<256>, grid, kBlock * 16, 0, p, st);
     default: return cudaErrorInvalidValue;
     }
 }

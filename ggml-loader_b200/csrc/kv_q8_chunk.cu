@@ -255,6 +255,16 @@ __device__ __forceinline__ float inverse_sum(float l, bool flash)
     return l == 0.0f ? (flash ? 0.0f : CUDART_NAN_F) : 1.0f / l;
 }
 
+// Element d (a multiple of 4) of row `in` of a cut pair's partial output: pieces
+// of 8 floats, a piece's rows neighbours, so that a warp's rows fill whole
+// sectors both where they are written and where they are read.
+template <int D>
+__device__ __forceinline__ int64_t part_at(int64_t block, int in, int d)
+{
+    constexpr int rows = 128 * CL<D>::NT;
+    return ((block * (D / 8) + (d >> 3)) * rows + in) * 8 + (d & 7);
+}
+
 // what the weights' pass reads of a row: weight = 2^((t - m) * unit) * y
 __device__ __forceinline__ float2 row_stat_of(float m, float l)
 {
@@ -617,7 +627,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             if (!ok || !(ok = __all_sync(0xffffffffu, wait(o_full, seg & 1)))) break;
             tc_fence_after();
             const bool whole = w.whole();
-            const int64_t at = ((int64_t)cta + w.pair) * (128 * L::NT) + g * 128 + row;   // (CTA, pair) in order: their sum counts them
+            const int64_t block = (int64_t)cta + w.pair;   // (CTA, pair) in order: their sum counts them
+            const int in = g * 128 + row;
             float scl = 1.0f;
             if constexpr (MASKED) {   // both sums relative to e^m alone
                 scl = pow2((int)me);
@@ -625,7 +636,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             }
             if (whole) scl *= inverse_sum(l, p.flash != 0);
             if (valid) {
-                if (!whole) p.stat[at] = make_float2(m, l);
+                if (!whole) p.stat[block * (128 * L::NT) + in] = make_float2(m, l);
                 else if (p.row_stat) p.row_stat[(int64_t)h * p.n_new * p.r + (int64_t)tok * p.r + hd] = row_stat_of(m, l);
             }
             const int64_t dst = (int64_t)tok * p.out_stride + (int64_t)(h * p.r + hd) * D;
@@ -641,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                     const float4 x = make_float4(__fmaf_rn(__uint_as_float(o[4 * q]), scl, bad), __fmaf_rn(__uint_as_float(o[4 * q + 1]), scl, bad),
                                                  __fmaf_rn(__uint_as_float(o[4 * q + 2]), scl, bad), __fmaf_rn(__uint_as_float(o[4 * q + 3]), scl, bad));
                     if (whole) store_out4(p, dst + ch * 32 + 4 * q, x);
-                    else st_v4_hint(p.part + at * D + ch * 32 + 4 * q, x, pol);
+                    else st_v4_hint(p.part + part_at<D>(block, in, ch * 32 + 4 * q), x, pol);
                 }
             }
             tc_fence_before();
@@ -658,6 +669,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
 }
 
 // Joins the pairs cut between CTAs, a warp a query row; row_stat of their rows.
+constexpr int kFoldU = 4;
+
 template <int D, bool MASKED>
 __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
 {
@@ -672,28 +685,46 @@ __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
     const int c0 = (int)(((x0 + 1) * p.n_cta - 1) / W), c1 = (int)(((x1 + 1) * p.n_cta - 1) / W);
     pdl_wait();
     if (c0 == c1 || tk >= p.tok_tile || tok >= p.n_new) return;
-    float M = -CUDART_INF_F;
-    for (int c = c0; c <= c1; c++) M = fmaxf(M, p.stat[((int64_t)c + pair) * rows_blk + in].x);
-    const float ref = M == -CUDART_INF_F ? 0.0f : M;
     constexpr int V = (D / 4 + 31) / 32;
     float4 x[V];
 #pragma unroll
     for (int v = 0; v < V; v++) x[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float l = 0.0f;
-#pragma unroll 4
-    for (int c = c0; c <= c1; c++) {
-        const int64_t at = ((int64_t)c + pair) * rows_blk + in;
-        const float2 s = p.stat[at];
-        const float f = ex2_approx((s.x - ref) * unit);
-        l = __fmaf_rn(s.y, f, l);
+    float M = -CUDART_INF_F, l = 0.0f;
+    // kFoldU parts and their (m, l) in flight together
+    for (int c = c0; c <= c1; c += kFoldU) {
+        float2 s[kFoldU];
+        float4 y[kFoldU][V];
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            if (lane + 32 * v >= D / 4) continue;
-            const float4 y = __ldcg(reinterpret_cast<const float4 *>(p.part + at * D) + lane + 32 * v);
-            x[v].x = __fmaf_rn(y.x, f, x[v].x);
-            x[v].y = __fmaf_rn(y.y, f, x[v].y);
-            x[v].z = __fmaf_rn(y.z, f, x[v].z);
-            x[v].w = __fmaf_rn(y.w, f, x[v].w);
+        for (int u = 0; u < kFoldU; u++) {
+            const bool have = c + u <= c1;
+            const int64_t block = (int64_t)c + u + pair;
+            s[u] = have ? p.stat[block * rows_blk + in] : make_float2(-CUDART_INF_F, 0.0f);
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                y[u][v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (have && lane + 32 * v < D / 4)
+                    y[u][v] = __ldcg(reinterpret_cast<const float4 *>(p.part + part_at<D>(block, in, (lane + 32 * v) * 4)));
+            }
+        }
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < kFoldU; u++) top = fmaxf(top, s[u].x);
+        const float ref = top == -CUDART_INF_F ? 0.0f : top, f0 = ex2_approx((M - ref) * unit);
+        M = top;
+        l *= f0;
+#pragma unroll
+        for (int v = 0; v < V; v++) x[v] = make_float4(x[v].x * f0, x[v].y * f0, x[v].z * f0, x[v].w * f0);
+#pragma unroll
+        for (int u = 0; u < kFoldU; u++) {
+            const float f = ex2_approx((s[u].x - ref) * unit);
+            l = __fmaf_rn(s[u].y, f, l);
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                x[v].x = __fmaf_rn(y[u][v].x, f, x[v].x);
+                x[v].y = __fmaf_rn(y[u][v].y, f, x[v].y);
+                x[v].z = __fmaf_rn(y[u][v].z, f, x[v].z);
+                x[v].w = __fmaf_rn(y[u][v].w, f, x[v].w);
+            }
         }
     }
     const float z = inverse_sum(l, p.flash != 0);
