@@ -74,6 +74,7 @@ struct AttendParams {
     int32_t l2_ahead;       // rows: blocks a CTA asks for in L2 while the kernel before ends
     int32_t tok_tile, tok_blk, n_blk;   // chunk: tokens of a query tile and of a CTA's tiles, such blocks
     int64_t subs;           // chunk: sub-tiles of 64 keys of one KV head, over its blocks
+    int32_t gap;            // chunk: what a pair's beginning counts for where the work is cut, in sub-tiles
     float *part;            // [n_cta + n_vh][rows][D] partial outputs of a (CTA, head or pair); rows: 16,
                             // or a chunk block's 128 * n_tile
     float2 *stat;           // [n_cta + n_vh][rows] their (maximum, sum)

@@ -67,8 +67,8 @@ struct CL {
     static constexpr size_t o_k = o_q + NT * (size_t)q_tile;
     static constexpr size_t o_v = o_k + KS * (size_t)tile;
     static constexpr size_t o_raw = o_v + VS * (size_t)tile;
-    static constexpr size_t o_off = o_raw + RS * (size_t)unit;   // [128] where a tile's query rows are
-    static constexpr size_t o_bar = o_off + 128 * 8;
+    static constexpr size_t o_off = o_raw + RS * (size_t)unit;   // [NT][128] where the tiles' query rows are
+    static constexpr size_t o_bar = o_off + NT * 128 * 8;
     static constexpr int n_bar = 2 + 2 * KS + 2 * VS + 12 + 2 + 3 + 2 * RS;
     static constexpr size_t o_tm = o_bar + n_bar * 8;
     static constexpr size_t bytes = o_tm + 16;
@@ -82,51 +82,57 @@ __device__ __forceinline__ int subs_of(const AttendParams &p, int b)
     return (int)((last + kSub - 1) / kSub);
 }
 
+// The axis that is cut: of each pair p.gap units, what its beginning costs in
+// sub-tiles, then its sub-tiles.
+__device__ __forceinline__ int64_t axis_head(const AttendParams &p) { return p.subs + (int64_t)p.n_blk * p.gap; }
+
 __device__ __forceinline__ int64_t pair_start(const AttendParams &p, int pair)
 {
     const int b = pair % p.n_blk;
-    int64_t x = (int64_t)(pair / p.n_blk) * p.subs;
-    for (int i = 0; i < b; i++) x += subs_of(p, i);
+    int64_t x = (int64_t)(pair / p.n_blk) * axis_head(p);
+    for (int i = 0; i < b; i++) x += subs_of(p, i) + p.gap;
     return x;
 }
 
 __device__ __forceinline__ int64_t cta_begin(const AttendParams &p, int c)
 {
-    return (int64_t)c * (p.c.H * p.subs) / p.n_cta;
+    return (int64_t)c * (p.c.H * axis_head(p)) / p.n_cta;
 }
 
-// A walk over a CTA's sub-tiles: pair, sub-tile t of [t0, t1) of it (whole: all of the pair's).
+// A walk over a CTA's sub-tiles: pair, sub-tile t of [t0, t1) of its n.
 struct Walk {
     int pair, t0, t, t1, n;
-    int64_t left;   // sub-tiles from t0 of this pair on
+    int64_t at, end;   // axis: where the pair's sub-tile 0 is, the CTA's end
     __device__ __forceinline__ void begin(const AttendParams &p, int c)
     {
         const int64_t x = cta_begin(p, c);
-        left = cta_begin(p, c + 1) - x;
-        const int h = (int)(x / p.subs);
-        int64_t rem = x - (int64_t)h * p.subs;
+        end = cta_begin(p, c + 1);
+        const int h = (int)(x / axis_head(p));
+        int64_t rem = x - (int64_t)h * axis_head(p);
         int b = 0;
         for (; b < p.n_blk - 1; b++) {
-            const int k = subs_of(p, b);
+            const int k = subs_of(p, b) + p.gap;
             if (rem < k) break;
             rem -= k;
         }
         pair = h * p.n_blk + b;
-        t0 = t = (int)rem;
+        at = x - rem + p.gap;
+        t0 = t = (int)max((int64_t)0, rem - p.gap);
         span(p);
     }
     __device__ __forceinline__ void span(const AttendParams &p)
     {
         n = subs_of(p, pair % p.n_blk);
-        t1 = (int)min((int64_t)n, t0 + left);
+        t1 = (int)min((int64_t)n, end - at);   // (below t0: none of this pair's)
     }
-    __device__ __forceinline__ bool more() const { return left > 0; }
+    __device__ __forceinline__ bool more() const { return t0 < t1; }   // (an axis that ends in a gap: no pair after it)
     __device__ __forceinline__ void next_pair(const AttendParams &p)
     {
-        left -= t1 - t0;
         pair++;
         t0 = t = 0;
-        if (left > 0) span(p);
+        at += n + p.gap;
+        t1 = 0;
+        if (at < end) span(p);
     }
     __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == n; }
 };
@@ -152,34 +158,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
-__device__ __forceinline__ uint64_t pk2(float lo, float hi)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-
-__device__ __forceinline__ float2 up2(uint64_t v)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 
@@ -250,6 +228,27 @@ __device__ __forceinline__ void store_out4(const AttendParams &p, int64_t i, flo
     }
 }
 
+__device__ __forceinline__ void st_v8(float *p, const float (&x)[8])
+{
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]),
+                 "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+                 : "memory");
+}
+
+__device__ __forceinline__ void store_out8(const AttendParams &p, int64_t i, const float (&x)[8])
+{
+    if (p.out_f16 && p.out_vec) {
+        uint4 w;
+        __half2 *h = reinterpret_cast<__half2 *>(&w);
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = __floats2half2_rn(x[2 * e], x[2 * e + 1]);
+        *reinterpret_cast<uint4 *>(static_cast<__half *>(p.out) + i) = w;
+    } else {
+        store_out4(p, i, make_float4(x[0], x[1], x[2], x[3]));
+        store_out4(p, i + 4, make_float4(x[4], x[5], x[6], x[7]));
+    }
+}
+
 __device__ __forceinline__ float inverse_sum(float l, bool flash)
 {
     return l == 0.0f ? (flash ? 0.0f : CUDART_NAN_F) : 1.0f / l;
@@ -308,10 +307,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tm_slot;
+    Walk w;
+    w.begin(p, cta);
     pdl_launch_dependents();
     pdl_wait();
 
-    Walk w;
     if (warp < 4) {
         regs_dec<96>();
         if (lane == 0 && warp == 3) {
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const uint32_t raw = smem_addr(smem + L::o_raw);
             int u = 0;
             bool ok = true;
-            for (w.begin(p, cta); ok && w.more(); w.next_pair(p)) {
+            for (; ok && w.more(); w.next_pair(p)) {
                 const int64_t head = (int64_t)(w.pair / p.n_blk) * p.c.rows;
                 for (int t = w.t0; ok && t < w.t1; t++) {
                     const int64_t key0 = (int64_t)t * kSub;
@@ -349,7 +349,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             };
             int i = 0;   // sub-tiles of the CTA so far
             bool ok = true;
-            w.begin(p, cta);
             if (warp < 2) {
                 const int g = warp;
                 int n = 0;   // sub-tiles of tile g so far
@@ -448,18 +447,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             }
             return true;
         };
-        w.begin(p, cta);
         for (int seg = 0; ok && w.more(); seg++, w.next_pair(p)) {
             const int h = w.pair / p.n_blk, b = w.pair % p.n_blk, nt = tiles_of(p, b);
             if (seg > 0 && !(ok = wait(q_empty, (seg - 1) & 1))) break;
-            for (int g = 0; g < nt; g++) {
-                const int tk = st / p.r, tok = b * p.tok_blk + g * p.tok_tile + tk;
-                named_sync(1, 128);   // (the tile before has been staged)
-                off[st] = tk < p.tok_tile && tok < p.n_new
-                              ? tok * p.q_stride + (int64_t)(h * p.r + st - tk * p.r) * D : -1;
-                named_sync(1, 128);
-                stage_queries<D>(p, smem_addr(smem + L::o_q) + g * L::q_tile, 16384, off, st);
+            named_sync(1, 128);   // (the tiles before have been staged)
+            const int tk = st / p.r, in = st - tk * p.r;
+#pragma unroll
+            for (int g = 0; g < L::NT; g++) {
+                const int tok = b * p.tok_blk + g * p.tok_tile + tk;
+                off[g * 128 + st] = tk < p.tok_tile && tok < p.n_new ? tok * p.q_stride + (int64_t)(h * p.r + in) * D : -1;
             }
+            named_sync(1, 128);
+            for (int g = 0; g < nt; g++) stage_queries<D>(p, smem_addr(smem + L::o_q) + g * L::q_tile, 16384, off + g * 128, st);
+            cp_async_wait<0>();
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
@@ -484,7 +484,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         const int64_t n_sc = p.c.rows / kBlock;
         int n = 0;
         bool ok = true;
-        w.begin(p, cta);
         for (int seg = 0; ok && w.more(); seg++, w.next_pair(p)) {
             const int h = w.pair / p.n_blk, b = w.pair % p.n_blk;
             if (g >= tiles_of(p, b)) {   // no rows in this tile: keep step with the other one
@@ -640,7 +639,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                 else if (p.row_stat) p.row_stat[(int64_t)h * p.n_new * p.r + (int64_t)tok * p.r + hd] = row_stat_of(m, l);
             }
             const int64_t dst = (int64_t)tok * p.out_stride + (int64_t)(h * p.r + hd) * D;
-            const uint64_t pol = policy_evict_last();   // a cut pair's rows stay in L2 for the fold
 #pragma unroll 1
             for (int ch = 0; ch < D / 32; ch++) {
                 uint32_t o[32];
@@ -648,11 +646,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                 tmem_wait_ld();
                 if (!valid) continue;
 #pragma unroll
-                for (int q = 0; q < 8; q++) {
-                    const float4 x = make_float4(__fmaf_rn(__uint_as_float(o[4 * q]), scl, bad), __fmaf_rn(__uint_as_float(o[4 * q + 1]), scl, bad),
-                                                 __fmaf_rn(__uint_as_float(o[4 * q + 2]), scl, bad), __fmaf_rn(__uint_as_float(o[4 * q + 3]), scl, bad));
-                    if (whole) store_out4(p, dst + ch * 32 + 4 * q, x);
-                    else st_v4_hint(p.part + part_at<D>(block, in, ch * 32 + 4 * q), x, pol);
+                for (int q = 0; q < 4; q++) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = __fmaf_rn(__uint_as_float(o[8 * q + e]), scl, bad);
+                    if (whole) store_out8(p, dst + ch * 32 + 8 * q, x);
+                    else st_v8(p.part + part_at<D>(block, in, ch * 32 + 8 * q), x);
                 }
             }
             tc_fence_before();
@@ -681,7 +680,7 @@ __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
     const int pair = blockIdx.x / (rows_blk / 8), in = blockIdx.x % (rows_blk / 8) * 8 + warp;
     const int h = pair / p.n_blk, b = pair % p.n_blk, tk = (in & 127) / p.r, hd = (in & 127) - tk * p.r;
     const int tok = b * p.tok_blk + (in >> 7) * p.tok_tile + tk;
-    const int64_t W = p.c.H * p.subs, x0 = pair_start(p, pair), x1 = x0 + subs_of(p, b) - 1;
+    const int64_t W = p.c.H * axis_head(p), x0 = pair_start(p, pair) + p.gap, x1 = x0 + subs_of(p, b) - 1;
     const int c0 = (int)(((x0 + 1) * p.n_cta - 1) / W), c1 = (int)(((x1 + 1) * p.n_cta - 1) / W);
     pdl_wait();
     if (c0 == c1 || tk >= p.tok_tile || tok >= p.n_new) return;
@@ -766,6 +765,10 @@ void chunk_split(AttendParams &p)
         p.subs += (last + kSub - 1) / kSub;
     }
     p.n_cta = (int)std::min<int64_t>(kSMs, p.c.H * p.subs);
+    // A pair's beginning and end cost a CTA about 8 us, 6 sub-tiles (512 tokens
+    // at 4k: CTAs of one pair were done after 50 us, of two after 67); where
+    // the ranges are short they stay even, for the sake of more CTAs.
+    p.gap = (int)std::min<int64_t>(6, p.c.H * p.subs / p.n_cta / 8);
 }
 
 cudaError_t launch_chunk(const AttendParams &p, cudaStream_t st)

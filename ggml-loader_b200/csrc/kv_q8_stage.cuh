@@ -25,6 +25,35 @@ __device__ __forceinline__ void sts128(uint32_t at, uint4 v)
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// ---- packed F32 pairs
+__device__ __forceinline__ uint64_t pk2(float lo, float hi)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+__device__ __forceinline__ float2 up2(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 // n bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory, completed on `bar`
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t n, uint64_t *bar)
 {
@@ -41,8 +70,8 @@ __device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void *sr
 
 // 128 query rows as F16 in the swizzled layout, by 128 threads (t); off[row] is
 // where a row's elements start, -1 for a row of zeros (shared memory, complete).
-// Aligned F16 rows go straight to shared memory; others through registers, four
-// loads in flight.
+// Aligned F16 rows go straight to shared memory (complete after cp_async_wait);
+// others through registers, four loads in flight.
 template <int D>
 __device__ __forceinline__ void stage_queries(const AttendParams &p, uint32_t dst, uint32_t box, const int64_t *off, int t)
 {
@@ -57,7 +86,6 @@ __device__ __forceinline__ void stage_queries(const AttendParams &p, uint32_t ds
                                 q + (at < 0 ? 0 : at + c * 8), at >= 0);
         }
         sm100::cp_async_commit();
-        sm100::cp_async_wait<0>();
     } else {
 #pragma unroll 1
         for (int x0 = t; x0 < 128 * C; x0 += 4 * 128) {

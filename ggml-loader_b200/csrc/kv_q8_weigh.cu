@@ -37,7 +37,7 @@ struct WL {
     static constexpr int n_ld = 128 * D / 16 / 128;    // 16-byte loads a staging thread makes for an item's codes
     static constexpr int ctas = D == 256 ? 1 : 2;      // an SM
     static constexpr size_t o_k = 0, o_q = tile;
-    static constexpr size_t o_st = o_q + 2 * (size_t)tile;   // [2][128] (m, 1 / Z)
+    static constexpr size_t o_st = o_q + 2 * (size_t)tile;   // [2][64] two rows' (-m, -m, 1 / Z, 1 / Z)
     static constexpr size_t o_lim = o_st + 2 * 128 * 8;      // [2][128] the last key a row may see
     static constexpr size_t o_off = o_lim + 2 * 128 * 4;     // [2][128] where a row's queries are, -1: nowhere
     static constexpr size_t o_bar = o_off + 2 * 128 * 8;
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
     uint64_t *drain = bar + 10;
     uint32_t *tm_slot = reinterpret_cast<uint32_t *>(smem + L::o_tm);
     volatile int *flag = reinterpret_cast<volatile int *>(smem + L::o_tm + 8);
-    float2 *row_st = reinterpret_cast<float2 *>(smem + L::o_st);
+    float4 *row_st = reinterpret_cast<float4 *>(smem + L::o_st);
     int *row_lim = reinterpret_cast<int *>(smem + L::o_lim);
     int64_t *row_off = reinterpret_cast<int64_t *>(smem + L::o_off);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -131,6 +131,8 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tm_slot;
+    Steps w;
+    w.begin(p, blockIdx.x, gridDim.x);
     pdl_launch_dependents();
     pdl_wait();
     auto wait = [&](uint64_t *b, uint32_t par) {
@@ -139,8 +141,6 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
         return false;
     };
 
-    Steps w;
-    w.begin(p, blockIdx.x, gridDim.x);
     bool ok = true;
     int q = -1, s = 0, items = 0;   // query tiles staged (the present one's number), steps, items begun
     if (warp < 4) {
@@ -156,50 +156,57 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
             ok = __all_sync(0xffffffffu, wait(&q_full[q & 1], (q >> 1) & 1) && wait(&s_full[s & 1], (s >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
-            const float4 *st = reinterpret_cast<const float4 *>(row_st + (q & 1) * 128);
+            const float4 *st = row_st + (q & 1) * 64;
             const int *lim = row_lim + (q & 1) * 128;
-            const int row0 = w.qt * 128, n_rows = min(128, p.n_new * p.r - row0);
+            const int row0 = w.qt * 128, n_rows = min(128, p.n_new * p.r - row0), n_ch = (n_rows + 31) / 32;
             const bool all = MASKED || w.key0 + 127 <= p.n_past + row0 / p.r;   // every row sees every key
             const bool in = key < p.n_kv;
-            float part = 0.0f;
-#pragma unroll 1
-            for (int ch = 0; ch < 4; ch++) {
-                if (ch * 32 >= n_rows) break;
-                uint32_t v[32];
-                tmem_ld32(tS + (s & 1) * 128 + ch * 32, v);
-                tmem_wait_ld();
+            uint64_t part = 0ull;   // two sums
+            const uint64_t c2 = pk2(c, c);
+            // 32 rows' scores
+            auto rows = [&](int ch, uint32_t (&v)[32]) {
                 if constexpr (MASKED) {
                     int tok = -1;
-                    float mk = 0.0f;
+                    float mk = 0.0f, a = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
                         const int row = row0 + ch * 32 + e;
                         if (row - row0 >= n_rows) break;
-                        const float2 y = row_st[(q & 1) * 128 + ch * 32 + e];
+                        const float4 y4 = st[ch * 16 + e / 2];
+                        const float m = e & 1 ? y4.y : y4.x, y = e & 1 ? y4.w : y4.z;
+                        if (y == 0.0f) continue;   // (its mask may be infinite)
                         if (row / p.r != tok) {   // (the same for all lanes)
                             tok = row / p.r;
                             const int64_t i = tok * p.mask_stride + key;
                             mk = -CUDART_INF_F;
                             if (in) mk = p.mask_f16 ? __half2float(static_cast<const __half *>(p.mask)[i]) : static_cast<const float *>(p.mask)[i];
                         }
-                        if (y.y == 0.0f) continue;   // (its mask may be infinite)
-                        part = __fmaf_rn(ex2_approx((__fmaf_rn(__uint_as_float(v[e]), c, mk) - y.x) * kLog2e), y.y, part);
+                        a = __fmaf_rn(ex2_approx((__fmaf_rn(__uint_as_float(v[e]), c, mk) + m) * kLog2e), y, a);
                     }
+                    part = add2(part, pk2(a, 0.0f));
                 } else {
                     if (!all) {
 #pragma unroll
                         for (int e = 0; e < 32; e++)
                             if (key > lim[ch * 32 + e]) v[e] = __float_as_uint(-CUDART_INF_F);
                     }
-                    float a = 0.0f, b = 0.0f;
+                    uint64_t s0 = 0ull, s1 = 0ull;
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const float4 y = st[ch * 16 + e];   // two rows' (m, 1 / Z)
-                        a = __fmaf_rn(ex2_approx(__fmaf_rn(__uint_as_float(v[2 * e]), c, -y.x)), y.y, a);
-                        b = __fmaf_rn(ex2_approx(__fmaf_rn(__uint_as_float(v[2 * e + 1]), c, -y.z)), y.w, b);
+                        const float4 y = st[ch * 16 + e];
+                        const float2 x = up2(fma2(pk2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, pk2(y.x, y.y)));
+                        uint64_t &sum = e & 1 ? s1 : s0;
+                        sum = fma2(pk2(ex2_approx(x.x), ex2_approx(x.y)), pk2(y.z, y.w), sum);
                     }
-                    part += a + b;
+                    part = add2(part, add2(s0, s1));
                 }
+            };
+#pragma unroll 1
+            for (int ch = 0; ch < n_ch; ch++) {
+                uint32_t v[32];
+                tmem_ld32(tS + (s & 1) * 128 + ch * 32, v);
+                tmem_wait_ld();
+                rows(ch, v);
             }
             tc_fence_before();
             __syncwarp();
@@ -207,7 +214,10 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
                 mbar_arrive(&s_empty[s & 1]);
                 if (w.done_with_q(p)) mbar_arrive(&q_empty[q & 1]);
             }
-            sum += part;
+            {
+                const float2 x = up2(part);
+                sum += x.x + x.y;
+            }
             if (w.last()) {
                 if (in) p.c.weight[(int64_t)w.h * p.c.rows + key] += sum;
                 sum = 0.0f;
@@ -255,12 +265,15 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
                 // a row that adds nothing has 1 / Z = 0: its queries are zeros, so that its products are finite
                 const float2 y = row0 + t < R ? stat[t] : make_float2(0.0f, 0.0f);
                 const int tok = (row0 + t) / p.r, j = row0 + t - tok * p.r;
-                row_st[(q & 1) * 128 + t] = y;
+                float *rs = reinterpret_cast<float *>(row_st + (q & 1) * 64 + t / 2) + (t & 1);
+                rs[0] = -y.x;
+                rs[2] = y.y;
                 row_lim[(q & 1) * 128 + t] = (int)(p.n_past + tok);
                 off[t] = y.y != 0.0f ? tok * p.q_stride + (int64_t)(w.h * p.r + j) * D : -1;
             }
             named_sync(1, 128);
             stage_queries<D>(p, sq + (q & 1) * L::tile, L::box, off, t);
+            cp_async_wait<0>();
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[q & 1]);
