@@ -80,7 +80,7 @@ struct AttendParams {
     float2 *stat;           // [n_cta + n_vh][rows] their (maximum, sum)
     float *scores;          // [H][n_new * r][nb * kBlock] or null
     float2 *row_stat;       // [H][n_new * r] (maximum, 1 / sum or 0) or null
-    int32_t n_kt;           // weigh: tiles of 128 keys, ceil(n_kv / 128)
+    int32_t n_kt;           // weigh: a KV head's items of 128 or 256 keys
     unsigned *error;        // the device's record of waits that expired
 };
 // bytes of workspace (a function of the sizes alone)

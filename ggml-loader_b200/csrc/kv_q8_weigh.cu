@@ -7,12 +7,14 @@
 // its sum never leaves its registers: no atomics, one order.  Half the products
 // of the attention itself; the exponentials are the bound (16 a clock and SM).
 //
-// An item is (KV head, 128 keys); a CTA takes a range of items and for each
-// walks the query tiles that see them.  288 threads, two CTAs an SM up to
-// head_dim 128:
-//   warps 0-3  a key a thread: S^T from TMEM, exponentials, the sum
-//   warps 4-7  stage: the item's codes as F16, query tiles and their rows' (m, 1 / Z)
-//   warp 8     issues the MMAs, owns TMEM
+// An item is (KV head, NK tiles of 128 keys); a CTA takes a range of items and
+// for each walks the query tiles that see them, which L2 delivers again for
+// every item: with two tiles of keys an item half as often (512 tokens at 4k,
+// where that was the bound: 37 us with one tile, two CTAs an SM, against 26).
+//   4 warps a key tile  a key a thread: S^T from TMEM, exponentials, the sum
+//   4 warps             stage: the item's codes as F16, query tiles and their
+//                       rows' (m, 1 / Z)
+//   1 warp              issues the MMAs, owns TMEM
 #include <math_constants.h>
 
 #include <algorithm>
@@ -27,27 +29,29 @@ namespace {
 using namespace sm100;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kThreads = 288;
 
-template <int D>
+template <int D, int NK>
 struct WL {
+    static constexpr int threads = NK * 128 + 128 + 32;
     static constexpr int NB = (D + 63) / 64;
     static constexpr uint32_t box = 128 * 128;         // [128 rows][64 halves]
     static constexpr uint32_t tile = NB * box;         // K or Q tile
-    static constexpr int n_ld = 128 * D / 16 / 128;    // 16-byte loads a staging thread makes for an item's codes
-    static constexpr int ctas = D == 256 ? 1 : 2;      // an SM
-    static constexpr size_t o_k = 0, o_q = tile;
-    static constexpr size_t o_st = o_q + 2 * (size_t)tile;   // [2][64] two rows' (-m, -m, 1 / Z, 1 / Z)
-    static constexpr size_t o_lim = o_st + 2 * 128 * 8;      // [2][128] the last key a row may see
-    static constexpr size_t o_off = o_lim + 2 * 128 * 4;     // [2][128] where a row's queries are, -1: nowhere
-    static constexpr size_t o_bar = o_off + 2 * 128 * 8;
-    static constexpr int n_bar = 2 + 4 + 4 + 1;
+    static constexpr int n_ld = NK * D / 16;           // 16-byte loads a staging thread makes for an item's codes
+    static constexpr int ctas = D == 256 || NK == 2 ? 1 : 2;   // an SM
+    static constexpr int QS = NK == 2 ? 4 : 2;         // query tiles staged or in use
+    static constexpr size_t o_k = 0, o_q = NK * (size_t)tile;
+    static constexpr size_t o_st = o_q + QS * (size_t)tile;   // [QS][64] two rows' (-m, -m, 1 / Z, 1 / Z)
+    static constexpr size_t o_lim = o_st + QS * 128 * 8;      // [QS][128] the last key a row may see
+    static constexpr size_t o_off = o_lim + QS * 128 * 4;     // [QS][128] where a row's queries are, -1: nowhere
+    static constexpr size_t o_bar = o_off + QS * 128 * 8;
+    static constexpr int n_bar = 2 + 2 * QS + 4 + 1;
     static constexpr size_t o_tm = o_bar + n_bar * 8;
     static constexpr size_t bytes = o_tm + 16;
     static_assert(bytes * ctas <= 226 * 1024, "shared memory");
 };
 
 // A walk over a CTA's (item, query tile) steps, the same in every warp.
+template <int NK>
 struct Steps {
     int64_t item, end;
     int h, qt, n_qt;
@@ -67,7 +71,7 @@ struct Steps {
     __device__ __forceinline__ void enter(const AttendParams &p)
     {
         h = (int)(item / p.n_kt);
-        key0 = (item - (int64_t)h * p.n_kt) * 128;
+        key0 = (item - (int64_t)h * p.n_kt) * (128 * NK);
         // tiles whose last token comes before the keys do not see them
         const int64_t tok0 = p.mask ? 0 : max((int64_t)0, key0 - p.n_past);
         qt = (int)(tok0 * p.r / 128);
@@ -96,14 +100,15 @@ struct Steps {
     }
 };
 
-template <int D, bool MASKED>
-__global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const AttendParams p)
+template <int D, int NK, bool MASKED>
+__global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_kernel(const AttendParams p)
 {
-    using L = WL<D>;
+    using L = WL<D, NK>;
+    constexpr int QS = L::QS, kStage = NK * 4, kIssue = kStage + 4;   // the first staging warp, the issuing warp
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::o_bar);
-    uint64_t *k_full = bar, *k_empty = bar + 1, *q_full = bar + 2, *q_empty = bar + 4, *s_full = bar + 6, *s_empty = bar + 8;
-    uint64_t *drain = bar + 10;
+    uint64_t *k_full = bar, *k_empty = bar + 1, *q_full = bar + 2, *q_empty = q_full + QS, *s_full = q_empty + QS;
+    uint64_t *s_empty = s_full + 2, *drain = s_empty + 2;
     uint32_t *tm_slot = reinterpret_cast<uint32_t *>(smem + L::o_tm);
     volatile int *flag = reinterpret_cast<volatile int *>(smem + L::o_tm + 8);
     float4 *row_st = reinterpret_cast<float4 *>(smem + L::o_st);
@@ -113,25 +118,27 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
     if (tid == 0) {
         mbar_init(k_full, 4);
         mbar_init(k_empty, 1);
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < QS; i++) {
             mbar_init(&q_full[i], 4);
-            mbar_init(&q_empty[i], 5);   // the MMAs that read it, and the 4 warps that read its rows' numbers
+            mbar_init(&q_empty[i], 1 + kStage);   // the MMAs that read it, and the warps that read its rows' numbers
+        }
+        for (int i = 0; i < 2; i++) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&s_empty[i], 4);
+            mbar_init(&s_empty[i], kStage);
         }
         mbar_init(drain, 1);
         *flag = 0;
         fence_mbar_init();
     }
-    if (warp == 8) {
-        tmem_alloc(tm_slot, 256);
+    if (warp == kIssue) {
+        tmem_alloc(tm_slot, 256 * NK);
         tmem_relinquish();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tm_slot;
-    Steps w;
+    Steps<NK> w;
     w.begin(p, blockIdx.x, gridDim.x);
     pdl_launch_dependents();
     pdl_wait();
@@ -143,23 +150,29 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
 
     bool ok = true;
     int q = -1, s = 0, items = 0;   // query tiles staged (the present one's number), steps, items begun
-    if (warp < 4) {
-        const uint32_t tS = tmem + ((uint32_t)(warp * 32) << 16);
-        float sum = 0.0f;
+    if (warp < kStage) {
+        const int kt = warp >> 2;   // key tile of the item
+        const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kt * 128;
+        float sum = 0.0f, c = 0.0f;
+        int64_t now = -1;
         for (; ok && w.more(); s++) {
             if (w.fresh) q++;
-            const int64_t key = w.key0 + tid;
-            // (key 0 of the tile is a row of the cache: the block of a lane past the cache is the last one)
-            const int64_t blk = min(key / kBlock, p.c.rows / kBlock - 1);
-            const uint32_t kw = __ldg(reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)w.h * (p.c.rows / kBlock) + blk);
-            const float c = p.scale * pow2(scale_exp(kw)) * (MASKED ? 1.0f : kLog2e);
-            ok = __all_sync(0xffffffffu, wait(&q_full[q & 1], (q >> 1) & 1) && wait(&s_full[s & 1], (s >> 1) & 1));
+            const int64_t key = w.key0 + tid;   // (the warps of a tile are in lane order)
+            const int qs = q % QS;
+            if (w.item != now) {
+                // (key 0 of the item is a row of the cache: the block of a lane past the cache is the last one)
+                now = w.item;
+                const int64_t blk = min(key / kBlock, p.c.rows / kBlock - 1);
+                const uint32_t kw = __ldg(reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)w.h * (p.c.rows / kBlock) + blk);
+                c = p.scale * pow2(scale_exp(kw)) * (MASKED ? 1.0f : kLog2e);
+            }
+            ok = __all_sync(0xffffffffu, wait(&q_full[qs], (q / QS) & 1) && wait(&s_full[s & 1], (s >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
-            const float4 *st = row_st + (q & 1) * 64;
-            const int *lim = row_lim + (q & 1) * 128;
+            const float4 *st = row_st + qs * 64;
+            const int *lim = row_lim + qs * 128;
             const int row0 = w.qt * 128, n_rows = min(128, p.n_new * p.r - row0), n_ch = (n_rows + 31) / 32;
-            const bool all = MASKED || w.key0 + 127 <= p.n_past + row0 / p.r;   // every row sees every key
+            const bool all = MASKED || w.key0 + kt * 128 + 127 <= p.n_past + row0 / p.r;   // every row sees every key
             const bool in = key < p.n_kv;
             uint64_t part = 0ull;   // two sums
             const uint64_t c2 = pk2(c, c);
@@ -204,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
 #pragma unroll 1
             for (int ch = 0; ch < n_ch; ch++) {
                 uint32_t v[32];
-                tmem_ld32(tS + (s & 1) * 128 + ch * 32, v);
+                tmem_ld32(tS + (s & 1) * (128 * NK) + ch * 32, v);
                 tmem_wait_ld();
                 rows(ch, v);
             }
@@ -212,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&s_empty[s & 1]);
-                if (w.done_with_q(p)) mbar_arrive(&q_empty[q & 1]);
+                if (w.done_with_q(p)) mbar_arrive(&q_empty[qs]);
             }
             {
                 const float2 x = up2(part);
@@ -224,12 +237,12 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
             }
             w.next(p);
         }
-    } else if (warp < 8) {
-        const int t = tid - 128;
+    } else if (warp < kIssue) {
+        const int t = tid - kStage * 32;
         uint4 buf[L::n_ld];
         auto load = [&](int64_t item) {
             const int h = (int)(item / p.n_kt);
-            const int64_t key0 = (item - (int64_t)h * p.n_kt) * 128;
+            const int64_t key0 = (item - (int64_t)h * p.n_kt) * (128 * NK);
             const uint4 *src = reinterpret_cast<const uint4 *>(p.c.k + ((int64_t)h * p.c.rows + key0) * D);
 #pragma unroll
             for (int j = 0; j < L::n_ld; j++) {
@@ -246,7 +259,8 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
 #pragma unroll
                 for (int j = 0; j < L::n_ld; j++) {
                     const int i = t + 128 * j;
-                    store_codes(sk, L::box, i / (D / 16), i % (D / 16), buf[j]);
+                    const int r = i / (D / 16);
+                    store_codes(sk + (r >> 7) * L::tile, L::box, r & 127, i % (D / 16), buf[j]);
                 }
                 fence_async_smem();
                 __syncwarp();
@@ -257,26 +271,27 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
             }
             if (!w.fresh) continue;
             q++;
-            if (q >= 2 && !(ok = all_wait(&q_empty[q & 1], ((q >> 1) - 1) & 1))) break;
+            const int qs = q % QS;
+            if (q >= QS && !(ok = all_wait(&q_empty[qs], (q / QS - 1) & 1))) break;
             const int row0 = w.qt * 128, R = p.n_new * p.r;
             const float2 *stat = p.row_stat + (int64_t)w.h * R + row0;
-            int64_t *off = row_off + (q & 1) * 128;
+            int64_t *off = row_off + qs * 128;
             {
                 // a row that adds nothing has 1 / Z = 0: its queries are zeros, so that its products are finite
                 const float2 y = row0 + t < R ? stat[t] : make_float2(0.0f, 0.0f);
                 const int tok = (row0 + t) / p.r, j = row0 + t - tok * p.r;
-                float *rs = reinterpret_cast<float *>(row_st + (q & 1) * 64 + t / 2) + (t & 1);
+                float *rs = reinterpret_cast<float *>(row_st + qs * 64 + t / 2) + (t & 1);
                 rs[0] = -y.x;
                 rs[2] = y.y;
-                row_lim[(q & 1) * 128 + t] = (int)(p.n_past + tok);
+                row_lim[qs * 128 + t] = (int)(p.n_past + tok);
                 off[t] = y.y != 0.0f ? tok * p.q_stride + (int64_t)(w.h * p.r + j) * D : -1;
             }
             named_sync(1, 128);
-            stage_queries<D>(p, sq + (q & 1) * L::tile, L::box, off, t);
+            stage_queries<D>(p, sq + qs * L::tile, L::box, off, t);
             cp_async_wait<0>();
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[q & 1]);
+            if (lane == 0) mbar_arrive(&q_full[qs]);
         }
     } else if (lane == 0) {
         constexpr uint32_t id = idesc_f16_f32(128, 128, false);
@@ -289,17 +304,20 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
             }
             if (w.fresh) {
                 q++;
-                if (!(ok = wait(&q_full[q & 1], (q >> 1) & 1))) break;
+                if (!(ok = wait(&q_full[q % QS], (q / QS) & 1))) break;
             }
             if (s >= 2 && !(ok = wait(&s_empty[s & 1], ((s >> 1) - 1) & 1))) break;
             tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < D / 16; kk++) {
-                const uint32_t off = (kk >> 2) * L::box + (kk & 3) * 32;
-                umma_ss(tmem + (s & 1) * 128, sdesc_k_sw128(sk + off), sdesc_k_sw128(sq + (q & 1) * L::tile + off), id, kk > 0);
-            }
+            for (int k = 0; k < NK; k++)
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    const uint32_t off = (kk >> 2) * L::box + (kk & 3) * 32;
+                    umma_ss(tmem + (s & 1) * (128 * NK) + k * 128, sdesc_k_sw128(sk + k * L::tile + off),
+                            sdesc_k_sw128(sq + (q % QS) * L::tile + off), id, kk > 0);
+                }
             umma_commit(&s_full[s & 1]);
-            if (w.done_with_q(p)) umma_commit(&q_empty[q & 1]);
+            if (w.done_with_q(p)) umma_commit(&q_empty[q % QS]);
             if (w.last()) umma_commit(k_empty);
         }
         umma_commit(drain);
@@ -307,23 +325,33 @@ __global__ void __launch_bounds__(kThreads, WL<D>::ctas) weigh_kernel(const Atte
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kIssue) {
         tc_fence_after();
-        tmem_dealloc(tmem, 256);
+        tmem_dealloc(tmem, 256 * NK);
     }
 }
 
-template <int D, bool MASKED>
-cudaError_t run(const AttendParams &p, cudaStream_t st)
+template <int D, int NK, bool MASKED>
+cudaError_t run(AttendParams p, cudaStream_t st)
 {
-    using L = WL<D>;
+    using L = WL<D, NK>;
     static Once once;
     cudaError_t e = once.on_device([] {
-        return cudaFuncSetAttribute(weigh_kernel<D, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::bytes);
+        return cudaFuncSetAttribute(weigh_kernel<D, NK, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::bytes);
     });
     if (e != cudaSuccess) return e;
+    p.n_kt = (int)((p.n_kv + 128 * NK - 1) / (128 * NK));
     const unsigned grid = (unsigned)std::min<int64_t>((int64_t)p.c.H * p.n_kt, kSMs * L::ctas);
-    return launch_pdl(weigh_kernel<D, MASKED>, grid, kThreads, L::bytes, p, st);
+    return launch_pdl(weigh_kernel<D, NK, MASKED>, grid, L::threads, L::bytes, p, st);
+}
+
+template <int D, bool MASKED>
+cudaError_t run_d(const AttendParams &p, cudaStream_t st)
+{
+    // two tiles of keys an item where that leaves most SMs one (at head_dim 256 their codes would not fit)
+    if constexpr (D < 256)
+        if (p.c.H * ((p.n_kv + 255) / 256) >= kSMs / 2) return run<D, 2, MASKED>(p, st);
+    return run<D, 1, MASKED>(p, st);
 }
 
 }  // namespace
@@ -331,10 +359,10 @@ cudaError_t run(const AttendParams &p, cudaStream_t st)
 cudaError_t launch_weigh(const AttendParams &p, cudaStream_t st)
 {
     switch (p.c.D) {
-    case 64: return p.mask ? run<64, true>(p, st) : run<64, false>(p, st);
-    case 96: return p.mask ? run<96, true>(p, st) : run<96, false>(p, st);
-    case 128: return p.mask ? run<128, true>(p, st) : run<128, false>(p, st);
-    case 256: return p.mask ? run<256, true>(p, st) : run<256, false>(p, st);
+    case 64: return p.mask ? run_d<64, true>(p, st) : run_d<64, false>(p, st);
+    case 96: return p.mask ? run_d<96, true>(p, st) : run_d<96, false>(p, st);
+    case 128: return p.mask ? run_d<128, true>(p, st) : run_d<128, false>(p, st);
+    case 256: return p.mask ? run_d<256, true>(p, st) : run_d<256, false>(p, st);
     default: return cudaErrorInvalidValue;
     }
 }

@@ -211,7 +211,8 @@ def test_attend_causal(d, h, hq, n_new, n_past):
 
 @pytest.mark.parametrize("d, h, hq, n_past, n_new", [(128, 2, 8, 9000, 1), (64, 1, 7, 20011, 1), (96, 2, 2, 5000, 6),
                                                      (256, 1, 4, 4100, 3), (128, 1, 4, 6000, 40), (64, 2, 4, 3000, 300),
-                                                     (128, 8, 32, 2500, 1), (128, 1, 8, 2049, 129)])
+                                                     (128, 8, 32, 2500, 1), (128, 1, 8, 2049, 129), (64, 8, 8, 2600, 33),
+                                                     (96, 8, 24, 2450, 70), (128, 8, 32, 2500, 40), (128, 16, 16, 1300, 600)])
 @pytest.mark.parametrize("weight", [False, True])
 def test_attend_long(d, h, hq, n_past, n_new, weight):
     c = filled(h, n_past + n_new, d, weight=weight, seed=1)
@@ -223,9 +224,10 @@ def test_attend_long(d, h, hq, n_past, n_new, weight):
 
 @pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("flash", [False, True])
-@pytest.mark.parametrize("h, hq, n_new", [(2, 8, 1), (2, 8, 3), (1, 5, 9), (2, 12, 30)])
-def test_attend_mask(f16, flash, h, hq, n_new):
-    n_past, d = 333, 128
+@pytest.mark.parametrize("h, hq, n_new, n_past", [(2, 8, 1, 333), (2, 8, 3, 333), (1, 5, 9, 333), (2, 12, 30, 333),
+                                                  (10, 20, 21, 2000)])
+def test_attend_mask(f16, flash, h, hq, n_new, n_past):
+    d = 128
     n_kv = n_past + n_new
     c = filled(h, n_kv, d, weight=True)
     g = torch.Generator().manual_seed(4)
