@@ -497,14 +497,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.c.k_scale) + h * n_sc;
             const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.c.v_scale) + h * n_sc;
             float m = -CUDART_INF_F, me = 0.0f, l = 0.0f, bad = 0.0f;
-            // a sub-tile's scale words, one sub-tile ahead (the last block of a cache may be the first of the two)
+            // a sub-tile's scale words, one sub-tile ahead; a block behind the keys holds anything: 1 stands for its scale
             uint32_t kw[2], vw[2];
             auto scales = [&](int t) {
-                const int64_t i0 = min(2 * (int64_t)t, n_sc - 1), i1 = min(2 * (int64_t)t + 1, n_sc - 1);
-                kw[0] = __ldg(ksc + i0);
-                kw[1] = __ldg(ksc + i1);
-                vw[0] = __ldg(vsc + i0);
-                vw[1] = __ldg(vsc + i1);
+                const int64_t i = 2 * (int64_t)t;
+                const bool two = (i + 1) * kBlock < p.n_kv;
+                kw[0] = __ldg(ksc + i);
+                vw[0] = __ldg(vsc + i);
+                kw[1] = two ? __ldg(ksc + i + 1) : 0x3f800000u;
+                vw[1] = two ? __ldg(vsc + i + 1) : 0x3f800000u;
             };
             scales(w.t0);
             const int n0 = n;

@@ -24,9 +24,13 @@ class Cache:
 
     def __init__(self, h, rows, d, weight=False, seed=0):
         rng = np.random.default_rng(seed)
-        # what no row was stored in holds rubbish: codes of every kind, NaN scales
+        # what no row was stored in holds rubbish: codes of every kind, scales that are zeros, NaN, inf or no powers of two
         self.codes = [rng.integers(-128, 128, (h, rows, d)).astype(np.int8) for _ in range(2)]
-        self.words = [np.full((h, rows // B), 0x7FC00000 | 127, np.uint32) for _ in range(2)]
+        rubbish = np.array([0, 0x7FC00000 | 127, 0x7F800000, 0xFF800000, 0x80000000, 0x7FFFFFFF, 0x00000001, 0x7F7FFFFF, 0xC1234567],
+                           np.uint32)
+        self.words = [rubbish[rng.integers(0, len(rubbish), (h, rows // B))] for _ in range(2)]
+        for w in self.words:
+            w[:, 0] = 0x7FC00000 | 127
         dev = [torch.from_numpy(c).cuda() for c in self.codes]
         dev += [torch.from_numpy(w.view(np.float32)).cuda() for w in self.words]
         self.w = torch.zeros(h, rows, device="cuda") if weight else None
