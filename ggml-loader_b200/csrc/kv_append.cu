@@ -54,11 +54,12 @@ __device__ __forceinline__ void store8_f16(__half *dst, const float x[8])
 }
 
 // cache row of token t: its position, or the position modulo the ring's cells
-// (a ring cache, dory.c:459-472)
+// (a ring cache, dory.c:459-472), or from row_sub on (rows staged for the 8-bit
+// cache: token t in row t)
 __device__ __forceinline__ int64_t cache_row(const AppendParams &p, int t)
 {
     const int64_t pos = p.n_past + t;
-    return p.ring ? pos % p.ring : pos;
+    return p.ring ? pos % p.ring : pos - p.row_sub;
 }
 
 // row -> (token, kind 0 Q / 1 K / 2 V, head); false past the last row

@@ -26,6 +26,7 @@
 #include "kv_api.h"
 #include "kv_bench.h"
 #include "kv_internal.h"
+#include "kv_q8.h"
 
 namespace {
 
@@ -316,6 +317,22 @@ struct kv_ctx {
 
     ncclComm_t comm = nullptr;
 
+    // an 8-bit cache (cfg.cache_type KV_CACHE_Q8): every layer's buffers, and a
+    // spare set that kv_evict writes and changes for the layer's
+    struct Q8Layer {
+        kvb::q8::Cache c;
+        int64_t used = 0;    // rows in use
+        int64_t gone = 0;    // positions less rows: position p is in row p - gone
+        int64_t floor = 0;   // rows that n_past cannot go back behind
+    };
+    std::vector<Q8Layer> q8;
+    kvb::q8::Cache q8_spare{};
+    char *q8_mem = nullptr;      // all of them
+    __half *q8_new = nullptr;    // [2][n_batch_max][hkv_loc][D]: a call's rows on their way into the cache
+    int32_t *q8_kept = nullptr;  // [hkv_loc][rows]
+    void *q8_ws = nullptr;       // kv_attend's workspace
+    bool is_q8() const { return !q8.empty(); }
+
     std::atomic<int64_t> launches{0};
 #ifdef KV_PHASE_STAMPS
     // measurement builds: phase stamps of the last kStampRing attention launches
@@ -365,6 +382,15 @@ bool shape_ok(const kv_config *c, std::string &why)
     if (c->n_batch_max < 0) { why = "n_batch_max must be >= 0"; return false; }
     if (c->ring_cells < 0) { why = "ring_cells must be >= 0"; return false; }
     if (c->ring_cells > 0 && c->n_ctx <= 0) { why = "a ring cache needs n_ctx (its positions) > 0"; return false; }
+    if (c->cache_type != KV_CACHE_F16 && c->cache_type != KV_CACHE_Q8) { why = "unknown cache_type"; return false; }
+    if (c->cache_rows < 0) { why = "cache_rows must be >= 0"; return false; }
+    if (c->cache_type != KV_CACHE_Q8 && (c->cache_rows || c->track_weights)) { why = "cache_rows and track_weights need cache_type KV_CACHE_Q8"; return false; }
+    if (c->cache_type == KV_CACHE_Q8) {
+        if (ns > 1 || c->ring_cells > 0) { why = "an 8-bit cache has one shard and no ring"; return false; }
+        if (c->cache_rows > 0 && c->n_ctx <= 0) { why = "cache_rows needs n_ctx (the positions) > 0"; return false; }
+        if (c->cache_rows > 0 && c->cache_rows < c->n_ctx && !c->track_weights) { why = "fewer cache_rows than n_ctx need track_weights (kv_evict)"; return false; }
+        if (c->n_head / c->n_head_kv > 128) { why = "more than 128 query heads a KV head"; return false; }
+    }
     // TMA descriptors address at most 2^32 rows; 2^31 positions already exceed
     // any device's memory at every supported shape, and keep the sizing
     // arithmetic far from overflow
@@ -372,9 +398,25 @@ bool shape_ok(const kv_config *c, std::string &why)
     return true;
 }
 
+// bytes of one layer's block of rows of an 8-bit cache: codes, scales, weights
+uint64_t q8_block_bytes(const kv_config *c)
+{
+    return (uint64_t)c->n_head_kv *
+           (2u * KV_Q8_BLOCK * (uint64_t)c->head_dim + 2u * sizeof(float) + (c->track_weights ? KV_Q8_BLOCK * sizeof(float) : 0u));
+}
+
+int64_t q8_rows(const kv_config *c, int64_t n_ctx)
+{
+    const int64_t rows = c->cache_rows > 0 ? std::min(c->cache_rows, n_ctx) : n_ctx;
+    return (rows + KV_Q8_BLOCK - 1) / KV_Q8_BLOCK * KV_Q8_BLOCK;
+}
+
 uint64_t per_position_bytes(const kv_config *c)
 {
     const int ns = c->n_shards <= 1 ? 1 : c->n_shards;
+    if (c->cache_type == KV_CACHE_Q8)   // (a set of spare buffers with weights)
+        return ((uint64_t)(c->n_layer + (c->track_weights ? 1 : 0)) * q8_block_bytes(c) + KV_Q8_BLOCK - 1) / KV_Q8_BLOCK +
+               (uint64_t)(c->n_rot / 2) * sizeof(float2);
     const uint64_t cache = (uint64_t)c->n_layer * (uint64_t)(c->n_head_kv / ns) * (uint64_t)c->head_dim * 2u * 2u;
     const uint64_t rope = (uint64_t)(c->n_rot / 2) * sizeof(float2);
     return cache + rope;
@@ -593,7 +635,7 @@ void free_all(kv_ctx *ctx)
     unmap_peers(ctx);
     if (ctx->comm && nccl().CommDestroy) nccl().CommDestroy(ctx->comm);
     ctx->comm = nullptr;
-    void *ptrs[] = {ctx->cache, ctx->rope, ctx->qbuf, ctx->S, ctx->stats, ctx->acc, ctx->ctl, ctx->err,
+    void *ptrs[] = {ctx->q8_mem, ctx->q8_new, ctx->q8_kept, ctx->q8_ws, ctx->cache, ctx->rope, ctx->qbuf, ctx->S, ctx->stats, ctx->acc, ctx->ctl, ctx->err,
                     ctx->local_out, ctx->gathered, ctx->pf_stat, ctx->pf_out, ctx->pf_rstat, ctx->ring_mask};
     for (void *p : ptrs)
         if (p) cudaFree(p);
@@ -687,6 +729,20 @@ void unmap_peers(kv_ctx *ctx)
 }
 
 // The single-token append a kv_append deferred to the following kv_attend.
+// the rows kv_append wrote to q8_new, into the 8-bit cache
+int store_new_rows(kv_ctx *ctx, int layer, int64_t row0, int n_new, cudaStream_t st)
+{
+    kvb::q8::StoreParams p{};
+    p.c = ctx->q8[layer].c;
+    p.k = ctx->q8_new;
+    p.v = ctx->q8_new + (int64_t)ctx->cfg.n_batch_max * ctx->hkv_loc * ctx->D;
+    p.k_stride = p.v_stride = (int64_t)ctx->hkv_loc * ctx->D;
+    p.row0 = row0;
+    p.n_new = n_new;
+    p.f16 = p.vec = 1;
+    return launch(ctx, KV_K_APPEND, st, "8-bit store kernel", [&] { return kvb::q8::launch_store(p, st); });
+}
+
 int run_append(kv_ctx *ctx, const Pending &pd)
 {
     const kv_config &c = ctx->cfg;
@@ -702,13 +758,22 @@ int run_append(kv_ctx *ctx, const Pending &pd)
     p.eps = c.qk_norm == 2 ? c.rms_eps / (float)ctx->D : c.rms_eps;
     p.post = 1.0f / sqrtf((float)ctx->D);
     p.rope = ctx->rope;
-    p.kc = ctx->k_layer(pd.layer); p.vc = ctx->v_layer(pd.layer);
+    if (ctx->is_q8()) {
+        p.kc = ctx->q8_new;
+        p.vc = ctx->q8_new + (int64_t)c.n_batch_max * ctx->hkv_loc * ctx->D;
+    } else {
+        p.kc = ctx->k_layer(pd.layer);
+        p.vc = ctx->v_layer(pd.layer);
+    }
     p.ring = ctx->ring;
+    p.row_sub = ctx->is_q8() ? pd.n_past : 0;
     p.qbuf = ctx->qbuf;
     auto al16 = [](const void *x) { return ((uintptr_t)x & 15u) == 0; };
     const bool vec = al16(pd.q) && al16(pd.k) && al16(pd.v) && al16(pd.qn) && al16(pd.kn) &&
                      (pd.n_new == 1 || ((pd.q_stride | pd.k_stride | pd.v_stride) & 3) == 0);
-    return launch(ctx, KV_K_APPEND, pd.st, "append kernel", [&] { return kvb::launch_append(ctx->D, vec, p, pd.st); });
+    const int rc = launch(ctx, KV_K_APPEND, pd.st, "append kernel", [&] { return kvb::launch_append(ctx->D, vec, p, pd.st); });
+    if (rc || !ctx->is_q8()) return rc;
+    return store_new_rows(ctx, pd.layer, pd.n_past - ctx->q8[pd.layer].gone, pd.n_new, pd.st);
 }
 
 int flush_pending(kv_ctx *ctx)
@@ -743,6 +808,10 @@ int kv_config_init(kv_config *cfg)
 uint64_t kv_cache_bytes(const kv_config *cfg, int64_t n_ctx)
 {
     if (!cfg || n_ctx < 0) return 0;
+    if (cfg->cache_type == KV_CACHE_Q8) {
+        const uint64_t block = (uint64_t)cfg->n_layer * q8_block_bytes(cfg), n = (uint64_t)q8_rows(cfg, n_ctx) / KV_Q8_BLOCK;
+        return block > 0 && n > UINT64_MAX / block ? UINT64_MAX : block * n;
+    }
     const uint64_t per_token = (uint64_t)cfg->n_layer * (uint64_t)cfg->head_dim * (uint64_t)cfg->n_head_kv * 2u * 2u;
     // a ring holds min(ring_cells, n_ctx) rows whatever the positions (dory_kv_cost, dory.c:373-389)
     const int64_t rows = cfg->ring_cells > 0 ? std::min<int64_t>(cfg->ring_cells, n_ctx) : n_ctx;
@@ -766,6 +835,56 @@ int64_t kv_auto_n_ctx(const kv_config *cfg, int64_t free_bytes)
     if (n_ctx > limit) n_ctx = limit;
     if (n_ctx < 512) n_ctx = std::min<int64_t>(512, limit);
     return n_ctx;
+}
+
+// An 8-bit context's memory: every layer's codes, scales and weights (and a
+// spare set with weights, for kv_evict), the rotated queries, the rows on their
+// way into the cache, kv_attend's workspace.
+static int alloc_q8(kv_ctx *ctx)
+{
+    const kv_config &c = ctx->cfg;
+    const int64_t H = ctx->hkv_loc, D = ctx->D, rows = ctx->rows;
+    const bool weigh = c.track_weights != 0;
+    const int sets = c.n_layer + (weigh ? 1 : 0);
+    if ((double)sets * (double)rows * (double)H * (double)(2 * D + 5) > 0x1p60)   // beyond any device, and near size_t's range
+        return fail(KV_E_OOM, "a cache of %lld rows x %d layers is beyond any device's memory", (long long)rows, c.n_layer);
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    const size_t codes = up((size_t)(H * rows * D)), scales = up((size_t)(H * (rows / KV_Q8_BLOCK)) * sizeof(float));
+    const size_t weights = weigh ? up((size_t)(H * rows) * sizeof(float)) : 0, set = 2 * codes + 2 * scales + weights;
+    cudaError_t e = cudaMalloc(&ctx->q8_mem, (size_t)sets * set);
+    if (e != cudaSuccess)
+        return fail(KV_E_OOM, "failed to allocate KV cache (%lld rows x %d layers, %.0f MiB requested): %s", (long long)rows,
+                    c.n_layer, (double)sets * (double)set / (1024.0 * 1024.0), cudaGetErrorString(e));
+    // (no code or scale is read before it is stored; zeros, so that a row not stored yet reads back as one)
+    e = cudaMemset(ctx->q8_mem, 0, (size_t)sets * set);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemset");
+    ctx->q8.resize(c.n_layer);
+    for (int l = 0; l < sets; l++) {
+        char *m = ctx->q8_mem + (size_t)l * set;
+        kvb::q8::Cache &x = l < c.n_layer ? ctx->q8[l].c : ctx->q8_spare;
+        x.k = reinterpret_cast<int8_t *>(m);
+        x.v = reinterpret_cast<int8_t *>(m + codes);
+        x.k_scale = reinterpret_cast<float *>(m + 2 * codes);
+        x.v_scale = reinterpret_cast<float *>(m + 2 * codes + scales);
+        x.weight = weigh ? reinterpret_cast<float *>(m + 2 * codes + 2 * scales) : nullptr;
+        x.rows = rows;
+        x.H = (int32_t)H;
+        x.D = (int32_t)D;
+    }
+    kvb::q8::AttendParams p{};
+    p.c = ctx->q8[0].c;
+    p.Hq = ctx->hq_loc;
+    p.r = ctx->r;
+    p.n_new = c.n_batch_max;
+    p.n_kv = rows;
+    p.n_past = rows - c.n_batch_max;
+    const size_t batch = (size_t)c.n_batch_max * (size_t)D * sizeof(__half);
+    e = cudaMalloc(&ctx->q8_ws, (size_t)kvb::q8::attend_workspace(p));
+    if (e == cudaSuccess) e = cudaMalloc(&ctx->qbuf, batch * (size_t)ctx->hq_loc);
+    if (e == cudaSuccess) e = cudaMalloc(&ctx->q8_new, 2 * batch * (size_t)H);
+    if (e == cudaSuccess && weigh) e = cudaMalloc(&ctx->q8_kept, (size_t)(H * rows) * sizeof(int32_t));
+    if (e != cudaSuccess) return fail(KV_E_OOM, "scratch allocation: %s", cudaGetErrorString(e));
+    return KV_OK;
 }
 
 static int alloc_impl(const kv_config *cfg_in, kv_ctx **out)
@@ -833,15 +952,24 @@ static int alloc_impl(const kv_config *cfg_in, kv_ctx **out)
     ctx->ring = c.ring_cells > 0 ? std::min<int64_t>(c.ring_cells, ctx->n_ctx) : 0;
     ctx->rows = ctx->ring ? ctx->ring : ctx->n_ctx;
     c.ring_cells = ctx->ring;
+    const bool q8 = c.cache_type == KV_CACHE_Q8;
+    if (q8) {
+        ctx->rows = q8_rows(&c, ctx->n_ctx);
+        if (ctx->rows > kMaxPositions - KV_Q8_BLOCK) return bail(fail(KV_E_ARG, "kv_alloc: n_ctx above 2^31 - 64 positions"));
+    }
     if (c.n_batch_max > ctx->rows) c.n_batch_max = (int32_t)ctx->rows;
 
     const int64_t D = ctx->D;
+    if (q8) {
+        const int rc = alloc_q8(ctx);
+        if (rc) return bail(rc);
+    }
     ctx->layer_elems = ctx->rows * ctx->hkv_loc * D;   // <= 2^31 x 64 x 256
     if ((double)c.n_layer * 4.0 * (double)ctx->layer_elems > 0x1p60)   // beyond any device, and near size_t's range
         return bail(fail(KV_E_OOM, "a cache of %lld rows x %d layers is beyond any device's memory",
                          (long long)ctx->rows, c.n_layer));
     const size_t cache_bytes = (size_t)c.n_layer * 2u * (size_t)ctx->layer_elems * sizeof(__half);
-    e = cudaMalloc(&ctx->cache, cache_bytes);
+    e = q8 ? cudaSuccess : cudaMalloc(&ctx->cache, cache_bytes);
     if (e != cudaSuccess) {
         return bail(fail(KV_E_OOM, "failed to allocate KV cache (%lld rows x %d layers, %.0f MiB requested): %s",
                          (long long)ctx->rows, c.n_layer, (double)cache_bytes / (1024.0 * 1024.0),
@@ -859,6 +987,14 @@ static int alloc_impl(const kv_config *cfg_in, kv_ctx **out)
         if (e != cudaSuccess) return bail(fail(KV_E_OOM, "RoPE table allocation: %s", cudaGetErrorString(e)));
         e = cudaMemcpy(ctx->rope, table.data(), table.size() * sizeof(float), cudaMemcpyHostToDevice);
         if (e != cudaSuccess) return bail(cuda_fail(e, "RoPE table upload"));
+    }
+
+    if (q8) {   // (nothing of what follows is the 8-bit kernels')
+        e = cudaDeviceSynchronize();
+        if (e != cudaSuccess) return bail(cuda_fail(e, "kv_alloc sync"));
+        own.p = nullptr;
+        *out = ctx;
+        return KV_OK;
     }
 
     // score scratch: CTA c of a launch owns S_tiles(n_kv) tiles from
@@ -1098,6 +1234,17 @@ int kv_append_bias(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new,
     if (c.qk_norm == 2 && !q_norm_w) return fail(KV_E_ARG, "the nGPT norm needs q_norm_w (Q's per-channel scale)");
     int rc = ensure_device(ctx);
     if (rc) return rc;
+    if (ctx->is_q8()) {
+        kv_ctx::Q8Layer &l = ctx->q8[layer];
+        const int64_t gone = n_past == 0 ? 0 : l.gone, row = n_past - gone;
+        if (n_past > 0 && row < l.floor)
+            return fail(KV_E_RANGE, "position %lld of layer %d lies among evicted rows", (long long)n_past, layer);
+        if (row > ctx->rows - n_new)
+            return fail(KV_E_RANGE, "rows [%lld, %lld) exceed the layer's %lld: kv_evict makes room", (long long)row,
+                        (long long)(row + n_new), (long long)ctx->rows);
+        if (n_past == 0) l.gone = l.floor = 0;
+        l.used = row + n_new;
+    }
     rc = flush_pending(ctx);
     if (rc) return rc;
 
@@ -1114,7 +1261,7 @@ int kv_append_bias(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new,
     ctx->last_layer = layer;
     ctx->last_n_past = n_past;
     ctx->last_n_new = n_new;
-    if (n_new == 1 && ctx->r <= kvb::attn_rows() && !ctx->ring && c.qk_norm != 2) {
+    if (n_new == 1 && ctx->r <= kvb::attn_rows() && !ctx->ring && c.qk_norm != 2 && !ctx->is_q8()) {
         // one token: the attention kernels do the append themselves (same bits);
         // any other call on this context first performs it with the append kernel
         ctx->pend = pd;
@@ -1228,6 +1375,33 @@ int prefill(kv_ctx *ctx, const CUtensorMap &km, const CUtensorMap &vm, const CUt
 
 }  // namespace
 
+// kv_attend over an 8-bit layer: the rows in use, the new ones the last of them
+static int attend_q8(kv_ctx *ctx, int32_t layer, int32_t n_new, const MaskArg &mk, float *out, cudaStream_t st)
+{
+    const int64_t D = ctx->D;
+    kvb::q8::AttendParams p{};
+    p.c = ctx->q8[layer].c;
+    p.Hq = ctx->hq_loc;
+    p.r = ctx->r;
+    p.n_new = n_new;
+    p.n_kv = ctx->q8[layer].used;
+    p.n_past = p.n_kv - n_new;
+    p.q = ctx->qbuf;
+    p.q_stride = p.out_stride = ctx->hq_loc * D;
+    p.q_f16 = p.q_vec = 1;
+    p.mask = mk.ptr;
+    p.mask_stride = mk.stride;
+    p.mask_f16 = mk.f16 ? 1 : 0;
+    p.flash = mk.flash ? 1 : 0;
+    p.out = out;
+    p.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0;
+    p.scale = ctx->scale;
+    if (mk.ptr && mk.stride < p.n_kv)
+        return fail(KV_E_ARG, "mask_stride %lld < the %lld keys attended", (long long)mk.stride, (long long)p.n_kv);
+    return launch(ctx, n_new * ctx->r > 16 ? KV_K_PREFILL : KV_K_ATTN, st, "8-bit attention kernels",
+                  [&] { return kvb::q8::launch_attend(p, ctx->q8_ws, st); });
+}
+
 static int attend_impl(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new, const MaskArg &mk_in, float *out,
                 void *stream)
 {
@@ -1240,6 +1414,7 @@ static int attend_impl(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new
     if (rc) return rc;
     const kv_config &c = ctx->cfg;
     const cudaStream_t st = to_stream(stream);
+    if (ctx->is_q8()) return attend_q8(ctx, layer, n_new, mk_in, out, st);
     // the deferred single-token append runs inside the attention kernels when it
     // belongs to this call and stream; otherwise it is performed now
     const bool fused = ctx->pend.on && ctx->pend.layer == layer && ctx->pend.n_past == n_past &&
@@ -1442,6 +1617,58 @@ int kv_forward(kv_ctx *ctx, int64_t n_past, int32_t n_new,
     return KV_OK;
 }
 
+// The same for an 8-bit cache, on an idle device.  Imported rows are stored
+// with the rows behind them in the last block, at their present values, and
+// the other of K and V likewise, at its own: kv_q8_store takes both.
+static int rows_io_q8(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0, int64_t nrows, void *host, bool to_host)
+{
+    const kvb::q8::Cache &c = ctx->q8[layer].c;
+    const int64_t width = (int64_t)c.H * c.D;
+    const int64_t end = to_host ? row0 + nrows : (row0 + nrows + KV_Q8_BLOCK - 1) / KV_Q8_BLOCK * KV_Q8_BLOCK, n = end - row0;
+    struct Tmp {
+        __half *p = nullptr;
+        ~Tmp()
+        {
+            if (p) cudaFree(p);
+        }
+    } tmp;
+    if (cudaMalloc(&tmp.p, (size_t)(2 * n * width) * sizeof(__half)) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(KV_E_OOM, "row buffer");
+    }
+    __half *k = tmp.p, *v = tmp.p + n * width, *mine = which == 0 ? k : v;
+    kvb::q8::LoadParams lp{};
+    lp.c = c;
+    lp.k = to_host && which != 0 ? nullptr : k;
+    lp.v = to_host && which == 0 ? nullptr : v;
+    lp.stride = width;
+    lp.row0 = row0;
+    lp.n = n;
+    lp.f16 = lp.vec = 1;
+    KV_CUDA(kvb::q8::launch_load(lp, nullptr));
+    KV_CUDA(cudaStreamSynchronize(nullptr));
+    const size_t bytes = (size_t)(nrows * width) * sizeof(__half);
+    if (to_host) {
+        KV_CUDA(cudaMemcpy(host, mine, bytes, cudaMemcpyDeviceToHost));
+        return KV_OK;
+    }
+    KV_CUDA(cudaMemcpy(mine, host, bytes, cudaMemcpyHostToDevice));
+    kvb::q8::StoreParams sp{};
+    sp.c = c;
+    sp.c.weight = nullptr;   // (imported rows keep their weights)
+    sp.k = k;
+    sp.v = v;
+    sp.k_stride = sp.v_stride = width;
+    sp.row0 = row0;
+    sp.n_new = (int32_t)n;
+    sp.f16 = sp.vec = 1;
+    KV_CUDA(kvb::q8::launch_store(sp, nullptr));
+    KV_CUDA(cudaStreamSynchronize(nullptr));
+    kv_ctx::Q8Layer &l = ctx->q8[layer];
+    l.used = std::max(l.used, row0 + nrows);
+    return KV_OK;
+}
+
 static int rows_io(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0, int64_t nrows, void *host, bool to_host)
 {
     if (!ctx || !host) return fail(KV_E_ARG, "NULL argument");
@@ -1453,10 +1680,12 @@ static int rows_io(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0, int6
     if (rc) return rc;
     rc = flush_pending(ctx);
     if (rc) return rc;
-    __half *base = (which == 0 ? ctx->k_layer(layer) : ctx->v_layer(layer)) + row0 * (int64_t)ctx->hkv_loc * ctx->D;
+    __half *base = ctx->is_q8() ? nullptr
+                                : (which == 0 ? ctx->k_layer(layer) : ctx->v_layer(layer)) + row0 * (int64_t)ctx->hkv_loc * ctx->D;
     const size_t bytes = (size_t)nrows * ctx->hkv_loc * ctx->D * sizeof(__half);
     if (bytes == 0) return KV_OK;
     KV_CUDA(cudaDeviceSynchronize());
+    if (ctx->is_q8()) return rows_io_q8(ctx, layer, which, row0, nrows, host, to_host);
     if (to_host) KV_CUDA(cudaMemcpy(host, base, bytes, cudaMemcpyDeviceToHost));
     else KV_CUDA(cudaMemcpy(base, host, bytes, cudaMemcpyHostToDevice));
     return KV_OK;
@@ -1470,6 +1699,50 @@ int kv_export_rows(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0, int6
 int kv_import_rows(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0, int64_t nrows, const uint16_t *host_src)
 {
     return rows_io(ctx, layer, which, row0, nrows, const_cast<uint16_t *>(host_src), false);
+}
+
+int kv_layer_rows(const kv_ctx *ctx, int32_t layer, int64_t *used, int64_t *capacity)
+{
+    if (!ctx) return fail(KV_E_ARG, "NULL context");
+    if (layer < 0 || layer >= ctx->cfg.n_layer) return fail(KV_E_ARG, "layer %d out of range", layer);
+    if (!ctx->is_q8() && used) return fail(KV_E_UNSUPPORTED, "kv_layer_rows: only an 8-bit context counts its rows in use");
+    if (used) *used = ctx->q8[layer].used;
+    if (capacity) *capacity = ctx->rows;
+    return KV_OK;
+}
+
+int kv_evict(kv_ctx *ctx, int32_t layer, int64_t keep, int64_t recent, int32_t *kept, void *stream)
+{
+    if (!ctx) return fail(KV_E_ARG, "NULL context");
+    if (!ctx->is_q8() || !ctx->cfg.track_weights)
+        return fail(KV_E_UNSUPPORTED, "kv_evict needs an 8-bit context with track_weights");
+    if (layer < 0 || layer >= ctx->cfg.n_layer) return fail(KV_E_ARG, "layer %d out of range", layer);
+    kv_ctx::Q8Layer &l = ctx->q8[layer];
+    if (keep < 1 || recent < 0 || recent > keep || keep > l.used)
+        return fail(KV_E_ARG, "kv_evict: 0 <= recent <= keep <= the %lld rows in use and keep >= 1 are required", (long long)l.used);
+    if (reinterpret_cast<uintptr_t>(kept) % 4) return fail(KV_E_ARG, "kv_evict: misaligned kept");
+    int rc = ensure_device(ctx);
+    if (rc) return rc;
+    const cudaStream_t st = to_stream(stream);
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    KV_CUDA(cudaStreamIsCapturing(st, &cap));
+    if (cap != cudaStreamCaptureStatusNone)
+        return fail(KV_E_STATE, "kv_evict on a stream that is being captured: the layer's buffers change places");
+    kvb::q8::EvictParams p{};
+    p.src = l.c;
+    p.dst = ctx->q8_spare;
+    p.n_rows = l.used;
+    p.keep = keep;
+    p.recent = recent;
+    p.kept = kept ? kept : ctx->q8_kept;
+    rc = launch(ctx, KV_K_APPEND, st, "eviction kernels", [&] { return kvb::q8::launch_evict(p, st); });
+    if (rc) return rc;
+    std::swap(l.c, ctx->q8_spare);
+    l.gone += l.used - keep;
+    l.used = keep;
+    l.floor = keep - recent;
+    if (ctx->last_layer == layer) ctx->last_layer = -1;   // (kv_attend follows a kv_append)
+    return KV_OK;
 }
 
 int kv_comm_unique_id(void *id_out)
@@ -1509,6 +1782,7 @@ int kv_status(kv_ctx *ctx, void *stream)
     if (rc) return rc;
     rc = flush_pending(ctx);
     if (rc) return rc;
+    if (ctx->is_q8()) return kv_q8_status(stream);
     KV_CUDA(cudaStreamSynchronize(to_stream(stream)));
     unsigned word = 0;
     KV_CUDA(cudaMemcpy(&word, ctx->err, sizeof(word), cudaMemcpyDeviceToHost));
@@ -1526,6 +1800,7 @@ int kv_debug_inject(kv_ctx *ctx, int32_t what, uint64_t limit_ns)
 {
     if (!ctx) return fail(KV_E_ARG, "NULL context");
     if (what != 0 && what != 1) return fail(KV_E_ARG, "unknown injection %d", what);
+    if (ctx->is_q8()) return fail(KV_E_UNSUPPORTED, "kv_debug_inject: the F16 cache's kernels only");
     ctx->inject = what;
     if (limit_ns) ctx->limit_ns = limit_ns;
     return KV_OK;
@@ -1538,6 +1813,7 @@ int kv_fill_synthetic(kv_ctx *ctx, uint64_t seed, uint64_t stream_base, int64_t 
     if (!ctx) return fail(KV_E_ARG, "NULL context");
     if (row0 < 0 || nrows < 0 || row0 > ctx->rows || nrows > ctx->rows - row0)
         return fail(KV_E_RANGE, "rows outside the cache");
+    if (ctx->is_q8()) return fail(KV_E_UNSUPPORTED, "kv_fill_synthetic: an F16 cache only");
     int rc = ensure_device(ctx);
     if (rc) return rc;
     rc = flush_pending(ctx);

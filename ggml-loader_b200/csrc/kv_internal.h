@@ -28,6 +28,7 @@ struct AppendParams {
     __half *kc, *vc;                 // layer cache [rows][hkv_loc][D]
     __half *qbuf;                    // [n_new][hq_loc][D]  rotated Q, F16
     int64_t ring;                    // 0: position p in row p; > 0: in row p % ring (ring cache)
+    int64_t row_sub;                 // ring 0: position p in row p - row_sub
 };
 
 cudaError_t launch_append(int D, bool vec_loads, const AppendParams &p, cudaStream_t st);

@@ -26,6 +26,9 @@ KV_E_TIMEOUT = -6
 KV_E_STATE = -7
 KV_E_UNSUPPORTED = -8
 
+KV_CACHE_F16 = 0
+KV_CACHE_Q8 = 1
+
 KERNELS = {"append": 0, "attn": 1, "prefill": 2, "pfold": 3, "gather": 4, "prefill2": 5}
 
 _vp = ctypes.c_void_p
@@ -51,6 +54,7 @@ class KvConfig(ctypes.Structure):
         ("comm_id", _vp),
         ("ring_cells", _i64),
         ("flash_attn", _i32),
+        ("cache_type", _i32), ("cache_rows", _i64), ("track_weights", _i32),
     ]
 
 
@@ -107,6 +111,8 @@ def lib():
         "kv_launch_count": (_i64, [_vp]),
         "kv_debug_stamps": (_i64, [_vp, _vp, ctypes.POINTER(_i32), ctypes.POINTER(_i32)]),
         "kv_attend_decode_noalloc": (ctypes.c_int, [_vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp]),
+        "kv_evict": (ctypes.c_int, [_vp, _i32, _i64, _i64, _vp, _vp]),
+        "kv_layer_rows": (ctypes.c_int, [_vp, _i32, ctypes.POINTER(_i64), ctypes.POINTER(_i64)]),
         "kv_q8_store": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _vp]),
         "kv_q8_load": (ctypes.c_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp]),
         "kv_q8_attend_workspace": (_u64, [_vp, _i32, _i64, _i32]),
@@ -171,10 +177,12 @@ def _stream(s):
 
 
 def make_config(spec, n_ctx=None, n_batch_max=None, device=-1, n_shards=1, shard=0, comm_id=None, ring_cells=0,
-                flash_attn=False):
+                flash_attn=False, cache_type=0, cache_rows=0, track_weights=False):
     """A KvConfig from a specs.py dict.  Keeps referenced buffers alive on the
     returned object (freq factors, comm id).  ring_cells > 0 makes a ring cache
-    (positions bounded by n_ctx, rows = ring_cells)."""
+    (positions bounded by n_ctx, rows = ring_cells).  cache_type KV_CACHE_Q8
+    makes an 8-bit cache, of cache_rows rows (0: n_ctx); track_weights keeps its
+    rows' attention weights, which Context.evict goes by."""
     import numpy as np
     c = KvConfig()
     lib().kv_config_init(ctypes.byref(c))
@@ -205,6 +213,9 @@ def make_config(spec, n_ctx=None, n_batch_max=None, device=-1, n_shards=1, shard
     c.shard = shard
     c.ring_cells = ring_cells
     c.flash_attn = 1 if flash_attn else 0
+    c.cache_type = cache_type
+    c.cache_rows = cache_rows
+    c.track_weights = 1 if track_weights else 0
     if comm_id is not None:
         c._id = ctypes.create_string_buffer(bytes(comm_id), 128)
         c.comm_id = ctypes.cast(c._id, _vp)
@@ -308,6 +319,20 @@ class Context:
                                        v_stride, in_layer_stride, _ptr(q_norm_w), _ptr(k_norm_w),
                                        norm_layer_stride, _ptr(out), out_layer_stride, _stream(stream)),
                       "kv_forward")
+
+    def evict(self, layer, keep, recent, kept=None, stream=None):
+        """kv_evict: the layer's last `recent` rows and the heaviest others stay, `keep`
+        in all; kept: a CUDA int32 tensor [n_head_kv][keep] of their numbers, or None."""
+        if kept is not None:
+            import torch
+            assert kept.dtype == torch.int32 and kept.is_contiguous() and kept.shape == (self.n_kv_heads, keep)
+        return _check(lib().kv_evict(self.h, layer, keep, recent, _ptr(kept), _stream(stream)), "kv_evict")
+
+    def layer_rows(self, layer):
+        """(rows in use, rows held) of a layer of an 8-bit context."""
+        used, held = _i64(), _i64()
+        _check(lib().kv_layer_rows(self.h, layer, ctypes.byref(used), ctypes.byref(held)), "kv_layer_rows")
+        return used.value, held.value
 
     # -- rows ---------------------------------------------------------------
     def export_rows(self, layer, which, row0, nrows):

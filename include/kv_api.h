@@ -102,11 +102,27 @@ typedef struct kv_config {
                                    branch, as decode_session::use_flash_attn
                                    selects it (model.h:381-384); see
                                    KV_ATTN_FLASH at kv_attend_mask              */
+    int32_t cache_type;         /* KV_CACHE_F16, or KV_CACHE_Q8: the cache in 8-bit
+                                   codes (see kv_q8_cache), half the bytes       */
+    int64_t cache_rows;         /* KV_CACHE_Q8: rows a layer holds (rounded up to a
+                                   multiple of 32), 0 = n_ctx.  Fewer than n_ctx:
+                                   kv_evict makes room                           */
+    int32_t track_weights;      /* KV_CACHE_Q8: 1 = kv_attend accumulates each row's
+                                   attention weight, which kv_evict goes by      */
 } kv_config;
 
+#define KV_CACHE_F16 0
+#define KV_CACHE_Q8  1
+
 /* Defaults: NEOX RoPE, base 10000, scale 1, attn factor 1, no YaRN, eps 1e-6,
- * n_ctx 0 (auto), n_batch_max 512, device -1, one shard, linear cache.  Shape
- * fields 0.
+ * n_ctx 0 (auto), n_batch_max 512, device -1, one shard, linear F16 cache.
+ * Shape fields 0.
+ *
+ * 8-bit caches (cache_type KV_CACHE_Q8): the calls below are the same; kv_append
+ * rotates and norms as it does for F16 and stores the F16 rows' codes, kv_attend
+ * is kv_q8_attend's operator (queries rounded to F16, F32 out; the default and
+ * the flash-attn branch differ only in a row without a visible key).  One
+ * shard, no ring.
  *
  * Ring caches (ring_cells > 0; dory's sliding and global rings, one context
  * per ring size, per-loop slots as extra layers): kv_append's n_past is the
@@ -120,8 +136,8 @@ int kv_config_init(kv_config *cfg);
 
 /* Bytes of the whole K+V cache at n_ctx positions, all layers and all shards:
  * exactly kv_cache_bytes() of the reference (model.cpp:869-885); a ring
- * configuration holds min(ring_cells, n_ctx) rows.  UINT64_MAX when the product
- * does not fit 64 bits. */
+ * configuration holds min(ring_cells, n_ctx) rows; an 8-bit one its codes,
+ * scales and weights.  UINT64_MAX when the product does not fit 64 bits. */
 uint64_t kv_cache_bytes(const kv_config *cfg, int64_t n_ctx);
 
 /* Context auto-sizing rule of auto_n_ctx() (model.cpp:1002-1059) applied to
@@ -269,6 +285,24 @@ int kv_attend_decode_noalloc(const uint16_t *k_cache, const uint16_t *v_cache,
                              int32_t n_head, int32_t n_head_kv, int32_t head_dim, int64_t n_kv,
                              const float *q, float *out, void *stream);
 
+/*
+ * Evict rows of `layer` of an 8-bit context with track_weights: each KV head
+ * keeps the layer's last `recent` rows and the heaviest others, `keep` in all
+ * (kv_q8_evict; keep at most the rows in use).  Positions are not renumbered:
+ * the kept keys stay rotated as they are, the next kv_append is again at the
+ * next position, n_past, and kv_attend attends over the rows that are left.
+ * Every layer is evicted by its own call.  Rewinding n_past is possible by up
+ * to `recent` tokens (KV_E_RANGE beyond), or to 0.  kept: DEVICE int32
+ * [n_head_kv][keep], each head's kept rows (their numbers before the call), or
+ * NULL.  The layer's buffers change places with a spare set, so a stream that is
+ * being captured is refused (KV_E_STATE), and a graph captured before must not
+ * be replayed after.
+ */
+int kv_evict(kv_ctx *ctx, int32_t layer, int64_t keep, int64_t recent, int32_t *kept, void *stream);
+
+/* Rows of `layer` in use, and rows it holds (either may be NULL). */
+int kv_layer_rows(const kv_ctx *ctx, int32_t layer, int64_t *used, int64_t *capacity);
+
 /* ---- the cache in 8 bits -------------------------------------------------- */
 /*
  * One layer's K and V in 8-bit codes with one scale for each KV head and block
@@ -375,7 +409,9 @@ int kv_q8_evict(const kv_q8_cache *src, int64_t n_rows, int64_t keep, int64_t re
 
 /* Copy cache rows [row0, row0+nrows) of K (which = 0) or V (which = 1) of
  * `layer` to / from host memory in the reference layout [row][head][dim] F16
- * (this context's heads only).  Synchronous.  Used for checking, for the
+ * (this context's heads only; an 8-bit cache's values, exact in F16, or stored
+ * as kv_q8_store stores them: the rows before row0 in its block, and the ones
+ * behind in the last block, are stored again at the block's scale).  Synchronous.  Used for checking, for the
  * reference's /save-/load style rebuilds and for tests. */
 int kv_export_rows(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0,
                    int64_t nrows, uint16_t *host_dst);

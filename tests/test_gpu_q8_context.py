@@ -1,0 +1,281 @@
+"""GPU tests of an 8-bit context (cache_type KV_CACHE_Q8): kv_append, kv_attend,
+kv_attend_mask, kv_forward, row export and import, and kv_evict, against the
+F16 context on the same values and the 64-bit restatement."""
+import numpy as np
+import pytest
+import torch
+
+import kv_b200 as K
+import q8_reference as R
+
+pytestmark = pytest.mark.gpu
+B = R.BLOCK
+
+
+def spec(d=128, hq=8, h=2, layers=2, **kw):
+    return dict(dict(n_layer=layers, n_head=hq, n_head_kv=h, head_dim=d, n_rot=d, rope_mode=2, rope_base=10000.0, n_ctx=512), **kw)
+
+
+def inputs(seed, n, hq, h, d):
+    g = torch.Generator().manual_seed(seed)
+    fused = torch.randn(n, (hq + 2 * h) * d, generator=g).cuda()
+    return fused[:, :hq * d], fused[:, hq * d:(hq + h) * d], fused[:, (hq + h) * d:]
+
+
+def append(ctx, layer, n_past, qkv, norms=(None, None)):
+    q, k, v = qkv
+    ctx.append(layer, n_past, q.shape[0], q, q.stride(0), k, k.stride(0), v, v.stride(0), *norms)
+
+
+def q8_context(sp, **kw):
+    return K.Context(K.make_config(sp, cache_type=K.KV_CACHE_Q8, **kw))
+
+
+def quantised(rows_u16):
+    """[n][h][d] F16 bits -> the values an 8-bit cache holds, when the rows were stored in one call."""
+    x = rows_u16.view(np.float16).astype(np.float64)
+    out = np.empty_like(x)
+    for h in range(x.shape[1]):
+        for b in range(0, x.shape[0], B):
+            c, w = R.quantise_block(x[b:b + B, h])
+            out[b:b + B, h] = R.row_values(c, np.array([w], np.uint32))
+    return out
+
+
+SPECS = {"plain": spec(), "normal-rope": spec(rope_mode=0, d=64, hq=6, h=3), "qk-norm": spec(qk_norm=1, rms_eps=1e-6),
+         "partial-rope": spec(d=96, hq=4, h=4, n_rot=48), "ngpt-256": spec(d=256, hq=8, h=2, qk_norm=2)}
+
+
+@pytest.mark.parametrize("name", list(SPECS))
+def test_rows_are_the_f16_context_s_in_8_bits(name):
+    sp = SPECS[name]
+    hq, h, d = sp["n_head"], sp["n_head_kv"], sp["head_dim"]
+    g = torch.Generator().manual_seed(1)
+    qn = torch.rand(hq * d if sp.get("qk_norm") == 2 else d, generator=g).cuda() + 0.5
+    norms = {1: (qn, torch.rand(d, generator=g).cuda() + 0.5), 2: (qn, None)}.get(sp.get("qk_norm"), (None, None))
+    with q8_context(sp) as a, K.Context(K.make_config(sp)) as b:
+        qkv = inputs(3, 70, hq, h, d)
+        for ctx in (a, b):
+            append(ctx, 1, 0, qkv, norms)
+        torch.cuda.synchronize()
+        for which in (0, 1):
+            want = quantised(b.export_rows(1, which, 0, 70))
+            got = a.export_rows(1, which, 0, 70).view(np.float16).astype(np.float64)
+            assert np.array_equal(got, want)
+        assert a.layer_rows(1) == (70, 512) and a.layer_rows(0) == (0, 512)
+
+
+def close(got, want):
+    """The framework's attention tolerance (two roundings of the weights to F16)."""
+    got, want = got.double(), want.double()
+    assert torch.isfinite(got).all()
+    assert (got - want).abs().max() <= 2e-3 * max(1.0, float(want.abs().max()))
+    assert float((got - want).norm() / want.norm()) <= 1e-3
+
+
+@pytest.mark.parametrize("name", list(SPECS))
+@pytest.mark.parametrize("n_past, n_new", [(0, 1), (33, 1), (200, 5), (90, 40), (5, 200)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attend_equals_the_f16_context_over_the_same_values(name, n_past, n_new, masked):
+    sp = SPECS[name]
+    hq, h, d = sp["n_head"], sp["n_head_kv"], sp["head_dim"]
+    qn = torch.ones(hq * d if sp.get("qk_norm") == 2 else d, device="cuda")
+    norms = {1: (qn, qn[:d]), 2: (qn, None)}.get(sp.get("qk_norm"), (None, None))
+    with q8_context(sp) as a, K.Context(K.make_config(sp)) as b:
+        if n_past:
+            append(a, 0, 0, inputs(1, n_past, hq, h, d), norms)
+        new = inputs(2, n_new, hq, h, d)
+        append(a, 0, n_past, new, norms)
+        append(b, 0, n_past, new, norms)
+        for which in (0, 1):
+            b.import_rows(0, which, 0, a.export_rows(0, which, 0, n_past + n_new))
+        mask = None
+        if masked:
+            mask = torch.randn(n_new, n_past + n_new + 3, device="cuda")
+            mask[torch.rand(mask.shape, device="cuda") < 0.3] = float("-inf")
+            mask[:, 0] = 0.0
+        outs = []
+        for ctx in (a, b):
+            out = torch.empty(n_new, hq * d, device="cuda")
+            if masked:
+                ctx.attend_mask(0, n_past, n_new, mask, out)
+            else:
+                ctx.attend(0, n_past, n_new, out)
+            ctx.status()
+            outs.append(out)
+        close(*outs)
+
+
+def test_forward_over_layers_and_replay():
+    sp = spec(layers=3)
+    hq, h, d = 8, 2, 128
+    g = torch.Generator().manual_seed(5)
+    with q8_context(sp) as ctx:
+        n = 100
+        q, k, v = (torch.randn(3, n + 1, w * d, generator=g).cuda() for w in (hq, h, h))
+        outs = [torch.zeros(3, n, hq * d, device="cuda"), torch.zeros(3, 1, hq * d, device="cuda")]
+
+        def layers(i):
+            a, m = (0, n) if i == 0 else (n, 1)
+            for l in range(3):
+                append(ctx, l, a, (q[l, a:a + m], k[l, a:a + m], v[l, a:a + m]))
+                ctx.attend(l, a, m, outs[i][l])
+
+        layers(0)
+        layers(1)
+        torch.cuda.synchronize()
+        want = outs[1].clone()
+        # the same token through kv_forward's layer loop, one layer stride for q, k and v: a fused buffer
+        fused = torch.cat([q[:, n], k[:, n], v[:, n]], 1).contiguous()
+        ctx.forward(n, 1, fused, 0, fused[:, hq * d:], 0, fused[:, (hq + h) * d:], 0, fused.stride(0), None, None, 0, outs[1],
+                    hq * d)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[1], want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ctx.forward(n, 1, fused, 0, fused[:, hq * d:], 0, fused[:, (hq + h) * d:], 0, fused.stride(0), None, None, 0,
+                        outs[1], hq * d, stream=torch.cuda.current_stream())
+        outs[1].zero_()
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[1], want)
+
+
+def test_import_and_export_round_trip():
+    sp = spec(d=64, hq=4, h=2, layers=1)
+    rng = np.random.default_rng(1)
+    with q8_context(sp) as ctx:
+        x = (rng.standard_normal((100, 2, 64)) * 2).astype(np.float16).view(np.uint16)
+        for which in (0, 1):
+            ctx.import_rows(0, which, 0, x)
+            assert np.array_equal(ctx.export_rows(0, which, 0, 100).view(np.float16).astype(np.float64), quantised(x))
+        before = [ctx.export_rows(0, w, 0, 100) for w in (0, 1)]
+        # what an 8-bit cache exported goes in again unchanged, also in the middle, rows behind it and V untouched
+        ctx.import_rows(0, 0, 0, before[0])
+        ctx.import_rows(0, 0, 37, before[0][37:50])
+        assert all(np.array_equal(ctx.export_rows(0, w, 0, 100), before[w]) for w in (0, 1))
+        assert ctx.layer_rows(0) == (100, 512)
+
+
+def test_a_budget_of_rows_over_a_long_sequence():
+    """Positions go on past the rows a layer holds; each layer is evicted whenever it is full."""
+    hq, h, d, budget, rows = 6, 2, 64, 40, 96
+    sp = spec(d=d, hq=hq, h=h, layers=2, n_rot=0, n_ctx=400)
+    rng = np.random.default_rng(4)
+    with q8_context(sp, cache_rows=rows, track_weights=True, n_batch_max=48) as ctx:
+        assert ctx.layer_rows(0) == (0, 96)
+        kept_rows = [[[] for _ in range(h)] for _ in range(2)]   # the reference's K and V values of each layer and head
+        weight = [np.zeros((h, 0)) for _ in range(2)]
+        n_past = 0
+        for step, n in enumerate([48, 30, 1, 1, 1, 1, 1, 20, 1, 1, 33, 17, 40, 1, 1, 1, 48, 25, 1, 30]):
+            for layer in range(2):
+                used = ctx.layer_rows(layer)[0]
+                if used + n > rows:
+                    q, k, v = inputs(999, n, hq, h, d)
+                    with pytest.raises(K.KvError) as e:
+                        append(ctx, layer, n_past, (q, k, v))
+                    assert e.value.code == K.KV_E_RANGE
+                    kept = torch.empty(h, budget - n % 7, dtype=torch.int32, device="cuda")
+                    keep = kept.shape[1]
+                    ctx.evict(layer, keep, 16, kept)
+                    for i in range(h):
+                        idx = kept[i].tolist()
+                        assert idx[-16:] == list(range(used - 16, used)) and idx == sorted(set(idx))
+                        # the order by the reference's weights, but where two are as near as the tolerance of a weight
+                        left = np.setdiff1d(np.arange(used - 16), idx)
+                        if len(left):
+                            assert weight[layer][i][left].max() <= weight[layer][i][idx[:-16]].min() * (1 + 1e-4) + 1e-7
+                        vals = [np.stack(kept_rows[layer][i])[idx][:, w] for w in (0, 1)]
+                        for w in (0, 1):
+                            for b in range(0, keep, B):
+                                c, word = R.quantise_block(vals[w][b:b + B])
+                                vals[w][b:b + B] = R.row_values(c, np.array([word], np.uint32))
+                        kept_rows[layer][i] = list(np.stack(vals, 1))
+                    weight[layer] = np.stack([weight[layer][i][kept[i].cpu().numpy()] for i in range(h)])
+                    assert ctx.layer_rows(layer) == (keep, rows)
+                    with pytest.raises(K.KvError) as e:
+                        ctx.attend(layer, n_past, n, torch.empty(n, hq * d, device="cuda"))
+                    assert e.value.code == K.KV_E_STATE
+                    used = keep
+                qkv = inputs(100 * step + layer, n, hq, h, d)
+                append(ctx, layer, n_past, qkv)
+                out = torch.empty(n, hq * d, device="cuda")
+                ctx.attend(layer, n_past, n, out)
+                ctx.status()
+                got = [ctx.export_rows(layer, w, 0, used + n).view(np.float16).astype(np.float64) for w in (0, 1)]
+                for i in range(h):
+                    old = used // B * B   # (rows before the first block of the new ones keep their values)
+                    if old:
+                        assert np.array_equal(np.stack([g[:old, i] for g in got], 1), np.stack(kept_rows[layer][i][:old]))
+                    kept_rows[layer][i] = list(np.stack([g[:, i] for g in got], 1))
+                weight[layer] = np.concatenate([weight[layer], np.zeros((h, n))], 1)
+                q = qkv[0].half().double().cpu().reshape(n, h, hq // h, d)
+                o = out.double().cpu().reshape(n, h, hq // h, d)
+                for i in range(h):
+                    kk, vv = (torch.from_numpy(g[:, i]) for g in got)
+                    want, wt, mag, err, top = R.attend(kk, vv, torch.ones(used + n, dtype=torch.float64), q[:, i], used)
+                    assert ((o[:, i] - want).abs() <= mag * 2.0 ** -10 + 1e-6).all()
+                    weight[layer][i] += wt.numpy()
+            n_past += n
+        assert n_past > 2 * rows
+
+
+def test_rewinding_after_an_eviction():
+    hq, h, d = 4, 2, 64
+    sp = spec(d=d, hq=hq, h=h, layers=1, n_rot=0, n_ctx=256)
+    with q8_context(sp, cache_rows=64, track_weights=True) as ctx:
+        out = torch.empty(60, hq * d, device="cuda")
+        append(ctx, 0, 0, inputs(1, 60, hq, h, d))
+        ctx.attend(0, 0, 60, out)
+        ctx.evict(0, 32, 8)
+        for n_past, ok in ((60, True), (55, True), (52, True), (51, False), (1, False)):
+            if ok:
+                append(ctx, 0, n_past, inputs(2, 1, hq, h, d))
+                ctx.attend(0, n_past, 1, out)
+                assert ctx.layer_rows(0)[0] == n_past - 28 + 1
+            else:
+                with pytest.raises(K.KvError) as e:
+                    append(ctx, 0, n_past, inputs(2, 1, hq, h, d))
+                assert e.value.code == K.KV_E_RANGE
+        append(ctx, 0, 0, inputs(3, 5, hq, h, d))   # from the start: nothing is gone
+        ctx.attend(0, 0, 5, out)
+        assert ctx.layer_rows(0) == (5, 64)
+        append(ctx, 0, 5, inputs(3, 1, hq, h, d))
+
+
+def test_refusals_of_a_context():
+    sp = spec(d=64, hq=4, h=2, layers=1, n_rot=0, n_ctx=100)
+    with q8_context(sp, track_weights=True) as ctx:
+        append(ctx, 0, 0, inputs(1, 40, 4, 2, 64))
+        for args, code in (((0, 41, 0), K.KV_E_ARG), ((0, 0, 0), K.KV_E_ARG), ((0, 10, 11), K.KV_E_ARG),
+                           ((0, 10, -1), K.KV_E_ARG), ((1, 10, 1), K.KV_E_ARG)):
+            with pytest.raises(K.KvError) as e:
+                ctx.evict(*args)
+            assert e.value.code == code
+        with pytest.raises(K.KvError) as e:
+            ctx.fill_synthetic(1, 0, 10)
+        assert e.value.code == K.KV_E_UNSUPPORTED
+        s = torch.cuda.Stream()
+        with pytest.raises(K.KvError) as e:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                ctx.evict(0, 10, 1, stream=s)
+        assert e.value.code == K.KV_E_STATE
+        ctx.evict(0, 10, 1)
+        torch.cuda.synchronize()
+    with q8_context(sp) as ctx, K.Context(K.make_config(sp)) as f16:
+        for c in (ctx, f16):
+            with pytest.raises(K.KvError) as e:
+                c.evict(0, 1, 0)
+            assert e.value.code == K.KV_E_UNSUPPORTED
+        with pytest.raises(K.KvError) as e:
+            f16.layer_rows(0)
+        assert e.value.code == K.KV_E_UNSUPPORTED
+
+
+def test_auto_sized_context():
+    sp = spec(d=64, hq=4, h=2, layers=1, n_ctx=0, n_ctx_train=3000)
+    with q8_context(sp) as ctx:
+        assert ctx.n_ctx == 3000
+        assert ctx.layer_rows(0) == (0, 3008)

@@ -145,3 +145,43 @@ def test_reference_evict_order():
     assert R.evict(w, 8, 8, 0) == list(range(8))
     assert R.evict(w, 8, 3, 3) == [5, 6, 7]
     assert R.evict(w, 7, 6, 0) == [0, 1, 2, 3, 4, 6]
+
+
+def config(**kw):
+    c = K.KvConfig()
+    K.lib().kv_config_init(ctypes.byref(c))
+    for k, v in dict(dict(n_layer=4, n_head=8, n_head_kv=2, head_dim=64, n_rot=64, n_ctx=1000, cache_type=K.KV_CACHE_Q8),
+                     **kw).items():
+        setattr(c, k, v)
+    return c
+
+
+@pytest.mark.parametrize("kw", [dict(cache_type=2), dict(cache_type=-1), dict(n_shards=2), dict(ring_cells=64),
+                                dict(cache_rows=-1), dict(cache_rows=100), dict(cache_rows=100, n_ctx=0, track_weights=1),
+                                dict(cache_type=0, cache_rows=5), dict(cache_type=0, track_weights=1),
+                                dict(n_head=2 * 129)])
+def test_configurations_that_are_refused(kw):
+    h = ctypes.c_void_p()
+    assert K.lib().kv_alloc(ctypes.byref(config(**kw)), ctypes.byref(h)) == K.KV_E_ARG and not h.value
+
+
+def test_cache_bytes_of_an_8_bit_configuration():
+    block = 2 * (2 * 32 * 64 + 8)
+    assert K.cache_bytes(config(), 1000) == 4 * 32 * block
+    assert K.cache_bytes(config(track_weights=1), 1000) == 4 * 32 * (block + 2 * 32 * 4)
+    assert K.cache_bytes(config(track_weights=1, cache_rows=100), 1000) == 4 * 4 * (block + 2 * 32 * 4)
+    assert K.cache_bytes(config(), 0) == 0
+    f16 = K.cache_bytes(config(cache_type=0), 1024)
+    assert 0.5 * f16 < K.cache_bytes(config(), 1024) < 0.51 * f16
+
+
+def test_auto_n_ctx_of_an_8_bit_configuration():
+    # about twice the F16 cache's positions in the same memory
+    a, b = (K.auto_n_ctx(config(cache_type=t, n_layer=32, n_head_kv=8, head_dim=128, n_ctx_train=1 << 30), 100 << 30) for t in (0, 1))
+    assert 1.9 * a < b <= 2.0 * a
+
+
+def test_null_contexts():
+    L = K.lib()
+    assert L.kv_evict(None, 0, 1, 0, None, None) == K.KV_E_ARG
+    assert L.kv_layer_rows(None, 0, None, None) == K.KV_E_ARG
