@@ -497,15 +497,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.c.k_scale) + h * n_sc;
             const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.c.v_scale) + h * n_sc;
             float m = -CUDART_INF_F, me = 0.0f, l = 0.0f, bad = 0.0f;
-            // a sub-tile's scale words, one sub-tile ahead; a block behind the keys holds anything: 1 stands for its scale
+            // a sub-tile's scale words, one sub-tile ahead; a block behind the keys holds anything: the last block's stand for its own
             uint32_t kw[2], vw[2];
+            const int64_t last_blk = (p.n_kv - 1) / kBlock;
             auto scales = [&](int t) {
-                const int64_t i = 2 * (int64_t)t;
-                const bool two = (i + 1) * kBlock < p.n_kv;
+                const int64_t i = min(2 * (int64_t)t, last_blk), j = min(2 * (int64_t)t + 1, last_blk);
                 kw[0] = __ldg(ksc + i);
+                kw[1] = __ldg(ksc + j);
                 vw[0] = __ldg(vsc + i);
-                kw[1] = two ? __ldg(ksc + i + 1) : 0x3f800000u;
-                vw[1] = two ? __ldg(vsc + i + 1) : 0x3f800000u;
+                vw[1] = __ldg(vsc + j);
             };
             scales(w.t0);
             const int n0 = n;
@@ -682,7 +682,14 @@ __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
     const int h = pair / p.n_blk, b = pair % p.n_blk, tk = (in & 127) / p.r, hd = (in & 127) - tk * p.r;
     const int tok = b * p.tok_blk + (in >> 7) * p.tok_tile + tk;
     const int64_t W = p.c.H * axis_head(p), x0 = pair_start(p, pair) + p.gap, x1 = x0 + subs_of(p, b) - 1;
-    const int c0 = (int)(((x0 + 1) * p.n_cta - 1) / W), c1 = (int)(((x1 + 1) * p.n_cta - 1) / W);
+    int c0, c1;
+    if ((W + 1) * p.n_cta < ((int64_t)1 << 31)) {   // (a 64-bit division is some hundred instructions)
+        c0 = (int)(((uint32_t)(x0 + 1) * (uint32_t)p.n_cta - 1u) / (uint32_t)W);
+        c1 = (int)(((uint32_t)(x1 + 1) * (uint32_t)p.n_cta - 1u) / (uint32_t)W);
+    } else {
+        c0 = (int)(((x0 + 1) * p.n_cta - 1) / W);
+        c1 = (int)(((x1 + 1) * p.n_cta - 1) / W);
+    }
     pdl_wait();
     if (c0 == c1 || tk >= p.tok_tile || tok >= p.n_new) return;
     constexpr int V = (D / 4 + 31) / 32;
