@@ -253,6 +253,8 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
         if (w.more()) load(w.item);
         auto all_wait = [&](uint64_t *b, uint32_t par) { return __all_sync(0xffffffffu, wait(b, par)); };
         const uint32_t sk = smem_addr(smem + L::o_k), sq = smem_addr(smem + L::o_q);
+        bool ahead = false;   // `next` holds the numbers of this thread's row of the next tile
+        float2 next = make_float2(0.0f, 0.0f);
         for (int64_t now = -1; ok && w.more(); w.next(p)) {
             if (w.item != now) {
                 if (items > 0 && !(ok = all_wait(k_empty, (items - 1) & 1))) break;
@@ -278,7 +280,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
             int64_t *off = row_off + qs * 128;
             {
                 // a row that adds nothing has 1 / Z = 0: its queries are zeros, so that its products are finite
-                const float2 y = row0 + t < R ? stat[t] : make_float2(0.0f, 0.0f);
+                const float2 y = ahead ? next : row0 + t < R ? stat[t] : make_float2(0.0f, 0.0f);
                 const int tok = (row0 + t) / p.r, j = row0 + t - tok * p.r;
                 float *rs = reinterpret_cast<float *>(row_st + qs * 64 + t / 2) + (t & 1);
                 rs[0] = -y.x;
@@ -292,6 +294,9 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[qs]);
+            // (not before the fence, which waits for loads in flight)
+            ahead = !w.last();
+            if (ahead) next = row0 + 128 + t < R ? stat[128 + t] : make_float2(0.0f, 0.0f);
         }
     } else if (lane == 0) {
         constexpr uint32_t id = idesc_f16_f32(128, 128, false);
