@@ -143,28 +143,26 @@ __global__ void __launch_bounds__(kBlock *D / 8) store_kernel(const StoreParams 
     if (fresh && !is_v && c == 0 && p.c.weight) p.c.weight[(int64_t)h * p.c.rows + row] = 0.0f;
 }
 
-// kLoadU pieces of 8 codes a thread, their loads in flight together; a token's
-// heads are neighbours in the output.  Bound by the output's bytes.
-constexpr int kLoadU = 4;
-
-template <int D, bool F16>
+// U pieces of 8 codes a thread, their loads in flight together; a token's heads
+// are neighbours in the output.  Bound by the output's bytes.
+template <int D, bool F16, int U>
 __global__ void __launch_bounds__(256) load_kernel(const LoadParams p)
 {
-    pdl_launch_dependents();
-    pdl_wait();
     const bool is_v = p.k ? blockIdx.y != 0 : true;
     void *out = is_v ? p.v : p.k;
     const int8_t *codes = is_v ? p.c.v : p.c.k;
     const uint32_t *scale = reinterpret_cast<const uint32_t *>(is_v ? p.c.v_scale : p.c.k_scale);
     // (a row has at most 1024 * 32 pieces, a CTA's rows are few: 32 bits from its first row on)
     const uint32_t pieces = p.c.H * (D / 8);
-    const int64_t first = (int64_t)blockIdx.x * (256 * kLoadU), t0 = first / pieces;
+    const int64_t first = (int64_t)blockIdx.x * (256 * U), t0 = first / pieces;
     const uint32_t base = (uint32_t)(first - t0 * pieces);
-    uint2 w[kLoadU];
-    uint32_t s[kLoadU];
-    int64_t at[kLoadU];
+    uint2 w[U];
+    uint32_t s[U];
+    int64_t at[U];
+    pdl_launch_dependents();
+    pdl_wait();
 #pragma unroll
-    for (int k = 0; k < kLoadU; k++) {
+    for (int k = 0; k < U; k++) {
         const uint32_t j = base + threadIdx.x + 256 * k, dt = j / pieces, c = j - dt * pieces;
         const int64_t t = t0 + dt, row = p.row0 + t;
         const uint32_t h = c / (D / 8), d = c % (D / 8) * 8;
@@ -175,20 +173,21 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadParams p)
         }
     }
 #pragma unroll
-    for (int k = 0; k < kLoadU; k++) {
+    for (int k = 0; k < U; k++) {
         if (at[k] < 0) continue;
-        const int e0 = scale_exp(s[k]);
+        const int e = scale_exp(s[k]);
+        const bool bad = (s[k] & 0x7f800000u) == 0x7f800000u;   // a block with values that are not finite
         if constexpr (F16) {
             __half *dst = static_cast<__half *>(out) + at[k];
             __half y[8];
-            if ((s[k] & 0x7f800000u) == 0x7f800000u) {   // a block with values that are not finite
+            if (bad) {
                 float x[8];
-                decode8(w[k], e0, x);
+                decode8(w[k], e, x);
 #pragma unroll
-                for (int e = 0; e < 8; e++) y[e] = __float2half_rn(x[e]);
+                for (int j = 0; j < 8; j++) y[j] = __float2half_rn(x[j]);
             } else {
-                // the codes as halves times 2^e0, both exact (2^-24 is the smallest half)
-                const __half2 f = __half2half2(__float2half_rn(pow2(e0)));
+                // the codes as halves times 2^e, both exact (2^-24 is the smallest half)
+                const __half2 f = __half2half2(__float2half_rn(pow2(e)));
                 const uint2 a = codes_to_half4(w[k].x), b = codes_to_half4(w[k].y);
                 __half2 *y2 = reinterpret_cast<__half2 *>(y);
                 y2[0] = __hmul2(*reinterpret_cast<const __half2 *>(&a.x), f);
@@ -200,18 +199,18 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadParams p)
                 *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; e++) dst[e] = y[e];
+                for (int j = 0; j < 8; j++) dst[j] = y[j];
             }
         } else {
             float *dst = static_cast<float *>(out) + at[k];
             float x[8];
-            decode8(w[k], e0, x);
+            decode8(w[k], e, x);
             if (p.vec) {
                 reinterpret_cast<float4 *>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
                 reinterpret_cast<float4 *>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; e++) dst[e] = x[e];
+                for (int j = 0; j < 8; j++) dst[j] = x[j];
             }
         }
     }
@@ -444,7 +443,8 @@ __device__ __forceinline__ void move_codes(uint4 &x, int k, bool bad)
 // each of K and of V.  Many small CTAs keep the gathers in flight (32k rows to
 // 16k with the selection and the read-back: 46 us, two blocks a CTA 47 us, four
 // 51 us); the codes' arithmetic is in halves, two at a time (with conversions
-// to float and back the conversions were the bound, 50 us).
+// to float and back the conversions were the bound, 50 us).  A warp a block, all
+// of its rows in flight, measured 52 us.
 template <int D>
 __global__ void __launch_bounds__(kBlock *D / 16) gather_kernel(const EvictParams p)
 {
@@ -516,11 +516,21 @@ cudaError_t store_d(const StoreParams &p, dim3 grid, cudaStream_t st)
                  : launch_pdl(store_kernel<D, false>, grid, kBlock * D / 8, 0, p, st);
 }
 
-template <int D>
-cudaError_t load_d(const LoadParams &p, dim3 grid, cudaStream_t st)
+template <int D, int U>
+cudaError_t load_du(const LoadParams &p, cudaStream_t st)
 {
-    return p.f16 ? launch_pdl(load_kernel<D, true>, grid, 256, 0, p, st)
-                 : launch_pdl(load_kernel<D, false>, grid, 256, 0, p, st);
+    const int64_t pieces = p.n * p.c.H * (D / 8);   // (2^31 CTAs would be a cache of 2^42 bytes)
+    const dim3 grid((unsigned)((pieces + 256 * U - 1) / (256 * U)), p.k && p.v ? 2 : 1);
+    return p.f16 ? launch_pdl(load_kernel<D, true, U>, grid, 256, 0, p, st)
+                 : launch_pdl(load_kernel<D, false, U>, grid, 256, 0, p, st);
+}
+
+template <int D>
+cudaError_t load_d(const LoadParams &p, cudaStream_t st)
+{
+    // four pieces a thread once they leave eight CTAs an SM (16k rows of 8 heads of 128: 1 piece 22 us, 2 18 us, 4
+    // 16 us; 9 rows: 1 piece 0.4 us less than 4)
+    return p.n * p.c.H * (D / 8) >= (int64_t)kSMs * 8 * 256 * 4 ? load_du<D, 4>(p, st) : load_du<D, 1>(p, st);
 }
 
 }  // namespace
@@ -540,13 +550,11 @@ cudaError_t launch_store(const StoreParams &p, cudaStream_t st)
 
 cudaError_t launch_load(const LoadParams &p, cudaStream_t st)
 {
-    const int64_t pieces = p.n * p.c.H * (p.c.D / 8);   // (at most 2^31 * 2^15 / 2^10 CTAs: checked by the entry point)
-    const dim3 grid((unsigned)((pieces + 256 * kLoadU - 1) / (256 * kLoadU)), p.k && p.v ? 2 : 1);
     switch (p.c.D) {
-    case 64: return load_d<64>(p, grid, st);
-    case 96: return load_d<96>(p, grid, st);
-    case 128: return load_d<128>(p, grid, st);
-    case 256: return load_d<256>(p, grid, st);
+    case 64: return load_d<64>(p, st);
+    case 96: return load_d<96>(p, st);
+    case 128: return load_d<128>(p, st);
+    case 256: return load_d<256>(p, st);
     default: return cudaErrorInvalidValue;
     }
 }

@@ -648,27 +648,41 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
     const int64_t key = (int64_t)(w - h * chunks) * 512 + tid * 4;
     int a, b;
     span_of(p, h, a, b);
+    const float *src = p.scores + (int64_t)h * R * p.nb * kBlock + key;
+    float *dst = p.c.weight + (int64_t)h * p.c.rows + key;
+    const int64_t pitch = (int64_t)p.nb * kBlock;
+    const int row = tid >> 3, sub = tid & 7;
     pdl_wait();
-    {
-        const int row = tid >> 3, sub = tid & 7;
-        float M = -CUDART_INF_F, l = 0.0f;
-        if (row < R) {
-            for (int c = a + sub; c <= b; c += 8) {
-                const float2 s = p.stat[((int64_t)c + h) * 16 + row];
-                const float top = fmaxf(M, s.x);
-                if (top > -CUDART_INF_F) l = __fmaf_rn(l, ex2_approx((M - top) * unit), s.y * ex2_approx((s.x - top) * unit));
-                else l += s.y;   // (0, or NaN)
-                M = top;
-            }
-        }
+    // all that is read, on its way at once: the first rows' scores, the weights so far, the parts' (m, l)
+    constexpr int kAhead = 4, kParts = 3;
+    float4 x[kAhead];
+    float old[4];
+    float2 ml[kParts];
 #pragma unroll
-        for (int k = 1; k < 8; k <<= 1) {
-            const float M2 = __shfl_xor_sync(0xffffffffu, M, k), l2 = __shfl_xor_sync(0xffffffffu, l, k);
+    for (int u = 0; u < kParts; u++)
+        ml[u] = row < R && a + sub + 8 * u <= b ? p.stat[((int64_t)a + sub + 8 * u + h) * 16 + row] : make_float2(-CUDART_INF_F, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kAhead; i++)
+        x[i] = key < p.n_kv && i < R ? *reinterpret_cast<const float4 *>(src + i * pitch) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 4; i++) old[i] = key + i < p.n_kv ? dst[i] : 0.0f;
+    {
+        float M = -CUDART_INF_F, l = 0.0f;
+        auto take = [&](float M2, float l2) {
             const float top = fmaxf(M, M2);
             if (top > -CUDART_INF_F) l = __fmaf_rn(l, ex2_approx((M - top) * unit), l2 * ex2_approx((M2 - top) * unit));
-            else l += l2;
+            else l += l2;   // (0, or NaN)
             M = top;
-        }
+        };
+#pragma unroll
+        for (int u = 0; u < kParts; u++) take(ml[u].x, ml[u].y);
+        if (row < R)
+            for (int c = a + sub + 8 * kParts; c <= b; c += 8) {
+                const float2 s = p.stat[((int64_t)c + h) * 16 + row];
+                take(s.x, s.y);
+            }
+#pragma unroll
+        for (int k = 1; k < 8; k <<= 1) take(__shfl_xor_sync(0xffffffffu, M, k), __shfl_xor_sync(0xffffffffu, l, k));
         if (sub == 0) {
             const bool adds = row < R && l > 0.0f && l < CUDART_INF_F && M < CUDART_INF_F;
             s_row[row] = adds ? make_float2(M, 1.0f / l) : make_float2(0.0f, 0.0f);
@@ -676,22 +690,22 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
     }
     __syncthreads();
     if (key >= p.n_kv) return;
-    const float *src = p.scores + (int64_t)h * R * p.nb * kBlock + key;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](float2 s, float4 y) {
+        if (s.y == 0.0f) return;   // (adds nothing, whatever its scores are)
+        sum[0] = __fmaf_rn(ex2_approx((y.x - s.x) * unit), s.y, sum[0]);
+        sum[1] = __fmaf_rn(ex2_approx((y.y - s.x) * unit), s.y, sum[1]);
+        sum[2] = __fmaf_rn(ex2_approx((y.z - s.x) * unit), s.y, sum[2]);
+        sum[3] = __fmaf_rn(ex2_approx((y.w - s.x) * unit), s.y, sum[3]);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; i++)
+        if (i < R) add(s_row[i], x[i]);
 #pragma unroll 4
-    for (int row = 0; row < R; row++) {
-        const float2 s = s_row[row];
-        const float4 x = *reinterpret_cast<const float4 *>(src + (int64_t)row * p.nb * kBlock);
-        if (s.y == 0.0f) continue;   // (adds nothing, whatever its scores are)
-        sum[0] = __fmaf_rn(ex2_approx((x.x - s.x) * unit), s.y, sum[0]);
-        sum[1] = __fmaf_rn(ex2_approx((x.y - s.x) * unit), s.y, sum[1]);
-        sum[2] = __fmaf_rn(ex2_approx((x.z - s.x) * unit), s.y, sum[2]);
-        sum[3] = __fmaf_rn(ex2_approx((x.w - s.x) * unit), s.y, sum[3]);
-    }
-    float *dst = p.c.weight + (int64_t)h * p.c.rows + key;
+    for (int i = kAhead; i < R; i++) add(s_row[i], *reinterpret_cast<const float4 *>(src + i * pitch));
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (key + i < p.n_kv) dst[i] += sum[i];
+        if (key + i < p.n_kv) dst[i] = old[i] + sum[i];
 }
 
 template <int D, bool HILO, bool MASKED>
