@@ -35,10 +35,14 @@ constexpr int kMaxCluster = 8;
 constexpr float kBias = 7.0f;    // a new reference's weight is 2^kBias,
 constexpr float kTop = 15.0f;    // and it moves where a weight would pass 2^kTop
 
-template <int D>
+template <int D, bool HILO, bool MASKED>
 struct Rows {
-    static constexpr int W = 8;                                      // warps
-    static constexpr int E = D == 64 ? 10 : D == 96 ? 7 : D == 128 ? 6 : 3;   // tiles in a warp's ring
+    // warps: the mask's loads and arithmetic want a third one a scheduler (5
+    // tokens of 32 heads of 96 at 4k: 13.7 us with 8, 12.7 with 12); without a
+    // mask 8 with the deeper ring are ahead (128k keys of 8 heads: 48.0 and
+    // 50.2 us), and the other instances' registers allow no more
+    static constexpr int W = HILO && MASKED && D < 256 ? 12 : 8;
+    static constexpr int E = 219 * 1024 / (W * kBlock * (D + 16));   // tiles in a warp's ring
     static constexpr int pitch = D + 16;                             // bytes a row: 8 rows fall on different banks
     static constexpr int tile = kBlock * pitch;                      // K or V of a block
     static constexpr int ring = E * tile;                            // a warp's
@@ -198,9 +202,9 @@ __device__ __forceinline__ void softmax_block(float (&s)[8], RowState &st, float
 // Else rows 0-15, weights in F16 (11 bits, half a step 2^-12 of each: the
 // outputs' own F16 rounding is as large).
 template <int D, bool HILO, bool MASKED>
-__global__ void __launch_bounds__(Rows<D>::W * 32, 1) rows_kernel(const AttendParams p)
+__global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(const AttendParams p)
 {
-    using G = Rows<D>;
+    using G = Rows<D, HILO, MASKED>;
     constexpr int RT = HILO ? 1 : 2;   // 8-row halves of softmax state
     extern __shared__ __align__(128) char smem[];
     __shared__ float2 s_stat[G::W][16];
@@ -711,7 +715,7 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
 template <int D, bool HILO, bool MASKED>
 cudaError_t run(const AttendParams &p, cudaStream_t st)
 {
-    using G = Rows<D>;
+    using G = Rows<D, HILO, MASKED>;
     static Once once;
     cudaError_t e = once.on_device([] {
         return cudaFuncSetAttribute(rows_kernel<D, HILO, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
