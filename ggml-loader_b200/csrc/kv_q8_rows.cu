@@ -12,6 +12,11 @@
 // sum of e^(t - m) adds W * 2^(me - ev) in float.  With a reference that only
 // moves when W would pass 2^15 the accumulators are seldom rescaled.
 //
+// The tensor cores (mma.sync m16n8k16; tcgen05 has 64 rows at least) are the
+// bound next to HBM: with the rows on their 16-wide side and the keys on the
+// 8-wide one, half of it empty, their pipe was 82 % busy at 4 rows.  So keys,
+// and then dims, are the 16-wide side and 8 rows the 8-wide one: half as many.
+//
 // A head's blocks are streamed once: warps take blocks of 32 keys in turn, each
 // with its own ring of shared memory (cp.async, nothing but warp barriers in
 // the loop), so HBM is the bound; partial (m, sum, out) rows of the CTAs of a
@@ -35,21 +40,22 @@ constexpr int kMaxCluster = 8;
 constexpr float kBias = 7.0f;    // a new reference's weight is 2^kBias,
 constexpr float kTop = 15.0f;    // and it moves where a weight would pass 2^kTop
 
-template <int D, bool HILO, bool MASKED>
+// NG: groups of 8 query rows.  DUP (up to 4 rows): columns 4-7 of the group
+// repeat rows 0-3 and carry the low halves of their weights, W - F16(W), so the
+// weights enter with 22 bits at no cost; otherwise in F16 (11 bits, half a step
+// 2^-12 of each: the outputs' own F16 rounding is as large).
+template <int D, int NG, bool MASKED>
 struct Rows {
-    // warps: the mask's loads and arithmetic want a third one a scheduler (5
-    // tokens of 32 heads of 96 at 4k: 13.7 us with 8, 12.7 with 12); without a
-    // mask 8 with the deeper ring are ahead (128k keys of 8 heads: 48.0 and
-    // 50.2 us), and the other instances' registers allow no more
-    static constexpr int W = HILO && MASKED && D < 256 ? 12 : 8;
+    static constexpr int W = 8;                                      // warps
     static constexpr int E = 219 * 1024 / (W * kBlock * (D + 16));   // tiles in a warp's ring
     static constexpr int pitch = D + 16;                             // bytes a row: 8 rows fall on different banks
     static constexpr int tile = kBlock * pitch;                      // K or V of a block
     static constexpr int ring = E * tile;                            // a warp's
-    static constexpr int smem = W * ring;                            // (at the end also the W warps' 16 output rows, and their sum)
+    static constexpr int NR = 8 * NG;
+    static constexpr int smem = W * ring;                            // (at the end also the W warps' output rows, and their sum)
     static constexpr int nk = D / 16;                                // 16-wide steps over D
-    static constexpr bool q_regs = D <= 128;                         // the queries stay in registers, else in shared memory
-    static_assert(smem >= (W + 1) * 16 * D * 4 && smem <= 225 * 1024, "shared memory");
+    static constexpr bool q_regs = D <= 128 || NG == 1;              // the queries stay in registers, else in shared memory
+    static_assert(smem >= (W + 1) * NR * D * 4 && smem <= 225 * 1024, "shared memory");
 };
 
 // two F16 pairs (codes 0, 1 | 2, 3 or 0, 2 | 1, 3) of four signed codes: 0x6400
@@ -64,6 +70,14 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t &a, uint32_t 
     const __half2 hx = __hsub2(*reinterpret_cast<__half2 *>(&x), off), hy = __hsub2(*reinterpret_cast<__half2 *>(&y), off);
     a = *reinterpret_cast<const uint32_t *>(&hx);
     b = *reinterpret_cast<const uint32_t *>(&hy);
+}
+
+// 8x8 halves, a row a 4 lanes, transposed
+__device__ __forceinline__ uint32_t transpose8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t pack(float lo, float hi)
@@ -154,28 +168,26 @@ __device__ __forceinline__ float inverse_sum(float l, bool flash)
     return l == 0.0f ? (flash ? 0.0f : CUDART_NAN_F) : 1.0f / l;
 }
 
-// One query row of the warp's running softmax (a thread holds 8 of a block's
-// 32 keys of it; the 4 threads of a row agree on m, me and l's share is each one's own)
+// One query row of the warp's running softmax (a thread holds 4 of a block's 32
+// keys of it; the 8 threads of a row agree on m, me and l's share is each one's own)
 struct RowState {
     float m, me, l, bad;   // bad: 0, or NaN once a visible key's V block was not finite
 };
 
-// The block's 8 scores of this thread -> weights; rescale is the factor for
-// the sums so far (1 when the reference stays).
+// The block's 4 scores of this thread -> weights; returns the factor for the
+// output so far (1 when the reference stays).
 template <bool MASKED>
-__device__ __forceinline__ void softmax_block(float (&s)[8], RowState &st, float ev, bool v_bad, float &rescale, float &orescale)
+__device__ __forceinline__ float softmax_block(float (&s)[4], RowState &st, float ev, bool v_bad)
 {
     // MASKED: natural units (a mask of the type's lowest value leaves no room for a factor); else log2
     constexpr float unit = MASKED ? kLog2e : 1.0f;
-    float top = s[0];
+    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
 #pragma unroll
-    for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    rescale = orescale = 1.0f;
+    for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    float orescale = 1.0f;
     if (top > -CUDART_INF_F && (st.m == -CUDART_INF_F || __fmaf_rn(top - st.m, unit, ev - st.me) > kTop)) {
         if (st.m > -CUDART_INF_F) {
-            rescale = ex2_approx((st.m - top) * unit);
+            st.l *= ex2_approx((st.m - top) * unit);
             orescale = ex2_approx(__fmaf_rn(st.m - top, unit, st.me - (ev - kBias)));
         }
         st.m = top;
@@ -183,29 +195,31 @@ __device__ __forceinline__ void softmax_block(float (&s)[8], RowState &st, float
     }
     if (v_bad && top > -CUDART_INF_F) st.bad = CUDART_NAN_F;
     const float m = st.m == -CUDART_INF_F ? 0.0f : st.m, up = ev - st.me;
-    float sum = 0.0f;
     if constexpr (MASKED) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) s[i] = ex2_approx(__fmaf_rn(s[i] - m, kLog2e, up));
+        for (int i = 0; i < 4; i++) s[i] = ex2_approx(__fmaf_rn(s[i] - m, kLog2e, up));
     } else {
         const float ref = up - m;
 #pragma unroll
-        for (int i = 0; i < 8; i++) s[i] = ex2_approx(s[i] + ref);
+        for (int i = 0; i < 4; i++) s[i] = ex2_approx(s[i] + ref);
     }
-#pragma unroll
-    for (int i = 0; i < 8; i++) sum += s[i];
-    st.l = __fmaf_rn(sum, pow2((int)-up), st.l * rescale);
+    st.l = __fmaf_rn((s[0] + s[1]) + (s[2] + s[3]), pow2((int)-up), st.l);
+    return orescale;
 }
 
-// HILO (up to 8 rows): the tensor cores' rows 8-15 carry the low half of rows
-// 0-7's weights, W - F16(W), so the weights enter with 22 bits at no cost.
-// Else rows 0-15, weights in F16 (11 bits, half a step 2^-12 of each: the
-// outputs' own F16 rounding is as large).
-template <int D, bool HILO, bool MASKED>
-__global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(const AttendParams p)
+// the i-th row of a thread
+template <bool DUP>
+__device__ __forceinline__ int row_of(int t4, int i)
 {
-    using G = Rows<D, HILO, MASKED>;
-    constexpr int RT = HILO ? 1 : 2;   // 8-row halves of softmax state
+    const int row = (i >> 1) * 8 + 2 * t4 + (i & 1);
+    return DUP ? row & 3 : row;
+}
+
+template <int D, int NG, bool DUP, bool MASKED>
+__global__ void __launch_bounds__(Rows<D, NG, MASKED>::W * 32, 1) rows_kernel(const AttendParams p)
+{
+    using G = Rows<D, NG, MASKED>;
+    constexpr int NS = 2 * NG;   // a thread's rows: of group i / 2, 2 t4 + i % 2
     extern __shared__ __align__(128) char smem[];
     __shared__ float2 s_stat[G::W][16];
     __shared__ float s_bad[G::W][16];
@@ -228,20 +242,25 @@ __global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(
         const int h = (int)(pos / p.nb), b0 = (int)(pos - (int64_t)h * p.nb);
         const int b1 = (int)min((int64_t)p.nb, b0 + hi - pos);
         pos += b1 - b0;
-        const int nrows = p.n_new * p.r;   // (at most 8 with HILO, else 16)
+        const int nrows = p.n_new * p.r;   // (at most 4 with DUP, else 8 NG)
         const int8_t *kc = p.c.k + (int64_t)h * p.c.rows * D, *vc = p.c.v + (int64_t)h * p.c.rows * D;
         const uint32_t *ksc = reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)h * (p.c.rows / kBlock);
         const uint32_t *vsc = reinterpret_cast<const uint32_t *>(p.c.v_scale) + (int64_t)h * (p.c.rows / kBlock);
-        // rows g and g + 8: token and where their queries start
-        int tok[RT];
-        int64_t qat[RT];
-        bool have[RT];
+        // where the queries of row g (of each group) start; the tokens of the thread's own rows
+        int64_t qat[NG];
+        bool have[NG];
+        int tok[NS];
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
-            const int row = g + 8 * i;
+        for (int i = 0; i < NG; i++) {
+            const int row = DUP ? g & 3 : g + 8 * i;
             have[i] = row < nrows;
-            tok[i] = have[i] ? row / p.r : 0;
-            qat[i] = tok[i] * p.q_stride + (int64_t)(h * p.r + (have[i] ? row - tok[i] * p.r : 0)) * D + t4 * 4;
+            const int t = have[i] ? row / p.r : 0;
+            qat[i] = t * p.q_stride + (int64_t)(h * p.r + (have[i] ? row - t * p.r : 0)) * D + t4 * 4;
+        }
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            const int row = row_of<DUP>(t4, i);
+            tok[i] = row < nrows ? row / p.r : 0;
         }
         if (!waited) pdl_wait();   // (nothing before it reads memory)
         waited = true;
@@ -255,25 +274,25 @@ __global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(
             vw = mine < b1 ? vsc[mine] : 0;
         };
         scales(b0 + warp);
-        // Q as the A operand: dims 4 t4 .. + 3 of each 16 (the order in which a
+        // Q as the B operand: dims 4 t4 .. + 3 of each 16 (the order in which a
         // thread holds a key's codes)
-        uint2 q[G::q_regs ? G::nk : 1][RT];
+        uint2 q[G::q_regs ? G::nk : 1][NG];
         if constexpr (G::q_regs) {
             if (p.q_f16 && p.q_vec) {
 #pragma unroll
-                for (int i = 0; i < RT; i++)
+                for (int i = 0; i < NG; i++)
 #pragma unroll
                     for (int k = 0; k < G::nk; k++)
                         q[k][i] = have[i] ? *reinterpret_cast<const uint2 *>(static_cast<const __half *>(p.q) + qat[i] + k * 16)
                                           : make_uint2(0, 0);
             } else {
 #pragma unroll
-                for (int i = 0; i < RT; i++)
+                for (int i = 0; i < NG; i++)
 #pragma unroll
                     for (int k = 0; k < G::nk; k++) q[k][i] = have[i] ? load_q4(p, qat[i] + k * 16) : make_uint2(0, 0);
             }
         } else {
-            for (int i = threadIdx.x; i < 8 * RT * (D / 4); i += G::W * 32) {
+            for (int i = threadIdx.x; i < G::NR * (D / 4); i += G::W * 32) {
                 const int row = i / (D / 4), c = i % (D / 4), t = row / p.r;
                 s_q[row][c] = row < nrows ? load_q4(p, t * p.q_stride + (int64_t)(h * p.r + row - t * p.r) * D + c * 4)
                                           : make_uint2(0, 0);
@@ -312,23 +331,26 @@ __global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(
         for (int i = 0; i < G::E - 1; i++) fetch();
         if constexpr (!G::q_regs) __syncthreads();
 
-        RowState st[RT];
+        RowState st[NS];
 #pragma unroll
-        for (int i = 0; i < RT; i++) st[i] = RowState{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
-        float o[2 * G::nk][4];
+        for (int i = 0; i < NS; i++) st[i] = RowState{-CUDART_INF_F, 0.0f, 0.0f, 0.0f};
+        // dims 16 c + 2 g (of the two rows), 16 c + 2 g + 1 (of the two rows)
+        float o[G::nk][NG][4];
 #pragma unroll
-        for (int i = 0; i < 2 * G::nk; i++)
+        for (int c = 0; c < G::nk; c++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[i][j] = 0.0f;
+            for (int i = 0; i < NG; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[c][i][j] = 0.0f;
 
-        // a block's mask values, one block ahead
-        float mk[MASKED ? RT : 1][8];
+        // a block's mask values, one block ahead; key j of a thread: g + 8 j
+        float mk[MASKED ? NS : 1][4];
         auto masks = [&](int b) {
 #pragma unroll
-            for (int i = 0; i < RT; i++)
+            for (int i = 0; i < NS; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int64_t key = (int64_t)b * kBlock + (j >> 1) * 8 + 2 * t4 + (j & 1);
+                for (int j = 0; j < 4; j++) {
+                    const int64_t key = (int64_t)b * kBlock + 8 * j + g;
                     mk[MASKED ? i : 0][j] = key < p.n_kv ? mask_value(p, tok[i], key) : -CUDART_INF_F;
                 }
         };
@@ -339,138 +361,136 @@ __global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(
             const bool k_bad = (kword & 0x7f800000u) == 0x7f800000u, v_bad = (vword & 0x7f800000u) == 0x7f800000u;
             const float ks = k_bad ? CUDART_NAN_F : pow2(scale_exp(kword)), ev = (float)scale_exp(vword);
             const int64_t key0 = (int64_t)b * kBlock;
-            // S = Q K^T: 4 groups of 8 keys, 32 dims at a time
-            const uint32_t kt = next_tile() + (lane & 7) * G::pitch + (lane >> 3) * 16;
-            float acc[4][4];
+
+            // S^T = K Q^T: two tiles of 16 keys, 32 dims at a time (lanes 0-7 and
+            // 16-23 address keys 0-7 of a tile, the others 8-15; lanes 16-31 the
+            // second 16 dims)
+            const uint32_t kt = next_tile() + (lane & 15) * G::pitch + (lane >> 4) * 16;
+            float acc[2][NG][4];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[j][i] = 0.0f;
+                for (int i = 0; i < NG; i++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[j][i][k] = 0.0f;
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
-                uint2 qa[2][RT];
+                uint2 qb[2][NG];
 #pragma unroll
                 for (int k = 0; k < 2; k++)
 #pragma unroll
-                    for (int i = 0; i < RT; i++) {
-                        if constexpr (G::q_regs) qa[k][i] = q[2 * c + k][i];
-                        else qa[k][i] = s_q[g + 8 * i][(2 * c + k) * 4 + t4];
+                    for (int i = 0; i < NG; i++) {
+                        if constexpr (G::q_regs) qb[k][i] = q[2 * c + k][i];
+                        else qb[k][i] = s_q[g + 8 * i][(2 * c + k) * 4 + t4];
                     }
 #pragma unroll
-                for (int jj = 0; jj < 2; jj++) {
-                    // lanes 0-15: keys of group 2 jj (two 16-dim chunks), 16-31: of group 2 jj + 1
+                for (int j = 0; j < 2; j++) {
                     uint32_t w[4];
-                    ldsm_x4(kt + (jj * 16 + (lane >> 4) * 8) * G::pitch + c * 32 - (lane >> 4) * 32, w[0], w[1], w[2], w[3]);
+                    ldsm_x4(kt + j * 16 * G::pitch + c * 32, w[0], w[1], w[2], w[3]);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        uint32_t x, y;
-                        codes_to_half<false>(w[i], x, y);
-                        float(&d)[4] = acc[2 * jj + (i >> 1)];
-                        const uint2 *a = qa[i & 1];
-                        if constexpr (HILO) mma_16816(d, a[0].x, 0u, a[0].y, 0u, x, y);
-                        else mma_16816(d, a[0].x, a[RT - 1].x, a[0].y, a[RT - 1].y, x, y);
+                    for (int k = 0; k < 2; k++) {
+                        uint32_t x0, y0, x1, y1;
+                        codes_to_half<false>(w[2 * k], x0, y0);
+                        codes_to_half<false>(w[2 * k + 1], x1, y1);
+#pragma unroll
+                        for (int i = 0; i < NG; i++) mma_16816(acc[j][i], x0, x1, y0, y1, qb[k][i].x, qb[k][i].y);
                     }
                 }
             }
 
             // scores, then weights
             const float cs = p.scale * ks * (MASKED ? 1.0f : kLog2e);
-            float w[RT][8];
-            float orescale[RT];
+            float w[NS][4], orescale[NS];
             bool moved = false;
 #pragma unroll
-            for (int i = 0; i < RT; i++) {
+            for (int i = 0; i < NS; i++) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float d = acc[j >> 1][2 * i + (j & 1)];
-                    if constexpr (MASKED) w[i][j] = mk[i][j] == -CUDART_INF_F ? mk[i][j] : __fmaf_rn(d, cs, mk[i][j]);
-                    else w[i][j] = d * cs;
+                for (int j = 0; j < 4; j++) {
+                    const float x = acc[j >> 1][i >> 1][2 * (j & 1) + (i & 1)];
+                    if constexpr (MASKED) w[i][j] = mk[i][j] == -CUDART_INF_F ? mk[i][j] : __fmaf_rn(x, cs, mk[i][j]);
+                    else w[i][j] = x * cs;
                 }
-                if (MASKED && i == RT - 1 && b + G::W < b1) masks(b + G::W);
                 if (!MASKED && key0 + kBlock > p.n_past) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (key0 + (j >> 1) * 8 + 2 * t4 + (j & 1) > p.n_past + tok[i]) w[i][j] = -CUDART_INF_F;
-                }
-                if (p.scores && g + 8 * i < nrows) {
-                    float *dst = p.scores + ((int64_t)h * p.n_new * p.r + g + 8 * i) * p.nb * kBlock + key0 + 2 * t4;
-#pragma unroll
                     for (int j = 0; j < 4; j++)
-                        *reinterpret_cast<float2 *>(dst + 8 * j) = make_float2(w[i][2 * j], w[i][2 * j + 1]);
+                        if (key0 + 8 * j + g > p.n_past + tok[i]) w[i][j] = -CUDART_INF_F;
                 }
-                float rescale;
-                softmax_block<MASKED>(w[i], st[i], ev, v_bad, rescale, orescale[i]);
+                if (p.scores && row_of<DUP>(t4, i) < nrows && (!DUP || t4 < 2)) {
+                    float *dst = p.scores + ((int64_t)h * nrows + row_of<DUP>(t4, i)) * p.nb * kBlock + key0 + g;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) dst[8 * j] = w[i][j];
+                }
+                orescale[i] = softmax_block<MASKED>(w[i], st[i], ev, v_bad);
                 moved |= orescale[i] != 1.0f;
             }
+            if (MASKED && b + G::W < b1) masks(b + G::W);
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int i = 0; i < 2 * G::nk; i++) {
-                    o[i][0] *= orescale[0];
-                    o[i][1] *= orescale[0];
-                    o[i][2] *= orescale[RT - 1];
-                    o[i][3] *= orescale[RT - 1];
-                }
+                for (int c = 0; c < G::nk; c++)
+#pragma unroll
+                    for (int i = 0; i < NG; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[c][i][j] *= orescale[2 * i + (j & 1)];
             }
 
-            // O += W V: two steps of 16 keys
-            uint32_t pa[2][4];
+            // O^T += V^T W^T: two steps of 16 keys
+            uint32_t pb[2][NG][2];
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
+            for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const float e0 = w[0][4 * s + 2 * x], e1 = w[0][4 * s + 2 * x + 1];
-                    pa[s][2 * x] = pack(e0, e1);
-                    if constexpr (HILO) {
-                        const __half2 hi2 = *reinterpret_cast<const __half2 *>(&pa[s][2 * x]);
-                        pa[s][2 * x + 1] = pack(e0 - __low2float(hi2), e1 - __high2float(hi2));
-                    } else {
-                        pa[s][2 * x + 1] = pack(w[RT - 1][4 * s + 2 * x], w[RT - 1][4 * s + 2 * x + 1]);
+                for (int i = 0; i < NG; i++)
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        float e0 = w[2 * i][2 * k + x], e1 = w[2 * i + 1][2 * k + x];
+                        uint32_t y = pack(e0, e1);
+                        if constexpr (DUP) {
+                            const __half2 hi2 = *reinterpret_cast<const __half2 *>(&y);
+                            const uint32_t lo = pack(e0 - __low2float(hi2), e1 - __high2float(hi2));
+                            y = t4 < 2 ? y : lo;
+                        }
+                        pb[k][i][x] = transpose8(y);
                     }
-                }
-            }
             const uint32_t vt = next_tile();
 #pragma unroll
             for (int c = 0; c < G::nk; c++) {
                 uint32_t v[4];
                 ldsm_x4_t(vt + lane * G::pitch + c * 16, v[0], v[1], v[2], v[3]);
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
+                for (int k = 0; k < 2; k++) {
                     uint32_t e0, d0, e1, d1;   // even and odd dims, keys 0-7 and 8-15 of the step
-                    codes_to_half<true>(v[2 * s], e0, d0);
-                    codes_to_half<true>(v[2 * s + 1], e1, d1);
-                    mma_16816(o[2 * c], pa[s][0], pa[s][1], pa[s][2], pa[s][3], e0, e1);
-                    mma_16816(o[2 * c + 1], pa[s][0], pa[s][1], pa[s][2], pa[s][3], d0, d1);
+                    codes_to_half<true>(v[2 * k], e0, d0);
+                    codes_to_half<true>(v[2 * k + 1], e1, d1);
+#pragma unroll
+                    for (int i = 0; i < NG; i++) mma_16816(o[c][i], e0, d0, e1, d1, pb[k][i][0], pb[k][i][1]);
                 }
             }
         }
 
         // the warps' rows: (m, l) and O 2^me to shared memory, summed there
-        constexpr int NR = 8 * RT;
         float *os = reinterpret_cast<float *>(smem);
         cp_async_wait<0>();
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < RT; i++) {
+        for (int i = 0; i < NS; i++) {
             float l = st[i].l;
-            l += __shfl_xor_sync(0xffffffffu, l, 1);
-            l += __shfl_xor_sync(0xffffffffu, l, 2);
-            const int row = g + 8 * i;
-            if (t4 == 0) {
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) l += __shfl_xor_sync(0xffffffffu, l, k);
+            const int row = row_of<DUP>(t4, i);
+            const bool mine = !DUP || t4 < 2;
+            if (g == 0 && mine) {
                 s_stat[warp][row] = make_float2(st[i].m, l);
                 s_bad[warp][row] = st[i].bad;
             }
             const float f = pow2((int)st[i].me);
-            float *dst = os + ((int64_t)warp * NR + row) * D;
+            float *dst = os + ((int64_t)warp * G::NR + row) * D + 2 * g;
 #pragma unroll
             for (int c = 0; c < G::nk; c++) {
-                // columns 2 t4, 2 t4 + 1 of the even and odd tile: dims 16 c + 4 t4 .. + 3
-                float4 x;
-                if constexpr (HILO)
-                    x = make_float4(o[2 * c][0] + o[2 * c][2], o[2 * c + 1][0] + o[2 * c + 1][2],
-                                    o[2 * c][1] + o[2 * c][3], o[2 * c + 1][1] + o[2 * c + 1][3]);
-                else
-                    x = make_float4(o[2 * c][2 * i], o[2 * c + 1][2 * i], o[2 * c][2 * i + 1], o[2 * c + 1][2 * i + 1]);
-                *reinterpret_cast<float4 *>(dst + c * 16 + t4 * 4) = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+                float x = o[c][i >> 1][i & 1], y = o[c][i >> 1][2 + (i & 1)];
+                if constexpr (DUP) {   // the low halves' sums
+                    x += __shfl_xor_sync(0xffffffffu, x, 2);
+                    y += __shfl_xor_sync(0xffffffffu, y, 2);
+                }
+                if (mine) *reinterpret_cast<float2 *>(dst + c * 16) = make_float2(x * f, y * f);
             }
         }
         __syncthreads();
@@ -489,7 +509,7 @@ __global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(
             for (int w = 0; w < G::W; w++) {
                 const float2 s = s_stat[w][row];
                 const float f = ex2_approx((s.x - ref) * unit), bad = s_bad[w][row];
-                const float4 y = *reinterpret_cast<const float4 *>(os + ((int64_t)w * NR + row) * D + c);
+                const float4 y = *reinterpret_cast<const float4 *>(os + ((int64_t)w * G::NR + row) * D + c);
                 // (a warp without a visible key: m = -inf, f = 0, its sums 0 -- or NaN, which must stay)
                 l = __fmaf_rn(s.y, f, l);
                 x.x = __fmaf_rn(y.x, f, x.x + bad);
@@ -498,7 +518,7 @@ __global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(
                 x.w = __fmaf_rn(y.w, f, x.w + bad);
             }
             if (p.cq) {
-                *reinterpret_cast<float4 *>(os + G::W * NR * D + row * D + c) = x;
+                *reinterpret_cast<float4 *>(os + G::W * G::NR * D + row * D + c) = x;
                 if (c == 0) s_row[row] = make_float2(M, l);
                 continue;
             }
@@ -513,7 +533,7 @@ __global__ void __launch_bounds__(Rows<D, HILO, MASKED>::W * 32, 1) rows_kernel(
             cluster_sync_all();
             for (int i = cluster_rank() * (G::W * 32) + threadIdx.x; i < nrows * (D / 4); i += p.cq * G::W * 32) {
                 const int row = i / (D / 4), c = i % (D / 4) * 4;
-                const uint32_t at = smem_addr(&s_row[row]), xat = smem_addr(os + G::W * NR * D + row * D + c);
+                const uint32_t at = smem_addr(&s_row[row]), xat = smem_addr(os + G::W * G::NR * D + row * D + c);
                 float2 s[kMaxCluster];
                 float4 y[kMaxCluster];
                 float M = -CUDART_INF_F;
@@ -712,15 +732,15 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
         if (key + i < p.n_kv) dst[i] = old[i] + sum[i];
 }
 
-template <int D, bool HILO, bool MASKED>
+template <int D, int NG, bool DUP, bool MASKED>
 cudaError_t run(const AttendParams &p, cudaStream_t st)
 {
-    using G = Rows<D, HILO, MASKED>;
+    using G = Rows<D, NG, MASKED>;
     static Once once;
     cudaError_t e = once.on_device([] {
-        return cudaFuncSetAttribute(rows_kernel<D, HILO, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
+        return cudaFuncSetAttribute(rows_kernel<D, NG, DUP, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
     });
-    if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, HILO, MASKED>, p.n_cta, G::W * 32, G::smem, p, st, p.cq);
+    if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, NG, DUP, MASKED>, p.n_cta, G::W * 32, G::smem, p, st, p.cq);
     if (e != cudaSuccess || p.cq) return e;
     const bool split = p.n_cta > p.n_vh || p.n_vh % p.n_cta != 0;   // else every head lies in one CTA
     if (!split && !p.scores) return cudaSuccess;
@@ -729,12 +749,17 @@ cudaError_t run(const AttendParams &p, cudaStream_t st)
     return launch_pdl(join_kernel<D, MASKED>, grid, 128, 0, p, st);
 }
 
+template <int D, bool MASKED>
+cudaError_t run_m(const AttendParams &p, cudaStream_t st)
+{
+    const int64_t rows = (int64_t)p.n_new * p.r;
+    return rows <= 4 ? run<D, 1, true, MASKED>(p, st) : rows <= 8 ? run<D, 1, false, MASKED>(p, st) : run<D, 2, false, MASKED>(p, st);
+}
+
 template <int D>
 cudaError_t run_d(const AttendParams &p, cudaStream_t st)
 {
-    const bool hilo = (int64_t)p.n_new * p.r <= 8;
-    if (p.mask) return hilo ? run<D, true, true>(p, st) : run<D, false, true>(p, st);
-    return hilo ? run<D, true, false>(p, st) : run<D, false, false>(p, st);
+    return p.mask ? run_m<D, true>(p, st) : run_m<D, false>(p, st);
 }
 
 }  // namespace
