@@ -71,6 +71,7 @@ struct AttendParams {
     int32_t n_vh;           // what CTAs work on at a time: KV heads, or (chunk) pairs of one and a block, H * n_blk
     int32_t n_cta;
     int32_t cq;             // rows: CTAs of a head's cluster, 0: no clusters
+    int32_t warps;          // rows: a CTA's, 8 or 12
     int32_t l2_ahead;       // rows: blocks a CTA asks for in L2 while the kernel before ends
     int32_t tok_tile, tok_blk, n_blk;   // chunk: tokens of a query tile and of a CTA's tiles, such blocks
     int64_t subs;           // chunk: sub-tiles of 64 keys of one KV head, over its blocks

@@ -44,9 +44,9 @@ constexpr float kTop = 15.0f;    // and it moves where a weight would pass 2^kTo
 // repeat rows 0-3 and carry the low halves of their weights, W - F16(W), so the
 // weights enter with 22 bits at no cost; otherwise in F16 (11 bits, half a step
 // 2^-12 of each: the outputs' own F16 rounding is as large).
-template <int D, int NG, bool MASKED>
+template <int D, int NG, int W_>
 struct Rows {
-    static constexpr int W = 8;                                      // warps
+    static constexpr int W = W_;                                     // warps
     static constexpr int E = 219 * 1024 / (W * kBlock * (D + 16));   // tiles in a warp's ring
     static constexpr int pitch = D + 16;                             // bytes a row: 8 rows fall on different banks
     static constexpr int tile = kBlock * pitch;                      // K or V of a block
@@ -215,10 +215,10 @@ __device__ __forceinline__ int row_of(int t4, int i)
     return DUP ? row & 3 : row;
 }
 
-template <int D, int NG, bool DUP, bool MASKED>
-__global__ void __launch_bounds__(Rows<D, NG, MASKED>::W * 32, 1) rows_kernel(const AttendParams p)
+template <int D, int NG, int W, bool DUP, bool MASKED>
+__global__ void __launch_bounds__(W * 32, 1) rows_kernel(const AttendParams p)
 {
-    using G = Rows<D, NG, MASKED>;
+    using G = Rows<D, NG, W>;
     constexpr int NS = 2 * NG;   // a thread's rows: of group i / 2, 2 t4 + i % 2
     extern __shared__ __align__(128) char smem[];
     __shared__ float2 s_stat[G::W][16];
@@ -732,15 +732,15 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
         if (key + i < p.n_kv) dst[i] = old[i] + sum[i];
 }
 
-template <int D, int NG, bool DUP, bool MASKED>
+template <int D, int NG, int W, bool DUP, bool MASKED>
 cudaError_t run(const AttendParams &p, cudaStream_t st)
 {
-    using G = Rows<D, NG, MASKED>;
+    using G = Rows<D, NG, W>;
     static Once once;
     cudaError_t e = once.on_device([] {
-        return cudaFuncSetAttribute(rows_kernel<D, NG, DUP, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
+        return cudaFuncSetAttribute(rows_kernel<D, NG, W, DUP, MASKED>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem);
     });
-    if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, NG, DUP, MASKED>, p.n_cta, G::W * 32, G::smem, p, st, p.cq);
+    if (e == cudaSuccess) e = launch_pdl(rows_kernel<D, NG, W, DUP, MASKED>, p.n_cta, G::W * 32, G::smem, p, st, p.cq);
     if (e != cudaSuccess || p.cq) return e;
     const bool split = p.n_cta > p.n_vh || p.n_vh % p.n_cta != 0;   // else every head lies in one CTA
     if (!split && !p.scores) return cudaSuccess;
@@ -753,7 +753,9 @@ template <int D, bool MASKED>
 cudaError_t run_m(const AttendParams &p, cudaStream_t st)
 {
     const int64_t rows = (int64_t)p.n_new * p.r;
-    return rows <= 4 ? run<D, 1, true, MASKED>(p, st) : rows <= 8 ? run<D, 1, false, MASKED>(p, st) : run<D, 2, false, MASKED>(p, st);
+    if constexpr (D < 256)
+        if (rows <= 8 && p.warps == 12) return rows <= 4 ? run<D, 1, 12, true, MASKED>(p, st) : run<D, 1, 12, false, MASKED>(p, st);
+    return rows <= 4 ? run<D, 1, 8, true, MASKED>(p, st) : rows <= 8 ? run<D, 1, 8, false, MASKED>(p, st) : run<D, 2, 8, false, MASKED>(p, st);
 }
 
 template <int D>
@@ -786,20 +788,25 @@ void rows_split(AttendParams &p)
         if (up <= kSMs) C = std::min(up, T);
         else if (T / down - T / C <= 21) C = down;
     }
-    // Up to 8 CTAs a head join in their cluster instead of by a second kernel,
+    // 2 to 8 CTAs a head join in their cluster instead of by a second kernel,
     // where the device holds all clusters at once (these numbers of them, by
-    // the occupancy query at this shared memory).  Heads of up to 128 blocks of
-    // 128-wide rows are cut in 8 for it, two blocks a warp.  2000 keys, device
-    // time with the join and without: 2 heads of 64 4.9 and 4.1 us, 8 of 128
-    // 8.0 and 5.2 us.
+    // the occupancy query at this shared memory): 2000 keys of 8 heads 8.0 ->
+    // 5.2 us of device time.  Longer heads are not cut in 8 for it: 4000 keys
+    // 7.1 us so, and 5.8 us over 128 CTAs and with the second kernel.
     constexpr int most[kMaxCluster + 1] = {0, 0, 74, 45, 33, 22, 22, 15, 15};
     p.cq = 0;
     if (!p.c.weight) {
-        if (C > kMaxCluster * p.n_vh && (int64_t)p.nb * p.c.D <= 2 * W * kMaxCluster * 128 && p.n_vh <= most[kMaxCluster]) C = kMaxCluster * p.n_vh;
         const int64_t q = C / p.n_vh;
         if (C % p.n_vh == 0 && q >= 2 && q <= kMaxCluster && p.n_vh <= most[q]) p.cq = (int)q;
     }
     p.n_cta = (int)C;
+    // 12 warps from 28 blocks a CTA on: the loop's chain of loads, conversions
+    // and products has more to hide it, the CTA's end has more rows to add.  8
+    // and 12 warps: 2000 keys of 8 heads 5.2 and 5.5 us, 16k 11.2 and 11.4, 32k
+    // 17.6 and 16.8, 131k 52.8 and 51.6; 16k of 32 heads of 96, 5 masked tokens,
+    // 39.2 and 32.9.  (Two groups of rows, or 256 dims, do not fit 168 registers
+    // a thread: 12 warps 60.9 us against 39.8, and 36.2 against 29.5.)
+    p.warps = T >= 28 * C ? 12 : W;
     p.l2_ahead = W;   // a block of each warp: 20.5 -> 19.5 us at 32k keys of 8 heads; 16 gain the same, 32 nothing
 }
 
