@@ -1738,9 +1738,10 @@ int kv_evict(kv_ctx *ctx, int32_t layer, int64_t keep, int64_t recent, int32_t *
     rc = launch(ctx, KV_K_APPEND, st, "eviction kernels", [&] { return kvb::q8::launch_evict(p, st); });
     if (rc) return rc;
     std::swap(l.c, ctx->q8_spare);
+    // (of the `recent` rows, those behind an earlier eviction's floor follow one another in position)
+    l.floor = std::max(keep - recent, l.floor - (l.used - keep));
     l.gone += l.used - keep;
     l.used = keep;
-    l.floor = keep - recent;
     if (ctx->last_layer == layer) ctx->last_layer = -1;   // (kv_attend follows a kv_append)
     return KV_OK;
 }

@@ -292,7 +292,8 @@ int kv_attend_decode_noalloc(const uint16_t *k_cache, const uint16_t *v_cache,
  * the kept keys stay rotated as they are, the next kv_append is again at the
  * next position, n_past, and kv_attend attends over the rows that are left.
  * Every layer is evicted by its own call.  Rewinding n_past is possible by up
- * to `recent` tokens (KV_E_RANGE beyond), or to 0.  kept: DEVICE int32
+ * to `recent` tokens, as far as an earlier eviction allowed it (KV_E_RANGE
+ * beyond), or to 0.  kept: DEVICE int32
  * [n_head_kv][keep], each head's kept rows (their numbers before the call), or
  * NULL.  The layer's buffers change places with a spare set, so a stream that is
  * being captured is refused (KV_E_STATE), and a graph captured before must not
@@ -362,7 +363,8 @@ int kv_q8_load(const kv_q8_cache *cache, int64_t row0, int64_t n, void *k_out, v
 
 /* Bytes of workspace kv_q8_attend needs for these sizes (0: bad arguments).  It
  * grows with n_past and n_new: ask once for the largest of both.  The contents
- * need no preparation; calls that overlap on the device need one each. */
+ * need no preparation; calls that overlap on the device need one each (and on
+ * a cache that keeps weights no two calls may overlap). */
 uint64_t kv_q8_attend_workspace(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32_t n_new);
 
 /*

@@ -244,6 +244,27 @@ def test_rewinding_after_an_eviction():
         append(ctx, 0, 5, inputs(3, 1, hq, h, d))
 
 
+def test_rewinding_after_two_evictions():
+    """The second one's recent rows reach back behind the first one's: those do not follow one another in position."""
+    hq, h, d = 4, 2, 64
+    sp = spec(d=d, hq=hq, h=h, layers=1, n_rot=0, n_ctx=256)
+    with q8_context(sp, cache_rows=64, track_weights=True) as ctx:
+        out = torch.empty(60, hq * d, device="cuda")
+        append(ctx, 0, 0, inputs(1, 60, hq, h, d))
+        ctx.attend(0, 0, 60, out)
+        ctx.evict(0, 32, 8)   # positions 52 to 59 are the last 8 rows
+        append(ctx, 0, 60, inputs(2, 2, hq, h, d))
+        ctx.attend(0, 60, 2, out)
+        ctx.evict(0, 30, 20)
+        for n_past in (51, 45, 42):
+            with pytest.raises(K.KvError) as e:
+                append(ctx, 0, n_past, inputs(3, 1, hq, h, d))
+            assert e.value.code == K.KV_E_RANGE
+        append(ctx, 0, 52, inputs(3, 1, hq, h, d))
+        ctx.attend(0, 52, 1, out)
+        assert ctx.layer_rows(0) == (21, 64)
+
+
 def test_refusals_of_a_context():
     sp = spec(d=64, hq=4, h=2, layers=1, n_rot=0, n_ctx=100)
     with q8_context(sp, track_weights=True) as ctx:
