@@ -436,6 +436,8 @@ class Q8Cache:
         for name, t, shape, dtype in want:
             if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != k.device:
                 raise ValueError("%s must be a contiguous %s tensor %s on %s" % (name, dtype, shape, k.device))
+        if not k.is_cuda:
+            raise ValueError("a Q8Cache's tensors must be on a CUDA device")
         self.tensors = k, v, k_scale, v_scale, weight   # kept alive
         self.n_head_kv, self.rows, self.head_dim = h, rows, d
         self._c = KvQ8Cache(*[_ptr(t) for t in self.tensors], rows, h, d)
@@ -443,11 +445,11 @@ class Q8Cache:
         self._lib, self._calls, self._index = lib(), _calls(), k.get_device()
         self._width = h * d
         self._torch = torch
-        self._current = torch._C._cuda_getDevice if self._index >= 0 else None
+        self._current = torch._C._cuda_getDevice
 
     def _on_device(self, fn, *args):
         """fn(*args), which returns a KV_* code, on the cache's device."""
-        if self._current is None or self._current() == self._index:
+        if self._current() == self._index:
             rc = fn(*args)
         else:
             with self._torch.cuda.device(self._index):

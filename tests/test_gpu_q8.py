@@ -327,6 +327,82 @@ def test_strided_queries_and_outputs(pad, shift):
     assert (got[:, :shift] == 9.0).all() and (got[:, shift + hq * d:] == 9.0).all()
 
 
+# enough blocks a CTA that the few-row kernel takes its wider form: heads that lie in one CTA, and heads cut between CTAs
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("d, h, r, n_past, n_new", [(64, 148, 1, 930, 1), (128, 148, 2, 900, 3), (96, 150, 1, 990, 4),
+                                                    (128, 6, 4, 22300, 1), (64, 7, 7, 20000, 1), (96, 5, 2, 28700, 2)])
+def test_attend_many_blocks(d, h, r, n_past, n_new, masked):
+    n_kv, weight = n_past + n_new, h == 6
+    c = filled(h, n_kv, d, weight=weight, seed=3)
+    mask = None
+    if masked:
+        mask = torch.randn(n_new, n_kv, generator=torch.Generator().manual_seed(5))
+        mask[:, 40:n_kv // 2] = float("-inf")
+        if n_new > 1:
+            mask[0] = float("-inf")
+        mask = mask.half().cuda()
+    check(c, h * r, n_past, n_new, queries(8, n_new, h * r, d), mask=mask, flash=True)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams, each with its workspace, give the bits of the same calls one after the other."""
+    c = filled(8, 6000, 128)
+    calls = [(1, 5999), (4, 5000), (40, 3000), (100, 5900)]
+    qs = [queries(i, n, 32, 128) for i, (n, _) in enumerate(calls)]
+    wss = [torch.empty(max(c.q8.attend_workspace(32, p, n) for n, p in calls), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    want = []
+    for q, (n, past) in zip(qs, calls):
+        want.append(torch.empty(n, 32 * 128, device="cuda"))
+        c.q8.attend(32, past, n, q, want[-1], workspace=wss[0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[torch.full_like(w, 9.0) for w in want] for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i in range(len(calls)):
+            for j, st in enumerate(streams):   # (the second stream takes them in the other order)
+                m = len(calls) - 1 - i if j else i
+                c.q8.attend(32, calls[m][1], calls[m][0], qs[m], outs[j][m], workspace=wss[j], stream=st)
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(x, w) for x, w in zip(o, want))
+
+
+@pytest.mark.parametrize("n_new", [1, 3, 9, 40])
+def test_offsets_that_pass_32_bits(n_new):
+    """A cache of 6.4 GB each of K and V: rows at both ends of every head, the keys between them masked."""
+    h, d, rows = 3, 256, 8400000 // B * B
+    n_past = rows - n_new - 5
+    n_kv = n_past + n_new
+    g = torch.Generator(device="cuda").manual_seed(2)
+    codes = [torch.empty(h, rows, d, dtype=torch.int8, device="cuda") for _ in range(2)]
+    for x in codes:
+        for i in range(h):   # (zeros but for the two ends; no row is read that is not one of these)
+            x[i].zero_()
+            x[i, :64] = torch.randint(-127, 128, (64, d), generator=g, device="cuda", dtype=torch.int8)
+            x[i, -96:] = torch.randint(-127, 128, (96, d), generator=g, device="cuda", dtype=torch.int8)
+    scales = [torch.full((h, rows // B), 2.0 ** -6, device="cuda") for _ in range(2)]
+    q8 = K.Q8Cache(*codes, *scales)
+    seen = torch.cat([torch.arange(60), torch.arange(n_kv - 70, n_kv)])
+    mask = torch.full((n_new, n_kv), float("-inf"), dtype=torch.float16, device="cuda")
+    mask[:, seen.cuda()] = torch.randn(n_new, len(seen), generator=g, device="cuda").half()
+    q = queries(4, n_new, h, d)
+    out = torch.empty(n_new, h * d, device="cuda")
+    ws = torch.empty(q8.attend_workspace(h, n_past, n_new), dtype=torch.uint8, device="cuda")
+    q8.attend(h, n_past, n_new, q, out, mask=mask, workspace=ws)
+    back = [torch.empty(70, h, d, device="cuda") for _ in range(2)]
+    q8.load(n_kv - 70, 70, *back)
+    qq, m = q.double().cpu().view(n_new, h, 1, d), mask[:, seen.cuda()].float().cpu()
+    for i in range(h):
+        k, v = (torch.cat([x[i, :60], x[i, n_kv - 70:n_kv]]).double().cpu() * 2.0 ** -6 for x in codes)
+        want, _, mag, err, _ = R.attend(k, v, torch.ones(len(seen), dtype=torch.float64), qq[:, i], 0, m)
+        # (the tolerance of `check`, for the keys that are seen)
+        tol = mag * ((2 * err + 2.0 ** -21 + len(seen) * 2.0 ** -24)[..., None] + 2.0 ** -11) + 130 * 127 * 2.0 ** -38 + 2.0 ** -24
+        assert ((out.double().cpu().view(n_new, h, 1, d)[:, i] - want).abs() <= tol).all()
+        for x, y in zip(back, (k, v)):
+            assert torch.equal(x[:, i].double().cpu(), y[60:])
+
+
 def test_the_same_call_gives_the_same_bits():
     c = filled(4, 5000, 128, weight=True)
     q = queries(1, 2, 16, 128)
@@ -369,6 +445,16 @@ def run_evict(c, n, keep, recent, with_weight=True, seed=1):
 def test_evict(h, d, n, keep, recent):
     c = filled(h, n, d, weight=True, spread=3.0)
     c.w.copy_(torch.randn(c.w.shape, generator=torch.Generator().manual_seed(n)).exp())
+    run_evict(c, n, keep, recent)
+
+
+def test_evict_more_candidates_than_shared_memory_holds():
+    n, keep, recent, d = 8 * 32768 + 5001, 70001, 1001, 64
+    c = Cache(1, -(-n // B) * B, d, weight=True)
+    for w, dw in zip(c.words, c.dev[2:]):
+        w[:] = 127 - 6 << 23
+        dw.copy_(torch.from_numpy(w.view(np.float32)))
+    c.w.copy_(torch.randint(0, 60000, c.w.shape, generator=torch.Generator().manual_seed(1)).float())   # (with ties)
     run_evict(c, n, keep, recent)
 
 

@@ -185,3 +185,63 @@ def test_null_contexts():
     L = K.lib()
     assert L.kv_evict(None, 0, 1, 0, None, None) == K.KV_E_ARG
     assert L.kv_layer_rows(None, 0, None, None) == K.KV_E_ARG
+
+
+# ---- the Python binding -------------------------------------------------------
+def test_a_q8cache_refuses_other_tensors():
+    torch = pytest.importorskip("torch")
+
+    def make(k=(2, 64, 64), dtype=torch.int8, v=(2, 64, 64), scale=(2, 2), weight=None, t=False):
+        x = torch.zeros(k, dtype=dtype)
+        return K.Q8Cache(x.transpose(0, 1) if t else x, torch.zeros(v, dtype=torch.int8), torch.zeros(scale), torch.zeros(scale),
+                         None if weight is None else torch.zeros(weight))
+
+    for kw in (dict(dtype=torch.uint8), dict(v=(2, 32, 64)), dict(scale=(2, 64)), dict(weight=(2, 2)), dict(t=True),
+               dict()):   # (the last: not on a GPU)
+        with pytest.raises(ValueError):
+            make(**kw)
+
+
+def test_the_binding_refuses_other_rows():
+    """Its C module's checks, with CPU tensors for a cache on "device -1": nothing here reaches the library but calls it refuses."""
+    torch = pytest.importorskip("torch")
+    try:
+        calls = K._calls()
+    except ImportError:
+        pytest.skip("the binding's C module is not built")
+    c = cache()
+    ref = ctypes.addressof(c)
+    f, half = lambda *s: torch.zeros(s), lambda *s: torch.zeros(s, dtype=torch.float16)
+    good = f(3, 128)
+    for k, v in ((f(2, 128), good), (good, f(3, 127)), (good, half(3, 128)), (good.double(), good), (f(3, 256)[:, ::2], good),
+                 (f(128, 3).t(), good), (f(128), good), (good, torch.tensor(1.0)), (f(3, 128, 2)[..., 0], good)):
+        with pytest.raises(ValueError):
+            calls.store(ref, -1, 128, 0, 3, k, v, None)
+    with pytest.raises(ValueError):
+        calls.store(ref, 0, 128, 0, 3, good, good, None)          # another device
+    with pytest.raises(AttributeError):
+        calls.store(ref, -1, 128, 0, 3, None, good, None)
+    with pytest.raises(TypeError):
+        calls.store(ref, -1, 128, 0, 3, good)
+    assert calls.store(ref, -1, 128, 1022, 3, good, f(3, 2, 64), None) == K.KV_E_RANGE
+    for ko, vo in ((good, half(3, 128)), (good, f(3, 200)[:, :128]), (f(4, 128), None)):
+        with pytest.raises(ValueError):
+            calls.load(ref, -1, 128, 0, 3, ko, vo, None)
+    assert calls.load(ref, -1, 128, 0, 3, None, None, None) == K.KV_E_ARG
+    assert calls.load(ref, -1, 128, 1 << 62, 3, good, None, None) == K.KV_E_RANGE
+    q, out, ws = f(3, 256), half(3, 4, 64), torch.zeros(64, dtype=torch.uint8)
+
+    def attend(q=q, out=out, mask=None, ws=ws, n_head=4, past=10):
+        return calls.attend(ref, -1, 64, n_head, past, 3, q, out, mask, False, ws, None)
+
+    for kw in (dict(q=f(3, 255)), dict(out=f(2, 256)), dict(mask=f(3, 12)), dict(mask=f(2, 13)), dict(mask=f(3, 26)[:, ::2]),
+               dict(mask=f(13)), dict(mask=f(3, 13).int()), dict(ws=None), dict(ws=torch.zeros(8, 8)[:, ::2]), dict(n_head=6)):
+        with pytest.raises(ValueError):
+            attend(**kw)
+    assert attend(past=1022) == K.KV_E_RANGE
+    kept = torch.zeros(2, 5, dtype=torch.int32)
+    d = other()
+    for x, dev in ((kept.long(), -1), (kept[:, :4], -1), (kept.t().contiguous(), -1), (kept, 0)):
+        with pytest.raises(ValueError):
+            calls.evict(ref, -1, 2, 100, 5, 1, ctypes.addressof(d), dev, x, None)
+    assert calls.evict(ref, -1, 2, 2000, 5, 1, ctypes.addressof(d), -1, kept, None) == K.KV_E_RANGE
