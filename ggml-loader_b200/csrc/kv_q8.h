@@ -67,7 +67,7 @@ struct AttendParams {
     float scale;
     // scratch of the workspace, set by launch_attend
     int32_t nb;             // blocks of kBlock keys: ceil(n_kv / kBlock)
-    int32_t n_tile;         // query-row tiles a CTA holds
+    int32_t n_tile;         // chunk: query-row tiles a CTA holds (rows: 1)
     int32_t n_vh;           // what CTAs work on at a time: KV heads, or (chunk) pairs of one and a block, H * n_blk
     int32_t n_cta;
     int32_t cq;             // rows: CTAs of a head's cluster, 0: no clusters

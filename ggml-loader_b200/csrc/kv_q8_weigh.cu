@@ -5,12 +5,14 @@
 // The scores are formed again as S^T = K Q^T on the tensor cores (keys on the
 // 128 TMEM lanes, 128 query rows in the columns), so a thread holds one key and
 // its sum never leaves its registers: no atomics, one order.  Half the products
-// of the attention itself; the exponentials are the bound (16 a clock and SM).
+// of the attention itself; the exponentials (16 a clock and SM) are busy half
+// of the time, the rest is the chain of a tile: products, exponentials, and the
+// tile's columns handed back (512 tokens at 4k, 8 heads of 128: 36 us).
 //
 // An item is (KV head, NK tiles of 128 keys); a CTA takes a range of items and
 // for each walks the query tiles that see them, which L2 delivers again for
-// every item: with two tiles of keys an item half as often (512 tokens at 4k,
-// where that was the bound: 37 us with one tile, two CTAs an SM, against 26).
+// every item: with two tiles of keys an item half as often (the same call: 37
+// us with one tile, two CTAs an SM).
 //   4 warps a key tile  a key a thread: S^T from TMEM, exponentials, the sum
 //   4 warps             stage: the item's codes as F16, query tiles and their
 //                       rows' (m, 1 / Z)
