@@ -5,14 +5,19 @@
 // The scores are formed again as S^T = K Q^T on the tensor cores (keys on the
 // 128 TMEM lanes, 128 query rows in the columns), so a thread holds one key and
 // its sum never leaves its registers: no atomics, one order.  Half the products
-// of the attention itself; the exponentials (16 a clock and SM) are busy half
-// of the time, the rest is the chain of a tile: products, exponentials, and the
-// tile's columns handed back (512 tokens at 4k, 8 heads of 128: 36 us).
+// of the attention itself.  Without a mask 1 / Z goes into the exponent, e^(t -
+// m - ln Z): one number a row to read (and one more rounding, at the size of the
+// score m or of log2 Z <= 31: as the score's own, or half a step 2^-20).
+// 512 tokens at 4k, 8 heads of 128: 33 us.  A pair of tiles takes 2 us, 1.1 of
+// it the exponentials' units (16 a clock and SM); two warps a scheduler do not
+// hide the rest of the chain (wait, read TMEM, exponentials, hand back), and the
+// staging warps take 1.85 us a query tile, most of it L2's delivery.
 //
 // An item is (KV head, NK tiles of 128 keys); a CTA takes a range of items and
 // for each walks the query tiles that see them, which L2 delivers again for
 // every item: with two tiles of keys an item half as often (the same call: 37
-// us with one tile, two CTAs an SM).
+// us with one tile, two CTAs an SM).  Each tile has its own barriers, so that one
+// tile's wait falls into the other's exponentials.
 //   4 warps a key tile  a key a thread: S^T from TMEM, exponentials, the sum
 //   4 warps             stage: the item's codes as F16, query tiles and their
 //                       rows' (m, 1 / Z)
@@ -42,11 +47,10 @@ struct WL {
     static constexpr int ctas = D == 256 || NK == 2 ? 1 : 2;   // an SM
     static constexpr int QS = NK == 2 ? 4 : 2;         // query tiles staged or in use
     static constexpr size_t o_k = 0, o_q = NK * (size_t)tile;
-    static constexpr size_t o_st = o_q + QS * (size_t)tile;   // [QS][64] two rows' (-m, -m, 1 / Z, 1 / Z)
-    static constexpr size_t o_lim = o_st + QS * 128 * 8;      // [QS][128] the last key a row may see
-    static constexpr size_t o_off = o_lim + QS * 128 * 4;     // [QS][128] where a row's queries are, -1: nowhere
+    static constexpr size_t o_st = o_q + QS * (size_t)tile;   // [QS][64] two rows' (-m, -m, 1 / Z, 1 / Z); without a mask four rows' -m - log2 Z
+    static constexpr size_t o_off = o_st + QS * 128 * 8;      // [QS][128] where a row's queries are, -1: nowhere
     static constexpr size_t o_bar = o_off + QS * 128 * 8;
-    static constexpr int n_bar = 2 + 2 * QS + 4 + 1;
+    static constexpr int n_bar = 2 + 2 * QS + 4 * NK + 1;
     static constexpr size_t o_tm = o_bar + n_bar * 8;
     static constexpr size_t bytes = o_tm + 16;
     static_assert(bytes * ctas <= 226 * 1024, "shared memory");
@@ -110,11 +114,10 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
     extern __shared__ __align__(1024) unsigned char smem[];
     uint64_t *bar = reinterpret_cast<uint64_t *>(smem + L::o_bar);
     uint64_t *k_full = bar, *k_empty = bar + 1, *q_full = bar + 2, *q_empty = q_full + QS, *s_full = q_empty + QS;
-    uint64_t *s_empty = s_full + 2, *drain = s_empty + 2;
+    uint64_t *s_empty = s_full + 2 * NK, *drain = s_empty + 2 * NK;   // [buffer][key tile]
     uint32_t *tm_slot = reinterpret_cast<uint32_t *>(smem + L::o_tm);
     volatile int *flag = reinterpret_cast<volatile int *>(smem + L::o_tm + 8);
     float4 *row_st = reinterpret_cast<float4 *>(smem + L::o_st);
-    int *row_lim = reinterpret_cast<int *>(smem + L::o_lim);
     int64_t *row_off = reinterpret_cast<int64_t *>(smem + L::o_off);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -124,9 +127,9 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
             mbar_init(&q_full[i], 4);
             mbar_init(&q_empty[i], 1 + kStage);   // the MMAs that read it, and the warps that read its rows' numbers
         }
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 2 * NK; i++) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&s_empty[i], kStage);
+            mbar_init(&s_empty[i], 4);
         }
         mbar_init(drain, 1);
         *flag = 0;
@@ -156,6 +159,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
         const int kt = warp >> 2;   // key tile of the item
         const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + kt * 128;
         float sum = 0.0f, c = 0.0f;
+        int first = 0;   // the first row that sees the thread's key (without a mask)
         int64_t now = -1;
         for (; ok && w.more(); s++) {
             if (w.fresh) q++;
@@ -167,27 +171,27 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
                 const int64_t blk = min(key / kBlock, p.c.rows / kBlock - 1);
                 const uint32_t kw = __ldg(reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)w.h * (p.c.rows / kBlock) + blk);
                 c = p.scale * pow2(scale_exp(kw)) * (MASKED ? 1.0f : kLog2e);
+                first = (int)max((int64_t)0, min((int64_t)p.n_new, key - p.n_past)) * p.r;
             }
-            ok = __all_sync(0xffffffffu, wait(&q_full[qs], (q / QS) & 1) && wait(&s_full[s & 1], (s >> 1) & 1));
+            ok = __all_sync(0xffffffffu, wait(&q_full[qs], (q / QS) & 1) && wait(&s_full[(s & 1) * NK + kt], (s >> 1) & 1));
             if (!ok) break;
             tc_fence_after();
             const float4 *st = row_st + qs * 64;
-            const int *lim = row_lim + qs * 128;
-            const int row0 = w.qt * 128, n_rows = min(128, p.n_new * p.r - row0), n_ch = (n_rows + 31) / 32;
-            const bool all = MASKED || w.key0 + kt * 128 + 127 <= p.n_past + row0 / p.r;   // every row sees every key
+            const int row0 = w.qt * 128, n_rows = min(128, p.n_new * p.r - row0);
             const bool in = key < p.n_kv;
             uint64_t part = 0ull;   // two sums
             const uint64_t c2 = pk2(c, c);
-            // 32 rows' scores
-            auto rows = [&](int ch, uint32_t (&v)[32]) {
+            // N rows' scores
+            constexpr int N = 32;
+            auto rows = [&](int ch, uint32_t (&v)[N]) {
                 if constexpr (MASKED) {
                     int tok = -1;
                     float mk = 0.0f, a = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const int row = row0 + ch * 32 + e;
+                    for (int e = 0; e < N; e++) {
+                        const int row = row0 + ch * N + e;
                         if (row - row0 >= n_rows) break;
-                        const float4 y4 = st[ch * 16 + e / 2];
+                        const float4 y4 = st[ch * (N / 2) + e / 2];
                         const float m = e & 1 ? y4.y : y4.x, y = e & 1 ? y4.w : y4.z;
                         if (y == 0.0f) continue;   // (its mask may be infinite)
                         if (row / p.r != tok) {   // (the same for all lanes)
@@ -200,33 +204,50 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
                     }
                     part = add2(part, pk2(a, 0.0f));
                 } else {
-                    if (!all) {
+                    const int hide = first - row0 - ch * N;   // rows of these that do not see the key
+                    if (__all_sync(0xffffffffu, hide >= N)) return;
+                    if (__any_sync(0xffffffffu, hide > 0)) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            if (key > lim[ch * 32 + e]) v[e] = __float_as_uint(-CUDART_INF_F);
+                        for (int e = 0; e < N; e++)
+                            if (e < hide) v[e] = __float_as_uint(-CUDART_INF_F);
                     }
                     uint64_t s0 = 0ull, s1 = 0ull;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float4 y = st[ch * 16 + e];
-                        const float2 x = up2(fma2(pk2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), c2, pk2(y.x, y.y)));
-                        uint64_t &sum = e & 1 ? s1 : s0;
-                        sum = fma2(pk2(ex2_approx(x.x), ex2_approx(x.y)), pk2(y.z, y.w), sum);
+                    for (int e = 0; e < N / 4; e++) {
+                        const float4 y = st[ch * (N / 4) + e];
+                        const float2 a = up2(fma2(pk2(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1])), c2, pk2(y.x, y.y)));
+                        const float2 b = up2(fma2(pk2(__uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3])), c2, pk2(y.z, y.w)));
+                        s0 = add2(s0, pk2(ex2_approx(a.x), ex2_approx(a.y)));
+                        s1 = add2(s1, pk2(ex2_approx(b.x), ex2_approx(b.y)));
                     }
                     part = add2(part, add2(s0, s1));
                 }
             };
+            const uint32_t at = tS + (s & 1) * (128 * NK);
+            if constexpr (MASKED || L::ctas == 2) {   // (two CTAs an SM: 96 registers a thread)
 #pragma unroll 1
-            for (int ch = 0; ch < n_ch; ch++) {
-                uint32_t v[32];
-                tmem_ld32(tS + (s & 1) * (128 * NK) + ch * 32, v);
-                tmem_wait_ld();
-                rows(ch, v);
+                for (int ch = 0; ch * N < n_rows; ch++) {
+                    uint32_t v[N];
+                    tmem_ld32(at + ch * N, v);
+                    tmem_wait_ld();
+                    rows(ch, v);
+                }
+            } else {
+                // the next rows' scores on their way during the exponentials
+                uint32_t v[2][N];
+                tmem_ld32(at, v[0]);
+#pragma unroll
+                for (int ch = 0; ch < 128 / N; ch++) {
+                    if (ch * N >= n_rows) break;
+                    tmem_wait_ld();
+                    if (ch * N + N < n_rows) tmem_ld32(at + ch * N + N, v[(ch + 1) & 1]);
+                    rows(ch, v[ch & 1]);
+                }
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                mbar_arrive(&s_empty[s & 1]);
+                mbar_arrive(&s_empty[(s & 1) * NK + kt]);
                 if (w.done_with_q(p)) mbar_arrive(&q_empty[qs]);
             }
             {
@@ -284,10 +305,13 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
                 // a row that adds nothing has 1 / Z = 0: its queries are zeros, so that its products are finite
                 const float2 y = ahead ? next : row0 + t < R ? stat[t] : make_float2(0.0f, 0.0f);
                 const int tok = (row0 + t) / p.r, j = row0 + t - tok * p.r;
-                float *rs = reinterpret_cast<float *>(row_st + qs * 64 + t / 2) + (t & 1);
-                rs[0] = -y.x;
-                rs[2] = y.y;
-                row_lim[qs * 128 + t] = (int)(p.n_past + tok);
+                if constexpr (MASKED) {
+                    float *rs = reinterpret_cast<float *>(row_st + qs * 64 + t / 2) + (t & 1);
+                    rs[0] = -y.x;
+                    rs[2] = y.y;
+                } else {
+                    reinterpret_cast<float *>(row_st + qs * 64)[t] = log2f(y.y) - y.x;   // (1 / Z = 0: -inf)
+                }
                 off[t] = y.y != 0.0f ? tok * p.q_stride + (int64_t)(w.h * p.r + j) * D : -1;
             }
             named_sync(1, 128);
@@ -313,17 +337,20 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
                 q++;
                 if (!(ok = wait(&q_full[q % QS], (q / QS) & 1))) break;
             }
-            if (s >= 2 && !(ok = wait(&s_empty[s & 1], ((s >> 1) - 1) & 1))) break;
-            tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < NK; k++)
+            for (int k = 0; k < NK; k++) {
+                const int buf = (s & 1) * NK + k;
+                if (s >= 2 && !(ok = wait(&s_empty[buf], ((s >> 1) - 1) & 1))) break;
+                tc_fence_after();
 #pragma unroll
                 for (int kk = 0; kk < D / 16; kk++) {
                     const uint32_t off = (kk >> 2) * L::box + (kk & 3) * 32;
-                    umma_ss(tmem + (s & 1) * (128 * NK) + k * 128, sdesc_k_sw128(sk + k * L::tile + off),
-                            sdesc_k_sw128(sq + (q % QS) * L::tile + off), id, kk > 0);
+                    umma_ss(tmem + buf * 128, sdesc_k_sw128(sk + k * L::tile + off), sdesc_k_sw128(sq + (q % QS) * L::tile + off), id,
+                            kk > 0);
                 }
-            umma_commit(&s_full[s & 1]);
+                umma_commit(&s_full[buf]);
+            }
+            if (!ok) break;
             if (w.done_with_q(p)) umma_commit(&q_empty[q % QS]);
             if (w.last()) umma_commit(k_empty);
         }
