@@ -269,9 +269,9 @@ __device__ __forceinline__ int before_warp(const int *s_scan, int warp, int lane
 
 // The digit (from the top) in which the want-th largest key lies, by the
 // cluster's counts: thread t takes BINS / 1024 digits from the top down.
-// `want` becomes what is to be taken within it.
+// `want` becomes what is to be taken within it, `have` what it holds.
 template <int BINS>
-__device__ __forceinline__ uint32_t find_digit(const int *s_all, int *s_scan, int *s_found, int &want)
+__device__ __forceinline__ uint32_t find_digit(const int *s_all, int *s_scan, int *s_found, int &want, int &have)
 {
     constexpr int M = BINS / kSelThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -298,9 +298,11 @@ __device__ __forceinline__ uint32_t find_digit(const int *s_all, int *s_scan, in
             }
         s_found[0] = digit;
         s_found[1] = want - before;
+        s_found[2] = s_all[digit];
     }
     __syncthreads();
     want = s_found[1];
+    have = s_found[2];
     return s_found[0];
 }
 
@@ -318,7 +320,7 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
     int *s_all = s_mine + kSelBins;                      // [2][kSelBins] the cluster's, by digit in turn
     uint32_t *s_key = s_dyn + 3 * kSelBins;
     __shared__ int s_scan[2 * kSelWarps];
-    __shared__ int s_found[2];
+    __shared__ int s_found[3];
     __shared__ int s_count[2];         // this CTA's keys above the edge, and on it
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = (int)cluster_rank(), h = blockIdx.x / kSelCtas;
@@ -344,16 +346,18 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
         atomicAdd(&s_mine[k >> 20], 1);
     }
     auto key = [&](int i) { return held ? s_key[i] : weight_key(w[lo + i]); };
-    int want = take;   // still to be taken among the keys with the prefix
+    int want = take, have;   // still to be taken among the keys with the prefix, and their number
     __syncthreads();
     send_counts<4096>(s_mine, s_all);
     cluster_sync_all();
-    uint32_t prefix = find_digit<4096>(s_all, s_scan, s_found, want);
+    uint32_t prefix = find_digit<4096>(s_all, s_scan, s_found, want, have);
     // (find_digit's barrier: the first counts are read; they are zeros again before the last digit's come in)
     s_all[tid] = 0;
+    // (where all keys with the prefix are taken -- the cluster's CTAs know the same numbers -- the other digits do not matter)
+    int shift = 20;
 #pragma unroll 1
-    for (int d = 0; d < 2; d++) {
-        const int shift = 10 - 10 * d;
+    for (int d = 0; d < 2 && want < have; d++) {
+        shift -= 10;
         int *all = s_all + (d ? 0 : kSelBins);
         for (int i = tid; i < n; i += kSelThreads) {
             const uint32_t k = key(i);
@@ -362,14 +366,14 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
         __syncthreads();
         send_counts<1024>(s_mine, all);
         cluster_sync_all();
-        prefix = prefix << 10 | find_digit<1024>(all, s_scan, s_found, want);
+        prefix = prefix << 10 | find_digit<1024>(all, s_scan, s_found, want, have);
     }
 
     // a thread's keys are neighbours: m of them from m tid on
     const int m = (n + kSelThreads * 4 - 1) / (kSelThreads * 4) * 4, i0 = min(n, m * tid), i1 = min(n, i0 + m);
     int above = 0, on = 0;
     for (int i = i0; i < i1; i++) {
-        const uint32_t k = key(i);
+        const uint32_t k = key(i) >> shift;
         above += k > prefix;
         on += k == prefix;
     }
@@ -406,7 +410,7 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
     sm100::cluster_arrive();
     // rows before this thread's first: a above the edge and min(e, want) on it
     for (int i = i0; i < i1; i++) {
-        const uint32_t k = key(i);
+        const uint32_t k = key(i) >> shift;
         const bool tie = k == prefix;
         if (k > prefix || (tie && e < want)) kept[a + min(e, want)] = lo + i;
         a += k > prefix;
