@@ -671,14 +671,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
 // Joins the pairs cut between CTAs, a warp a query row; row_stat of their rows.
 constexpr int kFoldU = 4;
 
-template <int D, bool MASKED>
+template <int D, bool MASKED, bool WIDE>
 __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
 {
+    __shared__ float4 s_o[WIDE ? 8 : 1][D / 4];
+    __shared__ float2 s_ml[8];
     constexpr int rows_blk = 128 * CL<D>::NT;
     constexpr float unit = MASKED ? kLog2e : 1.0f;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch_dependents();
-    const int pair = blockIdx.x / (rows_blk / 8), in = blockIdx.x % (rows_blk / 8) * 8 + warp;
+    constexpr int rows_cta = WIDE ? 1 : 8;
+    const int pair = blockIdx.x / (rows_blk / rows_cta), in = blockIdx.x % (rows_blk / rows_cta) * rows_cta + (WIDE ? 0 : warp);
     const int h = pair / p.n_blk, b = pair % p.n_blk, tk = (in & 127) / p.r, hd = (in & 127) - tk * p.r;
     const int tok = b * p.tok_blk + (in >> 7) * p.tok_tile + tk;
     const int64_t W = p.c.H * axis_head(p), x0 = pair_start(p, pair) + p.gap, x1 = x0 + subs_of(p, b) - 1;
@@ -698,7 +701,7 @@ __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
     for (int v = 0; v < V; v++) x[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float M = -CUDART_INF_F, l = 0.0f;
     // kFoldU parts and their (m, l) in flight together
-    for (int c = c0; c <= c1; c += kFoldU) {
+    for (int c = c0 + (WIDE ? warp * kFoldU : 0); c <= c1; c += WIDE ? 8 * kFoldU : kFoldU) {
         float2 s[kFoldU];
         float4 y[kFoldU][V];
 #pragma unroll
@@ -734,6 +737,33 @@ __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
             }
         }
     }
+    if constexpr (WIDE) {
+        // the warps' sums, each relative to its own maximum
+#pragma unroll
+        for (int v = 0; v < V; v++)
+            if (lane + 32 * v < D / 4) s_o[warp][lane + 32 * v] = x[v];
+        if (lane == 0) s_ml[warp] = make_float2(M, l);
+        __syncthreads();
+        if (warp) return;
+        M = -CUDART_INF_F;
+        l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) M = fmaxf(M, s_ml[k].x);
+        const float ref = M == -CUDART_INF_F ? 0.0f : M;
+#pragma unroll
+        for (int v = 0; v < V; v++) x[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float f = ex2_approx((s_ml[k].x - ref) * unit);
+            l = __fmaf_rn(s_ml[k].y, f, l);
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                if (lane + 32 * v >= D / 4) continue;
+                const float4 y = s_o[k][lane + 32 * v];
+                x[v] = make_float4(__fmaf_rn(y.x, f, x[v].x), __fmaf_rn(y.y, f, x[v].y), __fmaf_rn(y.z, f, x[v].z), __fmaf_rn(y.w, f, x[v].w));
+            }
+        }
+    }
     const float z = inverse_sum(l, p.flash != 0);
     const int64_t dst = (int64_t)tok * p.out_stride + (int64_t)(h * p.r + hd) * D;
 #pragma unroll
@@ -755,7 +785,9 @@ cudaError_t run(const AttendParams &p, cudaStream_t st)
     if (e != cudaSuccess) return e;
     // every pair in one CTA: as many CTAs as pairs of equal length, or one CTA
     if (p.n_cta == 1 || (p.n_blk == 1 && p.c.H % p.n_cta == 0)) return cudaSuccess;
-    return launch_pdl(fold_kernel<D, MASKED>, (unsigned)p.n_vh * (128 * L::NT / 8), 256, 0, p, st);
+    // pairs of many parts: a CTA a row, its warps share the parts (one head over 21k keys, 148 parts: 98 us with a warp a row)
+    if (p.n_cta > 12 * p.n_vh) return launch_pdl(fold_kernel<D, MASKED, true>, (unsigned)p.n_vh * (128 * L::NT), 256, 0, p, st);
+    return launch_pdl(fold_kernel<D, MASKED, false>, (unsigned)p.n_vh * (128 * L::NT / 8), 256, 0, p, st);
 }
 
 }  // namespace

@@ -181,26 +181,18 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
             const bool in = key < p.n_kv;
             uint64_t part = 0ull;   // two sums
             const uint64_t c2 = pk2(c, c);
-            // N rows' scores
-            constexpr int N = 32;
+            // N rows' scores, and with a mask its values
+            constexpr int N = MASKED ? 16 : 32;
+            float mk[MASKED ? N : 1];
             auto rows = [&](int ch, uint32_t (&v)[N]) {
                 if constexpr (MASKED) {
-                    int tok = -1;
-                    float mk = 0.0f, a = 0.0f;
+                    float a = 0.0f;
 #pragma unroll
                     for (int e = 0; e < N; e++) {
-                        const int row = row0 + ch * N + e;
-                        if (row - row0 >= n_rows) break;
-                        const float4 y4 = st[ch * (N / 2) + e / 2];
+                        const float4 y4 = st[(ch * N + e) / 2];
                         const float m = e & 1 ? y4.y : y4.x, y = e & 1 ? y4.w : y4.z;
-                        if (y == 0.0f) continue;   // (its mask may be infinite)
-                        if (row / p.r != tok) {   // (the same for all lanes)
-                            tok = row / p.r;
-                            const int64_t i = tok * p.mask_stride + key;
-                            mk = -CUDART_INF_F;
-                            if (in) mk = p.mask_f16 ? __half2float(static_cast<const __half *>(p.mask)[i]) : static_cast<const float *>(p.mask)[i];
-                        }
-                        a = __fmaf_rn(ex2_approx((__fmaf_rn(__uint_as_float(v[e]), c, mk) + m) * kLog2e), y, a);
+                        const float x = ex2_approx((__fmaf_rn(__uint_as_float(v[e]), c, mk[e]) + m) * kLog2e);
+                        a = y == 0.0f ? a : __fmaf_rn(x, y, a);   // (1 / Z = 0: its mask may be infinite)
                     }
                     part = add2(part, pk2(a, 0.0f));
                 } else {
@@ -224,7 +216,30 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
                 }
             };
             const uint32_t at = tS + (s & 1) * (128 * NK);
-            if constexpr (MASKED || L::ctas == 2) {   // (two CTAs an SM: 96 registers a thread)
+            if constexpr (MASKED) {
+                int tok = row0 / p.r, j = row0 - tok * p.r;   // of the next row
+                const void *src = p.mask;
+#pragma unroll 1
+                for (int ch = 0; ch * N < n_rows; ch++) {
+                    uint32_t v[N], raw[N];
+                    tmem_ld16(at + ch * N, v);
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        // (at clamped places, so that the loads are in flight together; a token's rows read the same values, from L1)
+                        const int64_t i = min(tok, p.n_new - 1) * p.mask_stride + min(key, p.n_kv - 1);
+                        raw[e] = p.mask_f16 ? static_cast<const unsigned short *>(src)[i] : static_cast<const uint32_t *>(src)[i];
+                        if (++j == p.r) {
+                            j = 0;
+                            tok++;
+                        }
+                    }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        mk[e] = !in ? -CUDART_INF_F : p.mask_f16 ? __half2float(__ushort_as_half((unsigned short)raw[e])) : __uint_as_float(raw[e]);
+                    rows(ch, v);
+                }
+            } else if constexpr (L::ctas == 2) {   // (two CTAs an SM: 96 registers a thread)
 #pragma unroll 1
                 for (int ch = 0; ch * N < n_rows; ch++) {
                     uint32_t v[N];
