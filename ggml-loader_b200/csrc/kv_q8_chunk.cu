@@ -182,14 +182,21 @@ __device__ __forceinline__ void add_mask(const AttendParams &p, int tok, int64_t
     const int64_t base = (int64_t)tok * p.mask_stride + kb;
 #pragma unroll 1
     for (int q = 0; q < 4; q++) {
+        // (at clamped places, so that the loads are in flight together)
+        uint32_t raw[16];
+        const int last = (int)min((int64_t)kSub, p.n_kv - kb) - 1;
+        if (p.mask_f16) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) raw[e] = static_cast<const unsigned short *>(p.mask)[base + min(16 * q + e, last)];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) raw[e] = static_cast<const uint32_t *>(p.mask)[base + min(16 * q + e, last)];
+        }
         float m[16];
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            m[e] = -CUDART_INF_F;
-            if (16 * q + e < nvis)
-                m[e] = p.mask_f16 ? __half2float(static_cast<const __half *>(p.mask)[base + 16 * q + e])
-                                  : static_cast<const float *>(p.mask)[base + 16 * q + e];
-        }
+        for (int e = 0; e < 16; e++)
+            m[e] = 16 * q + e >= nvis ? -CUDART_INF_F
+                   : p.mask_f16 ? __half2float(__ushort_as_half((unsigned short)raw[e])) : __uint_as_float(raw[e]);
         const float sc = q < 2 ? sc0 : sc1;
 #pragma unroll
         for (int qq = 0; qq < 4; qq++) {
