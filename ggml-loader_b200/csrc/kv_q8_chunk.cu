@@ -182,7 +182,8 @@ __device__ __forceinline__ void add_mask(const AttendParams &p, int tok, int64_t
     const int64_t base = (int64_t)tok * p.mask_stride + kb;
 #pragma unroll 1
     for (int q = 0; q < 4; q++) {
-        // (at clamped places, so that the loads are in flight together)
+        // (at clamped places, so that the loads are in flight together: 22 tokens over 44k keys 170 us; each under its
+        // condition they went one after the other, 257 us)
         uint32_t raw[16];
         const int last = (int)min((int64_t)kSub, p.n_kv - kb) - 1;
         if (p.mask_f16) {
