@@ -855,7 +855,7 @@ static int alloc_q8(kv_ctx *ctx)
     if (e != cudaSuccess)
         return fail(KV_E_OOM, "failed to allocate KV cache (%lld rows x %d layers, %.0f MiB requested): %s", (long long)rows,
                     c.n_layer, (double)sets * (double)set / (1024.0 * 1024.0), cudaGetErrorString(e));
-    // (no code or scale is read before it is stored; zeros, so that a row not stored yet reads back as one)
+    // (zeros are a row of zeros at any scale: a row not stored yet reads back as one)
     e = cudaMemset(ctx->q8_mem, 0, (size_t)sets * set);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMemset");
     ctx->q8.resize(c.n_layer);

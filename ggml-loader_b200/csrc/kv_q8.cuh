@@ -10,10 +10,15 @@ namespace q8 {
 constexpr int kBad = -128;   // the code of a value that F16 does not hold as a finite number
 
 // A scale word is the float 2^e, or, for a block with a kBad code, a NaN that
-// keeps e + 127 in its low byte (so a rewound block can be stored again).
+// keeps e + 127 in its low byte (so a rewound block can be stored again).  A
+// block in which nothing was stored holds any word, and may be read under a mask
+// that hides its keys: its exponent is brought into the format's range, so that
+// what is multiplied by the hidden keys' weights of 0 is finite (from other
+// exponents a power of two could be infinite), and zeros are rows of zeros.
 __device__ __forceinline__ int scale_exp(uint32_t w)
 {
-    return (int)((w & 0x7f800000u) == 0x7f800000u ? (w & 0xffu) : w >> 23) - 127;
+    const int e = (int)((w & 0x7f800000u) == 0x7f800000u ? (w & 0xffu) : w >> 23) - 127;
+    return max(kExpMin, min(kExpMax, e));
 }
 
 __device__ __forceinline__ uint32_t scale_word(int e, bool bad)

@@ -568,3 +568,30 @@ def test_captured_steps_replay():
             got.append([t.clone() for t in (out, back, kept, c.w)])
         assert all(torch.equal(x, y) for x, y in zip(*got))
         assert torch.isfinite(got[0][0]).all()
+
+
+@pytest.mark.parametrize("n_new", [1, 5, 12, 40])
+@pytest.mark.parametrize("size", [30000.0, 1.0, 1e-6])
+def test_masked_blocks_in_which_nothing_was_stored(n_new, size):
+    """Blocks whose codes and scale words are whatever the memory held, all of their keys masked with -inf."""
+    h, hq, d, n_past = 40, 40, 64, 2000
+    n_kv = n_past + n_new
+    c = Cache(h, -(-n_kv // B) * B + B, d, weight=True)
+    words = np.array([0, 0x7FFFFFFF, 0x7F800000, 0xFF800000, 0x80000000, 1, 0x7F7FFFFF, 0x7FC000E5, 0x00800000, 0xC1234567], np.uint32)
+    rng = np.random.default_rng(3)
+    mask = torch.zeros(n_new, n_kv)
+    hidden = [b for b in range(n_past // B) if b % 3 == 1]
+    for w, dw in zip(c.words, c.dev[2:]):
+        for j, b in enumerate(hidden):
+            w[:, b] = words[(np.arange(h) + j) % len(words)]
+        dw.copy_(torch.from_numpy(w.view(np.float32)))
+    for b in hidden:
+        mask[:, b * B:(b + 1) * B] = float("-inf")
+    at = 0
+    for b in hidden + [None]:   # the rows between them, and the rest
+        end = n_kv if b is None else b * B
+        k = rng.standard_normal((end - at, h, d)).astype(np.float32)
+        v = (rng.uniform(-1, 1, (end - at, h, d)) * size).astype(np.float32)
+        c.store(at, k, v)
+        at = n_kv if b is None else (b + 1) * B
+    check(c, hq, n_past, n_new, queries(3, n_new, hq, d), mask=mask.cuda())
