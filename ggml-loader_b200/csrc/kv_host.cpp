@@ -1618,13 +1618,21 @@ int kv_forward(kv_ctx *ctx, int64_t n_past, int32_t n_new,
 }
 
 // The same for an 8-bit cache, on an idle device.  Imported rows are stored
-// with the rows behind them in the last block, at their present values, and
-// the other of K and V likewise, at its own: kv_q8_store takes both.
+// with the rows in use behind them in the last block, at their present values,
+// and the other of K and V likewise, at its own: kv_q8_store takes both.  What
+// the buffers hold behind the rows in use (of a rewind, or of another layer
+// before an eviction) has no part in it: there the other of K and V, and the
+// rows between those in use and the imported ones, become zeros, and the
+// weights 0.
 static int rows_io_q8(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0, int64_t nrows, void *host, bool to_host)
 {
-    const kvb::q8::Cache &c = ctx->q8[layer].c;
-    const int64_t width = (int64_t)c.H * c.D;
-    const int64_t end = to_host ? row0 + nrows : (row0 + nrows + KV_Q8_BLOCK - 1) / KV_Q8_BLOCK * KV_Q8_BLOCK, n = end - row0;
+    kv_ctx::Q8Layer &l = ctx->q8[layer];
+    const kvb::q8::Cache &c = l.c;
+    const int64_t width = (int64_t)c.H * c.D, used = std::max(l.used, row0 + nrows);
+    const int64_t from = to_host ? row0 : std::min(row0, l.used);
+    const int64_t end = to_host ? row0 + nrows
+                                : std::min(used, (row0 + nrows + KV_Q8_BLOCK - 1) / KV_Q8_BLOCK * KV_Q8_BLOCK);
+    const int64_t n = end - from, present = to_host ? n : std::min(end, l.used) - from;
     struct Tmp {
         __half *p = nullptr;
         ~Tmp()
@@ -1637,35 +1645,40 @@ static int rows_io_q8(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0, i
         return fail(KV_E_OOM, "row buffer");
     }
     __half *k = tmp.p, *v = tmp.p + n * width, *mine = which == 0 ? k : v;
-    kvb::q8::LoadParams lp{};
-    lp.c = c;
-    lp.k = to_host && which != 0 ? nullptr : k;
-    lp.v = to_host && which == 0 ? nullptr : v;
-    lp.stride = width;
-    lp.row0 = row0;
-    lp.n = n;
-    lp.f16 = lp.vec = 1;
-    KV_CUDA(kvb::q8::launch_load(lp, nullptr));
+    if (present < n) KV_CUDA(cudaMemset(tmp.p, 0, (size_t)(2 * n * width) * sizeof(__half)));
+    if (present > 0) {
+        kvb::q8::LoadParams lp{};
+        lp.c = c;
+        lp.k = to_host && which != 0 ? nullptr : k;
+        lp.v = to_host && which == 0 ? nullptr : v;
+        lp.stride = width;
+        lp.row0 = from;
+        lp.n = present;
+        lp.f16 = lp.vec = 1;
+        KV_CUDA(kvb::q8::launch_load(lp, nullptr));
+    }
     KV_CUDA(cudaStreamSynchronize(nullptr));
     const size_t bytes = (size_t)(nrows * width) * sizeof(__half);
     if (to_host) {
         KV_CUDA(cudaMemcpy(host, mine, bytes, cudaMemcpyDeviceToHost));
         return KV_OK;
     }
-    KV_CUDA(cudaMemcpy(mine, host, bytes, cudaMemcpyHostToDevice));
+    KV_CUDA(cudaMemcpy(mine + (row0 - from) * width, host, bytes, cudaMemcpyHostToDevice));
     kvb::q8::StoreParams sp{};
     sp.c = c;
-    sp.c.weight = nullptr;   // (imported rows keep their weights)
+    sp.c.weight = nullptr;   // (rows in use keep their weights)
     sp.k = k;
     sp.v = v;
     sp.k_stride = sp.v_stride = width;
-    sp.row0 = row0;
+    sp.row0 = from;
     sp.n_new = (int32_t)n;
     sp.f16 = sp.vec = 1;
     KV_CUDA(kvb::q8::launch_store(sp, nullptr));
+    if (c.weight && used > l.used)
+        KV_CUDA(cudaMemset2DAsync(c.weight + l.used, (size_t)c.rows * sizeof(float), 0, (size_t)(used - l.used) * sizeof(float),
+                                  (size_t)c.H, nullptr));
     KV_CUDA(cudaStreamSynchronize(nullptr));
-    kv_ctx::Q8Layer &l = ctx->q8[layer];
-    l.used = std::max(l.used, row0 + nrows);
+    l.used = used;
     return KV_OK;
 }
 

@@ -412,9 +412,16 @@ int kv_q8_evict(const kv_q8_cache *src, int64_t n_rows, int64_t keep, int64_t re
 /* Copy cache rows [row0, row0+nrows) of K (which = 0) or V (which = 1) of
  * `layer` to / from host memory in the reference layout [row][head][dim] F16
  * (this context's heads only; an 8-bit cache's values, exact in F16, or stored
- * as kv_q8_store stores them: the rows before row0 in its block, and the ones
- * behind in the last block, are stored again at the block's scale).  Synchronous.  Used for checking, for the
- * reference's /save-/load style rebuilds and for tests. */
+ * as kv_q8_store stores them: the rows in use before row0 in its block, and
+ * those behind in the last block, are stored again at the block's scale).
+ * Synchronous.  Used for checking, for the reference's /save-/load style
+ * rebuilds and for tests.  On an 8-bit context rows are counted as
+ * kv_layer_rows counts them, and imported rows are in use from then on: those
+ * that were not have weight 0, and zeros in the other of K and V (and, where
+ * row0 lies behind the rows in use, in the rows between) until that is imported
+ * too.  An import does not undo an eviction: positions stay as far from rows as
+ * kv_evict left them, so a session that was saved whole goes into a context of
+ * its own, or one that began again at n_past 0. */
 int kv_export_rows(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0,
                    int64_t nrows, uint16_t *host_dst);
 int kv_import_rows(kv_ctx *ctx, int32_t layer, int32_t which, int64_t row0,

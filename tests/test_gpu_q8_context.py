@@ -300,3 +300,79 @@ def test_auto_sized_context():
     with q8_context(sp) as ctx:
         assert ctx.n_ctx == 3000
         assert ctx.layer_rows(0) == (0, 3008)
+
+
+def exported(ctx, layer, row0, n):
+    return [ctx.export_rows(layer, w, row0, n) for w in (0, 1)]
+
+
+def random_rows(seed, n, h, d, size=1.0):
+    x = np.random.default_rng(seed).standard_normal((n, h, d)) * size
+    return x.astype(np.float16).view(np.uint16)
+
+
+def test_import_after_a_rewind_takes_no_old_row():
+    """What a rewind left behind the rows in use, large values and infinities among them, has no part in an import."""
+    hq, h, d = 4, 2, 64
+    with q8_context(spec(d=d, hq=hq, h=h, layers=1, n_rot=0)) as ctx:
+        big = [x.clone() * 1000.0 for x in inputs(1, 40, hq, h, d)]
+        big[1][25, 3] = float("inf")
+        append(ctx, 0, 0, big)
+        append(ctx, 0, 0, inputs(2, 21, hq, h, d))
+        v = exported(ctx, 0, 0, 21)[1]
+        x = random_rows(3, 21, h, d)
+        ctx.import_rows(0, 0, 0, x)
+        got = exported(ctx, 0, 0, 21)
+        assert np.array_equal(got[0].view(np.float16).astype(np.float64), quantised(x))
+        assert np.array_equal(got[1], v) and ctx.layer_rows(0) == (21, 512)
+        # rows behind those in use: the other of K and V holds zeros there until it is imported
+        y = random_rows(4, 19, h, d)
+        ctx.import_rows(0, 1, 21, y)
+        got = exported(ctx, 0, 0, 40)
+        assert np.array_equal(got[0][:21].view(np.float16).astype(np.float64), quantised(x)) and not got[0][21:].any()
+        both = np.concatenate([v, y])
+        # (row 21's block was stored twice: V's rows before it were codes already)
+        assert np.array_equal(got[1][32:].view(np.float16).astype(np.float64), quantised(both)[32:])
+        assert ctx.layer_rows(0) == (40, 512)
+
+
+def test_import_behind_the_rows_in_use_leaves_zeros_between():
+    hq, h, d = 4, 2, 64
+    with q8_context(spec(d=d, hq=hq, h=h, layers=1, n_rot=0)) as ctx:
+        append(ctx, 0, 0, inputs(1, 200, hq, h, d))
+        append(ctx, 0, 0, inputs(2, 37, hq, h, d))
+        before = exported(ctx, 0, 0, 37)
+        x = random_rows(3, 10, h, d)
+        for w in (0, 1):
+            ctx.import_rows(0, w, 100, x)
+        got = exported(ctx, 0, 0, 110)
+        alone = np.zeros((110, h, d), np.uint16)
+        alone[100:] = x
+        for g, b in zip(got, before):
+            assert np.array_equal(g[:37], b) and not g[37:100].any()
+            assert np.array_equal(g[96:].view(np.float16).astype(np.float64), quantised(alone)[96:])
+        assert ctx.layer_rows(0) == (110, 512)
+
+
+def test_import_after_an_eviction_takes_no_row_or_weight_of_another_layer():
+    hq, h, d = 4, 2, 64
+    sp = spec(d=d, hq=hq, h=h, layers=2, n_rot=0, n_ctx=256)
+    with q8_context(sp, cache_rows=64, track_weights=True) as ctx:
+        out = torch.empty(60, hq * d, device="cuda")
+        for layer, size in ((0, 1.0), (1, 100.0)):
+            q, k, v = inputs(layer, 60, hq, h, d)
+            append(ctx, layer, 0, (q, k * size if layer else k, v * size))
+            ctx.attend(layer, 0, 60, out)
+        ctx.evict(1, 40, 8)
+        ctx.evict(0, 40, 8)            # layer 0 now has the buffers that were layer 1's
+        before = exported(ctx, 0, 0, 40)
+        for w in (0, 1):
+            ctx.import_rows(0, w, 0, before[w])
+        assert all(np.array_equal(a, b) for a, b in zip(exported(ctx, 0, 0, 40), before))
+        x = random_rows(7, 12, h, d)
+        for w in (0, 1):
+            ctx.import_rows(0, w, 40, x)
+        assert ctx.layer_rows(0) == (52, 64)
+        kept = torch.empty(h, 40, dtype=torch.int32, device="cuda")
+        ctx.evict(0, 40, 0, kept)      # the imported rows have no weight, all others some
+        assert kept.tolist() == [list(range(40))] * h
