@@ -324,6 +324,7 @@ struct kv_ctx {
         int64_t used = 0;    // rows in use
         int64_t gone = 0;    // positions less rows: position p is in row p - gone
         int64_t floor = 0;   // rows that n_past cannot go back behind
+        int64_t row(int64_t n_past) const { return n_past == 0 ? 0 : n_past - gone; }   // (from the start: nothing is gone)
     };
     std::vector<Q8Layer> q8;
     kvb::q8::Cache q8_spare{};
@@ -773,7 +774,7 @@ int run_append(kv_ctx *ctx, const Pending &pd)
                      (pd.n_new == 1 || ((pd.q_stride | pd.k_stride | pd.v_stride) & 3) == 0);
     const int rc = launch(ctx, KV_K_APPEND, pd.st, "append kernel", [&] { return kvb::launch_append(ctx->D, vec, p, pd.st); });
     if (rc || !ctx->is_q8()) return rc;
-    return store_new_rows(ctx, pd.layer, pd.n_past - ctx->q8[pd.layer].gone, pd.n_new, pd.st);
+    return store_new_rows(ctx, pd.layer, ctx->q8[pd.layer].row(pd.n_past), pd.n_new, pd.st);
 }
 
 int flush_pending(kv_ctx *ctx)
@@ -1211,6 +1212,25 @@ int kv_append(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new,
                           nullptr, nullptr, nullptr, stream);
 }
 
+// Whether a layer of an 8-bit context takes n_new rows at n_past: next to the
+// rows in use or over the last of them, at rows that the layer has.  (Behind a
+// gap are rows of a rewind or, since kv_evict changes buffers, of another
+// layer.)
+static int q8_room(const kv_ctx *ctx, int layer, int64_t n_past, int n_new)
+{
+    const kv_ctx::Q8Layer &l = ctx->q8[layer];
+    const int64_t row = l.row(n_past);
+    if (n_past > 0 && row < l.floor)
+        return fail(KV_E_RANGE, "position %lld of layer %d lies among evicted rows", (long long)n_past, layer);
+    if (row > l.used)
+        return fail(KV_E_RANGE, "position %lld of layer %d leaves a gap: its next position is %lld", (long long)n_past, layer,
+                    (long long)(l.used + l.gone));
+    if (row > ctx->rows - n_new)
+        return fail(KV_E_RANGE, "rows [%lld, %lld) exceed the %lld of layer %d: kv_evict makes room", (long long)row,
+                    (long long)(row + n_new), (long long)ctx->rows, layer);
+    return KV_OK;
+}
+
 int kv_append_bias(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new,
                    const float *q, int64_t q_stride, const float *k, int64_t k_stride,
                    const float *v, int64_t v_stride, const float *q_norm_w, const float *k_norm_w,
@@ -1235,15 +1255,11 @@ int kv_append_bias(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new,
     int rc = ensure_device(ctx);
     if (rc) return rc;
     if (ctx->is_q8()) {
+        rc = q8_room(ctx, layer, n_past, n_new);
+        if (rc) return rc;
         kv_ctx::Q8Layer &l = ctx->q8[layer];
-        const int64_t gone = n_past == 0 ? 0 : l.gone, row = n_past - gone;
-        if (n_past > 0 && row < l.floor)
-            return fail(KV_E_RANGE, "position %lld of layer %d lies among evicted rows", (long long)n_past, layer);
-        if (row > ctx->rows - n_new)
-            return fail(KV_E_RANGE, "rows [%lld, %lld) exceed the layer's %lld: kv_evict makes room", (long long)row,
-                        (long long)(row + n_new), (long long)ctx->rows);
         if (n_past == 0) l.gone = l.floor = 0;
-        l.used = row + n_new;
+        l.used = l.row(n_past) + n_new;
     }
     rc = flush_pending(ctx);
     if (rc) return rc;

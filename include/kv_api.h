@@ -121,8 +121,9 @@ typedef struct kv_config {
  * 8-bit caches (cache_type KV_CACHE_Q8): the calls below are the same; kv_append
  * rotates and norms as it does for F16 and stores the F16 rows' codes, kv_attend
  * is kv_q8_attend's operator (queries rounded to F16, F32 out; the default and
- * the flash-attn branch differ only in a row without a visible key).  One
- * shard, no ring.
+ * the flash-attn branch differ only in a row without a visible key).  A layer's
+ * positions have no gaps: kv_append refuses an n_past beyond the next one
+ * (KV_E_RANGE).  One shard, no ring.
  *
  * Ring caches (ring_cells > 0; dory's sliding and global rings, one context
  * per ring size, per-loop slots as extra layers): kv_append's n_past is the

@@ -376,3 +376,34 @@ def test_import_after_an_eviction_takes_no_row_or_weight_of_another_layer():
         kept = torch.empty(h, 40, dtype=torch.int32, device="cuda")
         ctx.evict(0, 40, 0, kept)      # the imported rows have no weight, all others some
         assert kept.tolist() == [list(range(40))] * h
+
+
+def test_a_gap_in_the_positions_is_refused():
+    """n_past beyond the rows in use: on a fresh context, after a rewind, and after an eviction."""
+    hq, h, d = 4, 2, 64
+    sp = spec(d=d, hq=hq, h=h, layers=1, n_rot=0, n_ctx=256)
+    with q8_context(sp, cache_rows=128, track_weights=True) as ctx:
+        out = torch.empty(60, hq * d, device="cuda")
+
+        def refused(n_past, n=1):
+            before = ctx.layer_rows(0)
+            with pytest.raises(K.KvError) as e:
+                append(ctx, 0, n_past, inputs(9, n, hq, h, d))
+            assert e.value.code == K.KV_E_RANGE and ctx.layer_rows(0) == before
+
+        refused(1)
+        refused(40, 5)
+        append(ctx, 0, 0, inputs(1, 60, hq, h, d))
+        ctx.attend(0, 0, 60, out)
+        refused(61)
+        append(ctx, 0, 10, inputs(2, 1, hq, h, d))   # a rewind: rows 11 to 59 are no longer in use
+        refused(12)
+        refused(60)
+        ctx.attend(0, 10, 1, out)                     # (a refused call leaves the one before it as it was)
+        append(ctx, 0, 11, inputs(2, 49, hq, h, d))
+        ctx.attend(0, 11, 49, out)
+        ctx.evict(0, 32, 8)
+        refused(61)
+        append(ctx, 0, 60, inputs(3, 1, hq, h, d))
+        ctx.attend(0, 60, 1, out)
+        assert ctx.layer_rows(0) == (33, 128) and torch.isfinite(out).all()
