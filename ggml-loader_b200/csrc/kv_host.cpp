@@ -1257,9 +1257,6 @@ int kv_append_bias(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new,
     if (ctx->is_q8()) {
         rc = q8_room(ctx, layer, n_past, n_new);
         if (rc) return rc;
-        kv_ctx::Q8Layer &l = ctx->q8[layer];
-        if (n_past == 0) l.gone = l.floor = 0;
-        l.used = l.row(n_past) + n_new;
     }
     rc = flush_pending(ctx);
     if (rc) return rc;
@@ -1283,7 +1280,17 @@ int kv_append_bias(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new,
         ctx->pend = pd;
         return KV_OK;
     }
-    return run_append(ctx, pd);
+    rc = run_append(ctx, pd);
+    if (ctx->is_q8()) {   // (the rows are in use once their kernels are on the stream)
+        kv_ctx::Q8Layer &l = ctx->q8[layer];
+        if (rc == KV_OK) {
+            if (n_past == 0) l.gone = l.floor = 0;
+            l.used = l.row(n_past) + n_new;
+        } else {
+            ctx->last_layer = -1;
+        }
+    }
+    return rc;
 }
 
 namespace {

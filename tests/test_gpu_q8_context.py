@@ -407,3 +407,55 @@ def test_a_gap_in_the_positions_is_refused():
         append(ctx, 0, 60, inputs(3, 1, hq, h, d))
         ctx.attend(0, 60, 1, out)
         assert ctx.layer_rows(0) == (33, 128) and torch.isfinite(out).all()
+
+
+FAILED_APPEND = """
+import ctypes, sys
+import torch
+import kv_b200 as K
+sp = dict(n_layer=1, n_head=4, n_head_kv=2, head_dim=64, n_rot=0, n_ctx=256)
+ctx = K.Context(K.make_config(sp, cache_type=K.KV_CACHE_Q8, track_weights=True))
+x = torch.randn(40, 8 * 64, device="cuda")
+def append(n_past, n, s=None):
+    ctx.append(0, n_past, n, x, 512, x[:, 256:], 512, x[:, 384:], 512, stream=s)
+append(0, 40)
+ctx.evict(0, 20, 8)
+out = torch.empty(1, 256, device="cuda")
+s = torch.cuda.Stream()
+torch.cuda.synchronize()
+rt = ctypes.CDLL("libcudart.so.12")
+# a capture that an unsupported call has ended: the runtime refuses every launch into its stream
+assert rt.cudaStreamBeginCapture(ctypes.c_void_p(s.cuda_stream), 0) == 0
+assert rt.cudaDeviceSynchronize() != 0
+for n_past in (40, 0):
+    try:
+        append(n_past, 1, s)
+        sys.exit("not refused")
+    except K.KvError as e:
+        assert e.code == K.KV_E_CUDA, e
+    assert ctx.layer_rows(0)[0] == 20
+    try:
+        ctx.attend(0, n_past, 1, out)
+        sys.exit("attend after a failed append")
+    except K.KvError as e:
+        assert e.code == K.KV_E_STATE, e
+g = ctypes.c_void_p()
+rt.cudaStreamEndCapture(ctypes.c_void_p(s.cuda_stream), ctypes.byref(g))
+rt.cudaGetLastError()
+append(40, 1, s)
+ctx.attend(0, 40, 1, out, stream=s)
+s.synchronize()
+assert ctx.layer_rows(0)[0] == 21 and torch.isfinite(out).all()
+print("fine")
+"""
+
+
+def test_an_append_that_fails_changes_nothing():
+    """In a process of its own, whose runtime refuses the launch."""
+    import os
+    import subprocess
+    import sys
+    path = os.path.dirname(os.path.dirname(os.path.abspath(K.__file__)))
+    r = subprocess.run([sys.executable, "-c", FAILED_APPEND], env=dict(os.environ, PYTHONPATH=path), capture_output=True, text=True,
+                       timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "fine", r.stdout + r.stderr
