@@ -1398,8 +1398,9 @@ int prefill(kv_ctx *ctx, const CUtensorMap &km, const CUtensorMap &vm, const CUt
 
 }  // namespace
 
-// kv_attend over an 8-bit layer: the rows in use, the new ones the last of them
-static int attend_q8(kv_ctx *ctx, int32_t layer, int32_t n_new, const MaskArg &mk, float *out, cudaStream_t st)
+// kv_attend over an 8-bit layer: the rows up to the last one of its kv_append
+// (an import since then may have put more in use)
+static int attend_q8(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new, const MaskArg &mk, float *out, cudaStream_t st)
 {
     const int64_t D = ctx->D;
     kvb::q8::AttendParams p{};
@@ -1407,8 +1408,8 @@ static int attend_q8(kv_ctx *ctx, int32_t layer, int32_t n_new, const MaskArg &m
     p.Hq = ctx->hq_loc;
     p.r = ctx->r;
     p.n_new = n_new;
-    p.n_kv = ctx->q8[layer].used;
-    p.n_past = p.n_kv - n_new;
+    p.n_past = ctx->q8[layer].row(n_past);
+    p.n_kv = p.n_past + n_new;
     p.q = ctx->qbuf;
     p.q_stride = p.out_stride = ctx->hq_loc * D;
     p.q_f16 = p.q_vec = 1;
@@ -1437,7 +1438,7 @@ static int attend_impl(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new
     if (rc) return rc;
     const kv_config &c = ctx->cfg;
     const cudaStream_t st = to_stream(stream);
-    if (ctx->is_q8()) return attend_q8(ctx, layer, n_new, mk_in, out, st);
+    if (ctx->is_q8()) return attend_q8(ctx, layer, n_past, n_new, mk_in, out, st);
     // the deferred single-token append runs inside the attention kernels when it
     // belongs to this call and stream; otherwise it is performed now
     const bool fused = ctx->pend.on && ctx->pend.layer == layer && ctx->pend.n_past == n_past &&

@@ -459,3 +459,23 @@ def test_an_append_that_fails_changes_nothing():
     r = subprocess.run([sys.executable, "-c", FAILED_APPEND], env=dict(os.environ, PYTHONPATH=path), capture_output=True, text=True,
                        timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "fine", r.stdout + r.stderr
+
+
+def test_attend_after_an_import_of_more_rows():
+    """kv_attend goes over the rows up to its kv_append's last one, whatever was imported behind them."""
+    sp = spec(d=64, hq=4, h=2, layers=1, n_rot=0)
+    for n_past, n_new in ((0, 5), (30, 1), (30, 20)):
+        outs = []
+        with q8_context(sp) as a, K.Context(K.make_config(sp)) as b:
+            if n_past:
+                append(a, 0, 0, inputs(1, n_past, 4, 2, 64))
+            new = inputs(2, n_new, 4, 2, 64)
+            append(a, 0, n_past, new)
+            append(b, 0, n_past, new)
+            for w in (0, 1):
+                a.import_rows(0, w, n_past + n_new, random_rows(w, 90, 2, 64, 3.0))
+                b.import_rows(0, w, 0, a.export_rows(0, w, 0, n_past + n_new + 90))
+            for ctx in (a, b):
+                outs.append(torch.empty(n_new, 4 * 64, device="cuda"))
+                ctx.attend(0, n_past, n_new, outs[-1])
+            close(*outs)
