@@ -1629,6 +1629,12 @@ int kv_forward(kv_ctx *ctx, int64_t n_past, int32_t n_new,
                float *out, int64_t out_layer_stride, void *stream)
 {
     if (!ctx) return fail(KV_E_ARG, "NULL context");
+    // a layer without room is found before the first one adds to its weights
+    if (ctx->is_q8() && n_past >= 0 && n_new > 0)
+        for (int l = 0; l < ctx->cfg.n_layer; l++) {
+            const int rc = q8_room(ctx, l, n_past, n_new);
+            if (rc) return rc;
+        }
     for (int l = 0; l < ctx->cfg.n_layer; l++) {
         const int64_t io = (int64_t)l * in_layer_stride;
         const int64_t no = (int64_t)l * norm_layer_stride;

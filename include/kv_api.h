@@ -248,7 +248,9 @@ int kv_attend_mask(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new,
  * kv_append then kv_attend with inputs at q + l*in_layer_stride (likewise k,
  * v), gammas at q_norm_w + l*norm_layer_stride, output at
  * out + l*out_layer_stride.  The per-layer loop of forward_step
- * (model.cpp:1318, 1496-1597) restricted to this path, driven from C++.
+ * (model.cpp:1318, 1496-1597) restricted to this path, driven from C++.  On an
+ * 8-bit context a layer without room (KV_E_RANGE) is found before the first
+ * layer's work, so the call can be made again after kv_evict.
  */
 int kv_forward(kv_ctx *ctx, int64_t n_past, int32_t n_new,
                const float *q, int64_t q_stride,

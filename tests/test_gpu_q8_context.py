@@ -479,3 +479,24 @@ def test_attend_after_an_import_of_more_rows():
                 outs.append(torch.empty(n_new, 4 * 64, device="cuda"))
                 ctx.attend(0, n_past, n_new, outs[-1])
             close(*outs)
+
+
+def test_forward_refuses_before_the_first_layer():
+    """A layer without room: no layer's rows or weights change, so the call can be made again after kv_evict."""
+    hq, h, d = 4, 2, 64
+    sp = spec(d=d, hq=hq, h=h, layers=2, n_rot=0, n_ctx=256)
+    with q8_context(sp, cache_rows=64, track_weights=True) as ctx:
+        out = torch.empty(2, 64, hq * d, device="cuda")
+        for layer in (0, 1):
+            append(ctx, layer, 0, inputs(layer, 64, hq, h, d))
+            ctx.attend(layer, 0, 64, out[layer])
+        ctx.evict(0, 48, 8)
+        q, k, v = inputs(5, 4, hq, h, d)
+        args = (64, 4, q, q.stride(0), k, k.stride(0), v, v.stride(0), 0, None, None, 0, out, out.stride(0))
+        with pytest.raises(K.KvError) as e:
+            ctx.forward(*args)
+        assert e.value.code == K.KV_E_RANGE
+        assert ctx.layer_rows(0) == (48, 64) and ctx.layer_rows(1) == (64, 64)
+        ctx.evict(1, 48, 8)
+        ctx.forward(*args)
+        assert ctx.layer_rows(0) == (52, 64) and ctx.layer_rows(1) == (52, 64)
