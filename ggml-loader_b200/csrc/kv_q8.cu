@@ -127,8 +127,8 @@ __global__ void __launch_bounds__(kBlock *D / 8) store_kernel(const StoreParams 
     float *scale = (is_v ? p.c.v_scale : p.c.k_scale) + (int64_t)h * (p.c.rows / kBlock) + blk;
     float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     int e0 = 0;
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     if (fresh) {
         const int64_t at = (row - p.row0) * (is_v ? p.v_stride : p.k_stride) + h * D + c;
         load8<F16>(is_v ? p.v : p.k, at, p.vec, x);
@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadParams p)
     uint2 w[U];
     uint32_t s[U];
     int64_t at[U];
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
 #pragma unroll
     for (int k = 0; k < U; k++) {
         const uint32_t j = base + threadIdx.x + 256 * k, dt = j / pieces, c = j - dt * pieces;
@@ -332,9 +332,9 @@ __global__ void __cluster_dims__(kSelCtas, 1, 1) __launch_bounds__(kSelThreads) 
     const int lo = (int)min((int64_t)cand, (int64_t)rank * per), n = min(per, cand - lo);
     const bool held = per <= kSelSlice;
     for (int i = tid; i < 3 * kSelBins; i += kSelThreads) s_mine[i] = 0;
-    pdl_launch_dependents();
     cluster_sync_all();   // (counts may come in)
     pdl_wait();
+    pdl_launch_dependents();
     for (int64_t j = (int64_t)rank * kSelThreads + tid; j < p.recent; j += kSelCtas * kSelThreads)
         kept[take + j] = cand + (int32_t)j;
     if (take == 0) return;   // (the whole cluster)
@@ -460,8 +460,8 @@ __global__ void __launch_bounds__(kBlock *D / 16, 1536 / (kBlock * D / 16)) gath
     const int64_t row = (int64_t)blockIdx.x * kBlock + r;
     uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
     int e0[2] = {kExpMin, kExpMin};
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     const bool used = row < p.keep;
     if (used) {
         const int64_t from = p.kept[(int64_t)h * p.keep + row], at = ((int64_t)h * p.src.rows + from) * D + c;

@@ -54,7 +54,10 @@ __device__ __forceinline__ uint2 codes_to_half4(uint32_t w)
 }
 
 // A launch that may begin its set-up while the kernel before it in the stream
-// ends; every kernel launched so waits (pdl_wait) before it touches memory.
+// ends; every kernel launched so waits (pdl_wait) before it touches memory, and
+// lets the next one start (pdl_launch_dependents) only then, so that a kernel
+// that starts early may rely on all kernels older than the one before it: the
+// F16 cache's decode kernel does (kv_attend.cu).
 template <class K, class P>
 cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, const P &p, cudaStream_t st, unsigned cluster = 0)
 {

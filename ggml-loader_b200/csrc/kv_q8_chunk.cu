@@ -317,8 +317,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     const uint32_t tmem = *tm_slot;
     Walk w;
     w.begin(p, cta);
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
 
     if (warp < 4) {
         regs_dec<96>();
@@ -687,7 +687,6 @@ __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
     constexpr int rows_blk = 128 * CL<D>::NT;
     constexpr float unit = MASKED ? kLog2e : 1.0f;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_launch_dependents();
     constexpr int rows_cta = WIDE ? 1 : 8;
     const int pair = blockIdx.x / (rows_blk / rows_cta), in = blockIdx.x % (rows_blk / rows_cta) * rows_cta + (WIDE ? 0 : warp);
     const int h = pair / p.n_blk, b = pair % p.n_blk, tk = (in & 127) / p.r, hd = (in & 127) - tk * p.r;
@@ -702,6 +701,7 @@ __global__ void __launch_bounds__(256) fold_kernel(const AttendParams p)
         c1 = (int)(((x1 + 1) * p.n_cta - 1) / W);
     }
     pdl_wait();
+    pdl_launch_dependents();
     if (c0 == c1 || tk >= p.tok_tile || tok >= p.n_new) return;
     constexpr int V = (D / 4 + 31) / 32;
     float4 x[V];

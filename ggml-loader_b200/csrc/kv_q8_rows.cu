@@ -233,7 +233,6 @@ __global__ void __launch_bounds__(W * 32, 1) rows_kernel(const AttendParams p)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     char *ring = smem + warp * G::ring;
     const int64_t T = (int64_t)p.n_vh * p.nb, lo = blockIdx.x * T / p.n_cta, hi = (blockIdx.x + 1) * T / p.n_cta;
-    pdl_launch_dependents();
     if (threadIdx.x < 2 && lo < hi) {
         // While the kernel before this one ends, HBM brings the CTA's first codes
         // to L2 (a hint: what that kernel still writes is read anew below).
@@ -267,8 +266,11 @@ __global__ void __launch_bounds__(W * 32, 1) rows_kernel(const AttendParams p)
             const int row = row_of<DUP>(t4, i);
             tok[i] = row < nrows ? row / p.r : 0;
         }
-        if (!waited) pdl_wait();   // (nothing before it reads memory)
-        waited = true;
+        if (!waited) {   // (nothing before it reads memory)
+            pdl_wait();
+            pdl_launch_dependents();
+            waited = true;
+        }
 
         // The small loads first: behind the ring's they would wait for all of them.
         // the scale words of this warp's next 32 blocks, one a lane
@@ -593,7 +595,6 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
     constexpr float unit = MASKED ? kLog2e : 1.0f;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int R = p.n_new * p.r, n_join = p.n_vh * R;
-    pdl_launch_dependents();
     if ((int)blockIdx.x < n_join) {
         __shared__ float4 s_o[4][D / 4];
         __shared__ float2 s_ml[4];
@@ -603,6 +604,7 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
         const int t = row / p.r;
         const int64_t out = t * p.out_stride + (int64_t)(h * p.r + row - t * p.r) * D;
         pdl_wait();
+        pdl_launch_dependents();
         if (a == b) return;   // rows_kernel wrote the output
         constexpr int V = (D / 4 + 31) / 32;
         float4 x[V];
@@ -682,6 +684,7 @@ __global__ void __launch_bounds__(128) join_kernel(const AttendParams p)
     const int64_t pitch = (int64_t)p.nb * kBlock;
     const int row = tid >> 3, sub = tid & 7;
     pdl_wait();
+    pdl_launch_dependents();
     // all that is read, on its way at once: the first rows' scores, the weights so far, the parts' (m, l)
     constexpr int kAhead = 4, kParts = 3;
     float4 x[kAhead];

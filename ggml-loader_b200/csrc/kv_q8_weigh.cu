@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
     const uint32_t tmem = *tm_slot;
     Steps<NK> w;
     w.begin(p, blockIdx.x, gridDim.x);
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     auto wait = [&](uint64_t *b, uint32_t par) {
         if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
         give_up(p.error, flag, 8u);

@@ -500,3 +500,36 @@ def test_forward_refuses_before_the_first_layer():
         ctx.evict(1, 48, 8)
         ctx.forward(*args)
         assert ctx.layer_rows(0) == (52, 64) and ctx.layer_rows(1) == (52, 64)
+
+
+@pytest.mark.parametrize("n_new", [1, 3, 40])
+def test_an_f16_and_an_8_bit_context_in_turn_on_one_stream(n_new):
+    """Each step's kernels start while the other context's end; the bits are those of each context alone."""
+    sp = spec(layers=2, n_ctx=1200)
+    hq, h, d = 8, 2, 128
+    steps = [(0, 700), (700, 1), (701, n_new), (701 + n_new, 1), (702 + n_new, 30), (732 + n_new, 1)]
+    rows = [[inputs(10 * i + l, n, hq, h, d) for l in range(2)] for i, (_, n) in enumerate(steps)]
+
+    def run(contexts):
+        outs = [[torch.full((n, hq * d), 7.0, device="cuda") for _, n in steps for _ in range(2)] for _ in contexts]
+        torch.cuda.synchronize()
+        for i, (n_past, n) in enumerate(steps):
+            for l in range(2):
+                for ctx, out in zip(contexts, outs):
+                    append(ctx, l, n_past, rows[i][l])
+                    ctx.attend(l, n_past, n, out[2 * i + l])
+        torch.cuda.synchronize()
+        return outs
+
+    def contexts():
+        return K.Context(K.make_config(sp, n_batch_max=700)), q8_context(sp, n_batch_max=700)
+
+    a, b = contexts()
+    with a, b:
+        want = run([a]) + run([b])
+    for _ in range(3):
+        f16, q8 = contexts()
+        with f16, q8:
+            got = run([f16, q8])
+        for x, y in zip(got, want):
+            assert all(torch.equal(s, t) for s, t in zip(x, y))

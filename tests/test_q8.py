@@ -245,3 +245,26 @@ def test_the_binding_refuses_other_rows():
         with pytest.raises(ValueError):
             calls.evict(ref, -1, 2, 100, 5, 1, ctypes.addressof(d), dev, x, None)
     assert calls.evict(ref, -1, 2, 2000, 5, 1, ctypes.addressof(d), -1, kept, None) == K.KV_E_RANGE
+
+
+# ---- the kernels' launches ------------------------------------------------------
+def test_every_kernel_lets_the_next_one_start_after_its_own_wait():
+    """A kernel that starts early may rely on every kernel older than the one before it (the decode attention kernel's first
+    tile loads do): that holds where each kernel triggers its dependents only once its own wait is over."""
+    import glob
+    import os
+    import re
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(K.__file__))), "csrc")
+    seen = 0
+    for path in sorted(glob.glob(os.path.join(csrc, "*.cu"))):
+        with open(path) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        for kernel in re.split(r"__global__", text)[1:]:
+            name = re.search(r"(\w+)\s*\(const \w+", kernel)
+            triggers = [m.start() for m in re.finditer(r"pdl_launch_dependents\(\)", kernel)]
+            waits = [m.start() for m in re.finditer(r"pdl_wait\(\)", kernel)]
+            for i, t in enumerate(triggers):
+                # between one trigger and the next (branches of the kernel) there is a wait
+                assert any((triggers[i - 1] if i else 0) <= w < t for w in waits), (path, name and name.group(1))
+            seen += len(triggers)
+    assert seen >= 10
