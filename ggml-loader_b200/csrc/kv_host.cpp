@@ -1420,8 +1420,11 @@ static int attend_q8(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new, 
     p.out = out;
     p.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0;
     p.scale = ctx->scale;
+    p.limit_ns = ctx->limit_ns;
     if (mk.ptr && mk.stride < p.n_kv)
         return fail(KV_E_ARG, "mask_stride %lld < the %lld keys attended", (long long)mk.stride, (long long)p.n_kv);
+    p.inject = ctx->inject;
+    ctx->inject = 0;
     return launch(ctx, n_new * ctx->r > 16 ? KV_K_PREFILL : KV_K_ATTN, st, "8-bit attention kernels",
                   [&] { return kvb::q8::launch_attend(p, ctx->q8_ws, st); });
 }
@@ -1843,8 +1846,8 @@ int kv_status(kv_ctx *ctx, void *stream)
 int kv_debug_inject(kv_ctx *ctx, int32_t what, uint64_t limit_ns)
 {
     if (!ctx) return fail(KV_E_ARG, "NULL context");
-    if (what != 0 && what != 1) return fail(KV_E_ARG, "unknown injection %d", what);
-    if (ctx->is_q8()) return fail(KV_E_UNSUPPORTED, "kv_debug_inject: the F16 cache's kernels only");
+    if (what < 0 || what > (ctx->is_q8() ? 3 : 1))
+        return fail(KV_E_ARG, "unknown injection %d", what);
     ctx->inject = what;
     if (limit_ns) ctx->limit_ns = limit_ns;
     return KV_OK;

@@ -12,6 +12,7 @@ namespace q8 {
 
 constexpr int kBlock = 32;   // rows that share a scale (KV_Q8_BLOCK)
 constexpr int kSMs = 148;    // the most CTAs a split uses
+constexpr uint64_t kLimitNs = 1000000000ull;   // AttendParams::limit_ns of a call on the caller's buffers: 1 s
 constexpr int kExpMin = -24, kExpMax = 9;   // a scale is 2^e with e in this range
 
 struct Cache {
@@ -83,6 +84,8 @@ struct AttendParams {
     float2 *row_stat;       // [H][n_new * r] (maximum, 1 / sum or 0) or null
     int32_t n_kt;           // weigh: a KV head's items of 128 or 256 keys
     unsigned *error;        // the device's record of waits that expired
+    uint64_t limit_ns;      // bound of every wait in the chunk's and the weights' kernels
+    int32_t inject;         // test hook (kv_debug_inject): which wait's partner stays away
 };
 // bytes of workspace (a function of the sizes alone)
 uint64_t attend_workspace(const AttendParams &p);

@@ -302,7 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const bool staged = b == q_full || (b >= k_full && b < k_full + KS) || (b >= v_full && b < v_full + VS) ||
                                 b >= raw_empty;   // the four staging warps
             const bool both = b == q_empty || (b >= k_empty && b < k_empty + KS);   // both S issuers
-            mbar_init(&bar[i], staged || (b >= p_full && b < p_full + 4) ? 4 : b == o_empty ? 8 : both ? 2 : 1);
+            const bool stays_away = p.inject == 1 && b == raw_full + 1;   // test hook: one arrival too many is waited for
+            mbar_init(&bar[i], (staged || (b >= p_full && b < p_full + 4) ? 4 : b == o_empty ? 8 : both ? 2 : 1) + stays_away);
         }
         *flag = 0;
         fence_mbar_init();
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
 #pragma unroll
                     for (int v = 0; v < 2; v++, u++) {
                         const int s = u % L::RS;
-                        if (u >= L::RS && !mbar_wait_ab(&raw_empty[s], (u / L::RS - 1) & 1, kLimitNs, flag)) {
+                        if (u >= L::RS && !mbar_wait_ab(&raw_empty[s], (u / L::RS - 1) & 1, p.limit_ns, flag)) {
                             give_up(p.error, flag, 2u);
                             ok = false;
                             break;
@@ -346,12 +347,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                 }
             }
             // none may land after the CTA has gone
-            for (int x = u > L::RS ? u - L::RS : 0; x < u; x++) mbar_wait(&raw_full[x % L::RS], (x / L::RS) & 1, kLimitNs);
+            for (int x = u > L::RS ? u - L::RS : 0; x < u; x++) mbar_wait(&raw_full[x % L::RS], (x / L::RS) & 1, p.limit_ns);
         } else if (lane == 0) {
             constexpr uint32_t idS = idesc_f16_f32(128, kSub, false), idO = idesc_f16_f32(128, D, true);
             const uint32_t sq = smem_addr(smem + L::o_q), sk = smem_addr(smem + L::o_k), sv = smem_addr(smem + L::o_v);
             auto wait = [&](uint64_t *b, uint32_t par) {
-                if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
+                if (mbar_wait_ab(b, par, p.limit_ns, flag)) return true;
                 give_up(p.error, flag, 1u);
                 return false;
             };
@@ -415,14 +416,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             }
             // every MMA of this thread has completed before TMEM is freed
             umma_commit(&drain[warp]);
-            mbar_wait(&drain[warp], 0, kLimitNs);
+            mbar_wait(&drain[warp], 0, p.limit_ns);
         }
     } else if (warp < 8) {
         regs_dec<80>();
         const int st = tid - 128;
         auto wait = [&](uint64_t *b, uint32_t par) {
             // (one answer for the warp: its lanes arrive together)
-            const bool got = mbar_wait_ab(b, par, kLimitNs, flag);
+            const bool got = mbar_wait_ab(b, par, p.limit_ns, flag);
             if (!__all_sync(0xffffffffu, got)) {
                 give_up(p.error, flag, 2u);
                 return false;
@@ -437,15 +438,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const int s = u % L::RS;
             if (!wait(&raw_full[s], (u / L::RS) & 1)) return false;
             u++;
-            uint4 c[L::n_ld];
+            constexpr int N = L::n_ld > 4 ? 4 : L::n_ld;   // pieces at a time (8: registers spilled)
+            uint4 c[N];
             const uint4 *src = reinterpret_cast<const uint4 *>(smem + L::o_raw + s * L::unit);
 #pragma unroll
-            for (int j = 0; j < L::n_ld; j++) c[j] = src[st + 128 * j];
+            for (int j = 0; j < N; j++) c[j] = src[st + 128 * j];
             if (used && !wait(empty, par)) return false;
 #pragma unroll
-            for (int j = 0; j < L::n_ld; j++) {
-                const int x = st + 128 * j;
-                store_codes(smem_addr(tile), L::box, x / (D / 16), x % (D / 16), c[j]);
+            for (int j0 = 0; j0 < L::n_ld; j0 += N) {
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    const int x = st + 128 * (j0 + j);
+                    store_codes(smem_addr(tile), L::box, x / (D / 16), x % (D / 16), c[j]);
+                    if (j0 + N < L::n_ld) c[j] = src[x + 128 * N];
+                }
             }
             fence_async_smem();
             __syncwarp();
@@ -455,10 +461,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             }
             return true;
         };
-        for (int seg = 0; ok && w.more(); seg++, w.next_pair(p)) {
+        for (int seg = 0; w.more(); seg++, w.next_pair(p)) {
             const int h = w.pair / p.n_blk, b = w.pair % p.n_blk, nt = tiles_of(p, b);
-            if (seg > 0 && !(ok = wait(q_empty, (seg - 1) & 1))) break;
-            named_sync(1, 128);   // (the tiles before have been staged)
+            if (seg > 0 && ok) ok = wait(q_empty, (seg - 1) & 1);
+            // the tiles before have been staged; a warp that gave up comes here too, and all four leave together
+            if (named_sync_or(1, 128, !ok)) break;
             const int tk = st / p.r, in = st - tk * p.r;
 #pragma unroll
             for (int g = 0; g < L::NT; g++) {
@@ -471,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(q_full);
-            for (int t = w.t0; t < w.t1; t++, i++) {
+            for (int t = w.t0; t < w.t1; t++, i++) {   // (a warp that gives up here goes on to the next segment's barrier)
                 const int ks = i % KS, vs = i % VS;
                 if (!(ok = convert(smem + L::o_k + ks * L::tile, &k_full[ks], &k_empty[ks], i >= KS, (i / KS - 1) & 1))) break;
                 if (!(ok = convert(smem + L::o_v + vs * L::tile, &v_full[vs], &v_empty[vs], i >= VS, (i / VS - 1) & 1))) break;
@@ -485,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
         const uint32_t tS = tmem + lanes + g * 128, tO = tmem + lanes + kTmO + g * D;
         const int tok_in = row / p.r, hd = row - tok_in * p.r;
         auto wait = [&](uint64_t *b, uint32_t par) {
-            if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
+            if (mbar_wait_ab(b, par, p.limit_ns, flag)) return true;
             give_up(p.error, flag, 4u);
             return false;
         };

@@ -186,6 +186,7 @@ int kv_q8_attend(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32
     p.out_f16 = out_type == KV_F16;
     p.out_vec = vec_ok(out, p.out_stride, out_type);
     p.scale = 1.0f / sqrtf((float)p.c.D);
+    p.limit_ns = kvb::q8::kLimitNs;
     return cuda_rc(kvb::q8::launch_attend(p, workspace, static_cast<cudaStream_t>(stream)), what);
 }
 

@@ -8,8 +8,6 @@
 namespace kvb {
 namespace q8 {
 
-constexpr uint64_t kLimitNs = 1000000000ull;   // bound of every wait: 1 s
-
 __device__ __forceinline__ void give_up(unsigned *error, volatile int *flag, unsigned bit)
 {
     if (!*flag) {

@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
     int64_t *row_off = reinterpret_cast<int64_t *>(smem + L::o_off);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        mbar_init(k_full, 4);
+        mbar_init(k_full, p.inject == 2 ? 5 : 4);   // (test hook: one arrival too many is waited for)
         mbar_init(k_empty, 1);
         for (int i = 0; i < QS; i++) {
             mbar_init(&q_full[i], 4);
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
     pdl_wait();
     pdl_launch_dependents();
     auto wait = [&](uint64_t *b, uint32_t par) {
-        if (mbar_wait_ab(b, par, kLimitNs, flag)) return true;
+        if (mbar_wait_ab(b, par, p.limit_ns, flag)) return true;
         give_up(p.error, flag, 8u);
         return false;
     };
@@ -293,9 +293,11 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
         const uint32_t sk = smem_addr(smem + L::o_k), sq = smem_addr(smem + L::o_q);
         bool ahead = false;   // `next` holds the numbers of this thread's row of the next tile
         float2 next = make_float2(0.0f, 0.0f);
-        for (int64_t now = -1; ok && w.more(); w.next(p)) {
-            if (w.item != now) {
-                if (items > 0 && !(ok = all_wait(k_empty, (items - 1) & 1))) break;
+        ok = !(p.inject == 3 && warp == kStage);   // (test hook: this warp alone gives up)
+        // (a warp that gave up comes to the barrier below like the others, and all four leave together)
+        for (int64_t now = -1; w.more(); w.next(p)) {
+            if (ok && w.item != now && items > 0) ok = all_wait(k_empty, (items - 1) & 1);
+            if (ok && w.item != now) {
 #pragma unroll
                 for (int j = 0; j < L::n_ld; j++) {
                     const int i = t + 128 * j;
@@ -312,11 +314,11 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
             if (!w.fresh) continue;
             q++;
             const int qs = q % QS;
-            if (q >= QS && !(ok = all_wait(&q_empty[qs], (q / QS - 1) & 1))) break;
+            if (ok && q >= QS) ok = all_wait(&q_empty[qs], (q / QS - 1) & 1);
             const int row0 = w.qt * 128, R = p.n_new * p.r;
             const float2 *stat = p.row_stat + (int64_t)w.h * R + row0;
             int64_t *off = row_off + qs * 128;
-            {
+            if (ok) {
                 // a row that adds nothing has 1 / Z = 0: its queries are zeros, so that its products are finite
                 const float2 y = ahead ? next : row0 + t < R ? stat[t] : make_float2(0.0f, 0.0f);
                 const int tok = (row0 + t) / p.r, j = row0 + t - tok * p.r;
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
                 }
                 off[t] = y.y != 0.0f ? tok * p.q_stride + (int64_t)(w.h * p.r + j) * D : -1;
             }
-            named_sync(1, 128);
+            if (named_sync_or(1, 128, !ok)) break;
             stage_queries<D>(p, sq + qs * L::tile, L::box, off, t);
             cp_async_wait<0>();
             fence_async_smem();
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
             if (w.last()) umma_commit(k_empty);
         }
         umma_commit(drain);
-        mbar_wait(drain, 0, kLimitNs);
+        mbar_wait(drain, 0, p.limit_ns);
     }
     tc_fence_before();
     __syncthreads();

@@ -49,7 +49,10 @@ int64_t kv_launch_count(const kv_ctx *ctx);
 /* Failure injection for tests.  what = 1: in the next decode launch the tile
  * producer withholds one tile, so the consumers' bounded wait expires (the
  * call's output is invalid and kv_status reports KV_E_TIMEOUT; no fault, no
- * hang).  limit_ns > 0 also sets the bound of every device-side wait of this
+ * hang).  On an 8-bit context, for its next kv_attend: 1, the chunk kernel's
+ * second tile never counts as complete; 2, nor do the first keys of the weights'
+ * pass; 3, one of that pass's staging warps gives up by itself, as where its
+ * wait alone expired.  (Few rows have no such waits.)  limit_ns > 0 also sets the bound of every device-side wait of this
  * context (default 1 s); 0 keeps it. */
 int kv_debug_inject(kv_ctx *ctx, int32_t what, uint64_t limit_ns);
 

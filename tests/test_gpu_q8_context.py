@@ -533,3 +533,39 @@ def test_an_f16_and_an_8_bit_context_in_turn_on_one_stream(n_new):
             got = run([f16, q8])
         for x, y in zip(got, want):
             assert all(torch.equal(s, t) for s, t in zip(x, y))
+
+
+def prompt_context(**kw):
+    """More pairs of tiles than CTAs, several query tiles a KV head, weights kept."""
+    hq, h, d = 128, 64, 64
+    sp = spec(d=d, hq=hq, h=h, layers=1, n_rot=0, n_ctx=512)
+    return q8_context(sp, track_weights=True, **kw), inputs(1, 100, hq, h, d), inputs(2, 400, hq, h, d), hq * d
+
+
+def expires(what, limit_ms=100):
+    """A prompt's chunk with an injected failure: its status is a timeout, once, and the next calls are right."""
+    ctx, old, new, width = prompt_context()
+    twin = prompt_context()[0]
+    with ctx, twin:
+        for c in (ctx, twin):
+            append(c, 0, 0, old)
+        append(ctx, 0, 100, new)
+        ctx.debug_inject(what, limit_ns=limit_ms * 1_000_000)
+        ctx.attend(0, 100, 400, torch.empty(400, width, device="cuda"))
+        with pytest.raises(K.KvError) as e:
+            ctx.status()
+        assert e.value.code == K.KV_E_TIMEOUT
+        assert ctx.status() == K.KV_OK
+        ctx.debug_inject(0, limit_ns=1_000_000_000)
+        outs = []
+        for c in (ctx, twin):
+            append(c, 0, 100, new)
+            outs.append(torch.empty(400, width, device="cuda"))
+            c.attend(0, 100, 400, outs[-1])
+            assert c.status() == K.KV_OK
+        assert torch.equal(*outs)
+
+
+def test_a_staging_warp_that_gives_up_alone():
+    """The other three are not left at a barrier that it does not come to."""
+    expires(3)
