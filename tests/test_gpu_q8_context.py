@@ -569,3 +569,17 @@ def expires(what, limit_ms=100):
 def test_a_staging_warp_that_gives_up_alone():
     """The other three are not left at a barrier that it does not come to."""
     expires(3)
+
+
+@pytest.mark.parametrize("what", [1, 2])
+def test_a_wait_that_runs_out(what):
+    """In the chunk's kernel, and in the pass that sums its weights."""
+    expires(what)
+
+
+def test_injections_that_do_not_exist():
+    with q8_context(spec(d=64, hq=4, h=2, layers=1)) as a, K.Context(K.make_config(spec(d=64, hq=4, h=2, layers=1))) as b:
+        for ctx, what in ((a, -1), (a, 4), (b, 2), (b, 3)):
+            with pytest.raises(K.KvError) as e:
+                ctx.debug_inject(what)
+            assert e.value.code == K.KV_E_ARG
