@@ -882,9 +882,12 @@ static int alloc_q8(kv_ctx *ctx)
     const size_t batch = (size_t)c.n_batch_max * (size_t)D * sizeof(__half);
     e = cudaMalloc(&ctx->q8_ws, (size_t)kvb::q8::attend_workspace(p));
     if (e == cudaSuccess) e = cudaMalloc(&ctx->qbuf, batch * (size_t)ctx->hq_loc);
+    if (e == cudaSuccess) e = cudaMalloc(&ctx->err, 2 * sizeof(unsigned));   // (the second: the answer's way to the host)
     if (e == cudaSuccess) e = cudaMalloc(&ctx->q8_new, 2 * batch * (size_t)H);
     if (e == cudaSuccess && weigh) e = cudaMalloc(&ctx->q8_kept, (size_t)(H * rows) * sizeof(int32_t));
     if (e != cudaSuccess) return fail(KV_E_OOM, "scratch allocation: %s", cudaGetErrorString(e));
+    e = cudaMemset(ctx->err, 0, 2 * sizeof(unsigned));
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMemset");
     return KV_OK;
 }
 
@@ -1421,6 +1424,7 @@ static int attend_q8(kv_ctx *ctx, int32_t layer, int64_t n_past, int32_t n_new, 
     p.out_vec = reinterpret_cast<uintptr_t>(out) % 16 == 0;
     p.scale = ctx->scale;
     p.limit_ns = ctx->limit_ns;
+    p.error = ctx->err;
     if (mk.ptr && mk.stride < p.n_kv)
         return fail(KV_E_ARG, "mask_stride %lld < the %lld keys attended", (long long)mk.stride, (long long)p.n_kv);
     p.inject = ctx->inject;
@@ -1829,9 +1833,12 @@ int kv_status(kv_ctx *ctx, void *stream)
     if (rc) return rc;
     rc = flush_pending(ctx);
     if (rc) return rc;
-    if (ctx->is_q8()) return kv_q8_status(stream);
     KV_CUDA(cudaStreamSynchronize(to_stream(stream)));
     unsigned word = 0;
+    if (ctx->is_q8()) {
+        KV_CUDA(kvb::q8::take_error(ctx->err, to_stream(stream), &word));
+        return word == 0 ? KV_OK : fail(KV_E_TIMEOUT, "a device-side wait expired (error word 0x%x); the outputs of that call are invalid", word);
+    }
     KV_CUDA(cudaMemcpy(&word, ctx->err, sizeof(word), cudaMemcpyDeviceToHost));
     if (word == 0) return KV_OK;
     // a CTA that left early never counted itself in: restart the per-head

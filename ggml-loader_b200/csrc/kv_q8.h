@@ -83,7 +83,7 @@ struct AttendParams {
     float *scores;          // [H][n_new * r][nb * kBlock] or null
     float2 *row_stat;       // [H][n_new * r] (maximum, 1 / sum or 0) or null
     int32_t n_kt;           // weigh: a KV head's items of 128 or 256 keys
-    unsigned *error;        // the device's record of waits that expired
+    unsigned *error;        // the record of waits that expired: a context's, or null for the device's
     uint64_t limit_ns;      // bound of every wait in the chunk's and the weights' kernels
     int32_t inject;         // test hook (kv_debug_inject): which wait's partner stays away
 };
@@ -99,9 +99,10 @@ void chunk_split(AttendParams &p);
 cudaError_t launch_chunk(const AttendParams &p, cudaStream_t st);
 // kv_q8_weigh.cu: a chunk's softmax weights into the cache's accumulator
 cudaError_t launch_weigh(const AttendParams &p, cudaStream_t st);
-// the current device's record of waits that expired: its address, and its bits since the last call
+// the current device's record of waits that expired, of calls on the callers' buffers: its address
 cudaError_t error_word(unsigned **dev);
-cudaError_t take_error(unsigned *word);
+// a record's bits since the last call, behind what `st` holds (record: two words, one of them for the answer's way back)
+cudaError_t take_error(unsigned *record, cudaStream_t st, unsigned *word);
 
 // Runs a function once a device (a kernel's attributes last); devices past 63 run it every time.
 struct Once {

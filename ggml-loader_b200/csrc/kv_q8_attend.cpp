@@ -50,7 +50,7 @@ cudaError_t launch_attend(AttendParams p, void *ws, cudaStream_t st)
 {
     lay_out(p, static_cast<char *>(ws));
     if ((int64_t)p.n_new * p.r <= 16) return launch_rows(p, st);
-    cudaError_t e = error_word(&p.error);
+    cudaError_t e = p.error ? cudaSuccess : error_word(&p.error);
     if (e == cudaSuccess) e = launch_chunk(p, st);
     return e != cudaSuccess || !p.row_stat ? e : launch_weigh(p, st);
 }

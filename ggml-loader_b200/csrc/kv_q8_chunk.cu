@@ -40,7 +40,7 @@
 namespace kvb {
 namespace q8 {
 
-__device__ unsigned g_error;
+__device__ unsigned g_error[2];   // the record of calls on the callers' buffers, and what was taken from it last
 
 namespace {
 
@@ -805,6 +805,9 @@ cudaError_t run(const AttendParams &p, cudaStream_t st)
     return launch_pdl(fold_kernel<D, MASKED, false>, (unsigned)p.n_vh * (128 * L::NT / 8), 256, 0, p, st);
 }
 
+// a record's bits, cleared in the same step: one that another stream's kernel sets meanwhile is not lost
+__global__ void take_kernel(unsigned *record) { record[1] = atomicExch(record, 0u); }
+
 }  // namespace
 
 void chunk_split(AttendParams &p)
@@ -850,14 +853,12 @@ cudaError_t error_word(unsigned **dev)
     return e;
 }
 
-cudaError_t take_error(unsigned *word)
+cudaError_t take_error(unsigned *record, cudaStream_t st, unsigned *word)
 {
-    cudaError_t e = cudaMemcpyFromSymbol(word, g_error, sizeof(unsigned));
-    if (e == cudaSuccess && *word) {
-        const unsigned zero = 0;
-        e = cudaMemcpyToSymbol(g_error, &zero, sizeof(unsigned));
-    }
-    return e;
+    take_kernel<<<1, 1, 0, st>>>(record);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaMemcpyAsync(word, record + 1, sizeof(unsigned), cudaMemcpyDeviceToHost, st);
+    return e == cudaSuccess ? cudaStreamSynchronize(st) : e;
 }
 
 }  // namespace q8

@@ -1,8 +1,10 @@
 // kv_q8_host.cpp -- the C entry points of the 8-bit cache (include/kv_api.h):
-// argument checks and launches.  They keep no state and allocate nothing.
+// argument checks and launches.  They allocate nothing and keep no state but
+// the device's record of waits that expired.
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <mutex>
 
 #include "kv_api.h"
 #include "kv_internal.h"
@@ -194,8 +196,13 @@ int kv_q8_status(void *stream)
 {
     const char *what = "kv_q8_status";
     int rc = cuda_rc(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)), what);
-    unsigned word = 0;
-    if (rc == KV_OK) rc = cuda_rc(kvb::q8::take_error(&word), what);
+    unsigned word = 0, *record = nullptr;
+    if (rc == KV_OK) rc = cuda_rc(kvb::q8::error_word(&record), what);
+    if (rc == KV_OK) {
+        static std::mutex one;   // (one word a device for the answer's way back)
+        std::lock_guard<std::mutex> lock(one);
+        rc = cuda_rc(kvb::q8::take_error(record, static_cast<cudaStream_t>(stream), &word), what);
+    }
     if (rc == KV_OK && word)
         return fail(KV_E_TIMEOUT, "%s: a wait in an attention kernel expired (bits 0x%x); its outputs are not valid", what,
                     word);

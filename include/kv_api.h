@@ -396,7 +396,9 @@ int kv_q8_attend(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32
 /* Deferred device-side errors of kv_q8_attend on the current device, as
  * kv_status: waits for `stream`, then returns KV_E_TIMEOUT (and clears the
  * record) if a bounded wait inside one of its kernels expired since the last
- * check (the outputs of that call are not valid), else KV_OK. */
+ * check (the outputs of that call are not valid), else KV_OK.  One record a
+ * device, for all calls of kv_q8_attend there; a kv_ctx has its own, which
+ * kv_status reads. */
 int kv_q8_status(void *stream);
 
 /*

@@ -583,3 +583,23 @@ def test_injections_that_do_not_exist():
             with pytest.raises(K.KvError) as e:
                 ctx.debug_inject(what)
             assert e.value.code == K.KV_E_ARG
+
+
+def test_a_context_s_status_is_its_own():
+    """Neither another 8-bit context nor a caller of the operators takes or sees a context's expired wait."""
+    (a, old, new, width), b = prompt_context(), prompt_context()[0]
+    c = [torch.zeros(2, 64, 64, dtype=torch.int8, device="cuda") for _ in range(2)]
+    direct = K.Q8Cache(*c, *[torch.ones(2, 2, device="cuda") for _ in range(2)])
+    with a, b:
+        for ctx in (a, b):
+            append(ctx, 0, 0, old)
+            append(ctx, 0, 100, new)
+            if ctx is a:
+                a.debug_inject(1, limit_ns=100_000_000)
+            ctx.attend(0, 100, 400, torch.empty(400, width, device="cuda"))
+        assert b.status() == K.KV_OK and direct.status() == K.KV_OK
+        assert direct.status(torch.cuda.Stream()) == K.KV_OK
+        with pytest.raises(K.KvError) as e:
+            a.status()
+        assert e.value.code == K.KV_E_TIMEOUT
+        assert a.status() == K.KV_OK
