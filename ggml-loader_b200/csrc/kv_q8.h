@@ -82,6 +82,7 @@ struct AttendParams {
     float2 *stat;           // [n_cta + n_vh][rows] their (maximum, sum)
     float *scores;          // [H][n_new * r][nb * kBlock] or null
     float2 *row_stat;       // [H][n_new * r] (maximum, 1 / sum or 0) or null
+    unsigned *gave_up;      // [n_cta] whether a wait of the chunk's CTA expired, or null (no weights)
     int32_t n_kt;           // weigh: a KV head's items of 128 or 256 keys
     unsigned *error;        // the record of waits that expired: a context's, or null for the device's
     uint64_t limit_ns;      // bound of every wait in the chunk's and the weights' kernels

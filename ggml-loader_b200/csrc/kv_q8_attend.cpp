@@ -27,8 +27,12 @@ uint64_t lay_out(AttendParams &p, char *ws)
     p.stat = reinterpret_cast<float2 *>(take(slots * sizeof(float2)));
     p.scores = nullptr;
     p.row_stat = nullptr;
+    p.gave_up = nullptr;
     if (p.c.weight && !chunk) p.scores = reinterpret_cast<float *>(take(p.c.H * rows * p.nb * kBlock * sizeof(float)));
-    if (p.c.weight && chunk) p.row_stat = reinterpret_cast<float2 *>(take(p.c.H * rows * sizeof(float2)));
+    if (p.c.weight && chunk) {
+        p.row_stat = reinterpret_cast<float2 *>(take(p.c.H * rows * sizeof(float2)));
+        p.gave_up = reinterpret_cast<unsigned *>(take(kSMs * sizeof(unsigned)));
+    }
     return n;
 }
 

@@ -680,6 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
     if (warp == 3) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+        if (lane == 0 && p.gave_up) p.gave_up[cta] = *flag;
     }
 }
 

@@ -161,6 +161,10 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
         float sum = 0.0f, c = 0.0f;
         int first = 0;   // the first row that sees the thread's key (without a mask)
         int64_t now = -1;
+        // where a wait of the chunk's kernel expired, rows' (m, 1 / Z) are not this call's: nothing is added then
+        unsigned lost = 0;
+        for (int i = lane; i < p.n_cta; i += 32) lost |= p.gave_up[i];
+        const bool keeps = !__any_sync(0xffffffffu, lost);
         for (; ok && w.more(); s++) {
             if (w.fresh) q++;
             const int64_t key = w.key0 + tid;   // (the warps of a tile are in lane order)
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
                 sum += x.x + x.y;
             }
             if (w.last()) {
-                if (in) p.c.weight[(int64_t)w.h * p.c.rows + key] += sum;
+                if (in && keeps) p.c.weight[(int64_t)w.h * p.c.rows + key] += sum;
                 sum = 0.0f;
             }
             w.next(p);

@@ -396,8 +396,9 @@ int kv_q8_attend(const kv_q8_cache *cache, int32_t n_head, int64_t n_past, int32
 /* Deferred device-side errors of kv_q8_attend on the current device, as
  * kv_status: waits for `stream`, then returns KV_E_TIMEOUT (and clears the
  * record) if a bounded wait inside one of its kernels expired since the last
- * check (the outputs of that call are not valid), else KV_OK.  One record a
- * device, for all calls of kv_q8_attend there; a kv_ctx has its own, which
+ * check (the outputs of that call are not valid, and its softmax weights are
+ * added to none of the rows or, where the wait was in the weights' own pass, to
+ * some), else KV_OK.  One record a device, for all calls of kv_q8_attend there; a kv_ctx has its own, which
  * kv_status reads. */
 int kv_q8_status(void *stream);
 
@@ -445,7 +446,8 @@ int kv_comm_unique_id(void *id_out);
 /* Deferred device-side errors: waits for `stream`, then returns KV_E_TIMEOUT
  * (and clears the record) if a bounded wait inside one of this context's
  * kernels expired since the last check -- the outputs of that call are not
- * valid -- else KV_OK.  The context stays usable either way. */
+ * valid (and its weights, on an 8-bit context, as kv_q8_status says) -- else
+ * KV_OK.  The context stays usable either way. */
 int kv_status(kv_ctx *ctx, void *stream);
 
 const char *kv_strerror(int code);

@@ -603,3 +603,26 @@ def test_a_context_s_status_is_its_own():
             a.status()
         assert e.value.code == K.KV_E_TIMEOUT
         assert a.status() == K.KV_OK
+
+
+def test_a_chunk_whose_wait_ran_out_adds_no_weights():
+    """What kv_evict goes by stays as it was before that call."""
+    (a, old, new, width), b = prompt_context(), prompt_context()[0]
+    out = torch.empty(400, width, device="cuda")
+    kept = []
+    with a, b:
+        for ctx in (a, b):
+            append(ctx, 0, 0, old)
+            append(ctx, 0, 100, new)
+            ctx.attend(0, 100, 400, out)
+            append(ctx, 0, 100, inputs(3, 400, 128, 64, 64))   # the same rows again: their weights are 0
+            if ctx is a:
+                a.debug_inject(1, limit_ns=100_000_000)
+                a.attend(0, 100, 400, out)
+                with pytest.raises(K.KvError) as e:
+                    a.status()
+                assert e.value.code == K.KV_E_TIMEOUT
+            kept.append(torch.empty(64, 60, dtype=torch.int32, device="cuda"))
+            ctx.evict(0, 60, 0, kept[-1])
+        torch.cuda.synchronize()
+        assert torch.equal(*kept) and int(kept[0].max()) < 100
