@@ -517,10 +517,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const int64_t last_blk = (p.n_kv - 1) / kBlock;
             auto scales = [&](int t) {
                 const int64_t i = min(2 * (int64_t)t, last_blk), j = min(2 * (int64_t)t + 1, last_blk);
-                kw[0] = __ldg(ksc + i);
-                kw[1] = __ldg(ksc + j);
-                vw[0] = __ldg(vsc + i);
-                vw[1] = __ldg(vsc + j);
+                kw[0] = ksc[i];
+                kw[1] = ksc[j];
+                vw[0] = vsc[i];
+                vw[1] = vsc[j];
             };
             scales(w.t0);
             const int n0 = n;

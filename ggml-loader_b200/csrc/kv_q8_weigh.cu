@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
                 // (key 0 of the item is a row of the cache: the block of a lane past the cache is the last one)
                 now = w.item;
                 const int64_t blk = min(key / kBlock, p.c.rows / kBlock - 1);
-                const uint32_t kw = __ldg(reinterpret_cast<const uint32_t *>(p.c.k_scale) + (int64_t)w.h * (p.c.rows / kBlock) + blk);
+                const uint32_t kw = reinterpret_cast<const uint32_t *>(p.c.k_scale)[(int64_t)w.h * (p.c.rows / kBlock) + blk];
                 c = p.scale * pow2(scale_exp(kw)) * (MASKED ? 1.0f : kLog2e);
                 first = (int)max((int64_t)0, min((int64_t)p.n_new, key - p.n_past)) * p.r;
             }
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(WL<D, NK>::threads, WL<D, NK>::ctas) weigh_ker
 #pragma unroll
             for (int j = 0; j < L::n_ld; j++) {
                 const int i = t + 128 * j;
-                buf[j] = key0 + i / (D / 16) < p.c.rows ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
+                buf[j] = key0 + i / (D / 16) < p.c.rows ? src[i] : make_uint4(0, 0, 0, 0);
             }
         };
         if (w.more()) load(w.item);

@@ -268,3 +268,16 @@ def test_every_kernel_lets_the_next_one_start_after_its_own_wait():
                 assert any((triggers[i - 1] if i else 0) <= w < t for w in waits), (path, name and name.group(1))
             seen += len(triggers)
     assert seen >= 10
+
+
+def test_the_8_bit_kernels_load_nothing_as_read_only():
+    """A kernel that starts while the one before it ends must not load what that one writes as constant over its own run."""
+    import glob
+    import os
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(K.__file__))), "csrc")
+    files = glob.glob(os.path.join(csrc, "kv_q8*.cu*"))
+    assert len(files) >= 6
+    for path in files:
+        with open(path) as f:
+            text = f.read()
+        assert "__ldg" not in text and "global.nc" not in text and "__restrict__" not in text, path
