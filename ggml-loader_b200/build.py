@@ -1,5 +1,7 @@
 """Build the KV path library in-tree: ggml-loader_b200/lib/libkv_b200.so (and
-the Python binding's C module, ggml-loader_b200/kv_b200/_q8call.so).
+the Python binding's C module, ggml-loader_b200/kv_b200/_q8call with this
+interpreter's suffix: by $CC or gcc and Python's headers.  Without those the
+library is built all the same, and kv_b200.Q8Cache says what is missing).
 
 Every CUDA source is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a); host sources go through nvcc to
@@ -10,6 +12,7 @@ ggml-loader_b200/_build and rebuilt when a source or header is newer.
 import concurrent.futures as cf
 import glob
 import os
+import shlex
 import subprocess
 import sys
 import sysconfig
@@ -20,7 +23,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "lib", "libkv_b200.so")
 INCLUDE = os.path.join(ROOT, "include")
-CALLS = os.path.join(HERE, "kv_b200", "_q8call.so")
+CALLS = os.path.join(HERE, "kv_b200", "_q8call" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -71,7 +74,10 @@ def build(verbose=False, lib=LIB, obj_dir=OBJ, defines=()):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("link failed:\n%s\n%s" % (" ".join(cmd), r.stderr))
-    build_calls()
+    try:
+        build_calls()
+    except (OSError, RuntimeError) as e:
+        sys.stderr.write("the Python binding's C module, which kv_b200.Q8Cache needs, was not built: %s\n" % e)
     return lib
 
 
@@ -79,10 +85,11 @@ def build_calls():
     """The Python binding's C module (kv_b200/q8call.c)."""
     src = os.path.join(HERE, "kv_b200", "q8call.c")
     if _stale(CALLS, [src] + _headers()):
-        cmd = ["gcc", "-O2", "-shared", "-fPIC", "-Wall", "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], src, "-o", CALLS]
+        cmd = shlex.split(os.environ.get("CC") or "gcc")
+        cmd += ["-O2", "-shared", "-fPIC", "-Wall", "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], src, "-o", CALLS]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError("gcc failed for %s:\n%s\n%s" % (src, " ".join(cmd), r.stderr))
+            raise RuntimeError("the C compiler failed for %s:\n%s\n%s" % (src, " ".join(cmd), r.stderr))
     return CALLS
 
 

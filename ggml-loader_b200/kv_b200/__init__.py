@@ -409,7 +409,7 @@ def _calls():
         try:
             from . import _q8call
         except ImportError as e:
-            raise ImportError("kv_b200/_q8call.so is not built (%s); run ggml-loader_b200/build.py" % e)
+            raise ImportError("kv_b200._q8call is not built for this interpreter (%s); run ggml-loader_b200/build.py" % e)
         address = [ctypes.cast(getattr(lib(), n), _vp).value
                    for n in ("kv_q8_store", "kv_q8_load", "kv_q8_attend", "kv_q8_evict")]
         _q8call.init(torch.float32, torch.float16, torch.int32, *address)

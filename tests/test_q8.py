@@ -281,3 +281,21 @@ def test_the_8_bit_kernels_load_nothing_as_read_only():
         with open(path) as f:
             text = f.read()
         assert "__ldg" not in text and "global.nc" not in text and "__restrict__" not in text, path
+
+
+@pytest.mark.parametrize("compiler", ["no-such-compiler", "false"])
+def test_the_library_builds_without_a_c_compiler_for_the_binding(tmp_path, monkeypatch, capfd, compiler):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(K.__file__))), "build.py")
+    spec = importlib.util.spec_from_file_location("a_build", path)
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    monkeypatch.setenv("CC", compiler)
+    monkeypatch.setattr(b, "CALLS", str(tmp_path / "calls.so"))
+    monkeypatch.setattr(b, "_compile", lambda src, *a: src)
+    monkeypatch.setattr(b, "_stale", lambda target, deps: target == b.CALLS)   # (the library is up to date)
+    assert b.build() == b.LIB
+    assert "Q8Cache" in capfd.readouterr().err and not os.path.exists(b.CALLS)
+    with pytest.raises((OSError, RuntimeError)):
+        b.build_calls()
