@@ -406,10 +406,11 @@ uint64_t q8_block_bytes(const kv_config *c)
            (2u * KV_Q8_BLOCK * (uint64_t)c->head_dim + 2u * sizeof(float) + (c->track_weights ? KV_Q8_BLOCK * sizeof(float) : 0u));
 }
 
-int64_t q8_rows(const kv_config *c, int64_t n_ctx)
+// blocks of rows that a layer of an 8-bit cache holds
+int64_t q8_blocks(const kv_config *c, int64_t n_ctx)
 {
     const int64_t rows = c->cache_rows > 0 ? std::min(c->cache_rows, n_ctx) : n_ctx;
-    return (rows + KV_Q8_BLOCK - 1) / KV_Q8_BLOCK * KV_Q8_BLOCK;
+    return rows / KV_Q8_BLOCK + (rows % KV_Q8_BLOCK != 0);   // (n_ctx may be any number)
 }
 
 uint64_t per_position_bytes(const kv_config *c)
@@ -810,7 +811,7 @@ uint64_t kv_cache_bytes(const kv_config *cfg, int64_t n_ctx)
 {
     if (!cfg || n_ctx < 0) return 0;
     if (cfg->cache_type == KV_CACHE_Q8) {
-        const uint64_t block = (uint64_t)cfg->n_layer * q8_block_bytes(cfg), n = (uint64_t)q8_rows(cfg, n_ctx) / KV_Q8_BLOCK;
+        const uint64_t block = (uint64_t)cfg->n_layer * q8_block_bytes(cfg), n = (uint64_t)q8_blocks(cfg, n_ctx);
         return block > 0 && n > UINT64_MAX / block ? UINT64_MAX : block * n;
     }
     const uint64_t per_token = (uint64_t)cfg->n_layer * (uint64_t)cfg->head_dim * (uint64_t)cfg->n_head_kv * 2u * 2u;
@@ -958,7 +959,7 @@ static int alloc_impl(const kv_config *cfg_in, kv_ctx **out)
     c.ring_cells = ctx->ring;
     const bool q8 = c.cache_type == KV_CACHE_Q8;
     if (q8) {
-        ctx->rows = q8_rows(&c, ctx->n_ctx);
+        ctx->rows = q8_blocks(&c, ctx->n_ctx) * KV_Q8_BLOCK;
         if (ctx->rows > kMaxPositions - KV_Q8_BLOCK) return bail(fail(KV_E_ARG, "kv_alloc: n_ctx above 2^31 - 64 positions"));
     }
     if (c.n_batch_max > ctx->rows) c.n_batch_max = (int32_t)ctx->rows;

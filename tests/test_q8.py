@@ -299,3 +299,14 @@ def test_the_library_builds_without_a_c_compiler_for_the_binding(tmp_path, monke
     assert "Q8Cache" in capfd.readouterr().err and not os.path.exists(b.CALLS)
     with pytest.raises((OSError, RuntimeError)):
         b.build_calls()
+
+
+def test_cache_bytes_at_the_largest_sizes():
+    top = (1 << 64) - 1
+    assert K.cache_bytes(config(), (1 << 63) - 1) == top
+    assert K.cache_bytes(config(), 1 << 62) == top
+    one = K.cache_bytes(config(n_layer=1, n_head_kv=1, n_head=1), 32)
+    assert K.cache_bytes(config(n_layer=1, n_head_kv=1, n_head=1), 1 << 50) == one << 45
+    assert K.cache_bytes(config(n_layer=1, n_head_kv=1, n_head=1), (1 << 50) + 1) == (one << 45) + one
+    small = config(cache_rows=64, track_weights=1)
+    assert K.cache_bytes(small, (1 << 63) - 1) == K.cache_bytes(small, 64)
