@@ -595,3 +595,36 @@ def test_masked_blocks_in_which_nothing_was_stored(n_new, size):
         c.store(at, k, v)
         at = n_kv if b is None else (b + 1) * B
     check(c, hq, n_past, n_new, queries(3, n_new, hq, d), mask=mask.cuda())
+
+
+# ---- groups of more than 16 query heads ----------------------------------------
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("h, r, n_new, n_past", [(1, 17, 1, 0), (2, 33, 1, 500), (1, 71, 1, 90), (2, 71, 5, 700), (1, 100, 3, 333),
+                                                 (1, 128, 1, 1000), (2, 128, 3, 64), (3, 65, 9, 1500)])
+def test_attend_large_groups(d, h, r, n_new, n_past):
+    """Tiles of 128 / r tokens with rows left over; rows of the weights' pass that are cut across tokens."""
+    c = filled(h, n_past + n_new, d, weight=True, seed=n_past)
+    c.w.uniform_(0.0, 2.0)
+    check(c, h * r, n_past, n_new, queries(n_past, n_new, h * r, d), w0=c.w.cpu().clone())
+
+
+@pytest.mark.parametrize("r, n_new", [(17, 1), (71, 2), (100, 4), (128, 1)])
+@pytest.mark.parametrize("f16", [False, True])
+def test_attend_large_groups_under_a_mask(r, n_new, f16):
+    h, d, n_past = 2, 64, 300
+    n_kv = n_past + n_new
+    c = filled(h, n_kv, d, weight=True)
+    mask = torch.randn(n_new, n_kv + 5, generator=torch.Generator().manual_seed(4))
+    mask[torch.rand(mask.shape, generator=torch.Generator().manual_seed(5)) < 0.3] = float("-inf")
+    if n_new > 1:
+        mask[1] = float("-inf")
+    mask = mask.to(torch.float16 if f16 else torch.float32).cuda()
+    check(c, h * r, n_past, n_new, queries(9, n_new, h * r, d), mask=mask, flash=True)
+
+
+def test_a_status_is_fine_after_calls_that_are():
+    c = filled(2, 300, 64, weight=True)
+    for n_new in (1, 40):
+        check(c, 4, 300 - n_new, n_new, queries(1, n_new, 4, 64), w0=c.w.cpu().clone())
+        assert c.q8.status() == K.KV_OK
+        assert c.q8.status(torch.cuda.Stream()) == K.KV_OK

@@ -626,3 +626,21 @@ def test_a_chunk_whose_wait_ran_out_adds_no_weights():
             ctx.evict(0, 60, 0, kept[-1])
         torch.cuda.synchronize()
         assert torch.equal(*kept) and int(kept[0].max()) < 100
+
+
+@pytest.mark.parametrize("n_past, n_new", [(50, 1), (50, 3), (20, 150)])
+def test_many_query_heads_a_kv_head(n_past, n_new):
+    """A group of 48: a single token goes to the chunk's kernel."""
+    sp = spec(d=64, hq=48, h=1, layers=1)
+    with q8_context(sp, track_weights=True) as a, K.Context(K.make_config(sp)) as b:
+        append(a, 0, 0, inputs(1, n_past, 48, 1, 64))
+        outs = []
+        for ctx in (a, b):
+            append(ctx, 0, n_past, inputs(2, n_new, 48, 1, 64))
+        for which in (0, 1):
+            b.import_rows(0, which, 0, a.export_rows(0, which, 0, n_past + n_new))
+        for ctx in (a, b):
+            outs.append(torch.empty(n_new, 48 * 64, device="cuda"))
+            ctx.attend(0, n_past, n_new, outs[-1])
+            ctx.status()
+        close(*outs)
