@@ -628,6 +628,34 @@ def test_a_chunk_whose_wait_ran_out_adds_no_weights():
         assert torch.equal(*kept) and int(kept[0].max()) < 100
 
 
+@pytest.mark.parametrize("n_past, n_new", [(600, 1), (600, 40), (0, 300)])
+@pytest.mark.parametrize("shift", [0.0, 8.0])
+def test_the_error_that_the_codes_bring(n_past, n_new, shift):
+    """Both contexts on the same rows.  A code is off by up to half a scale, evenly: by scale / sqrt(12) in the mean.  With
+    queries and values of size 1 that is the error of a score, and so the relative one of a weight, and that of a value:
+    sqrt(sk^2 + sv^2) / sqrt(12) of the outputs, over thousands of them; 1.5 times that is allowed (weights are not all
+    small, scales differ from block to block)."""
+    hq, h, d = 8, 2, 128
+    sp = spec(layers=1, n_rot=0, n_ctx=1024)
+    with q8_context(sp) as a, K.Context(K.make_config(sp)) as b:
+        outs = []
+        for ctx in (a, b):
+            for at, n, seed in ((0, 200, 1), (200, n_past - 200, 2), (n_past, n_new, 3)) if n_past else ((0, n_new, 3),):
+                q, k, v = inputs(seed, n, hq, h, d)
+                k = k.clone()
+                k.view(n, h, d)[:, :, :4] += shift   # a few channels of K larger than the others
+                append(ctx, 0, at, (q, k, v))
+            outs.append(torch.empty(n_new, hq * d, device="cuda"))
+            ctx.attend(0, n_past, n_new, outs[-1])
+        scale = []
+        for which in (0, 1):
+            x = b.export_rows(0, which, 0, n_past + n_new).view(np.float16).astype(np.float64)
+            words = [R.quantise_block(x[i:i + B, j])[1] for i in range(0, len(x), B) for j in range(h)]
+            scale.append(np.sqrt(np.mean(4.0 ** R.word_exp(words))))
+        got = float((outs[0] - outs[1]).norm() / outs[1].norm())
+        assert 1e-3 < got <= 1.5 * np.hypot(*scale) / np.sqrt(12.0), (got, scale)
+
+
 @pytest.mark.parametrize("n_past, n_new", [(50, 1), (50, 3), (20, 150)])
 def test_many_query_heads_a_kv_head(n_past, n_new):
     """A group of 48: a single token goes to the chunk's kernel."""
