@@ -6,9 +6,14 @@
 // weights W = e^t 2^ev relative to a running reference of the row, F16, and
 //   out = sum W codes_v / sum W 2^-ev,
 // so both operands from the cache are its integer codes, exact in F16.
-// Reference: unmasked rows keep one number M (log2 units of e^t 2^ev); with a
-// mask it is a pair (m, me), since a mask of the type's lowest value leaves no
-// room next to it for an exponent.
+// Reference: unmasked rows keep one number M (log2 units of e^t 2^ev), a whole
+// one, so that ev - M is exact up to 2^24 and a weight's exponent is rounded
+// once.  Past it, a score of 10^7, a row is made NaN: weights would be off by the
+// lost exponents or leave F16's range.  (The pair that a mask has is exact there
+// too, but costs the loop without a mask a subtraction and an addition a score:
+// 512 tokens at 16k 188 us, so 180.)
+// With a mask it is a pair (m, me), since a mask of the type's lowest value
+// leaves no room next to it for an exponent.
 //
 // Work: a tile is 128 query rows of one KV head (row = token * r + head of the
 // group); a CTA holds two of them (one at head_dim 256), so a sub-tile of 64
@@ -47,6 +52,7 @@ namespace {
 using namespace sm100;
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kFar = 16777216.0f;           // rows without a mask whose reference is larger are NaN
 constexpr float kBias = 7.0f, kTop = 15.0f;   // as kv_q8_rows.cu: a new reference's weight is 2^7, it moves past 2^15
 constexpr int kThreads = 512;
 constexpr int kSub = 64;   // keys of a sub-tile
@@ -594,9 +600,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
                     const float x0 = max32(v), x1 = max32(v + 32);
                     const float z = fmaxf(__fmaf_rn(x0, c0, ev0), __fmaf_rn(x1, c1, ev1));
                     if (z > m + kTop) {   // (never without a visible key: z = -inf)
-                        f = ex2_approx(m - (z - kBias));   // 0 while m = -inf
+                        const float to = rintf(z) - kBias;
+                        f = ex2_approx(m - to);   // 0 while m = -inf
                         moved = m != -CUDART_INF_F;
-                        m = z - kBias;
+                        m = to;
                     }
                     if ((bad_scale(v0) && x0 > -CUDART_INF_F) || (bad_scale(v1) && x1 > -CUDART_INF_F)) bad = CUDART_NAN_F;
                     const float ref = m == -CUDART_INF_F ? 0.0f : m;
@@ -645,6 +652,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const AttendParams p
             const int64_t block = (int64_t)cta + w.pair;   // (CTA, pair) in order: their sum counts them
             const int in = g * 128 + row;
             float scl = 1.0f;
+            if constexpr (!MASKED) {   // (m = -inf: no visible key)
+                const float far = fabsf(m) >= kFar && m != -CUDART_INF_F ? CUDART_NAN_F : 0.0f;
+                l += far;
+                bad += far;
+            }
             if constexpr (MASKED) {   // both sums relative to e^m alone
                 scl = pow2((int)me);
                 l *= scl;

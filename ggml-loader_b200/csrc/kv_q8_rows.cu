@@ -204,9 +204,9 @@ __device__ __forceinline__ float softmax_block(float (&s)[4], RowState &st, floa
 #pragma unroll
         for (int i = 0; i < 4; i++) s[i] = ex2_approx(__fmaf_rn(s[i] - m, kLog2e, up));
     } else {
-        const float ref = up - m;
+        // (the difference first: beside a score past 2^24 the exponent would be lost)
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = ex2_approx(s[i] + ref);
+        for (int i = 0; i < 4; i++) s[i] = ex2_approx((s[i] - m) + up);
     }
     st.l = __fmaf_rn((s[0] + s[1]) + (s[2] + s[3]), pow2((int)-up), st.l);
     return orescale;

@@ -379,6 +379,9 @@ uint64_t kv_q8_attend_workspace(const kv_q8_cache *cache, int32_t n_head, int64_
  * mask, mask_type, mask_stride, flags: as kv_attend_mask (NULL: causal; the
  * flags change only a row without a visible key: NaN, or 0 with KV_ATTN_FLASH).
  * A key masked with -inf does not enter the row, whatever its block holds.
+ * Scores may be of any finite size with at most 16 query rows a KV head (n_new *
+ * n_head / n_head_kv), or with a mask; else one past 10^7 (or below -10^7) may
+ * make its row NaN, as one that is not finite does.
  * With cache->weight, weight[h][i] of every attended row i grows by the softmax
  * weights that the n_new tokens' query heads of KV head h gave it; a query row
  * whose softmax is not finite (no visible key, NaN or inf scores) adds nothing.

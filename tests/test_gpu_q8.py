@@ -628,3 +628,51 @@ def test_a_status_is_fine_after_calls_that_are():
         check(c, 4, 300 - n_new, n_new, queries(1, n_new, 4, 64), w0=c.w.cpu().clone())
         assert c.q8.status() == K.KV_OK
         assert c.q8.status(torch.cuda.Stream()) == K.KV_OK
+
+
+@pytest.mark.parametrize("n_new", [1, 3, 12, 40])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("size", [300.0, 3000.0, 30000.0])
+def test_scores_of_any_size(n_new, masked, size):
+    """Queries and keys up to F16's range: scores of up to 10^10, whose neighbours in 32 bits are far apart.  Values of
+    different sizes from block to block, so that blocks have different exponents beside such a score.  Chunks without a mask
+    are documented to hold scores of 10^7: a row with larger ones is right, or NaN and adds no weights."""
+    h, hq, d, n_past = 2, 8, 64, 700
+    n_kv, r = n_past + n_new, hq // h
+    rng = np.random.default_rng(6)
+    c = Cache(h, -(-n_kv // B) * B, d, weight=True)
+    k = np.clip(rows_of(rng, n_kv, h, d) * size / 2, -60000, 60000)
+    spread = np.repeat(2.0 ** rng.integers(-12, 12, n_kv // B + 1), B)[:n_kv, None, None]
+    c.store(0, k.astype(np.float32), (rows_of(rng, n_kv, h, d) * spread).astype(np.float32))
+    q = (queries(3, n_new, hq, d, f16=False) * size).clamp(-60000, 60000).half()
+    mask = torch.zeros(n_new, n_kv).cuda() if masked else None
+    kk = torch.from_numpy(np.stack([c.values(n_kv, i)[0].numpy() for i in range(h)]))
+    vv = torch.from_numpy(np.stack([c.values(n_kv, i)[1].numpy() for i in range(h)]))
+    s = torch.einsum("thrd,hnd->thrn", q.double().cpu().view(n_new, h, r, d), kk) / 8.0
+    if not masked:
+        s = s.masked_fill((torch.arange(n_kv)[None, :] > n_past + torch.arange(n_new)[:, None])[:, None, None, :], float("-inf"))
+    far = s.nan_to_num(neginf=0.0).abs().amax(-1) > 1e7
+    if masked or n_new * r <= 16 or not far.any():
+        far = torch.zeros_like(far)
+        out = check(c, hq, n_past, n_new, q, mask=mask)
+    else:
+        out = torch.zeros(n_new, hq * d, device="cuda")
+        ws = torch.empty(c.q8.attend_workspace(hq, n_past, n_new), dtype=torch.uint8, device="cuda")
+        c.q8.attend(hq, n_past, n_new, q, out, workspace=ws)
+        # rows whose largest score has not passed 2^24 / log2(e), 1.17e7, by its exponent and rounding, add 1 each (a weight's
+        # error is a factor of up to 2 there: an exponent's half step); no others do
+        total = c.w.cpu().double().sum(-1)
+        most = (s.amax(-1).abs() < 1.2e7).sum((0, 2)).double()
+        assert torch.isfinite(c.w).all() and (total <= most * 2.0 + 1e-3).all() and (c.w >= 0).all()
+    # all but the largest score's key is far below it: the outputs are its values
+    top = s.topk(2, -1)
+    # (the two largest apart by more than the sums' rounding, so that the second's weight is below 2^-24)
+    err = (d + 4) * 2.0 ** -24 * s.abs().nan_to_num(posinf=0.0, neginf=0.0).amax(-1) * 4
+    clear = top.values[..., 0] - top.values[..., 1] > 17.0 + err * 8
+    want = torch.gather(vv[None].expand(n_new, -1, -1, -1), 2, top.indices[..., :1].expand(-1, -1, -1, d))
+    got = out.double().cpu().view(n_new, h, r, d)
+    assert clear.float().mean() > 0.5
+    nan = torch.isnan(got).all(-1)
+    assert not (nan & ~far).any() and torch.equal(nan, (~torch.isfinite(got)).any(-1))
+    off = (got - want).abs() > want.abs() * 2.0 ** -10 + vv.abs().max() * 2.0 ** -23
+    assert not (off.any(-1) & clear & ~nan).any()
