@@ -446,7 +446,8 @@ cudaEvent_t pool_event(kv_ctx *ctx)
     return e;
 }
 
-// Wraps one kernel launch: counts it and, when profiling, brackets it with events.
+// Wraps one kernel launch (or an 8-bit call's, which count themselves): counts
+// it and, when profiling, brackets it with events.
 template <class F>
 int launch(kv_ctx *ctx, int kernel_id, cudaStream_t st, const char *what, F &&fn)
 {
@@ -456,9 +457,10 @@ int launch(kv_ctx *ctx, int kernel_id, cudaStream_t st, const char *what, F &&fn
         b = pool_event(ctx);
         cudaEventRecord(a, st);
     }
+    const int64_t before = kvb::q8::launched();
     cudaError_t e = fn();
     if (e != cudaSuccess) return cuda_fail(e, what);
-    ctx->launches.fetch_add(1, std::memory_order_relaxed);
+    ctx->launches.fetch_add(std::max<int64_t>(1, kvb::q8::launched() - before), std::memory_order_relaxed);
     if (ctx->prof_on) {
         cudaEventRecord(b, st);
         try {

@@ -74,7 +74,9 @@ cudaError_t launch_pdl(K kernel, dim3 grid, unsigned block, size_t smem, const P
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    launched() += e == cudaSuccess;
+    return e;
 }
 
 }  // namespace q8

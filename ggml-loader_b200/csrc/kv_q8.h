@@ -105,6 +105,9 @@ cudaError_t error_word(unsigned **dev);
 // a record's bits since the last call, behind what `st` holds (record: two words, one of them for the answer's way back)
 cudaError_t take_error(unsigned *record, cudaStream_t st, unsigned *word);
 
+// kernels that the calling thread has launched (launch_pdl counts them)
+int64_t &launched();
+
 // Runs a function once a device (a kernel's attributes last); devices past 63 run it every time.
 struct Once {
     std::atomic<uint64_t> done{0};

@@ -38,6 +38,12 @@ uint64_t lay_out(AttendParams &p, char *ws)
 
 }  // namespace
 
+int64_t &launched()
+{
+    static thread_local int64_t n = 0;
+    return n;
+}
+
 uint64_t attend_workspace(const AttendParams &p)
 {
     AttendParams q = p;

@@ -29,7 +29,8 @@ int kv_gen_normal_device(float *dst, uint64_t seed, uint64_t stream,
 
 /* Per-kernel timing with CUDA events recorded around each launch on the
  * launching stream.  Kernel ids below.  Enabling adds one event pair per
- * launch; totals accumulate until kv_profile_reset. */
+ * launch (one around all kernels of an 8-bit context's kv_attend or kv_evict);
+ * totals accumulate until kv_profile_reset. */
 #define KV_K_APPEND   0
 #define KV_K_ATTN     1
 #define KV_K_PREFILL  2   /* both tensor-core passes */

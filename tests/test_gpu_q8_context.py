@@ -672,3 +672,31 @@ def test_many_query_heads_a_kv_head(n_past, n_new):
             ctx.attend(0, n_past, n_new, outs[-1])
             ctx.status()
         close(*outs)
+
+
+def test_launches_are_counted_one_by_one():
+    with q8_context(spec(layers=1), track_weights=True) as a, q8_context(spec(layers=1)) as b:
+        out = torch.empty(64, 8 * 128, device="cuda")
+
+        def launches(ctx, fn):
+            n = ctx.launch_count()
+            fn()
+            return ctx.launch_count() - n
+
+        for ctx in (a, b):
+            assert launches(ctx, lambda: append(ctx, 0, 0, inputs(1, 64, 8, 2, 128))) == 2   # the append, the store
+        # 64 keys are one sub-tile of a KV head, which one CTA takes: the chunk alone; with weights also their pass
+        assert launches(a, lambda: a.attend(0, 0, 64, out)) == 2
+        assert launches(b, lambda: b.attend(0, 0, 64, out)) == 1
+        for ctx in (a, b):
+            append(ctx, 0, 64, inputs(2, 64, 8, 2, 128))
+        # 128 are two, cut between CTAs: a fold as well
+        assert launches(a, lambda: a.attend(0, 64, 64, out)) == 3
+        assert launches(b, lambda: b.attend(0, 64, 64, out)) == 2
+        for ctx in (a, b):
+            append(ctx, 0, 64, inputs(2, 1, 8, 2, 128))
+        # a token over 65 keys, a head a CTA: with weights the join's kernel adds them
+        assert launches(a, lambda: a.attend(0, 64, 1, out)) == 2
+        assert launches(b, lambda: b.attend(0, 64, 1, out)) == 1
+        assert launches(a, lambda: a.evict(0, 40, 4)) == 2
+        assert a.status() == b.status() == K.KV_OK
