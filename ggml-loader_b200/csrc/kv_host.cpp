@@ -732,8 +732,7 @@ void unmap_peers(kv_ctx *ctx)
     ctx->rx = nullptr;
 }
 
-// The single-token append a kv_append deferred to the following kv_attend.
-// the rows kv_append wrote to q8_new, into the 8-bit cache
+// The rows kv_append wrote to q8_new, into the 8-bit cache.
 int store_new_rows(kv_ctx *ctx, int layer, int64_t row0, int n_new, cudaStream_t st)
 {
     kvb::q8::StoreParams p{};
@@ -747,6 +746,7 @@ int store_new_rows(kv_ctx *ctx, int layer, int64_t row0, int n_new, cudaStream_t
     return launch(ctx, KV_K_APPEND, st, "8-bit store kernel", [&] { return kvb::q8::launch_store(p, st); });
 }
 
+// The single-token append a kv_append deferred to the following kv_attend.
 int run_append(kv_ctx *ctx, const Pending &pd)
 {
     const kv_config &c = ctx->cfg;

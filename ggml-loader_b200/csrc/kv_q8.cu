@@ -445,8 +445,8 @@ __device__ __forceinline__ void move_codes(uint4 &x, int k, bool bad)
 
 // One block of dst of a KV head a CTA, K and V: a row is D/16 threads, 16 codes
 // each of K and of V.  Many small CTAs keep the gathers in flight (32k rows to
-// 16k with the selection and the read-back: 44 us; with registers for 5 CTAs an
-// SM instead of 6 45.7 us, two blocks a CTA 47 us, four 51 us); the codes'
+// 16k with the selection and the read-back: 45 us; against each other, registers
+// for 6 CTAs an SM 44.1 us, for 5 45.7, two blocks a CTA 47, four 51); the codes'
 // arithmetic is in halves, two at a time (with conversions to float and back the
 // conversions were the bound, 50 us).  A warp a block, all of its rows in
 // flight, measured 52 us.

@@ -5,7 +5,10 @@
 // The mathematics is kv_q8_rows.cu's: scores t = (q . codes) * ks * scale,
 // weights W = e^t 2^ev relative to a running reference of the row, F16, and
 //   out = sum W codes_v / sum W 2^-ev,
-// so both operands from the cache are its integer codes, exact in F16.
+// so both operands from the cache are its integer codes, exact in F16.  The
+// weights are F16 with them (both operands of an MMA have one type), off by up to
+// 2^-11 of each, as the F16 cache's kernel rounds them; their low halves, 22 bits
+// in all, would be half as many MMAs again on a pipe that is 63 % busy.
 // Reference: unmasked rows keep one number M (log2 units of e^t 2^ev), a whole
 // one, so that ev - M is exact up to 2^24 and a weight's exponent is rounded
 // once.  Past it, a score of 10^7, a row is made NaN: weights would be off by the
@@ -29,7 +32,7 @@
 //   warp 3      brings the codes in (bulk copies, 32 KB in flight); owns TMEM
 //   warps 4-7   convert them to F16 in the 128-byte-swizzled layout the tensor
 //               cores read; also the queries.  (Codes loaded into registers some
-//               units ahead: 512 tokens at 16k 262 us, so 175: the fence before a
+//               units ahead: 512 tokens at 16k 262 us, so 175 then: the fence before a
 //               tile is handed over waits for every load in flight)
 //   warps 8-15  softmax of tile A and tile B, a query row a thread: S from TMEM,
 //               weights back as F16 pairs; rescales O when the reference moves;

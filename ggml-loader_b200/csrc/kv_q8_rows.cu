@@ -22,10 +22,10 @@
 // the loop); partial (m, sum, out) rows of the CTAs of a head are joined in
 // their cluster, or by a second kernel launched programmatically.
 //
-// One token, 8 heads of 128 with 4 query heads each: 131k keys 51.6 us, 5.2
+// One token, 8 heads of 128 with 4 query heads each: 131k keys 51 us, 5.2
 // TB/s (268 MB; at that length the power limit lowers the clock, and the SMs
-// issue an instruction in 54 % of their cycles), 32k keys 16.5 us, of which
-// about 6 are the launch, the first loads' latency and the joins.
+// issue an instruction in 54 % of their cycles), 32k keys 17.5 us, of which
+// about 7 are the launch, the first loads' latency and the joins.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -47,8 +47,9 @@ constexpr float kTop = 15.0f;    // and it moves where a weight would pass 2^kTo
 
 // NG: groups of 8 query rows.  DUP (up to 4 rows): columns 4-7 of the group
 // repeat rows 0-3 and carry the low halves of their weights, W - F16(W), so the
-// weights enter with 22 bits at no cost; otherwise in F16 (11 bits, half a step
-// 2^-12 of each: the outputs' own F16 rounding is as large).
+// weights enter with 22 bits at no cost; otherwise in F16 (11 bits, off by up to
+// 2^-11 of each, as the F16 cache's kernels round them and as an F16 output is
+// rounded once more; their low halves would be as many products again).
 template <int D, int NG, int W_>
 struct Rows {
     static constexpr int W = W_;                                     // warps

@@ -294,6 +294,8 @@ int kv_attend_decode_noalloc(const uint16_t *k_cache, const uint16_t *v_cache,
  * (kv_q8_evict; keep at most the rows in use).  Positions are not renumbered:
  * the kept keys stay rotated as they are, the next kv_append is again at the
  * next position, n_past, and kv_attend attends over the rows that are left.
+ * The weight is what every kv_attend since a row's kv_append gave it, those of
+ * tokens rewound since, and of calls made twice, among them.
  * Every layer is evicted by its own call.  Rewinding n_past is possible by up
  * to `recent` tokens, as far as an earlier eviction allowed it (KV_E_RANGE
  * beyond), or to 0.  kept: DEVICE int32
@@ -323,6 +325,14 @@ int kv_layer_rows(const kv_ctx *ctx, int32_t layer, int64_t *used, int64_t *capa
  *   F16 cache would hold it.  What is not finite then (inf, NaN) has code -128,
  *   which reads back as NaN, and its block's scale is NaN (the exponent kept in
  *   the low byte): attention takes every row of such a block as NaN.
+ *
+ * What that costs: a value is off by up to half its block's scale, scale /
+ * sqrt(12) in the mean, and 32 rows of a head share one scale, set by their largest
+ * magnitude.  With queries and values of size 1 an output is off by about
+ * sqrt(sk^2 + sv^2) / sqrt(12) of its size, sk and sv the scales: 1.7 % with normally
+ * distributed rows of 128, 3.8 % where four channels of K lie 8 deviations off the
+ * others, 14 % where two lie 30 off (2048 keys).  K with channels far larger than
+ * the rest is what this format is worst at.
  *
  * All pointers are DEVICE pointers on the current device, k and v 16-byte
  * aligned; rows is a multiple of KV_Q8_BLOCK, at most 2^31 - 32.  head_dim: 64,
@@ -385,7 +395,13 @@ uint64_t kv_q8_attend_workspace(const kv_q8_cache *cache, int32_t n_head, int64_
  * With cache->weight, weight[h][i] of every attended row i grows by the softmax
  * weights that the n_new tokens' query heads of KV head h gave it; a query row
  * whose softmax is not finite (no visible key, NaN or inf scores) adds nothing.
- * Results do not depend on timing (no atomics).
+ * The weights are a sum over calls: a call made twice for the same rows, a
+ * replayed graph, and draft tokens that are rewound afterwards have all left
+ * theirs in the rows that stay (kv_q8_store sets only its own rows' to 0).
+ * Results do not depend on timing (no atomics).  On their way to V the softmax
+ * weights are rounded to 22 bits with up to 4 query rows a KV head (n_new * n_head
+ * / n_head_kv) and to F16 with more, as kv_attend rounds them, so a token's bits
+ * alone and among others differ.
  * workspace: 256-byte aligned device memory of at least kv_q8_attend_workspace
  * bytes.  Returns KV_OK, KV_E_ARG, KV_E_RANGE (rows outside the cache, n_new or
  * workspace too small or large) or KV_E_CUDA.  n_new: at most 65535.

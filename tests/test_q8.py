@@ -310,3 +310,34 @@ def test_cache_bytes_at_the_largest_sizes():
     assert K.cache_bytes(config(n_layer=1, n_head_kv=1, n_head=1), (1 << 50) + 1) == (one << 45) + one
     small = config(cache_rows=64, track_weights=1)
     assert K.cache_bytes(small, (1 << 63) - 1) == K.cache_bytes(small, 64)
+
+
+@pytest.mark.parametrize("channels, shift, stated", [(0, 0.0, 0.017), (4, 8.0, 0.038), (2, 30.0, 0.14)])
+def test_the_accuracy_that_the_header_states(channels, shift, stated):
+    """The outputs' error that codes bring, by the definition alone: near the figures in kv_api.h and the rule beside them.
+    (A rule for the mean of thousands of outputs, whose weights are not all small: a quarter of it is allowed.)"""
+    got, rule = [], []
+    for seed in range(4):
+        rng = np.random.default_rng(seed)
+        k, v, q = (rng.standard_normal((n, 128)).astype(np.float16).astype(np.float64) for n in (2048, 2048, 64))
+        k[:, :channels] += shift
+
+        def held(x):
+            out, scale = np.empty_like(x), []
+            for b in range(0, len(x), R.BLOCK):
+                c, w = R.quantise_block(x[b:b + R.BLOCK])
+                out[b:b + R.BLOCK] = R.row_values(c, np.array([w], np.uint32))
+                scale.append(2.0 ** int(R.word_exp(w)))
+            return out, np.sqrt(np.mean(np.square(scale)))
+
+        def attend(k, v):
+            s = q @ k.T / np.sqrt(128.0)
+            p = np.exp(s - s.max(1, keepdims=True))
+            return p @ v / p.sum(1, keepdims=True)
+
+        (k8, sk), (v8, sv) = held(k), held(v)
+        want = attend(k, v)
+        got.append(np.linalg.norm(attend(k8, v8) - want) / np.linalg.norm(want))
+        rule.append(np.hypot(sk, sv) / np.sqrt(12.0))
+    assert abs(np.mean(got) / np.mean(rule) - 1.0) <= 0.25
+    assert abs(np.mean(got) / stated - 1.0) <= 0.1
