@@ -325,7 +325,8 @@ class Context:
         in all; kept: a CUDA int32 tensor [n_head_kv][keep] of their numbers, or None."""
         if kept is not None:
             import torch
-            assert kept.dtype == torch.int32 and kept.is_contiguous() and kept.shape == (self.n_kv_heads, keep)
+            if kept.dtype != torch.int32 or not kept.is_contiguous() or kept.shape != (self.n_kv_heads, keep) or not kept.is_cuda:
+                raise ValueError("kept must be a contiguous CUDA int32 tensor [%d][%d]" % (self.n_kv_heads, keep))
         return _check(lib().kv_evict(self.h, layer, keep, recent, _ptr(kept), _stream(stream)), "kv_evict")
 
     def layer_rows(self, layer):

@@ -341,3 +341,21 @@ def test_the_accuracy_that_the_header_states(channels, shift, stated):
         rule.append(np.hypot(sk, sv) / np.sqrt(12.0))
     assert abs(np.mean(got) / np.mean(rule) - 1.0) <= 0.25
     assert abs(np.mean(got) / stated - 1.0) <= 0.1
+
+
+def test_a_context_s_evict_refuses_other_tensors():
+    """A tensor in host memory among them, whose address the kernel would write to.  (The checks come before the library's call,
+    which refuses the missing context.)"""
+    torch = pytest.importorskip("torch")
+    ctx = object.__new__(K.Context)
+    ctx.h, ctx.n_kv_heads = None, 2
+    try:
+        for kept in (torch.zeros(2, 5, dtype=torch.int32), torch.zeros(2, 5, dtype=torch.int64), torch.zeros(2, 4, dtype=torch.int32),
+                     torch.zeros(5, 2, dtype=torch.int32).t()):
+            with pytest.raises(ValueError):
+                ctx.evict(0, 5, 1, kept)
+        with pytest.raises(K.KvError) as e:
+            ctx.evict(0, 5, 1)
+        assert e.value.code == K.KV_E_ARG
+    finally:
+        ctx.h = None
